@@ -468,4 +468,55 @@ int dsv3_mla_latent_gemm(const void* x, const float* x_s, const void* w, const f
                              pe_batch_stride, y, s, batch, rows, (int)q_rank, q_eps, kv_eps, (hipStream_t)stream);
 }
 
+// What the functions of the paged cache share (no GPU call).
+static int mla_pages_validate(const dsv3_mla_pages* cache, int64_t batch) {
+    if (!cache) return DSV3_ERR_NULL_POINTER;
+    if (cache->pages < 1 || cache->pages > 0x7fffffff || cache->page_size < 8 || cache->page_size > 65536 || cache->page_size % 8 != 0 ||
+        cache->table_width < 1 || cache->table_width > 0x7fffffff || batch < 0 || batch > 65535)
+        return DSV3_ERR_BAD_SHAPE;
+    if (batch == 0) return DSV3_OK;
+    if (!cache->kv || !cache->kv_scale || !cache->pe || !cache->table) return DSV3_ERR_NULL_POINTER;
+    if (!aligned(cache->kv, 16) || !aligned(cache->kv_scale, 4) || !aligned(cache->pe, 16) || !aligned(cache->table, 4)) return DSV3_ERR_MISALIGNED;
+    return DSV3_OK;
+}
+
+int dsv3_mla_latent_paged(const void* a, int64_t a_stride, const void* q_norm, const void* kv_norm, const float* freqs,
+                          const dsv3_mla_pages* cache, const int32_t* starts, const int32_t* counts, void* y, float* s, int64_t batch,
+                          int64_t rows, int64_t q_rank, int64_t kv_rank, int rope_dim, float q_eps, float kv_eps, void* stream) {
+    const int rc = mla_pages_validate(cache, batch);
+    if (rc != DSV3_OK) return rc;
+    if (kv_rank != 512 || rope_dim != 64 || q_rank < 0 || q_rank > 2048 || q_rank % 128 != 0 || rows < 0 || rows > 0x7fffff ||
+        batch * rows > 0x7fffffff || a_stride % 8 != 0 || a_stride < q_rank + kv_rank + rope_dim)
+        return DSV3_ERR_BAD_SHAPE;
+    if (batch == 0 || rows == 0) return DSV3_OK;
+    if (!a || !kv_norm || !freqs || !starts || !counts || (q_rank && (!q_norm || !y || !s))) return DSV3_ERR_NULL_POINTER;
+    if (!aligned(a, 16) || !aligned(kv_norm, 16) || !aligned(freqs, 8) || !aligned(starts, 4) || !aligned(counts, 4) ||
+        (q_rank && (!aligned(q_norm, 16) || !aligned(y, 8) || !aligned(s, 4))))
+        return DSV3_ERR_MISALIGNED;
+    return launch_mla_latent_paged(a, a_stride, q_norm, kv_norm, freqs, *cache, starts, counts, y, s, batch, rows, (int)q_rank, q_eps, kv_eps,
+                                   (hipStream_t)stream);
+}
+
+int dsv3_mla_cache_read(const dsv3_mla_pages* cache, const int32_t* lengths, void* kv, void* pe, int64_t batch, int64_t positions,
+                        void* stream) {
+    const int rc = mla_pages_validate(cache, batch);
+    if (rc != DSV3_OK) return rc;
+    if (positions < 0 || positions > 0x7fffff || batch * ((positions + 7) / 8) > 0x7fffffff) return DSV3_ERR_BAD_SHAPE;
+    if (batch == 0 || positions == 0) return DSV3_OK;
+    if (!lengths || !kv || !pe) return DSV3_ERR_NULL_POINTER;
+    if (!aligned(lengths, 4) || !aligned(kv, 16) || !aligned(pe, 16)) return DSV3_ERR_MISALIGNED;
+    return launch_mla_cache_read(*cache, lengths, kv, pe, batch, positions, (hipStream_t)stream);
+}
+
+int dsv3_mla_cache_keep(const dsv3_mla_pages* cache, const int32_t* starts, const int32_t* path, const int32_t* kept, int64_t batch,
+                        int most, void* stream) {
+    const int rc = mla_pages_validate(cache, batch);
+    if (rc != DSV3_OK) return rc;
+    if (most < 0 || most > 64) return DSV3_ERR_BAD_SHAPE;
+    if (batch == 0 || most == 0) return DSV3_OK;
+    if (!starts || !path || !kept) return DSV3_ERR_NULL_POINTER;
+    if (!aligned(starts, 4) || !aligned(path, 4) || !aligned(kept, 4)) return DSV3_ERR_MISALIGNED;
+    return launch_mla_cache_keep(*cache, starts, path, kept, batch, most, (hipStream_t)stream);
+}
+
 }  // extern "C"

@@ -330,6 +330,79 @@ Tensor mla_output(const Tensor& q, const Tensor& freqs, const Tensor& kv, const 
     return fp8_gemm(y, ys, wo, wo_s, DSV3_BF16);
 }
 
+// The paged cache of a layer, as its operators take it: kv e4m3 [pages, page, rank], scale fp32 [pages, page], pe bf16 [pages, page, rope],
+// and the sequences' page numbers, int32 [batch, width]
+dsv3_mla_pages checked_pages(const char* what, const Tensor& kv, const Tensor& scale, const Tensor& pe, const Tensor& table, int64_t batch) {
+    TORCH_CHECK(kv.dim() == 3 && kv.scalar_type() == kFp8 && kv.is_contiguous() && kv.size(0) > 0, what, ": kv_pages must be a contiguous e4m3 [pages, page, rank] of one page at least");
+    TORCH_CHECK(scale.dim() == 2 && scale.scalar_type() == at::kFloat && scale.is_contiguous() && scale.size(0) == kv.size(0) && scale.size(1) == kv.size(1),
+                what, ": kv_scale must be a contiguous fp32 [pages, page]");
+    TORCH_CHECK(pe.dim() == 3 && pe.scalar_type() == at::kBFloat16 && pe.is_contiguous() && pe.size(0) == kv.size(0) && pe.size(1) == kv.size(1),
+                what, ": pe_pages must be a contiguous bf16 [pages, page, rope]");
+    TORCH_CHECK(kv.size(1) >= 8 && kv.size(1) <= 65536 && kv.size(1) % 8 == 0, what, ": a page must have a multiple of 8 positions, up to 65536, got ", kv.size(1));
+    TORCH_CHECK(kv.size(2) == 512 && pe.size(2) == 64, what, ": latents of 512 and rotary keys of 64 are implemented, got ", kv.size(2), " and ", pe.size(2));
+    TORCH_CHECK(table.dim() == 2 && table.scalar_type() == at::kInt && table.is_contiguous() && table.size(0) == batch && table.size(1) > 0,
+                what, ": page_table must be a contiguous int32 [batch, width]");
+    return { kv.data_ptr(), (float*)scale.data_ptr(), pe.data_ptr(), kv.size(0), (int)kv.size(1), (const int32_t*)table.data_ptr(), table.size(1) };
+}
+const int32_t* checked_ints(const char* what, const char* name, const Tensor& t, int64_t batch) {
+    TORCH_CHECK(t.dim() == 1 && t.scalar_type() == at::kInt && t.is_contiguous() && t.size(0) == batch, what, ": ", name, " must be a contiguous int32 [batch]");
+    return (const int32_t*)t.data_ptr();
+}
+void check_row_freqs(const char* what, const Tensor& f, int64_t batch, int64_t rows, int64_t rope) {
+    TORCH_CHECK(f.scalar_type() == at::kComplexFloat && f.is_contiguous() && f.dim() == 3 && f.size(0) == batch && f.size(1) == rows &&
+                f.size(2) == rope / 2 && !f.is_conj() && !f.is_neg(), what, ": freqs must be a contiguous complex64 [batch, rows, rope / 2], not lazily conjugated");
+}
+
+// a [b, s, q_rank + 512 + 64] -> the normalised query latent, quantised, and the sequences' cache rows behind `starts`
+tuple<Tensor, Tensor> mla_latent_paged(const Tensor& a, const OptTensor& qn, const Tensor& kn, const Tensor& freqs, Tensor kv, Tensor scale, Tensor pe,
+                                       const Tensor& table, const Tensor& starts, const Tensor& counts, double q_eps, double kv_eps) {
+    const char* what = "mla_latent_paged";
+    TORCH_CHECK(a.dim() == 3 && a.is_contiguous() && a.scalar_type() == at::kBFloat16, what, ": a must be a contiguous bf16 [b, s, width]");
+    const int64_t b = a.size(0), s = a.size(1), qr = qn ? qn->numel() : 0;
+    const auto cache = checked_pages(what, kv, scale, pe, table, b);
+    const int32_t* at_start = checked_ints(what, "starts", starts, b);
+    const int32_t* count = checked_ints(what, "counts", counts, b);
+    check_row_freqs(what, freqs, b, s, pe.size(2));
+    TORCH_CHECK(kn.numel() == kv.size(2) && kn.scalar_type() == at::kBFloat16 && kn.is_contiguous() &&
+                (!qn || (qn->scalar_type() == at::kBFloat16 && qn->is_contiguous() && qr > 0)) && a.size(2) == qr + kv.size(2) + pe.size(2),
+                what, ": norm weights do not fit the row");
+    on_one_gpu(what, a, { qn ? &*qn : &a, &kn, &freqs, &kv, &scale, &pe, &table, &starts, &counts });
+    Tensor y = at::empty({b, s, qr}, a.options().dtype(kFp8)), ys = at::empty({b, s, qr / 128}, a.options().dtype(at::kFloat));
+    On on(a);
+    check(dsv3_mla_latent_paged(a.data_ptr(), a.size(2), qn ? qn->data_ptr() : nullptr, kn.data_ptr(), (const float*)freqs.data_ptr(), &cache, at_start,
+                                count, y.data_ptr(), (float*)ys.data_ptr(), b, s, qr, kv.size(2), (int)pe.size(2), (float)q_eps, (float)kv_eps,
+                                on.stream), "dsv3_mla_latent_paged");
+    return {y, ys};
+}
+
+// the first `positions` cache rows of every sequence as bf16 [b, positions, 512] and [.., 64], zeros from its length on
+tuple<Tensor, Tensor> mla_cache_read(const Tensor& kv, const Tensor& scale, const Tensor& pe, const Tensor& table, const Tensor& lengths, int64_t positions) {
+    const char* what = "mla_cache_read";
+    const int64_t b = table.dim() ? table.size(0) : 0;
+    const auto cache = checked_pages(what, kv, scale, pe, table, b);
+    const int32_t* length = checked_ints(what, "lengths", lengths, b);
+    TORCH_CHECK(positions >= 0 && positions <= 0x7fffff, what, ": positions must be 0 to ", 0x7fffff, ", got ", positions);
+    on_one_gpu(what, kv, { &scale, &pe, &table, &lengths });
+    Tensor out = at::empty({b, positions, kv.size(2)}, pe.options()), out_pe = at::empty({b, positions, pe.size(2)}, pe.options());
+    On on(kv);
+    check(dsv3_mla_cache_read(&cache, length, out.data_ptr(), out_pe.data_ptr(), b, positions, on.stream), "dsv3_mla_cache_read");
+    return {out, out_pe};
+}
+
+// cache rows starts + path[k] of every sequence to starts + k, k < kept
+void mla_cache_keep(Tensor kv, Tensor scale, Tensor pe, const Tensor& table, const Tensor& starts, const Tensor& path, const Tensor& kept) {
+    const char* what = "mla_cache_keep";
+    const int64_t b = table.dim() ? table.size(0) : 0;
+    const auto cache = checked_pages(what, kv, scale, pe, table, b);
+    const int32_t* start = checked_ints(what, "starts", starts, b);
+    const int32_t* n = checked_ints(what, "kept", kept, b);
+    TORCH_CHECK(path.dim() == 2 && path.scalar_type() == at::kInt && path.is_contiguous() && path.size(0) == b && path.size(1) <= 64,
+                what, ": path must be a contiguous int32 [batch, up to 64]");
+    on_one_gpu(what, kv, { &scale, &pe, &table, &starts, &path, &kept });
+    On on(kv);
+    check(dsv3_mla_cache_keep(&cache, start, (const int32_t*)path.data_ptr(), n, b, (int)path.size(1), on.stream), "dsv3_mla_cache_keep");
+}
+
 }  // namespace
 
 TORCH_LIBRARY_IMPL(dsv3fp8, CUDA, m) {
@@ -346,4 +419,7 @@ TORCH_LIBRARY_IMPL(dsv3fp8, CUDA, m) {
     m.impl("mla_latent", mla_latent);
     m.impl("mla_query", mla_query);
     m.impl("mla_output", mla_output);
+    m.impl("mla_latent_paged", mla_latent_paged);
+    m.impl("mla_cache_read", mla_cache_read);
+    m.impl("mla_cache_keep", mla_cache_keep);
 }

@@ -19,6 +19,14 @@ ABSORB_Q, ABSORB_V = 0, 1
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 OK = 0
 
+
+class MlaPages(ctypes.Structure):
+    """dsv3_mla_pages (include/dsv3_fp8.h)."""
+    _fields_ = [("kv", c_void_p), ("kv_scale", c_void_p), ("pe", c_void_p), ("pages", c_int64), ("page_size", c_int),
+                ("table", c_void_p), ("table_width", c_int64)]
+
+
+_pages_p = ctypes.POINTER(MlaPages)
 EXPORTS = {
     "dsv3_version": (c_int, []),
     "dsv3_status_string": (c_char_p, [c_int]),
@@ -73,6 +81,10 @@ EXPORTS = {
     "dsv3_mla_latent_gemm": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
                                      c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,
                                      c_int, c_float, c_float, c_void_p, c_size_t, c_void_p]),
+    "dsv3_mla_latent_paged": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, _pages_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                      c_int64, c_int64, c_int64, c_int64, c_int, c_float, c_float, c_void_p]),
+    "dsv3_mla_cache_read": (c_int, [_pages_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p]),
+    "dsv3_mla_cache_keep": (c_int, [_pages_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p]),
 }
 
 

@@ -2,7 +2,8 @@
 
 ``torch.ops.dsv3fp8.{act_quant, weight_dequant, weight_quant, fp8_gemm}`` and the grouped
 mixture-of-experts ops ``{gate_route, group_tiles, moe_route, fp8_gemm_grouped, swiglu_quant, moe_combine}`` and the
-attention ops ``{wkv_b_absorb, mla_latent, mla_decode, mla_decode_quant, mla_prefill, mla_query, mla_output}`` take and return torch tensors; the device
+attention ops ``{wkv_b_absorb, mla_latent, mla_decode, mla_decode_quant, mla_prefill, mla_query, mla_output}`` and the
+ones on a cache in pages ``{mla_latent_paged, mla_cache_read, mla_cache_keep}`` take and return torch tensors; the device
 implementations (native in libdsv3torch.so, the mixture-of-experts ones and ``wkv_b_absorb`` below) hand raw device pointers
 and the current HIP stream of the tensors' device to libdsv3fp8.so.  Only a device
 ("CUDA" dispatch key, which is HIP on ROCm) implementation and a shape-only Meta
@@ -49,6 +50,11 @@ _libdef.define("mla_query(Tensor x, Tensor wa, Tensor wa_scale, Tensor q_norm, T
                "Tensor(b!) pe_cache, int start, float q_eps, float kv_eps, Tensor wq_b, Tensor wq_b_scale, int heads) -> Tensor")
 _libdef.define("mla_output(Tensor q, Tensor freqs, Tensor kv_cache, Tensor pe_cache, Tensor wkv_b, Tensor scale, Tensor? mask, "
                "int positions, float softmax_scale, bool explicit, Tensor wo, Tensor wo_scale) -> Tensor")
+_libdef.define("mla_latent_paged(Tensor a, Tensor? q_norm, Tensor kv_norm, Tensor freqs, Tensor(a!) kv_pages, Tensor(b!) kv_scale, Tensor(c!) pe_pages, "
+               "Tensor page_table, Tensor starts, Tensor counts, float q_eps, float kv_eps) -> (Tensor, Tensor)")
+_libdef.define("mla_cache_read(Tensor kv_pages, Tensor kv_scale, Tensor pe_pages, Tensor page_table, Tensor lengths, int positions) -> (Tensor, Tensor)")
+_libdef.define("mla_cache_keep(Tensor(a!) kv_pages, Tensor(b!) kv_scale, Tensor(c!) pe_pages, Tensor page_table, Tensor starts, Tensor path, "
+               "Tensor kept) -> ()")
 _libdef.define("wkv_b_absorb(Tensor x, Tensor wkv_b, Tensor scale, int side, int nope_dim, int v_dim) -> Tensor")
 
 
@@ -300,6 +306,21 @@ def _mla_output_meta(q, freqs, kv_cache, pe_cache, wkv_b, scale, mask, positions
     return q.new_empty(q.size(0), q.size(1), wo.size(0))
 
 
+def _mla_latent_paged_meta(a, q_norm, kv_norm, freqs, kv_pages, kv_scale, pe_pages, page_table, starts, counts, q_eps, kv_eps):
+    b, s, _ = a.shape
+    rank = 0 if q_norm is None else q_norm.numel()
+    return a.new_empty(b, s, rank, dtype=FP8), a.new_empty(b, s, rank // 128, dtype=torch.float32)
+
+
+def _mla_cache_read_meta(kv_pages, kv_scale, pe_pages, page_table, lengths, positions):
+    b = page_table.size(0)
+    return pe_pages.new_empty(b, positions, kv_pages.size(2)), pe_pages.new_empty(b, positions, pe_pages.size(2))
+
+
+def _mla_cache_keep_meta(kv_pages, kv_scale, pe_pages, page_table, starts, path, kept):
+    return None
+
+
 _lib.require(_lib.TORCH_LIB_PATH)
 torch.ops.load_library(str(_lib.TORCH_LIB_PATH))       # the device implementations of csrc/torch_ops.cpp
 
@@ -314,6 +335,7 @@ for _name, _meta in (("act_quant", _act_quant_meta), ("weight_dequant", _weight_
                      ("linear_fp8", _linear_fp8_meta), ("swiglu_quant", _swiglu_quant_meta),
                      ("mla_prefill", _mla_prefill_meta), ("mla_decode", _mla_decode_meta), ("mla_decode_quant", _mla_prefill_meta), ("mla_latent", _mla_latent_meta),
                      ("mla_query", _mla_query_meta), ("mla_output", _mla_output_meta),
+                     ("mla_latent_paged", _mla_latent_paged_meta), ("mla_cache_read", _mla_cache_read_meta), ("mla_cache_keep", _mla_cache_keep_meta),
                      ("wkv_b_absorb", _wkv_b_absorb_meta), ("gate_route", _gate_route_meta),
                      ("group_tiles", _group_tiles_meta), ("moe_route", _moe_route_meta),
                      ("fp8_gemm_grouped", _fp8_gemm_grouped_meta), ("fp8_gemm_grouped_pow2", _fp8_gemm_grouped_meta),

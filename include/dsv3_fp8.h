@@ -400,6 +400,58 @@ int dsv3_mla_latent_gemm(const void* x, const float* x_s, const void* w, const f
                          int64_t pe_batch_stride, void* y, float* s, int64_t batch, int64_t rows, int64_t q_rank, int64_t kv_rank,
                          int rope_dim, float q_eps, float kv_eps, void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * ---- The latent cache of the attention layer in pages, in eight bits ----
+ *
+ * The reference keeps one dense bf16 cache per layer with a place for every position of every sequence (inference/model.py:443-444).
+ * Here sequences share pages of page_size positions (a multiple of 8, up to 65536): row j of a sequence is row
+ * table[b][j / page_size] * page_size + j % page_size of three arrays,
+ *     kv       e4m3 [pages, page_size, 512]     the latent's codes (16-byte aligned)
+ *     kv_scale binary32 [pages, page_size]      a power of two: latent = code * scale, a bf16 number (4-byte aligned)
+ *     pe       bf16 [pages, page_size, 64]      the rotated key (16-byte aligned)
+ * An entry of the table outside [0, pages) names no page: rows there are not written, are read as zeros and seen by no query.
+ * The struct lies in host memory and is read during the call; everything it points to is device memory.  Rows that the functions read
+ * are those that they have written, or zeros: codes that are NaN by themselves are none of these.
+ * `starts` and `counts` (int32 [batch], device): positions of a sequence in front of this step and its new rows, which take the positions
+ * behind them; of `rows` rows per sequence those from counts[b] on belong to nobody.  A negative count is 0, one above `rows` is `rows`.
+ */
+typedef struct dsv3_mla_pages {
+    void* kv;
+    float* kv_scale;
+    void* pe;
+    int64_t pages;
+    int page_size;
+    const int32_t* table;       /* int32 [batch, table_width] */
+    int64_t table_width;
+} dsv3_mla_pages;
+
+/*
+ * dsv3_mla_latent whose cache rows go into pages (inference/model.py:457-466, :480-483), for rows a[i] = [ query latent (q_rank) | latent (512) | rotary key (64) ]:
+ *     n = bf16( rms_norm(latent) * kv_norm ),  scale = 2^ceil(log2( max(amax n, 1e-4) / 448 )),  kv = e4m3( n / scale ),  pe = bf16( rotated key )
+ * at row starts[b] + i of sequence b, i < counts[b]; y, s as dsv3_mla_latent.  The norms' sums are binary64 here.  A latent that holds a
+ * NaN or an infinity is stored as zeros with a scale of NaN.  q_rank 0: no query latent (q_norm, y and s are not looked at).
+ * freqs: binary32 (cos, sin) pairs [batch, rows, 32], each row's own.  A negative start: none of the sequence's rows is written.
+ * Two rows that the table sends to one place leave either's values there, or parts of both.
+ */
+int dsv3_mla_latent_paged(const void* a, int64_t a_stride, const void* q_norm, const void* kv_norm, const float* freqs,
+                          const dsv3_mla_pages* cache, const int32_t* starts, const int32_t* counts, void* y, float* s, int64_t batch,
+                          int64_t rows, int64_t q_rank, int64_t kv_rank, int rope_dim, float q_eps, float kv_eps, void* stream);
+
+/*
+ * The first `positions` rows of every sequence as dense bf16 arrays, kv [batch, positions, 512] and pe [batch, positions, 64]: what
+ * dsv3_mla_prefill takes as caches.  Rows from lengths[b] (int32 [batch], device) on are zeros.
+ */
+int dsv3_mla_cache_read(const dsv3_mla_pages* cache, const int32_t* lengths, void* kv, void* pe, int64_t batch, int64_t positions,
+                        void* stream);
+
+/*
+ * Rows of a drafted tree that were accepted, moved to the front of this step's: row starts[b] + k becomes what row
+ * starts[b] + path[b, k] was, k < kept[b] (path: int32 [batch, most], most <= 64; kept: int32 [batch]).  All rows are read before any
+ * is written: a path may name them in any order.  Entries below 0 or in no page leave their row as it is.
+ */
+int dsv3_mla_cache_keep(const dsv3_mla_pages* cache, const int32_t* starts, const int32_t* path, const int32_t* kept, int64_t batch,
+                        int most, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

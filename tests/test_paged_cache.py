@@ -1,0 +1,170 @@
+"""The latent cache in pages, on the host: where a position lies, and what its functions refuse (no kernel runs)."""
+import ctypes
+import subprocess
+from pathlib import Path
+
+import pytest
+import torch
+
+from test_abi import A16, _gpu_body
+
+CSRC = Path(__file__).resolve().parent.parent / "deepseek-v3_amd" / "csrc"
+FP8 = torch.float8_e4m3fn
+
+
+@pytest.fixture(scope="module")
+def L():
+    from dsv3fp8 import _lib
+    return _lib
+
+
+@pytest.fixture(scope="module")
+def walk(tmp_path_factory):
+    """csrc/paged.hpp, which the kernels use, compiled for the host."""
+    at = tmp_path_factory.mktemp("paged")
+    (at / "walk.cpp").write_text('#include "paged.hpp"\n'
+                                 'extern "C" int64_t row(const int32_t* e, int64_t w, int64_t n, int p, int64_t at) { return dsv3::page_row(e, w, n, p, at); }\n'
+                                 'extern "C" void span(int s, int c, int r, int m, int* o) { auto x = dsv3::seq_span(s, c, r, m); o[0] = x.start; o[1] = x.end; o[2] = x.count; }\n')
+    subprocess.run(["g++", "-O1", "-shared", "-fPIC", "-fsanitize=undefined", "-fno-sanitize-recover", f"-I{CSRC}", str(at / "walk.cpp"), "-o", str(at / "walk.so")], check=True)
+    lib = ctypes.CDLL(str(at / "walk.so"))
+    lib.row.restype = ctypes.c_int64
+    lib.row.argtypes = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_int64]
+    lib.span.argtypes = [ctypes.c_int] * 4 + [ctypes.c_void_p]
+    return lib
+
+
+@pytest.mark.parametrize("page", [8, 24, 64, 65536])
+def test_row_of_a_position(walk, page):
+    pages = 2 ** 31 // page                                  # rows past 2^31, bytes past 2^40
+    table = torch.tensor([3, pages - 1, -1, pages, 2 ** 31 - 1, -2 ** 31, 0], dtype=torch.int32)
+    for pos in [0, 1, page - 1, page, page + 7, 2 * page - 1, 2 * page, 3 * page + 5, 4 * page, 5 * page + 1, 6 * page, 7 * page - 1]:
+        e = int(table[pos // page])
+        want = e * page + pos % page if 0 <= e < pages else -1
+        assert walk.row(table.data_ptr(), 7, pages, page, pos) == want
+    for pos in [-1, -2 ** 31, 7 * page, 2 ** 31 - 1 + 64, 2 ** 40]:         # in front of the sequence, behind its table
+        assert walk.row(table.data_ptr(), 7, pages, page, pos) == -1
+
+
+def test_span_of_a_sequence(walk):
+    o = (ctypes.c_int * 3)()
+    for (start, count, rows, most), want in {(5, 3, 4, 100): (5, 8, 3), (-4, 3, 4, 100): (0, 3, 3), (5, -1, 4, 100): (5, 5, 0), (5, 9, 4, 100): (5, 9, 4),
+                                             (98, 4, 4, 100): (98, 100, 4), (2 ** 31 - 1, 4, 4, 100): (100, 100, 4), (0, 0, 4, 100): (0, 0, 0),
+                                             (-2 ** 31, -2 ** 31, 64, 8388607): (0, 0, 0)}.items():
+        walk.span(start, count, rows, most, o)
+        assert tuple(o) == want
+
+
+def _cache(L, **change):
+    c = dict(kv=A16, kv_scale=A16, pe=A16, pages=4, page_size=64, table=A16, table_width=2) | change
+    return ctypes.byref(L.MlaPages(*c.values()))
+
+
+BAD_PAGES = [({"kv": None}, 1), ({"kv_scale": None}, 1), ({"pe": None}, 1), ({"table": None}, 1), ({"pages": 0}, 2), ({"pages": 2 ** 31}, 2),
+             ({"page_size": 0}, 2), ({"page_size": 12}, 2), ({"page_size": 4}, 2), ({"page_size": 65544}, 2), ({"table_width": 0}, 2),
+             ({"table_width": 2 ** 31}, 2), ({"kv": A16 + 8}, 4), ({"pe": A16 + 8}, 4), ({"kv_scale": A16 + 2}, 4), ({"table": A16 + 2}, 4)]
+
+
+def test_latent_paged_validation(L):
+    def call(a=A16, stride=2112, qw=A16, kw=A16, f=A16, cache=_cache(L), st=A16, n=A16, y=A16, s=A16, b=2, rows=3, qr=1536, c=512, rope=64):
+        return L.lib.dsv3_mla_latent_paged(a, stride, qw, kw, f, cache, st, n, y, s, b, rows, qr, c, rope, 1e-6, 1e-6, None)
+    for change, code in BAD_PAGES:
+        assert call(cache=_cache(L, **change)) == code
+    assert call(cache=None) == 1
+    for name in ("a", "qw", "kw", "f", "st", "n", "y", "s"):
+        assert call(**{name: None}) == 1 and call(**{name: A16 + 2}) == 4
+    for bad in (dict(stride=2104), dict(stride=2113), dict(b=-1), dict(b=65536), dict(rows=-1), dict(rows=1 << 23), dict(b=65535, rows=1 << 16), dict(qr=-128),
+                dict(qr=64), dict(qr=2176), dict(c=256), dict(rope=32)):
+        assert call(**bad) == 2
+    assert call(b=0, a=None) == 0 and call(rows=0, a=None) == 0
+    assert call(qr=0, qw=None, y=None, s=None, a=None) == 1          # no query latent: its pointers are not looked at
+
+
+def test_cache_read_validation(L):
+    def call(cache=_cache(L), n=A16, kv=A16, pe=A16, b=2, t=100):
+        return L.lib.dsv3_mla_cache_read(cache, n, kv, pe, b, t, None)
+    for change, code in BAD_PAGES:
+        assert call(cache=_cache(L, **change)) == code
+    for name in ("n", "kv", "pe"):
+        assert call(**{name: None}) == 1 and call(**{name: A16 + 2}) == 4
+    for bad in (dict(b=-1), dict(b=65536), dict(t=-1), dict(t=1 << 23)):
+        assert call(**bad) == 2
+    assert call(b=0, n=None) == 0 and call(t=0, n=None) == 0
+
+
+def test_cache_keep_validation(L):
+    def call(cache=_cache(L), st=A16, path=A16, kept=A16, b=2, most=5):
+        return L.lib.dsv3_mla_cache_keep(cache, st, path, kept, b, most, None)
+    for change, code in BAD_PAGES:
+        assert call(cache=_cache(L, **change)) == code
+    for name in ("st", "path", "kept"):
+        assert call(**{name: None}) == 1 and call(**{name: A16 + 2}) == 4
+    for bad in (dict(b=-1), dict(b=65536), dict(most=-1), dict(most=65)):
+        assert call(**bad) == 2
+    assert call(b=0, st=None) == 0 and call(most=0, st=None) == 0
+
+
+def _args(name):
+    z = torch.zeros
+    i32 = dict(dtype=torch.int32)
+    cache = [z(4, 16, 512, dtype=FP8), z(4, 16), z(4, 16, 64, dtype=torch.bfloat16), z(2, 3, **i32)]
+    if name == "mla_latent_paged":
+        return [z(2, 3, 128 + 576, dtype=torch.bfloat16), z(128, dtype=torch.bfloat16), z(512, dtype=torch.bfloat16), z(2, 3, 32, dtype=torch.complex64), *cache,
+                z(2, **i32), z(2, **i32), 1e-6, 1e-6]
+    if name == "mla_cache_read":
+        return [*cache, z(2, **i32), 20]
+    if name == "mla_cache_keep":
+        return [*cache, z(2, **i32), z(2, 5, **i32), z(2, **i32)]
+    return [z(2, 3, 4, 192, dtype=torch.bfloat16), z(2, 3, 32, dtype=torch.complex64), *cache, z(2, **i32), z(2, **i32), z(2, 3, dtype=torch.int64),
+            z(1024, 512, dtype=FP8), z(8, 4), 20, 0.1]
+
+
+# where the cache stands, and the int32 [batch] behind it
+OPERATORS = {"mla_latent_paged": (4, (8, 9)), "mla_cache_read": (0, (4,)), "mla_cache_keep": (0, (4, 6))}
+
+
+@pytest.mark.parametrize("name", OPERATORS)
+def test_operators_refuse_tensors_of_two_devices(name):
+    with pytest.raises(RuntimeError, match="on the GPU"):
+        _gpu_body(name, *_args(name))
+    for at, t in enumerate(_args(name)):
+        if isinstance(t, torch.Tensor):
+            args = _args(name)
+            args[at] = t.to("meta")
+            with pytest.raises(RuntimeError, match="one device"):
+                _gpu_body(name, *args)
+
+
+@pytest.mark.parametrize("name", OPERATORS)
+def test_operators_refuse_what_their_kernels_cannot_read(name):
+    at, ints = OPERATORS[name]
+    z = torch.zeros
+    bad = {at: [lambda t: t.bfloat16(), lambda t: t[:0], lambda t: z(4, 12, 512, dtype=FP8), lambda t: z(4, 16, 256, dtype=FP8), lambda t: t[0],
+                lambda t: z(4, 32, 512, dtype=FP8)[:, ::2]],
+           at + 1: [lambda t: t.bfloat16(), lambda t: t[:3], lambda t: t[:, :8].contiguous(), lambda t: t.flatten(), lambda t: z(16, 4).t()],
+           at + 2: [lambda t: t.float(), lambda t: t[:3], lambda t: z(4, 16, 32, dtype=t.dtype), lambda t: t[:, :8].contiguous(), lambda t: z(4, 16, 128, dtype=t.dtype)[..., ::2]],
+           at + 3: [lambda t: t.long(), lambda t: t[:1], lambda t: t[:, :0], lambda t: z(2, 6, dtype=t.dtype)[:, ::2], lambda t: t[0]]}
+    for i in ints:
+        bad[i] = [lambda t: t.long(), lambda t: t[:1], lambda t: z(4, dtype=t.dtype)[::2], lambda t: t[:, None]]
+    if name == "mla_latent_paged":
+        bad[0] = [lambda t: t.float(), lambda t: t[..., :-1].contiguous(), lambda t: t[0], lambda t: z(2, 6, 704, dtype=t.dtype)[:, ::2]]
+        bad[1] = [lambda t: t.float(), lambda t: t[:64], lambda t: z(256, dtype=t.dtype)[::2], lambda t: None, lambda t: t[:0]]
+        bad[2] = [lambda t: t.float(), lambda t: t[:511]]
+        bad[3] = [lambda t: t.conj(), lambda t: t[:1], lambda t: t[:, :2].contiguous(), lambda t: t[0], lambda t: t[..., :16].contiguous()]
+    if name == "mla_cache_read":
+        bad[5] = [lambda t: -1, lambda t: 1 << 23]
+    if name == "mla_cache_keep":
+        bad[5] = [lambda t: t.long(), lambda t: t[:1], lambda t: z(2, 65, dtype=t.dtype), lambda t: t[0], lambda t: z(2, 10, dtype=t.dtype)[:, ::2]]
+    for i, changes in bad.items():
+        for change in changes:
+            args = _args(name)
+            args[i] = change(args[i])
+            with pytest.raises(RuntimeError, match=name + r"[^:]*: (?!tensors|all tensors)"):
+                _gpu_body(name, *args)
+
+
+@pytest.mark.parametrize("name", OPERATORS)
+def test_shapes_without_a_device(name):
+    args = [t.to("meta") if isinstance(t, torch.Tensor) else t for t in _args(name)]
+    got = getattr(torch.ops.dsv3fp8, name)(*args)
+    shapes = {"mla_latent_paged": [(2, 3, 128), (2, 3, 1)], "mla_cache_read": [(2, 20, 512), (2, 20, 64)], "mla_cache_keep": []}[name]
+    assert [tuple(t.shape) for t in got or ()] == shapes
