@@ -38,7 +38,8 @@ HIPCC_FLAGS = [
 # or spills; exceptions are listed with their reasons.
 # The attention kernels keep their sums in registers for a whole loop and have none to spare (mla_decode_kernel: 32 x 512
 # sums in the 256 accumulation registers; an ordinary rescale of them spilled 300): a spill there is a copy per tile.
-NO_SPILL_SOURCES = {"fp8_gemm_skinny.hip", "fp8_gemm_stream.hip", "fp8_gemm_mid.hip", "mla_decode.hip", "mla_prefill.hip"}
+NO_SPILL_SOURCES = {"fp8_gemm_skinny.hip", "fp8_gemm_stream.hip", "fp8_gemm_mid.hip", "mla_decode.hip", "mla_prefill.hip",
+                    "mla_paged_decode.hip"}
 SGPR_SPILLS_ALLOWED = {
     # Scalars kept in lanes of a vector register are no scratch memory and cost nothing outside the tile loop: the limit for them.  (This build
     # reports none.)  The kernel takes all 256 vector registers, so a spilled one of these would be a copy per tile: refused.

@@ -519,4 +519,45 @@ int dsv3_mla_cache_keep(const dsv3_mla_pages* cache, const int32_t* starts, cons
     return launch_mla_cache_keep(*cache, starts, path, kept, batch, most, (hipStream_t)stream);
 }
 
+size_t dsv3_mla_decode_paged_workspace_bytes(int64_t batch, int64_t rows, int heads) {
+    if (batch <= 0 || batch > 65535 || rows <= 0 || rows > 64 || heads <= 0 || heads > 65535) return 0;
+    return mla_decode_paged_workspace_bytes(batch, rows, heads);
+}
+
+static int mla_decode_paged_checked(const void* q, const float* freqs, const dsv3_mla_pages* cache, const int32_t* starts, const int32_t* counts,
+                                    const int64_t* tree, const void* wkv_b, const float* wkv_b_scale, void* y, float* s, bool quant, int64_t batch,
+                                    int64_t rows, int64_t positions, int heads, int nope_dim, int rope_dim, int v_dim, int64_t kv_rank,
+                                    float softmax_scale, void* workspace, size_t workspace_bytes, void* stream) {
+    const int rc = mla_pages_validate(cache, batch);
+    if (rc != DSV3_OK) return rc;
+    if (nope_dim != 128 || rope_dim != 64 || v_dim != 128 || kv_rank != 512 || rows < 0 || rows > 64 || heads < 0 || heads > 65535 ||
+        positions < 1 || positions > 0x7fffff || positions > cache->table_width * cache->page_size ||
+        batch * ((positions + 31) / 32) > 0x7fffffff || !(softmax_scale > 1e-30f && softmax_scale < 1e30f))
+        return DSV3_ERR_BAD_SHAPE;
+    if (batch == 0 || rows == 0 || heads == 0) return DSV3_OK;
+    if (!q || !freqs || !starts || !counts || !wkv_b || !wkv_b_scale || !y || (quant && !s)) return DSV3_ERR_NULL_POINTER;
+    if (!aligned(q, 16) || !aligned(freqs, 8) || !aligned(starts, 4) || !aligned(counts, 4) || !aligned(tree, 8) || !aligned(wkv_b, 16) ||
+        !aligned(wkv_b_scale, 4) || !aligned(y, 16) || !aligned(s, 4))
+        return DSV3_ERR_MISALIGNED;
+    if (!workspace || !aligned(workspace, 256) || workspace_bytes < mla_decode_paged_workspace_bytes(batch, rows, heads)) return DSV3_ERR_WORKSPACE;
+    return launch_mla_decode_paged(q, freqs, *cache, starts, counts, tree, wkv_b, wkv_b_scale, y, s, batch, rows, positions, heads, softmax_scale,
+                                   workspace, (hipStream_t)stream);
+}
+
+int dsv3_mla_decode_paged(const void* q, const float* freqs, const dsv3_mla_pages* cache, const int32_t* starts, const int32_t* counts,
+                          const int64_t* tree, const void* wkv_b, const float* wkv_b_scale, void* y, int64_t batch, int64_t rows,
+                          int64_t positions, int heads, int nope_dim, int rope_dim, int v_dim, int64_t kv_rank, float softmax_scale,
+                          void* workspace, size_t workspace_bytes, void* stream) {
+    return mla_decode_paged_checked(q, freqs, cache, starts, counts, tree, wkv_b, wkv_b_scale, y, nullptr, false, batch, rows, positions, heads,
+                                    nope_dim, rope_dim, v_dim, kv_rank, softmax_scale, workspace, workspace_bytes, stream);
+}
+
+int dsv3_mla_decode_paged_quant(const void* q, const float* freqs, const dsv3_mla_pages* cache, const int32_t* starts, const int32_t* counts,
+                                const int64_t* tree, const void* wkv_b, const float* wkv_b_scale, void* y, float* s, int64_t batch, int64_t rows,
+                                int64_t positions, int heads, int nope_dim, int rope_dim, int v_dim, int64_t kv_rank, float softmax_scale,
+                                void* workspace, size_t workspace_bytes, void* stream) {
+    return mla_decode_paged_checked(q, freqs, cache, starts, counts, tree, wkv_b, wkv_b_scale, y, s, true, batch, rows, positions, heads,
+                                    nope_dim, rope_dim, v_dim, kv_rank, softmax_scale, workspace, workspace_bytes, stream);
+}
+
 }  // extern "C"

@@ -226,6 +226,10 @@ int launch_mla_latent_paged(const void* a, int64_t a_stride, const void* q_w, co
                             const int32_t* starts, const int32_t* counts, void* y, float* ys, int64_t batch, int64_t rows, int q_rank,
                             float q_eps, float kv_eps, hipStream_t st);
 int launch_mla_cache_read(const dsv3_mla_pages& cache, const int32_t* lengths, void* kv, void* pe, int64_t batch, int64_t positions, hipStream_t st);
+size_t mla_decode_paged_workspace_bytes(int64_t batch, int64_t tokens, int heads);
+int launch_mla_decode_paged(const void* q, const void* freqs, const dsv3_mla_pages& cache, const int32_t* starts, const int32_t* counts,
+                            const int64_t* tree, const void* w, const float* ws, void* y, float* ys, int64_t batch, int64_t tokens,
+                            int64_t positions, int heads, float scale, void* workspace, hipStream_t st);
 int launch_mla_cache_keep(const dsv3_mla_pages& cache, const int32_t* starts, const int32_t* path, const int32_t* kept, int64_t batch, int most,
                           hipStream_t st);
 

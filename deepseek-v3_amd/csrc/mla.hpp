@@ -8,6 +8,7 @@ namespace {
 
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) void* lptr_t;
+typedef __attribute__((address_space(3))) v2i* lds_v2i;
 
 __device__ __forceinline__ v16f mfma32(v4u a, v4u b, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
@@ -18,7 +19,12 @@ __device__ __forceinline__ void copy16(const void* base, uint32_t lane_off, uint
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
                  :: "v"(lane_off), "s"(base), "s"(lds_addr) : "memory", "m0");
 }
-// The same through a buffer descriptor (the range check answers requests past its end with zeros), into LDS at lds_addr + IMM
+// 256 bytes global -> LDS: lane l's four at base + lane_off land at lds_addr + 4 l
+__device__ __forceinline__ void copy4(const void* base, uint32_t lane_off, uint32_t lds_addr) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1"
+                 :: "v"(lane_off), "s"(base), "s"(lds_addr) : "memory", "m0");
+}
+// copy16 through a buffer descriptor (the range check answers requests past its end with zeros), into LDS at lds_addr + IMM
 __device__ __forceinline__ v4i buffer_of(const void* base, int bytes) {
     const uintptr_t a = (uintptr_t)base;
     return v4i{ (int)(uint32_t)a, (int)((uint32_t)(a >> 32) & 0xffffu), bytes, 0x00027000 };
@@ -41,6 +47,33 @@ __device__ __forceinline__ v2f halves32(float v) {
     const v2u r = __builtin_amdgcn_permlane32_swap(f32_as_u32(v), f32_as_u32(v), false, false);
     return v2f{ u32_as_f32(r[0]), u32_as_f32(r[1]) };
 }
+
+// v *= a on accumulators that stay in the accumulation registers: as an ordinary product the compiler moves all 256 of them
+// to and fro and spills.  At least 36 MFMAs with other results lie between the last write of v and this (the S products).
+__device__ __forceinline__ void scale_agprs(v16f& v, float a) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        float x = v[e], y;
+        asm volatile("v_accvgpr_read_b32 %1, %0\n\tv_mul_f32 %1, %1, %2\n\tv_accvgpr_write_b32 %0, %1" : "+a"(x), "=&v"(y) : "v"(a));
+        v[e] = x;
+    }
+}
+
+// mfma32 with its result in ordinary registers: the compiler would put it into accumulation registers, which are all taken, and move 16 sums
+// out and back per tile.  It does not know that these are MFMAs, so what it would keep apart stands here: two wait states in front
+// (an ordinary instruction may have written an operand); behind the last one, before its result is read, scores_ready.
+__device__ __forceinline__ void mfma32_first(v16f& d, v4u a, v4u b) {
+    asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(d) : "v"(a), "v"(b));
+}
+__device__ __forceinline__ void mfma32_next(v16f& d, v4u a, v4u b) {
+    asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(d) : "v"(a), "v"(b));
+}
+__device__ __forceinline__ void scores_ready(v16f& d) { asm volatile("s_nop 15" : "+v"(d)); }
+
+// n / d by a multiplication: magic is 2^32 / d rounded up, exact as long as n d < 2^32, or 0 where that does not hold (a division in front of
+// everything else costs a quarter of a microsecond)
+__device__ __forceinline__ int quotient(int n, int d, uint32_t magic) { return d == 1 ? n : magic ? (int)__umulhi((uint32_t)n, magic) : n / d; }
+inline uint32_t magic_of(int64_t most, int64_t d) { return d > 1 && most * d < (1ll << 32) ? (uint32_t)(((1ll << 32) + d - 1) / d) : 0u; }
 
 template <bool F32> __device__ __forceinline__ float mask_at(const void* m, int64_t i) {
     return F32 ? ((const float*)m)[i] : u32_as_f32((uint32_t)((const uint16_t*)m)[i] << 16);

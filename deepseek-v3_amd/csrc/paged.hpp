@@ -21,13 +21,13 @@ DSV3_HD int64_t page_row(const int32_t* entries, int64_t width, int64_t pages, i
     return entry * page + (pos - k * page);
 }
 
-// The positions of a sequence that are in the cache in front of this step and behind it: what is negative counts as none,
-// and nothing lies behind `most`.
+// A sequence's part in a step of `rows` rows at most: positions in front of it and behind it, rows.  Nothing lies behind `most`; a negative
+// start or count leaves nothing.
 struct SeqSpan { int start, end, count; };
 DSV3_HD SeqSpan seq_span(int start, int count, int rows, int most) {
-    const int s = start < 0 ? 0 : start > most ? most : start;
-    const int n = count < 0 ? 0 : count > rows ? rows : count;
-    return SeqSpan{ s, s + n < most ? s + n : most, n };
+    if (start < 0 || count <= 0) return SeqSpan{ 0, 0, 0 };
+    const int s = start > most ? most : start, n = count > rows ? rows : count;
+    return SeqSpan{ s, n < most - s ? s + n : most, n };
 }
 
 }  // namespace dsv3

@@ -389,6 +389,66 @@ tuple<Tensor, Tensor> mla_cache_read(const Tensor& kv, const Tensor& scale, cons
     return {out, out_pe};
 }
 
+// What the two attention operators on a cache in pages check and pass on alike; `call` gets the cache and the workspace.
+template <class Call>
+void attention_paged(const char* what, const Tensor& q, const Tensor& freqs, const Tensor& kv, const Tensor& scale, const Tensor& pe, const Tensor& table,
+                     const Tensor& starts, const Tensor& counts, const OptTensor& tree, const Tensor& w, const Tensor& ws, int64_t positions,
+                     double softmax_scale, Call call) {
+    TORCH_CHECK(q.dim() == 4 && q.is_contiguous() && q.scalar_type() == at::kBFloat16, what, ": q must be a contiguous bf16 [b, s, h, d]");
+    const int64_t b = q.size(0), s = q.size(1), h = q.size(2);
+    const auto cache = checked_pages(what, kv, scale, pe, table, b);
+    checked_ints(what, "starts", starts, b);
+    checked_ints(what, "counts", counts, b);
+    check_row_freqs(what, freqs, b, s, pe.size(2));
+    TORCH_CHECK(s <= 64, what, ": up to 64 new tokens a sequence are implemented, got ", s);
+    TORCH_CHECK(q.size(3) == 128 + pe.size(2), what, ": q must have 128 elements and the rotary ones a head, got ", q.size(3));
+    TORCH_CHECK(w.dim() == 2 && w.is_contiguous() && w.scalar_type() == kFp8 && w.size(1) == kv.size(2) && w.size(0) == h * 256, what,
+                ": wkv_b must be a contiguous fp8 [h * (128 + 128), kv_rank]");
+    TORCH_CHECK(ws.scalar_type() == at::kFloat && ws.dim() == 2 && ws.is_contiguous() && ws.size(0) == h * 2 && ws.size(1) == kv.size(2) / 128, what,
+                ": wkv_b's scales must be fp32, one per block of 128 x 128");
+    if (tree)
+        TORCH_CHECK(tree->dim() == 2 && tree->scalar_type() == at::kLong && tree->is_contiguous() && tree->size(0) == b && tree->size(1) == s, what,
+                    ": tree must be a contiguous int64 [b, s]");
+    TORCH_CHECK(positions >= 1 && positions <= 0x7fffff && positions <= table.size(1) * kv.size(1), what, ": positions must be 1 to what page_table has room for, got ", positions);
+    TORCH_CHECK(softmax_scale > 1e-30 && softmax_scale < 1e30, what, ": softmax_scale must be between 1e-30 and 1e30, got ", softmax_scale);
+    on_one_gpu(what, q, { &freqs, &kv, &scale, &pe, &table, &starts, &counts, tree ? &*tree : &q, &w, &ws });
+    On on(q);
+    const size_t need = dsv3_mla_decode_paged_workspace_bytes(b, s, (int)h);
+    Tensor buf = scratch(q, need);
+    call(cache, b, s, (int)h, tree ? (const int64_t*)tree->data_ptr() : nullptr, buf.data_ptr(), need, on.stream);
+}
+
+// queries of one new token or a tree of them per sequence -> [b, s, h * 128]
+Tensor mla_decode_paged(const Tensor& q, const Tensor& freqs, const Tensor& kv, const Tensor& scale, const Tensor& pe, const Tensor& table,
+                        const Tensor& starts, const Tensor& counts, const OptTensor& tree, const Tensor& w, const Tensor& ws, int64_t positions,
+                        double softmax_scale) {
+    Tensor y;
+    attention_paged("mla_decode_paged", q, freqs, kv, scale, pe, table, starts, counts, tree, w, ws, positions, softmax_scale,
+                    [&](const dsv3_mla_pages& cache, int64_t b, int64_t s, int h, const int64_t* bits, void* buf, size_t need, void* stream) {
+        y = at::empty({b, s, (int64_t)h * 128}, q.options());
+        check(dsv3_mla_decode_paged(q.data_ptr(), (const float*)freqs.data_ptr(), &cache, (const int32_t*)starts.data_ptr(), (const int32_t*)counts.data_ptr(),
+                                    bits, w.data_ptr(), (const float*)ws.data_ptr(), y.data_ptr(), b, s, positions, h, 128, 64, 128, 512,
+                                    (float)softmax_scale, buf, need, stream), "dsv3_mla_decode_paged");
+    });
+    return y;
+}
+// the same, rounded to bf16 and quantised per (token, head): the output projection's input
+tuple<Tensor, Tensor> mla_decode_paged_quant(const Tensor& q, const Tensor& freqs, const Tensor& kv, const Tensor& scale, const Tensor& pe,
+                                             const Tensor& table, const Tensor& starts, const Tensor& counts, const OptTensor& tree, const Tensor& w,
+                                             const Tensor& ws, int64_t positions, double softmax_scale) {
+    Tensor y, ys;
+    attention_paged("mla_decode_paged_quant", q, freqs, kv, scale, pe, table, starts, counts, tree, w, ws, positions, softmax_scale,
+                    [&](const dsv3_mla_pages& cache, int64_t b, int64_t s, int h, const int64_t* bits, void* buf, size_t need, void* stream) {
+        y = at::empty({b, s, (int64_t)h * 128}, q.options().dtype(kFp8));
+        ys = at::empty({b, s, h}, q.options().dtype(at::kFloat));
+        check(dsv3_mla_decode_paged_quant(q.data_ptr(), (const float*)freqs.data_ptr(), &cache, (const int32_t*)starts.data_ptr(),
+                                          (const int32_t*)counts.data_ptr(), bits, w.data_ptr(), (const float*)ws.data_ptr(), y.data_ptr(),
+                                          (float*)ys.data_ptr(), b, s, positions, h, 128, 64, 128, 512, (float)softmax_scale, buf, need, stream),
+              "dsv3_mla_decode_paged_quant");
+    });
+    return {y, ys};
+}
+
 // cache rows starts + path[k] of every sequence to starts + k, k < kept
 void mla_cache_keep(Tensor kv, Tensor scale, Tensor pe, const Tensor& table, const Tensor& starts, const Tensor& path, const Tensor& kept) {
     const char* what = "mla_cache_keep";
@@ -421,5 +481,7 @@ TORCH_LIBRARY_IMPL(dsv3fp8, CUDA, m) {
     m.impl("mla_output", mla_output);
     m.impl("mla_latent_paged", mla_latent_paged);
     m.impl("mla_cache_read", mla_cache_read);
+    m.impl("mla_decode_paged", mla_decode_paged);
+    m.impl("mla_decode_paged_quant", mla_decode_paged_quant);
     m.impl("mla_cache_keep", mla_cache_keep);
 }

@@ -84,6 +84,11 @@ EXPORTS = {
     "dsv3_mla_latent_paged": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, _pages_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                       c_int64, c_int64, c_int64, c_int64, c_int, c_float, c_float, c_void_p]),
     "dsv3_mla_cache_read": (c_int, [_pages_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p]),
+    "dsv3_mla_decode_paged_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int]),
+    "dsv3_mla_decode_paged": (c_int, [c_void_p, c_void_p, _pages_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                      c_int64, c_int64, c_int64, c_int, c_int, c_int, c_int, c_int64, c_float, c_void_p, c_size_t, c_void_p]),
+    "dsv3_mla_decode_paged_quant": (c_int, [c_void_p, c_void_p, _pages_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                            c_int64, c_int64, c_int64, c_int, c_int, c_int, c_int, c_int64, c_float, c_void_p, c_size_t, c_void_p]),
     "dsv3_mla_cache_keep": (c_int, [_pages_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p]),
 }
 

@@ -3,7 +3,8 @@
 ``torch.ops.dsv3fp8.{act_quant, weight_dequant, weight_quant, fp8_gemm}`` and the grouped
 mixture-of-experts ops ``{gate_route, group_tiles, moe_route, fp8_gemm_grouped, swiglu_quant, moe_combine}`` and the
 attention ops ``{wkv_b_absorb, mla_latent, mla_decode, mla_decode_quant, mla_prefill, mla_query, mla_output}`` and the
-ones on a cache in pages ``{mla_latent_paged, mla_cache_read, mla_cache_keep}`` take and return torch tensors; the device
+ones on a cache in pages ``{mla_latent_paged, mla_decode_paged, mla_decode_paged_quant, mla_cache_read,
+mla_cache_keep}`` take and return torch tensors; the device
 implementations (native in libdsv3torch.so, the mixture-of-experts ones and ``wkv_b_absorb`` below) hand raw device pointers
 and the current HIP stream of the tensors' device to libdsv3fp8.so.  Only a device
 ("CUDA" dispatch key, which is HIP on ROCm) implementation and a shape-only Meta
@@ -53,6 +54,9 @@ _libdef.define("mla_output(Tensor q, Tensor freqs, Tensor kv_cache, Tensor pe_ca
 _libdef.define("mla_latent_paged(Tensor a, Tensor? q_norm, Tensor kv_norm, Tensor freqs, Tensor(a!) kv_pages, Tensor(b!) kv_scale, Tensor(c!) pe_pages, "
                "Tensor page_table, Tensor starts, Tensor counts, float q_eps, float kv_eps) -> (Tensor, Tensor)")
 _libdef.define("mla_cache_read(Tensor kv_pages, Tensor kv_scale, Tensor pe_pages, Tensor page_table, Tensor lengths, int positions) -> (Tensor, Tensor)")
+for _name, _result in (("mla_decode_paged", "Tensor"), ("mla_decode_paged_quant", "(Tensor, Tensor)")):
+    _libdef.define(f"{_name}(Tensor q, Tensor freqs, Tensor kv_pages, Tensor kv_scale, Tensor pe_pages, Tensor page_table, Tensor starts, Tensor counts, "
+                   f"Tensor? tree, Tensor wkv_b, Tensor scale, int positions, float softmax_scale) -> {_result}")
 _libdef.define("mla_cache_keep(Tensor(a!) kv_pages, Tensor(b!) kv_scale, Tensor(c!) pe_pages, Tensor page_table, Tensor starts, Tensor path, "
                "Tensor kept) -> ()")
 _libdef.define("wkv_b_absorb(Tensor x, Tensor wkv_b, Tensor scale, int side, int nope_dim, int v_dim) -> Tensor")
@@ -317,6 +321,14 @@ def _mla_cache_read_meta(kv_pages, kv_scale, pe_pages, page_table, lengths, posi
     return pe_pages.new_empty(b, positions, kv_pages.size(2)), pe_pages.new_empty(b, positions, pe_pages.size(2))
 
 
+def _mla_decode_paged_meta(q, freqs, kv_pages, kv_scale, pe_pages, page_table, starts, counts, tree, wkv_b, scale, positions, softmax_scale):
+    return q.new_empty(q.size(0), q.size(1), q.size(2) * 128)
+
+
+def _mla_decode_paged_quant_meta(q, freqs, kv_pages, kv_scale, pe_pages, page_table, starts, counts, tree, wkv_b, scale, positions, softmax_scale):
+    return q.new_empty(q.size(0), q.size(1), q.size(2) * 128, dtype=FP8), q.new_empty(*q.shape[:3], dtype=torch.float32)
+
+
 def _mla_cache_keep_meta(kv_pages, kv_scale, pe_pages, page_table, starts, path, kept):
     return None
 
@@ -336,6 +348,7 @@ for _name, _meta in (("act_quant", _act_quant_meta), ("weight_dequant", _weight_
                      ("mla_prefill", _mla_prefill_meta), ("mla_decode", _mla_decode_meta), ("mla_decode_quant", _mla_prefill_meta), ("mla_latent", _mla_latent_meta),
                      ("mla_query", _mla_query_meta), ("mla_output", _mla_output_meta),
                      ("mla_latent_paged", _mla_latent_paged_meta), ("mla_cache_read", _mla_cache_read_meta), ("mla_cache_keep", _mla_cache_keep_meta),
+                     ("mla_decode_paged", _mla_decode_paged_meta), ("mla_decode_paged_quant", _mla_decode_paged_quant_meta),
                      ("wkv_b_absorb", _wkv_b_absorb_meta), ("gate_route", _gate_route_meta),
                      ("group_tiles", _group_tiles_meta), ("moe_route", _moe_route_meta),
                      ("fp8_gemm_grouped", _fp8_gemm_grouped_meta), ("fp8_gemm_grouped_pow2", _fp8_gemm_grouped_meta),

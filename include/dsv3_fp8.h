@@ -445,6 +445,29 @@ int dsv3_mla_cache_read(const dsv3_mla_pages* cache, const int32_t* lengths, voi
                         void* stream);
 
 /*
+ * Attention of MLA.forward for one new token, or a tree of up to 64 drafted ones, per sequence (inference/model.py:480-497 in the absorbed form
+ * of dsv3_mla_decode), on the cache in pages; the new rows are in it (dsv3_mla_latent_paged with the same starts and counts).  Token i of
+ * sequence b sees every position below starts[b], and position starts[b] + j where bit j of tree[b, i] is set and j < counts[b]
+ * (tree: int64 [batch, rows], 8-byte aligned, or NULL: bits 0 .. i).  Ancestors and the token itself for a tree; any other bits do.
+ * A token that sees nothing, and tokens from counts[b] on, give zeros.  A latent of NaN reaches the tokens that see it and no others.
+ * `positions`: no sequence has more (what lies behind is not seen); at most table_width * page_size.  It and the other sizes are all that
+ * the host knows: lengths are read on the device, the work is divided there.
+ * q: bf16 [batch, rows, heads, 192], its last 64 elements not yet rotated; freqs: binary32 (cos, sin) pairs [batch, rows, 32], each
+ * row's own; wkv_b, wkv_b_scale, softmax_scale as dsv3_mla_decode (the scale between 1e-30 and 1e30); y: bf16 [batch, rows, heads * 128].
+ * workspace: 256-byte aligned, dsv3_mla_decode_paged_workspace_bytes() bytes.
+ */
+size_t dsv3_mla_decode_paged_workspace_bytes(int64_t batch, int64_t rows, int heads);
+int dsv3_mla_decode_paged(const void* q, const float* freqs, const dsv3_mla_pages* cache, const int32_t* starts, const int32_t* counts,
+                          const int64_t* tree, const void* wkv_b, const float* wkv_b_scale, void* y, int64_t batch, int64_t rows,
+                          int64_t positions, int heads, int nope_dim, int rope_dim, int v_dim, int64_t kv_rank, float softmax_scale,
+                          void* workspace, size_t workspace_bytes, void* stream);
+/* The same, rounded to bf16 and quantised per (token, head) as dsv3_mla_decode_quant: y e4m3, s [batch, rows, heads]. */
+int dsv3_mla_decode_paged_quant(const void* q, const float* freqs, const dsv3_mla_pages* cache, const int32_t* starts, const int32_t* counts,
+                                const int64_t* tree, const void* wkv_b, const float* wkv_b_scale, void* y, float* s, int64_t batch, int64_t rows,
+                                int64_t positions, int heads, int nope_dim, int rope_dim, int v_dim, int64_t kv_rank, float softmax_scale,
+                                void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Rows of a drafted tree that were accepted, moved to the front of this step's: row starts[b] + k becomes what row
  * starts[b] + path[b, k] was, k < kept[b] (path: int32 [batch, most], most <= 64; kept: int32 [batch]).  All rows are read before any
  * is written: a path may name them in any order.  Entries below 0 or in no page leave their row as it is.

@@ -221,3 +221,289 @@ def test_rows_past_32_bits_of_bytes():
     rows = _rows(torch.tensor([[2, 0, 1]]), page, 3, 0, range(9000))
     assert torch.equal(got_kv[0].cpu(), (want[0].view(-1, C)[rows].float() * want[1].view(-1)[rows, None]).bfloat16())
     assert torch.equal(_bits(got_pe[0]), _bits(want[2].view(-1, ROPE)[rows]))
+
+
+# ------------------------------------------------------------------------------------------------------------ attention
+
+def _bits_of(rows):
+    """[batch][nodes] sets of nodes -> int64 [batch, nodes]."""
+    out = [[sum(1 << j for j in seen) for seen in seq] for seq in rows]
+    return torch.tensor([[v - (1 << 64) if v >> 63 else v for v in seq] for seq in out], dtype=torch.int64)
+
+
+def _trees(kind, g, b, s):
+    """What each new token sees of the new ones: None (those in front of it and itself), ancestors of a random tree, any bits (the
+    second token none)."""
+    if kind is None:
+        return None, [[set(range(i + 1)) for i in range(s)] for _ in range(b)]
+    rows = []
+    for _ in range(b):
+        seq = []
+        for i in range(s):
+            if kind == "any":
+                seq.append(set((torch.rand(s, generator=g) < 0.4).nonzero().flatten().tolist()) if i != 1 else set())
+            else:
+                parent = int(torch.randint(max(0, i - 5), i, (1,), generator=g)) if i else None
+                seq.append(({i} | seq[parent]) if i else {0})
+        rows.append(seq)
+    return _bits_of(rows), rows
+
+
+def _attention_case(b, s, h, context, page, kind, seed):
+    """Sequences of uneven lengths (the first the longest, the second with no more than the new tokens), fewer tokens in some, NaN in the
+    queries of tokens that a sequence does not have and in the cache rows behind every sequence."""
+    g = torch.Generator().manual_seed(seed)
+    lengths = [context] + [s + int(torch.randint(0, max(1, context - s + 1), (1,), generator=g)) for _ in range(b - 1)]
+    counts = [s] + [int(torch.randint(0, s + 1, (1,), generator=g)) for _ in range(b - 1)]
+    if b > 1:
+        lengths[1], counts[1] = s, s
+    if b > 3:
+        counts[3] = 0
+    starts = [n - s for n in lengths]
+    pages = sum(-(-n // page) for n in lengths) + 1
+    table, pool = _tables(g, lengths, page, pages), _pool(g, pages, page)
+    nan = torch.full((pages * page,), True)
+    for i in range(b):
+        nan[_rows(table, page, pages, i, range(starts[i] + counts[i]))] = False
+    pool[0].view(torch.uint8).view(-1, C)[nan] = 0x7f
+    pool[2].view(-1, ROPE)[nan] = float("nan")
+    q = (torch.randn(b, s, h, NOPE + ROPE, generator=g) * 2).bfloat16()
+    for i in range(b):
+        q[i, counts[i]:] = float("nan")
+    bits, seen = _trees(kind, g, b, s)
+    w8 = torch.randn(h * (NOPE + V), C, generator=g).to(FP8)
+    ws = torch.rand(h * 2, C // 128, generator=g) * 0.03 + 0.01
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    args = [q, _phases(g, b, s), *pool, table, i32(starts), i32(counts), bits, w8, ws, context, 0.08]
+    return [t.cuda() if isinstance(t, torch.Tensor) else t for t in args], seen
+
+
+def _attention_reference(args, seen):
+    """Binary64 with the absorbed form's roundings to bf16: weights, rotated and folded query, latent sum."""
+    q, freqs, kv, scale, pe, table, starts, counts, _, w8, ws, positions, softmax_scale = args
+    b, s, h, _ = q.shape
+    pages, page = scale.shape
+    w = (w8.float() * ws.repeat_interleave(128, 0).repeat_interleave(128, 1)).bfloat16().double().view(h, NOPE + V, C)
+    out = torch.zeros(b, s, h, V, dtype=torch.float64, device=q.device)
+    for i in range(b):
+        first, n = int(starts[i]), int(counts[i])
+        if n <= 0 or first < 0:
+            continue
+        end = min(first + n, positions)
+        rows = _rows(table.cpu(), page, pages, i, range(end))
+        visible = torch.zeros(n, end, dtype=torch.bool)
+        visible[:, :first] = True
+        for t in range(n):
+            for j in seen[i][t]:
+                if first + j < end:
+                    visible[t, first + j] = True
+        visible &= (rows >= 0)[None]
+        used = rows.clamp_min(0).cuda()
+        there = (rows >= 0).cuda()[:, None]
+        c = torch.where(there, kv.view(-1, C)[used].double() * scale.view(-1)[used, None].double(), 0.0)
+        k = torch.where(there, pe.view(-1, ROPE)[used].double(), 0.0)
+        turned = _rotated(q[i, :n, :, NOPE:], freqs[i, :n, None]).bfloat16().double()
+        visible = visible.cuda()
+        for a in range(h):
+            folded = (q[i, :n, a, :NOPE].double() @ w[a, :NOPE]).bfloat16().double()
+            score = (folded @ c.T + turned[:, a] @ k.T) * softmax_scale
+            p = score.masked_fill(~visible, float("-inf")).softmax(-1).masked_fill(~visible, 0)
+            for t in range(n):              # (a product with a weight of zero would bring in what the token does not see)
+                if bool(visible[t].any()):
+                    out[i, t, a] = (p[t, visible[t]] @ c[visible[t]]).bfloat16().double() @ w[a, NOPE:].T
+    return out
+
+
+def _close(got, ref):
+    # the latent sum and the result round to bf16 (2^-8 of the value at most each), the exponentials too; in the value product of 512 terms
+    # these errors average out against a result of the same size: 2^-7 of the row's norm
+    return ((got - ref).norm(dim=-1) <= 2.0 ** -7 * ref.norm(dim=-1)).all()
+
+
+# one token and 64; heads that fill no block of rows; contexts of one tile and many, of nothing but the new tokens; pages that end inside a
+# tile, hold a tile, hold everything; more sequences than compute units, more row blocks than compute units
+ATTEND = [(1, 1, 1, 1, 8, None), (1, 1, 128, 31, 64, None), (2, 1, 128, 33, 8, None), (1, 1, 128, 700, 64, None), (5, 1, 16, 1000, 24, None),
+          (70, 1, 128, 97, 16, None), (6, 5, 40, 257, 40, None), (3, 64, 3, 64, 8, "tree"), (2, 25, 128, 300, 24, "tree"), (4, 13, 20, 500, 64, "any"),
+          (1, 61, 128, 1500, 128, "tree"), (1, 1, 3, 9000, 4096, None), (300, 1, 4, 60, 8, None), (5, 64, 70, 90, 8, "any"), (1, 40, 100, 40, 48, "any"),
+          (9, 2, 64, 333, 16, "tree"), (20, 1, 16, 3000, 32, None), (130, 3, 64, 200, 64, "tree"), (1, 2, 32, 64, 64, None)]
+
+
+@pytest.mark.parametrize("grow", [False, True])
+@pytest.mark.parametrize("b,s,h,context,page,kind", ATTEND)
+def test_attention(b, s, h, context, page, kind, grow):
+    args, seen = _attention_case(b, s, h, context, page, kind, b + s + context)
+    if grow:                    # scores that grow along the positions by far more than 2^64: the running maximum is raised
+        if kind is not None or context < 8:
+            pytest.skip("one run per shape without a tree")
+        for i in range(b):
+            n = int(args[6][i] + args[7][i])
+            rows = _rows(args[5].cpu(), page, args[3].size(0), i, range(n)).cuda()
+            args[4].view(-1, ROPE)[rows] *= torch.linspace(0.01, 400, n, device="cuda").bfloat16()[:, None]
+    got = torch.ops.dsv3fp8.mla_decode_paged(*args).view(b, s, h, V).double()
+    ref = _attention_reference(args, seen)
+    assert torch.isfinite(got).all()
+    for i in range(b):
+        assert (got[i, max(0, int(args[7][i])):] == 0).all()
+    if kind == "any" and args[6].min() == 0:
+        i = int((args[6] == 0).nonzero()[0])
+        assert (got[i, 1] == 0).all()                               # a token that sees nothing
+    assert _close(got, ref)
+
+
+@pytest.mark.parametrize("b,s,h,context,page,kind", [(1, 1, 128, 33, 64, None), (1, 1, 8, 8192, 64, None), (3, 13, 24, 200, 24, "any"), (37, 1, 128, 70, 8, None), (2, 9, 128, 200, 40, "tree")])
+def test_attention_quantised_is_the_rounded_result_quantised(b, s, h, context, page, kind):
+    from dsv3fp8 import kernel
+    args, _ = _attention_case(b, s, h, context, page, kind, 5)
+    y = torch.ops.dsv3fp8.mla_decode_paged(*args)
+    yq, ys = torch.ops.dsv3fp8.mla_decode_paged_quant(*args)
+    rq, rs = kernel.act_quant(y)
+    assert torch.equal(yq.view(torch.uint8), rq.view(torch.uint8)) and torch.equal(ys.view(torch.int32), rs.view(torch.int32))
+    assert torch.equal(_bits(y), _bits(torch.ops.dsv3fp8.mla_decode_paged(*args)))          # and the same again
+
+
+@pytest.mark.parametrize("h,page", [(128, 64), (6, 24)])
+def test_rows_that_are_not_finite_reach_those_who_see_them(h, page):
+    """A latent of NaN (stored as zeros and a scale of NaN) and a key of NaN or infinity, in a drafted branch: the tokens of other branches do
+    not notice; then one in the context, which everybody sees."""
+    args, seen = _attention_case(2, 12, h, 150, page, "tree", 11)
+    clean = torch.ops.dsv3fp8.mla_decode_paged(*args)
+    first, pages = int(args[6][0]), args[3].size(0)
+    row = lambda j: int(_rows(args[5].cpu(), page, pages, 0, [j])[0])  # noqa: E731
+    for what in ("latent", "nan key", "inf key"):
+        node = 7
+        kv, scale, pe = args[2].clone(), args[3].clone(), args[4].clone()
+        if what == "latent":
+            kv.view(torch.uint8).view(-1, C)[row(first + node)] = 0
+            scale.view(-1)[row(first + node)] = float("nan")
+        else:
+            pe.view(-1, ROPE)[row(first + node), 3] = float("nan" if what == "nan key" else "inf")
+        got = torch.ops.dsv3fp8.mla_decode_paged(args[0], args[1], kv, scale, pe, *args[5:])
+        for t in range(12):
+            if node in seen[0][t]:
+                if what != "inf key":           # (an infinite score of the wrong sign only leaves the others)
+                    assert torch.isnan(got[0, t]).all()
+            else:
+                assert torch.equal(_bits(got[0, t]), _bits(clean[0, t]))
+        assert torch.equal(_bits(got[1]), _bits(clean[1]))
+    kv, scale = args[2].clone(), args[3].clone()
+    kv.view(torch.uint8).view(-1, C)[row(3)] = 0
+    scale.view(-1)[row(3)] = float("nan")
+    got = torch.ops.dsv3fp8.mla_decode_paged(args[0], args[1], kv, scale, *args[4:])
+    assert torch.isnan(got[0]).all() and torch.equal(_bits(got[1]), _bits(clean[1]))
+
+
+@pytest.mark.parametrize("page", [8, 40, 64])
+def test_attention_skips_what_is_no_page(page):
+    args, seen = _attention_case(3, 4, 20, 230, page, "tree", 2)
+    pages = args[3].size(0)
+    for i, k, entry in ((0, 1, -1), (0, 2, pages), (2, 0, 2 ** 31 - 1), (1, 0, -7)):
+        if k < args[5].size(1):
+            args[5][i, k] = entry
+    got = torch.ops.dsv3fp8.mla_decode_paged(*args).view(3, 4, 20, V).double()
+    assert torch.isfinite(got).all() and _close(got, _attention_reference(args, seen))
+
+
+def test_attention_past_the_stated_positions_and_negative_starts():
+    args, seen = _attention_case(4, 3, 16, 200, 16, None, 4)
+    args[11] = 150                                                  # the longest sequence is cut there
+    args[6][2] = -5                                                 # nothing
+    got = torch.ops.dsv3fp8.mla_decode_paged(*args).view(4, 3, 16, V).double()
+    assert (got[2] == 0).all() and torch.isfinite(got).all()
+    assert _close(got, _attention_reference(args, seen))
+
+
+def test_attention_of_nobody():
+    args, _ = _attention_case(3, 4, 16, 50, 16, "tree", 4)
+    args[7].zero_()
+    assert (torch.ops.dsv3fp8.mla_decode_paged(*args) == 0).all()
+    args, _ = _attention_case(1, 1, 16, 50, 16, None, 4)
+    args[0], args[1], args[5], args[6], args[7] = (args[k][:0] for k in (0, 1, 5, 6, 7))
+    assert torch.ops.dsv3fp8.mla_decode_paged(*args).shape == (0, 1, 16 * V)
+
+
+@pytest.mark.parametrize("b,s,h,context", [(3, 1, 128, 500), (2, 20, 16, 300)])
+def test_a_step_captured_and_replayed(b, s, h, context):
+    """Rows written, attended to and kept in one graph, on a stream of its own; two graphs; lengths, pages and queries change between replays."""
+    cases = [_attention_case(b, s, h, context, 24, "tree" if s > 1 else None, seed)[0] for seed in (1, 2, 3)]
+    pages = max(c[3].size(0) for c in cases)
+    def padded(c):
+        c = list(c)
+        for k in (2, 3, 4):
+            t = c[k]
+            big = torch.zeros(pages, *t.shape[1:], dtype=torch.uint8 if k == 2 else t.dtype, device="cuda")
+            big[:t.size(0)] = t.view(torch.uint8) if k == 2 else t
+            c[k] = big.view(FP8) if k == 2 else big
+        c[0] = c[0].nan_to_num(0.0)
+        return c
+    cases = [padded(c) for c in cases]
+    g = torch.Generator().manual_seed(9)
+    a = [torch.randn(b, s, C + ROPE, generator=g).bfloat16().cuda() for _ in cases]
+    kn = torch.ones(C).bfloat16().cuda()
+    path = torch.stack([torch.randperm(s, generator=g)[:min(4, s)] for _ in range(b)]).int().cuda()
+    kept = torch.full((b,), min(3, s), dtype=torch.int32, device="cuda")
+
+    def step(c, rows):
+        torch.ops.dsv3fp8.mla_latent_paged(rows, None, kn, c[1], *c[2:8], EPS, EPS)
+        y = torch.ops.dsv3fp8.mla_decode_paged(*c)
+        torch.ops.dsv3fp8.mla_cache_keep(*c[2:7], path, kept)
+        return y, *torch.ops.dsv3fp8.mla_cache_read(*c[2:6], c[6] + 1, context)
+
+    def fresh(c):
+        return [t.clone() if isinstance(t, torch.Tensor) else t for t in c]
+    want = []
+    for c, rows in zip(cases, a):
+        c = fresh(c)
+        want.append([t.clone() for t in (*step(c, rows), c[2].view(torch.uint8), c[3], c[4])])
+    graphs = []
+    for _ in range(2):
+        live, live_a = fresh(cases[0]), a[0].clone()
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            step(fresh(cases[0]), a[0])
+        torch.cuda.current_stream().wait_stream(stream)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(live, live_a)
+        graphs.append((graph, live, live_a, out))
+    for k in (1, 2, 0, 1):
+        for graph, live, live_a, out in graphs:
+            for t, new in zip(live, cases[k]):
+                if isinstance(t, torch.Tensor):
+                    t.copy_(new) if t.dtype != FP8 else t.view(torch.uint8).copy_(new.view(torch.uint8))
+            live_a.copy_(a[k])
+            graph.replay()
+            torch.ops.dsv3fp8.mla_decode_paged(*cases[k])           # eager work between the replays
+        for _, live, _, out in graphs:
+            for got, ref in zip((*out, live[2].view(torch.uint8), live[3], live[4]), want[k]):
+                assert torch.equal(_bits(got), _bits(ref))
+
+
+def test_two_streams_at_once():
+    one, seen1 = _attention_case(8, 1, 128, 900, 64, None, 21)
+    two, seen2 = _attention_case(3, 20, 16, 400, 24, "tree", 22)
+    want = [torch.ops.dsv3fp8.mla_decode_paged(*a) for a in (one, two)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(6):
+        for k, a in enumerate((one, two)):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(torch.ops.dsv3fp8.mla_decode_paged(*a))
+    torch.cuda.synchronize()
+    for k in (0, 1):
+        for y in got[k]:
+            assert torch.equal(_bits(y), _bits(want[k]))
+
+
+def test_attention_past_32_bits_of_bytes():
+    page, pages = 4096, 2200
+    args, seen = _attention_case(2, 3, 16, 9000, page, "tree", 6)
+    small = args[3].size(0)
+    kv = torch.zeros(pages, page, C, dtype=torch.uint8, device="cuda")
+    scale, pe = torch.ones(pages, page, device="cuda"), torch.zeros(pages, page, ROPE, device="cuda").bfloat16()
+    want = torch.ops.dsv3fp8.mla_decode_paged(*args)
+    kv[pages - small:], scale[pages - small:], pe[pages - small:] = args[2].view(torch.uint8), args[3], args[4]
+    table = torch.where((args[5] >= 0) & (args[5] < small), args[5] + (pages - small), -1).int()
+    got = torch.ops.dsv3fp8.mla_decode_paged(*args[:2], kv.view(FP8), scale, pe, table, *args[6:])
+    assert torch.equal(_bits(got), _bits(want)) and _close(got.view(2, 3, 16, V).double(), _attention_reference(args, seen))

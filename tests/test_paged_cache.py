@@ -47,9 +47,9 @@ def test_row_of_a_position(walk, page):
 
 def test_span_of_a_sequence(walk):
     o = (ctypes.c_int * 3)()
-    for (start, count, rows, most), want in {(5, 3, 4, 100): (5, 8, 3), (-4, 3, 4, 100): (0, 3, 3), (5, -1, 4, 100): (5, 5, 0), (5, 9, 4, 100): (5, 9, 4),
+    for (start, count, rows, most), want in {(5, 3, 4, 100): (5, 8, 3), (-4, 3, 4, 100): (0, 0, 0), (5, -1, 4, 100): (0, 0, 0), (5, 9, 4, 100): (5, 9, 4),
                                              (98, 4, 4, 100): (98, 100, 4), (2 ** 31 - 1, 4, 4, 100): (100, 100, 4), (0, 0, 4, 100): (0, 0, 0),
-                                             (-2 ** 31, -2 ** 31, 64, 8388607): (0, 0, 0)}.items():
+                                             (-2 ** 31, -2 ** 31, 64, 8388607): (0, 0, 0), (0, 2 ** 31 - 1, 64, 8388607): (0, 64, 64)}.items():
         walk.span(start, count, rows, most, o)
         assert tuple(o) == want
 
@@ -103,6 +103,35 @@ def test_cache_keep_validation(L):
     assert call(b=0, st=None) == 0 and call(most=0, st=None) == 0
 
 
+def test_decode_paged_validation(L):
+    base = dict(q=A16, f=A16, cache=_cache(L), st=A16, n=A16, tree=A16, w=A16, w_s=A16, y=A16, b=2, rows=3, pos=100, heads=4, nope=128, rope=64, v=128, c=512,
+                scale=0.1, ws=0x1000, wsb=1 << 30)
+    need = L.lib.dsv3_mla_decode_paged_workspace_bytes(2, 3, 4)
+    assert need > 0 and L.lib.dsv3_mla_decode_paged_workspace_bytes(0, 3, 4) == 0
+
+    def plain(**change):
+        a = base | change
+        return L.lib.dsv3_mla_decode_paged(*[a[k] for k in list(base)[:9]], *[a[k] for k in list(base)[9:]], None)
+
+    def quant(s=A16, **change):
+        a = base | change
+        return L.lib.dsv3_mla_decode_paged_quant(*[a[k] for k in list(base)[:9]], s, *[a[k] for k in list(base)[9:]], None)
+    for call in (plain, quant):
+        for change, code in BAD_PAGES:
+            assert call(cache=_cache(L, **change)) == code
+        for name in ("q", "f", "st", "n", "w", "w_s", "y"):
+            assert call(**{name: None}) == 1 and call(**{name: A16 + 2}) == 4
+        assert call(tree=A16 + 4) == 4 and call(cache=None) == 1
+        for bad in (dict(b=-1), dict(b=65536), dict(rows=-1), dict(rows=65), dict(heads=-1), dict(heads=65536), dict(pos=0), dict(pos=129), dict(nope=64), dict(rope=32),
+                    dict(v=64), dict(c=256), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=1e-40)):
+            assert call(**bad) == 2, bad
+        assert call(cache=_cache(L, table_width=1 << 20), pos=1 << 23) == 2
+        assert call(b=65535, cache=_cache(L, table_width=1 << 20), pos=(1 << 23) - 1) == 2        # tiles of all sequences past 31 bits
+        assert call(ws=None) == 6 and call(ws=0x1010) == 6 and call(wsb=need - 1) == 6
+        assert call(b=0, q=None) == 0 and call(rows=0, q=None) == 0 and call(heads=0, q=None) == 0
+    assert quant(s=None) == 1 and quant(s=A16 + 2) == 4
+
+
 def _args(name):
     z = torch.zeros
     i32 = dict(dtype=torch.int32)
@@ -119,7 +148,7 @@ def _args(name):
 
 
 # where the cache stands, and the int32 [batch] behind it
-OPERATORS = {"mla_latent_paged": (4, (8, 9)), "mla_cache_read": (0, (4,)), "mla_cache_keep": (0, (4, 6))}
+OPERATORS = {"mla_latent_paged": (4, (8, 9)), "mla_cache_read": (0, (4,)), "mla_cache_keep": (0, (4, 6)), "mla_decode_paged": (2, (6, 7)), "mla_decode_paged_quant": (2, (6, 7))}
 
 
 @pytest.mark.parametrize("name", OPERATORS)
@@ -154,6 +183,15 @@ def test_operators_refuse_what_their_kernels_cannot_read(name):
         bad[5] = [lambda t: -1, lambda t: 1 << 23]
     if name == "mla_cache_keep":
         bad[5] = [lambda t: t.long(), lambda t: t[:1], lambda t: z(2, 65, dtype=t.dtype), lambda t: t[0], lambda t: z(2, 10, dtype=t.dtype)[:, ::2]]
+    if name.startswith("mla_decode_paged"):
+        bad[0] = [lambda t: t.float(), lambda t: t[0], lambda t: z(2, 3, 8, 192, dtype=t.dtype)[:, :, ::2], lambda t: z(2, 3, 4, 128, dtype=t.dtype),
+                  lambda t: z(2, 65, 4, 192, dtype=t.dtype), lambda t: t[:, :, :3].contiguous()]
+        bad[1] = [lambda t: t.conj(), lambda t: t[:1], lambda t: t[:, :2].contiguous(), lambda t: t[0]]
+        bad[8] = [lambda t: t.int(), lambda t: t[:1], lambda t: t[:, :2].contiguous(), lambda t: z(2, 6, dtype=t.dtype)[:, ::2], lambda t: t[0]]
+        bad[9] = [lambda t: t.bfloat16(), lambda t: t[:1020], lambda t: t[:, :256].contiguous(), lambda t: z(1024, 1024, dtype=t.dtype)[:, ::2]]
+        bad[10] = [lambda t: t[:7], lambda t: t[:, :3].contiguous(), lambda t: t.bfloat16(), lambda t: t.flatten(), lambda t: z(4, 8).t()]
+        bad[11] = [lambda t: 0, lambda t: -1, lambda t: 49, lambda t: 1 << 23, lambda t: 2 ** 63 - 1]
+        bad[12] = [lambda t: 0.0, lambda t: -1.0, lambda t: float("nan"), lambda t: float("inf"), lambda t: 1e-40]
     for i, changes in bad.items():
         for change in changes:
             args = _args(name)
@@ -166,5 +204,6 @@ def test_operators_refuse_what_their_kernels_cannot_read(name):
 def test_shapes_without_a_device(name):
     args = [t.to("meta") if isinstance(t, torch.Tensor) else t for t in _args(name)]
     got = getattr(torch.ops.dsv3fp8, name)(*args)
-    shapes = {"mla_latent_paged": [(2, 3, 128), (2, 3, 1)], "mla_cache_read": [(2, 20, 512), (2, 20, 64)], "mla_cache_keep": []}[name]
+    shapes = {"mla_latent_paged": [(2, 3, 128), (2, 3, 1)], "mla_cache_read": [(2, 20, 512), (2, 20, 64)], "mla_cache_keep": [], "mla_decode_paged": [(2, 3, 512)], "mla_decode_paged_quant": [(2, 3, 512), (2, 3, 4)]}[name]
+    got = (got,) if isinstance(got, torch.Tensor) else got
     assert [tuple(t.shape) for t in got or ()] == shapes
