@@ -17,6 +17,10 @@ constexpr int kTile = 32;                               // positions per tile
 constexpr int kRopeOff = kTile * kC;                    // a stage: 32 rows of 512 codes, 32 rotary keys of 128 B, four groups of eight scales, 256 B each
 constexpr int kScaleOff = kRopeOff + kTile * kRope * 2;
 constexpr int kStage = kScaleOff + 1024;
+constexpr int kStages = 6;                              // tiles in LDS, computed or on their way
+constexpr int kCopies = 6;                              // of a tile, by each of the four wavefronts
+constexpr int kKeys = 4, kValues = 6;                   // reads from LDS ahead of the MFMAs that take them: keys (a read is two K steps), values
+constexpr int kSync = 27;                               // the value step behind which a tile's stage is free and the next tile's keys are read
 
 struct PagedArgs {
     const void* ql;                                     // folded queries [batch][rows][512], rows = tokens * heads, or in operand order
@@ -113,7 +117,7 @@ __device__ __forceinline__ v4u operand(uint32_t lo, uint32_t hi, float s) {
 template <bool PACK, int G>
 __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-    constexpr int RB = 4 / G;                           // row groups of a workgroup
+    constexpr int RB = 4 / G, R = kStages / G;          // row groups of a workgroup; steps that the stages hold
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = lane & 31, g = lane >> 5, rg = wave % RB, par = wave / RB;
     // a contiguous run of the ranges in use per XCD, the row blocks of a range next to each other: its rows are in the XCD's L2
@@ -133,35 +137,42 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     const int row = min(row0 + i, p.rows - 1);          // rows past the end repeat the last one; fold leaves them out
 
     // A wavefront copies eight rows of a tile, which lie in one page: four KiB of latents, a KiB of rotary keys, the scales (by
-    // all lanes, for what the first eight fetch).  Rows past the sequence's end are its last one again; what is no page's comes from `nothing`.
+    // all lanes, for what the first eight fetch).  Rows past the sequence's end are its last one again; what is no page's comes from `nothing`,
+    // so that every tile is as many copies, whose outstanding ones can be counted.
     const uint32_t lds0 = lds_addr_of(lds);
     const int32_t* entries = p.table + b * p.width;
-    auto copy_tile = [&](int t, int stage) {
-        const int pos = t * kTile + wave * 8;
-        const uint8_t* kv = nothing.kv;
-        const uint8_t* pe = nothing.pe;
-        const float* sc = nothing.scale;
-        int last = 0;
-        if (t < t1 && pos < seq.end) {
-            const int k = quotient(pos, p.page, p.page_magic), entry = scalar_load(entries, k);
-            if ((uint32_t)entry < (uint64_t)p.pages) {
-                const int64_t r = (int64_t)entry * p.page + (pos - k * p.page);
-                kv = p.kv + r * kC;
-                pe = p.pe + r * (kRope * 2);
-                sc = p.scales + r;
-                last = min(7, seq.end - 1 - pos);
-            }
-        }
-        const uint32_t at = lds0 + stage * kStage;
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {                   // row r's chunk c of 16 bytes lies at c ^ r (low four bits)
-            const int r = 2 * n + (lane >> 5), dst = wave * 8 + r;
-            copy16(kv, min(r, last) * kC + (((lane & 31) ^ (dst & 15)) << 4), at + wave * 4096 + n * 1024);
-        }
-        const int r = lane >> 3;                        // chunk c at c ^ r / 2 (low three bits)
-        copy16(pe, min(r, last) * (kRope * 2) + (((lane & 7) ^ (((wave * 8 + r) >> 1) & 7)) << 4), at + kRopeOff + wave * 1024);
-        copy4(sc, min(lane & 7, last) * 4, at + kScaleOff + wave * 256);
+    struct Source { const uint8_t* kv; const uint8_t* pe; const float* scales; int last; uint32_t at; };
+    auto entry_of = [&](int t) -> int {                 // the page number of the wavefront's rows of tile t (past the end: of the last ones)
+        return scalar_load(entries, quotient(min(t * kTile + wave * 8, seq.end - 1), p.page, p.page_magic));
     };
+    auto source = [&](int t, int entry, int stage) -> Source {
+        const int pos = t * kTile + wave * 8;
+        Source s = { nothing.kv, nothing.pe, nothing.scale, 0, lds0 + stage * kStage };
+        if (t < t1 && pos < seq.end && (uint32_t)entry < (uint64_t)p.pages) {
+            const int64_t r = (int64_t)entry * p.page + (pos - quotient(pos, p.page, p.page_magic) * p.page);
+            s.kv = p.kv + r * kC;
+            s.pe = p.pe + r * (kRope * 2);
+            s.scales = p.scales + r;
+            s.last = min(7, seq.end - 1 - pos);
+        }
+        return s;
+    };
+    auto issue = [&](const Source& s, auto which) {
+        constexpr int n = decltype(which)::value;
+        if constexpr (n < 4) {                          // row r's chunk c of 16 bytes lies at c ^ r (low four bits)
+            const int r = 2 * n + (lane >> 5);
+            copy16(s.kv, min(r, s.last) * kC + (((lane & 31) ^ ((wave * 8 + r) & 15)) << 4), s.at + wave * 4096 + n * 1024);
+        } else if constexpr (n == 4) {                  // chunk c at c ^ r / 2 (low three bits)
+            const int r = lane >> 3;
+            copy16(s.pe, min(r, s.last) * (kRope * 2) + (((lane & 7) ^ (((wave * 8 + r) >> 1) & 7)) << 4), s.at + kRopeOff + wave * 1024);
+        } else {
+            copy4(s.scales, min(lane & 7, s.last) * 4, s.at + kScaleOff + wave * 256);
+        }
+    };
+    for (int n = 0; n < (R - 1) * G; ++n) {
+        const Source s = source(t0 + n, entry_of(t0 + n), n);
+        unrolled<kCopies>([&](auto k) { issue(s, k); });
+    }
 
     v4u Q[36];
     {
@@ -195,20 +206,44 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     v16f O[16] = {};
     float m = -__builtin_inff(), l = 0.f;               // running maximum of the scores, this lane's share of the sum
     const float scale2 = p.scale * 1.44269504088896340736f;
-    auto tile = [&](int t, const uint8_t* base) {
-        const float sc = *(const float*)(base + kScaleOff + (i >> 3) * 256 + (i & 7) * 4);
+    // The reads' order and place are those that are written here (sched_barrier); a step's operand is made from its codes beside the MFMA
+    // in front of it: four conversions take no time there (33.6 cycles instead of 33.1), six do (38.6).
+    v4u keys[kKeys];
+    float sc;                                           // the scale of position i
+    auto key = [&](const uint8_t* base, int x) -> v4u {
+        return x < 16 ? *(const v4u*)(base + (kaddr ^ ((x & 7) << 5)) + (x >> 3) * 256) : *(const v4u*)(base + (raddr ^ ((x - 16) << 5)));
+    };
+    auto scale_at = [&](const uint8_t* base) { return *(const float*)(base + kScaleOff + (i >> 3) * 256 + (i & 7) * 4); };
+    // the next step's tiles are there, once this wavefront's copies of them are (those of the steps behind it stay in flight) and everybody's
+    auto arrived = [&] {
+        constexpr int left = (R - 2) * kCopies * G;
+        __builtin_amdgcn_s_waitcnt(0x0f70 | (left & 15) | (left >> 4) << 14);   // vmcnt
+        barrier_no_fence();
+    };
+    // One tile.  copy: beside the MFMA just issued.  The last value steps read the next tile's first keys.
+    auto tile = [&](int t, const uint8_t* base, const uint8_t* next, auto copy) {
+        const uint32_t vbase = lds_addr_of(base) + vaddr;
+        v2i values[kValues];
+        auto value = [&](int y) -> v2i {                // positions 16 (y / 16) .. of features 32 (y % 16) ..
+            return __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i)(uintptr_t)((vbase ^ ((y & 7) << 5)) + ((y >> 3) & 1) * 256 + (y >> 4) * 8192));
+        };
+        v4f w[4];
         v16f T[1];
         v16f& S = T[0];
-        unrolled<16>([&](auto pair) {
-            constexpr int n = decltype(pair)::value;
-            const v4u raw = *(const v4u*)(base + (kaddr ^ ((n & 7) << 5)) + (n >> 3) * 256);
-            if constexpr (n == 0) mfma32_first(S, operand(raw[0], raw[1], sc), Q[0]);
-            else mfma32_next(S, operand(raw[0], raw[1], sc), Q[2 * n]);
-            mfma32_next(S, operand(raw[2], raw[3], sc), Q[2 * n + 1]);
-        });
-        unrolled<4>([&](auto step) {
+        v4u cur = operand(keys[0][0], keys[0][1], sc);
+        __builtin_amdgcn_sched_barrier(0);
+        unrolled<36>([&](auto step) {
             constexpr int s = decltype(step)::value;
-            mfma32_next(S, *(const v4u*)(base + (raddr ^ (s << 5))), Q[32 + s]);
+            if constexpr (s == 0) mfma32_first(S, cur, Q[0]);
+            else mfma32_next(S, cur, Q[s]);
+            if constexpr (s < 31 && s % 2 == 0) cur = operand(keys[s / 2 % kKeys][2], keys[s / 2 % kKeys][3], sc);
+            else if constexpr (s < 31) cur = operand(keys[(s + 1) / 2 % kKeys][0], keys[(s + 1) / 2 % kKeys][1], sc);
+            else if constexpr (s < 35) cur = keys[(s - 15) % kKeys];
+            if constexpr (s < 32 && s % 2 == 0 && s / 2 + kKeys < 20) keys[s / 2 % kKeys] = key(base, s / 2 + kKeys);
+            if constexpr (s >= 26 && s < 26 + 4) w[s - 26] = *(const v4f*)(base + kScaleOff + (s - 26) * 256 + g * 16);
+            if constexpr (s >= 30) values[s - 30] = value(s - 30);
+            copy(step);
+            __builtin_amdgcn_sched_barrier(0);
         });
         scores_ready(S);
         // positions that nobody sees: past the end, of no page (a row that was not finite has scores of NaN already)
@@ -248,46 +283,71 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
             }
         }
         const float off = softmax_offset(T, m, scale2);
-        v4f w[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) w[k] = *(const v4f*)(base + kScaleOff + k * 256 + g * 16);
         if (__any(sc != sc)) {                          // NaN times an exponential of zero: these rows' codes are zeros, the scores say who sees them
 #pragma unroll
             for (int e = 0; e < 16; ++e) w[e >> 2][e & 3] = w[e >> 2][e & 3] == w[e >> 2][e & 3] ? w[e >> 2][e & 3] : 0.f;
         }
         float sum = 0.f;
         v4u P[2];
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) {
+        auto weights = [&](int e) {                     // two positions' exponentials
             const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(S[e], scale2, -off));
             const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(S[e + 1], scale2, -off));
             sum += x + y;
             P[e >> 3][(e & 7) >> 1] = pack_bf16(x * w[e >> 2][e & 3], y * w[e >> 2][(e & 3) + 1]);
-        }
-        const uint32_t vbase = lds_addr_of(base) + vaddr;
+        };
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) weights(e);
+        cur = operand((uint32_t)values[0][0], (uint32_t)values[0][1], 1.0f);
+        __builtin_amdgcn_sched_barrier(0);
         unrolled<32>([&](auto step) {
-            constexpr int s = decltype(step)::value;    // positions 16 (s / 16) .. of features 32 (s % 16) ..
-            const v2i raw = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i)(uintptr_t)((vbase ^ ((s & 7) << 5)) + ((s >> 3) & 1) * 256 + (s >> 4) * 8192));
-            O[s & 15] = mfma32(operand((uint32_t)raw[0], (uint32_t)raw[1], 1.0f), P[s >> 4], O[s & 15]);
+            constexpr int s = decltype(step)::value;
+            O[s & 15] = mfma32(cur, P[s >> 4], O[s & 15]);
+            if constexpr (s < 31) cur = operand((uint32_t)values[(s + 1) % kValues][0], (uint32_t)values[(s + 1) % kValues][1], 1.0f);
+            if constexpr (s + kValues < 32) values[s % kValues] = value(s + kValues);
+            if constexpr (s < 12 && s % 3 == 2) weights(8 + s / 3 * 2);         // the second half's, beside the first half's products
             __builtin_amdgcn_sched_barrier(0);
+            if constexpr (s == kSync) {                 // this tile's last codes are in registers: its stage is free behind the barrier
+                arrived();
+                sc = scale_at(next);
+            }
+            if constexpr (s >= kSync && s - kSync < kKeys) {
+                keys[s - kSync] = key(next, s - kSync);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         });
         l += sum;
 #pragma unroll
         for (int d = 0; d < 16; ++d) asm volatile("" : "+a"(O[d]));     // (the sums stay where they are)
     };
 
-    for (int t = t0; t < t1; t += G) {
-        barrier_no_fence();                             // everybody is done with the stages
+    arrived();
+    sc = scale_at(lds + par * kStage);
 #pragma unroll
-        for (int n = 0; n < G; ++n) copy_tile(t + n, n);
-        __builtin_amdgcn_s_waitcnt(0x0f70);             // vmcnt(0)
-        barrier_no_fence();
-        tile(t + par, lds + par * kStage);
+    for (int x = 0; x < kKeys; ++x) keys[x] = key(lds + par * kStage, x);
+    int st = 0, entry[G];
+#pragma unroll
+    for (int j = 0; j < G; ++j) entry[j] = entry_of(t0 + (R - 1) * G + j);
+    for (int t = t0; t < t1; t += G) {
+        const int st_next = st + 1 == R ? 0 : st + 1, st_free = st == 0 ? R - 1 : st - 1;
+        // Copies into the stage of the step before, which is free, every few MFMAs: the four wavefronts take turns on the compute unit's load
+        // path.  Page numbers are loaded a step ahead of the copies that need them.
+        Source ahead[G];
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+            ahead[j] = source(t + (R - 1) * G + j, entry[j], st_free * G + j);
+            entry[j] = entry_of(t + R * G + j);
+        }
+        tile(t + par, lds + (st * G + par) * kStage, lds + (st_next * G + par) * kStage, [&](auto step) {
+            constexpr int s = decltype(step)::value, E = 4 / G;
+            if constexpr (s % E == E - 1 && s / E < kCopies * G) issue(ahead[s / E / kCopies], std::integral_constant<int, s / E % kCopies>());
+        });
+        st = st_next;
     }
 
     const v2f parts = halves32(l);
     l = parts.x + parts.y;
     const int64_t slot = ((int64_t)range * p.blocks + blk) * (RB * 32);         // the workgroup's rows among all
+    __builtin_amdgcn_s_waitcnt(0x0f70);                 // (copies of the tiles past the range are still on their way into the stages)
     barrier_no_fence();
     // The sums leave as in mla_decode_kernel: 64 features of 32 rows at a time through LDS (16-byte chunks xor-ed with the row); the G
     // wavefronts of a row group first add theirs, each for 32 / G of the rows.
@@ -382,8 +442,8 @@ PagedSpace paged_space(const PagedPlan& a, int64_t batch) {
 template <int G> int launch_paged(const PagedArgs& a, bool pack, unsigned grid, hipStream_t st) {
     static void (*const kernels[2])(PagedArgs) = { mla_paged_kernel<false, G>, mla_paged_kernel<true, G> };
     static LdsGrant grant[2];
-    constexpr int bytes = 65536 + 1024;                 // (the sums' way out takes more than the stages)
-    static_assert(bytes >= G * kStage, "stages");
+    constexpr int bytes = kStages * kStage;
+    static_assert(bytes >= 65536 + 1024 && bytes <= 160 * 1024, "the sums leave through the stages");
     if (!grant[pack].ensure((const void*)kernels[pack], bytes)) return DSV3_ERR_LAUNCH;
     hipLaunchKernelGGL(kernels[pack], dim3(grid), dim3(256), bytes, st, a);
     return DSV3_OK;
