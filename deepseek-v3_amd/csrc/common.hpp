@@ -54,6 +54,25 @@ __device__ __forceinline__ uint32_t pack_fp8x4(float a, float b, float c, float 
 __device__ __forceinline__ v2f fp8x2_lo_to_f32(uint32_t p) { return __builtin_amdgcn_cvt_pk_f32_fp8((int)p, false); }
 __device__ __forceinline__ v2f fp8x2_hi_to_f32(uint32_t p) { return __builtin_amdgcn_cvt_pk_f32_fp8((int)p, true); }
 
+// Four binary32 as the sum of two e4m3 codes each, of scales 2^(e - 127) and a sixteenth of it (e from split_exponent): what the first code
+// leaves off, at most half a step of 2^-3, is the second's.  Off by 2^-9 of the value at most, half of what bf16 is, down to 2^-14 of the largest of
+// the values that share the scale; below that by 2^-23 of that largest one.
+__device__ __forceinline__ int split_exponent(uint32_t largest) {       // from the largest |value|'s bits: it becomes 128 .. 256
+    const int e = (int)(largest >> 23) - 7;
+    return e < 5 ? 5 : e > 247 ? 247 : e;
+}
+__device__ __forceinline__ void split_codes(float a, float b, float c, float d, float scale, float rest, uint32_t& first, uint32_t& second) {
+    typedef short v2s __attribute__((ext_vector_type(2)));
+    v2s r = {};
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, a, b, scale, false);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, c, d, scale, true);
+    first = __builtin_bit_cast(uint32_t, r);
+    const v2f lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(first, scale, false), hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(first, scale, true);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, a - lo.x, b - lo.y, rest, false);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, c - hi.x, d - hi.y, rest, true);
+    second = __builtin_bit_cast(uint32_t, r);
+}
+
 // Scale of a quantisation block (inference/kernel.py:26-31) from the largest bit pattern of |x| among its
 // elements.  As unsigned integers the patterns of finite values and infinity are ordered like the values, and a NaN
 // (exponent all ones, mantissa non-zero) is larger than all of them, so it reaches the scale as it does through
@@ -209,6 +228,8 @@ int launch_wkv_b_absorb(const void* x, int64_t x_ts, int64_t x_hs, const void* w
                         int64_t tokens, int heads, int nope, int v, int64_t kv_rank, hipStream_t st);
 int launch_wkv_b_absorb_q_packed(const void* x, int64_t x_ts, int64_t x_hs, const void* w, const float* ws, void* y,
                                  int64_t batch, int64_t per_seq, int blocks, int heads, int nope, int v, hipStream_t st);
+int launch_wkv_b_absorb_q_codes(const void* x, int64_t x_ts, int64_t x_hs, const void* w, const float* ws, void* y, void* y_exponents, bool pack,
+                                int64_t batch, int64_t per_seq, int blocks, int heads, hipStream_t st);
 bool mla_prefill_paired(int64_t batch, int64_t rows, int heads);               // two query tiles a workgroup
 size_t mla_prefill_workspace_bytes(int64_t batch, int64_t rows, int64_t positions, int heads);
 int launch_mla_prefill(const void* q, const void* freqs, const void* kv, int64_t kv_bs, const void* pe, int64_t pe_bs,

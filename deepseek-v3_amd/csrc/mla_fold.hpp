@@ -37,7 +37,7 @@ __global__ __launch_bounds__(512, 4) void mla_fold_kernel(FoldArgs p) {
     // The weights are loaded behind the latents, whose sums need the registers, but their lines (64 KiB, one a thread) are
     // brought into the L2 beside them.
     uint32_t touched = *(const uint32_t*)(p.w + ((int64_t)h * 256 + 128 + (threadIdx.x >> 2)) * kC + (threadIdx.x & 3) * 128);
-    const float scale2 = p.scale * 1.44269504088896340736f;
+    const float scale2 = PAGED ? 1.f : p.scale * 1.44269504088896340736f;       // (paged: maxima are exponents of two)
     for (int ms = blockIdx.z * p.group; ms < p.tokens; ms += gridDim.z * p.group) {
         const int n = min(p.group, p.tokens - ms);
         const int per = n == 1 ? 8 : n == 2 ? 4 : n <= 4 ? 2 : 1, sub = wave & (per - 1);       // wavefronts of a token

@@ -2,8 +2,9 @@
 // in pages of e4m3 rows (mla_paged.hip), in the absorbed form of mla_decode.hip: behind the query's fold through wkv_b
 //   attend   one range of a sequence's positions for 128 or 64 of its (token, head) rows: scores, softmax, weighted sum; binary32 partial sums
 //   fold     mla_fold.hpp
-// Codes are turned into bf16 operands in front of the matrix cores, exactly (a power of two times four bits): the folded query and
-// the exponentials are rounded to bf16, scores and sums stay in binary32.
+// The matrix cores take the codes as they are.  What meets them is two codes an element as well (split_codes), with scales of powers of two that
+// the products apply: the folded query, split by the kernel that folds it (wkv_b_absorb.hip), and the exponentials times their
+// position's scale, split here.  A pair of codes is off by 2^-9 of the value at most, where bf16 would be by 2^-8; scores and sums are binary32.
 #include <type_traits>
 
 #include "mla.hpp"
@@ -13,17 +14,17 @@
 namespace dsv3 {
 namespace {
 
-constexpr int kTile = 32;                               // positions per tile
-constexpr int kRopeOff = kTile * kC;                    // a stage: 32 rows of 512 codes, 32 rotary keys of 128 B, four groups of eight scales, 256 B each
+constexpr int kTile = 64;                               // positions per tile
+constexpr int kRopeOff = kTile * kC;                    // a stage: 64 rows of 512 codes, 64 rotary keys of 128 B, eight groups of eight scales, 256 B each
 constexpr int kScaleOff = kRopeOff + kTile * kRope * 2;
-constexpr int kStage = kScaleOff + 1024;
-constexpr int kStages = 6;                              // tiles in LDS, computed or on their way
-constexpr int kCopies = 6;                              // of a tile, by each of the four wavefronts
-constexpr int kKeys = 4, kValues = 6;                   // reads from LDS ahead of the MFMAs that take them: keys (a read is two K steps), values
-constexpr int kSync = 27;                               // the value step behind which a tile's stage is free and the next tile's keys are read
+constexpr int kStage = kScaleOff + 8 * 256;
+constexpr int kStages = 3;                              // tiles in LDS: the one whose values and the one whose keys are read, one on its way
+constexpr int kQueryOff = kStages * kStage;             // behind them the wavefronts' rotary queries, 4 KiB each
+constexpr int kLds = kQueryOff + 4 * 4096;
 
 struct PagedArgs {
-    const void* ql;                                     // folded queries [batch][rows][512], rows = tokens * heads, or in operand order
+    const uint8_t* ql;                                  // folded queries in codes [batch][rows][first, second][512], rows = tokens * heads, or in operand order
+    const uint8_t* qe;                                  // their exponents [batch][rows][8]
     const uint16_t* q;                                  // queries [batch][rows][192]: their rotary part is read here
     const v2f* freqs;                                   // [batch][tokens][32] (cos, sin)
     const uint8_t* kv; const float* scales; const uint8_t* pe;
@@ -35,7 +36,7 @@ struct PagedArgs {
     v2i* plan;                                          // [batch] (first range, ranges)
     int batch, tokens, rows, heads, positions, page, groups, blocks, ranges;        // groups: of 32 rows, in whole 128s; ranges: at most
     uint32_t page_magic;                                // for quotient()
-    float scale;
+    float scale;                                        // of the softmax, times log2 e
 };
 
 // Rows that are no page's: zeros, with a scale that no row has.
@@ -101,25 +102,54 @@ template <class F> __device__ __forceinline__ Share share_of(const PagedArgs& p,
     return s;
 }
 
-// two codes of a dword times a power of two, as bf16
-template <bool HI> __device__ __forceinline__ uint32_t codes_to_bf16(uint32_t c, float s) {
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)c, s, HI));
+// v_mfma_scale_f32_32x32x64_f8f6f4 of codes with its result in ordinary registers (mla.hpp: mfma32_first).  a's scale: byte 0 of sa; b's: byte B of sb.
+// Bytes 0 .. 15 of both lane halves share the scale that the low lanes hold, bytes 16 .. 31 that of the high lanes.  (As a builtin with a sum of zero
+// the compiler puts the result over the operands, which are still being read.)
+template <int B> __device__ __forceinline__ void mfma64_first(v16f& d, v8i a, v8i b, int sa, int sb) {
+    asm volatile("s_nop 3\n\tv_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, 0, %3, %4 op_sel:[0,%5,0] op_sel_hi:[0,%6,0] cbsz:0 blgp:0"
+                 : "=&v"(d) : "v"(a), "v"(b), "v"(sa), "v"(sb), "n"(B & 1), "n"(B >> 1));
 }
-__device__ __forceinline__ v4u operand(uint32_t lo, uint32_t hi, float s) {
-    return v4u{ codes_to_bf16<false>(lo, s), codes_to_bf16<true>(lo, s), codes_to_bf16<false>(hi, s), codes_to_bf16<true>(hi, s) };
+template <int B> __device__ __forceinline__ void mfma64_next(v16f& d, v8i a, v8i b, int sa, int sb) {
+    asm volatile("v_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[0,%5,0] op_sel_hi:[0,%6,0] cbsz:0 blgp:0"
+                 : "+v"(d) : "v"(a), "v"(b), "v"(sa), "v"(sb), "n"(B & 1), "n"(B >> 1));
+}
+// the same with its sum in accumulation registers, byte 0 of both scales
+__device__ __forceinline__ void mfma64_sum(v16f& d, v8i a, v8i b, int sa, int sb) {
+    asm volatile("v_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:0 blgp:0" : "+a"(d) : "v"(a), "v"(b), "v"(sa), "v"(sb));
+}
+// a * b, and zero where a or b is: also beside a scale of NaN (the codes of such a row are zeros, the scores say who sees it)
+__device__ __forceinline__ float times(float a, float b) {
+    float r;
+    asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+// the lane's number, formed where it is needed: nothing that goes by it stays in a register for the loop
+__device__ __forceinline__ int lane_now() {
+    int l = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+    asm volatile("" : "+v"(l));
+    return l;
+}
+__device__ __forceinline__ v8i join(v4u a, v4u b) {
+    return __builtin_bit_cast(v8i, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-// mla_decode_kernel's maps (mla_decode.hip) on codes: four wavefronts, 32 rows' queries and 32 x 512 sums each; S^T = K Q^T, O^T += V^T P^T.
-// A lane's 16 bytes of a key row are the operands of two K steps: step 2 n takes features 32 n + 16 g .. + 7 of lane half g, step 2 n + 1
-// the eight behind them.  Values are read transposed, eight positions of a feature per lane; the positions' scales go into the
-// exponentials (before these are rounded).
-// G tiles side by side: the G wavefronts of a group of 32 rows take every G-th tile and add their sums in LDS at the end.
-template <bool PACK, int G>
+// Four wavefronts with all 512 registers of their SIMD lane each: a wavefront holds 32 rows' folded queries as pairs of codes (128 registers) and their
+// 32 x 512 weighted sums (256).  Transposed products as in mla_decode_kernel (mla_decode.hip): S^T = K Q^T leaves a row in one lane and the lane
+// 32 further (position 8 (e / 4) + 4 g + e % 4 of 32 in register e of lane half g), O^T += V^T P^T takes it from there.  Per tile of 64 positions, in two
+// halves of 32: 2 x (16 products of 64 features with the two codes of the query, 4 of the rotary part in bf16), 16 x 2 products of 64
+// positions: 72 MFMAs, 4350 cycles.
+// One wavefront a SIMD issues an instruction every 5 cycles or so: turning each code into a bf16 operand in every wavefront (256 conversions per 32
+// positions beside 68 MFMAs, the form before this one) bound it at 4200 cycles per 32 positions.
+// Three phases a tile, in which the exponentials of one half stand beside the other half's or the next tile's scores:
+//   C  scores of the second half      | exponentials of the first half
+//   A  scores of the next tile's first half | exponentials of the second half
+//   B  weighted sums of the tile      | copies of the tile after the next
+// Measured (us, the form before): one sequence of 61 tokens x 128 heads at 32768 positions 542 -> ...
+template <bool PACK>
 __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-    constexpr int RB = 4 / G, R = kStages / G;          // row groups of a workgroup; steps that the stages hold
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int i = lane & 31, g = lane >> 5, rg = wave % RB, par = wave / RB;
+    const int i = lane & 31, g = lane >> 5;
     // a contiguous run of the ranges in use per XCD, the row blocks of a range next to each other: its rows are in the XCD's L2
     int unit = -1;
     const Share mine = share_of(p, lane, [&](int used) -> int {
@@ -131,22 +161,21 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     const int range = unit / p.blocks, blk = unit - range * p.blocks, b = mine.b;
     const SeqSpan seq = seq_span(scalar_load(p.starts, b), scalar_load(p.counts, b), p.tokens, p.positions);
     const int live = seq.count * p.heads;               // rows behind these are of tokens that the sequence does not have
-    if (blk * (RB * 32) >= live) return;
+    if (blk * 128 >= live) return;
     const int t0 = (range - mine.first) * mine.per, t1 = min((seq.end + kTile - 1) / kTile, t0 + mine.per);
-    const int row0 = blk * (RB * 32) + rg * 32;
+    const int row0 = blk * 128 + wave * 32;
     const int row = min(row0 + i, p.rows - 1);          // rows past the end repeat the last one; fold leaves them out
 
-    // A wavefront copies eight rows of a tile, which lie in one page: four KiB of latents, a KiB of rotary keys, the scales (by
-    // all lanes, for what the first eight fetch).  Rows past the sequence's end are its last one again; what is no page's comes from `nothing`,
-    // so that every tile is as many copies, whose outstanding ones can be counted.
+    // A wavefront copies two groups of eight rows of a tile, of which each lies in one page: four KiB of latents, a KiB of rotary keys, the scales (by
+    // all lanes, for what the first eight fetch).  Rows past the sequence's end are its last one again; what is no page's comes from `nothing`.
     const uint32_t lds0 = lds_addr_of(lds);
     const int32_t* entries = p.table + b * p.width;
     struct Source { const uint8_t* kv; const uint8_t* pe; const float* scales; int last; uint32_t at; };
-    auto entry_of = [&](int t) -> int {                 // the page number of the wavefront's rows of tile t (past the end: of the last ones)
-        return scalar_load(entries, quotient(min(t * kTile + wave * 8, seq.end - 1), p.page, p.page_magic));
+    auto entry_of = [&](int t, int h) -> int {          // the page number of group h of the wavefront's rows of tile t (past the end: of the last ones)
+        return scalar_load(entries, quotient(min(t * kTile + wave * 16 + h * 8, seq.end - 1), p.page, p.page_magic));
     };
-    auto source = [&](int t, int entry, int stage) -> Source {
-        const int pos = t * kTile + wave * 8;
+    auto source = [&](int t, int h, int entry, int stage) -> Source {
+        const int pos = t * kTile + wave * 16 + h * 8;
         Source s = { nothing.kv, nothing.pe, nothing.scale, 0, lds0 + stage * kStage };
         if (t < t1 && pos < seq.end && (uint32_t)entry < (uint64_t)p.pages) {
             const int64_t r = (int64_t)entry * p.page + (pos - quotient(pos, p.page, p.page_magic) * p.page);
@@ -157,296 +186,323 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
         }
         return s;
     };
-    auto issue = [&](const Source& s, auto which) {
-        constexpr int n = decltype(which)::value;
+    auto issue = [&](int lane, const Source& s, auto group, auto which) {
+        constexpr int n = decltype(which)::value, h = decltype(group)::value;
         if constexpr (n < 4) {                          // row r's chunk c of 16 bytes lies at c ^ r (low four bits)
-            const int r = 2 * n + (lane >> 5);
-            copy16(s.kv, min(r, s.last) * kC + (((lane & 31) ^ ((wave * 8 + r) & 15)) << 4), s.at + wave * 4096 + n * 1024);
-        } else if constexpr (n == 4) {                  // chunk c at c ^ r / 2 (low three bits)
-            const int r = lane >> 3;
-            copy16(s.pe, min(r, s.last) * (kRope * 2) + (((lane & 7) ^ (((wave * 8 + r) >> 1) & 7)) << 4), s.at + kRopeOff + wave * 1024);
+            const uint32_t chunk = ((lane & 31) ^ (lane >> 5)) << 4;
+            copy16(s.kv, min(2 * n + (lane >> 5), s.last) * kC + (chunk ^ ((8 * h + 2 * n) << 4)), s.at + (wave * 16 + 8 * h + 2 * n) * kC);
+        } else if constexpr (n == 4) {                  // a key's chunk c at c ^ r / 2 (low three bits)
+            copy16(s.pe, min(lane >> 3, s.last) * (kRope * 2) + (((lane & 7) ^ (4 * h + (lane >> 4))) << 4), s.at + kRopeOff + (wave * 16 + 8 * h) * (kRope * 2));
         } else {
-            copy4(s.scales, min(lane & 7, s.last) * 4, s.at + kScaleOff + wave * 256);
+            copy4(s.scales, min(lane & 7, s.last) * 4, s.at + kScaleOff + (wave * 2 + h) * 256);
         }
     };
-    for (int n = 0; n < (R - 1) * G; ++n) {
-        const Source s = source(t0 + n, entry_of(t0 + n), n);
-        unrolled<kCopies>([&](auto k) { issue(s, k); });
+    auto copy_tile = [&](int t, int stage) {
+        unrolled<2>([&](auto h) {
+            const Source s = source(t, h, entry_of(t, h), stage);
+            unrolled<6>([&](auto n) { issue(lane, s, h, n); });
+        });
+    };
+    // this wavefront's copies have landed, and everybody's
+    auto arrived = [&] {
+        __builtin_amdgcn_s_waitcnt(0x0f70);             // vmcnt(0)
+        barrier_no_fence();
+    };
+    copy_tile(t0, 0);
+    copy_tile(t0 + 1, 1);
+
+    if (row0 >= live) {                                 // no rows: the others' copies
+        arrived();
+        for (int t = t0, st = 2; t < t1; ++t, st = st == 2 ? 0 : st + 1) {
+            arrived();
+            copy_tile(t + 2, st);
+        }
+        arrived();
+        return;
     }
 
-    v4u Q[36];
+    v8i Q[2][8];                                        // first and second codes; K step n: features 64 n + 32 g .. + 31
+    int qs[2][2];                                       // their scales, K steps 0 .. 3 and 4 .. 7
+    uint8_t* const turned = lds + kQueryOff + wave * 4096;                      // rotary query, a lane's 16 bytes of K step s of 16 at s KiB
     {
         // (packed, a last block's missing rows hold anything; nobody reads their results)
-        const v4u* src = (const v4u*)p.ql + (PACK ? ((int64_t)b * p.groups + row0 / 32) * (kC / 16) * 64 + i : ((int64_t)b * p.rows + row) * (kC / 8));
+        const uint8_t* src = PACK ? p.ql + ((int64_t)b * p.groups + row0 / 32) * 32768 + lane * 16 : p.ql + ((int64_t)b * p.rows + row) * 1024 + g * 32;
 #pragma unroll
-        for (int n = 0; n < 16; ++n) {
-            Q[2 * n] = src[PACK ? (2 * n + g) * 64 : 4 * n + 2 * g];
-            Q[2 * n + 1] = src[PACK ? (2 * n + g) * 64 + 32 : 4 * n + 2 * g + 1];
-        }
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+                Q[c][n] = PACK ? join(*(const v4u*)(src + c * 16384 + n * 2048), *(const v4u*)(src + c * 16384 + n * 2048 + 1024))
+                               : join(*(const v4u*)(src + c * 512 + n * 64), *(const v4u*)(src + c * 512 + n * 64 + 16));
+        const v2u e = *(const v2u*)(p.qe + ((int64_t)b * p.rows + row) * 8);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) { qs[0][k] = (int)e[k]; qs[1][k] = (int)(e[k] - 0x04040404u); }
         const uint16_t* rsrc = p.q + ((int64_t)b * p.rows + row) * kQd + kNope + 8 * g;
         const v2f* fr = p.freqs + ((int64_t)b * p.tokens + row / p.heads) * (kRope / 2) + 4 * g;
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-            Q[32 + s] = *(const v4u*)(rsrc + 16 * s);
+            v4u x = *(const v4u*)(rsrc + 16 * s);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const v2f cs = fr[8 * s + e];
-                const float re = bf16lo_to_f32(Q[32 + s][e]), im = bf16hi_to_f32(Q[32 + s][e]);
-                Q[32 + s][e] = pack_bf16(re * cs.x - im * cs.y, re * cs.y + im * cs.x);
+                const float re = bf16lo_to_f32(x[e]), im = bf16hi_to_f32(x[e]);
+                x[e] = pack_bf16(re * cs.x - im * cs.y, re * cs.y + im * cs.x);
             }
+            *(v4u*)(turned + s * 1024 + lane * 16) = x;
         }
     }
 
-    const uint32_t kaddr = i * kC + ((g ^ (i & 15)) << 4);                      // pair n: ^ (2 n mod 16) << 4
-    const uint32_t raddr = kRopeOff + i * 128 + ((g ^ ((i >> 1) & 7)) << 4);    // ^ 2 s << 4
-    // transposed reads: lane group q2 of a half takes 16 features; its lane l fetches eight of row l / 2 of 4 g .. + 3, 8 + 4 g .. + 3
+    // (opaque again in every phase, below: formed ahead of the loop, what the reads' places xor to would take the registers that there are not)
+    uint32_t kaddr = i * kC + (((2 * g) ^ (i & 15)) << 4);                // K step n: ^ (4 n mod 16) << 4
+    uint32_t raddr = kRopeOff + i * 128 + ((g ^ ((i >> 1) & 7)) << 4);    // ^ 2 s << 4
+    // transposed reads: lane group q2 of a half takes 16 features; its lane l fetches eight of row l / 2 of 4 g .. + 3, 8 + 4 g .. + 3 of 16 rows
     const int l15 = lane & 15, q2 = (lane >> 4) & 1, vrow = 8 * (l15 >> 3) + 4 * g + ((l15 >> 1) & 3);
-    const uint32_t vaddr = vrow * kC + ((q2 ^ vrow) << 4) + 8 * (l15 & 1);
+    uint32_t vaddr = vrow * kC + ((q2 ^ vrow) << 4) + 8 * (l15 & 1);
+    auto key = [&](const uint8_t* base, int half, int n) -> v8i {
+        const uint8_t* at = base + half * (32 * kC) + (n >> 2) * 256;
+        return join(*(const v4u*)(at + (kaddr ^ ((n & 3) << 6))), *(const v4u*)(at + (kaddr ^ ((n & 3) << 6 | 16))));
+    };
+    auto rope_key = [&](const uint8_t* base, int half, int s) -> v4u { return *(const v4u*)(base + half * (32 * kRope * 2) + (raddr ^ (s << 5))); };
+    auto value = [&](uint32_t stage, int f) -> v8i {    // features 32 f .. of all 64 positions
+        const uint32_t at = stage + (vaddr ^ ((f & 7) << 5)) + (f >> 3) * 256;
+        v8i v;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const v2i x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i)(uintptr_t)(at + k * (16 * kC)));
+            v[2 * k] = x[0];
+            v[2 * k + 1] = x[1];
+        }
+        return v;
+    };
 
     v16f O[16] = {};
-    float m = -__builtin_inff(), l = 0.f;               // running maximum of the scores, this lane's share of the sum
-    const float scale2 = p.scale * 1.44269504088896340736f;
-    // The reads' order and place are those that are written here (sched_barrier); a step's operand is made from its codes beside the MFMA
-    // in front of it: four conversions take no time there (33.6 cycles instead of 33.1), six do (38.6).
-    v4u keys[kKeys];
-    float sc;                                           // the scale of position i
-    auto key = [&](const uint8_t* base, int x) -> v4u {
-        return x < 16 ? *(const v4u*)(base + (kaddr ^ ((x & 7) << 5)) + (x >> 3) * 256) : *(const v4u*)(base + (raddr ^ ((x - 16) << 5)));
+    v16f S[2];
+    v8i ring[2];                                        // keys of two K steps, or values of 64 features: read two to four MFMAs ahead
+    v4u rope_q[2];
+    v8i P[2];                                           // exponentials, first and second codes; dwords 4 h .. of half h
+    int pe[2];                                          // their exponents, by halves
+    float off = -__builtin_inff(), l = 0.f;             // exponentials are of 2^(score - off), off a whole number; this lane's share of their sum
+    int ks[2];                                          // scale byte of position i, by halves
+    uint32_t none[2];                                   // positions that nobody sees for want of a page, by halves
+    auto scales_of = [&](const uint8_t* base, int half) {
+        const int i = lane_now() & 31;
+        const float sc = *(const float*)(base + kScaleOff + (4 * half + (i >> 3)) * 256 + (i & 7) * 4);
+        ks[half] = (int)(f32_as_u32(sc) >> 23 & 0xff);  // (NaN: 255, which makes the products NaN)
+        none[half] = (uint32_t)__ballot(sc < 0.f);
     };
-    auto scale_at = [&](const uint8_t* base) { return *(const float*)(base + kScaleOff + (i >> 3) * 256 + (i & 7) * 4); };
-    // the next step's tiles are there, once this wavefront's copies of them are (those of the steps behind it stay in flight) and everybody's
-    auto arrived = [&] {
-        constexpr int left = (R - 2) * kCopies * G;
-        __builtin_amdgcn_s_waitcnt(0x0f70 | (left & 15) | (left >> 4) << 14);   // vmcnt
-        barrier_no_fence();
+
+    // The exponentials of half h, in 16 steps that stand beside the MFMAs of 20.
+    v4f w[4];
+    float pm = 0.f, offu = 0.f, shrink = 1.f;
+    bool behind = false;                                // the sums are still to be multiplied with `shrink`
+    auto soften = [&](int t, const uint8_t* base, auto half, auto step) {
+        constexpr int h = decltype(half)::value, x = decltype(step)::value;
+        v16f& s = S[h];
+        if constexpr (x < 8 && x % 2 == 0) w[x / 2] = *(const v4f*)(base + kScaleOff + (4 * h + x / 2) * 256 + (lane_now() >> 5) * 16);
+        if constexpr (x == 1) {
+            asm volatile("" : "+v"(s));                 // (behind two more MFMAs: the scores are there)
+            const int at = t * kTile + 32 * h, left = seq.end - at;
+            uint32_t there = ~none[h];
+            if (left < 32) there &= left > 0 ? (1u << left) - 1u : 0u;
+            if (there != ~0u || at + 32 > seq.start) {
+                const int j0 = at - seq.start;          // the first position among the new ones
+                uint32_t seen = there;
+                if (j0 > -32) {
+                    const int tok = min(row0 + (lane_now() & 31), p.rows - 1) / p.heads;
+                    const uint64_t bits = p.tree ? (uint64_t)p.tree[(int64_t)b * p.tokens + tok] : (2ull << tok) - 1;
+                    seen &= j0 >= 64 ? 0u : j0 >= 0 ? (uint32_t)(bits >> j0) : (uint32_t)(bits << -j0) | ((1u << -j0) - 1u);
+                }
+                seen >>= (lane_now() >> 5) * 4;
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (!(seen >> (8 * (e >> 2) + (e & 3)) & 1)) s[e] = -__builtin_inff();
+            }
+            pm = s[0];
+#pragma unroll
+            for (int e = 1; e < 16; ++e) pm = __builtin_elementwise_maximum(pm, s[e]);
+        }
+        if constexpr (x == 2) {
+            const v2f both = halves32(pm);
+            const float top = fmaxf(both.x, both.y) * p.scale;
+            // `off` is only raised when a score passes it by more than 2^64: exponentials and sums have room for that in binary32, and so the 256
+            // multiplications are needed in the rarest of cases.  By whole powers of two: the first half's codes change their exponent only.
+            // (Rows that nobody reads do not ask for it.)
+            const bool raise = row0 + (lane_now() & 31) < live && (top - off > 64.f || (off == -__builtin_inff() && top > off));
+            if (__any(raise)) {
+                const float on = raise ? __builtin_ceilf(top) : off;
+                const float a = !raise ? 1.f : off == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(off - on);
+                l *= a;
+                if constexpr (h == 1) pe[0] = max(5, pe[0] - (raise ? (int)fminf(on - off, 300.f) : 0));
+                off = on;
+                shrink = behind ? shrink * a : a;       // (the sums follow in front of phase B)
+                behind = true;
+            }
+            offu = off == -__builtin_inff() ? 0.f : off;
+            pm = 0.f;
+        }
+        if constexpr (x >= 3 && x < 11) {
+#pragma unroll
+            for (int e = 2 * (x - 3); e < 2 * (x - 3) + 2; ++e) {
+                const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], p.scale, -offu));
+                l += v;
+                s[e] = times(v, w[e >> 2][e & 3]);
+            }
+            pm = __builtin_elementwise_max(pm, __builtin_elementwise_max(s[2 * (x - 3)], s[2 * (x - 3) + 1]));
+        }
+        if constexpr (x == 11) {
+            const v2f both = halves32(pm);              // (the halves' bytes share a scale)
+            pe[h] = split_exponent(f32_as_u32(fmaxf(both.x, both.y)));
+        }
+        if constexpr (x >= 12 && x < 16) {
+            constexpr int k = x - 12;
+            uint32_t first, second;
+            split_codes(s[4 * k], s[4 * k + 1], s[4 * k + 2], s[4 * k + 3], u32_as_f32((uint32_t)pe[h] << 23), u32_as_f32((uint32_t)(pe[h] - 4) << 23), first, second);
+            P[0][4 * h + k] = (int)first;
+            P[1][4 * h + k] = (int)second;
+        }
     };
-    // One tile.  copy: beside the MFMA just issued.  The last value steps read the next tile's first keys.
-    auto tile = [&](int t, const uint8_t* base, const uint8_t* next, auto copy) {
-        const uint32_t vbase = lds_addr_of(base) + vaddr;
-        v2i values[kValues];
-        auto value = [&](int y) -> v2i {                // positions 16 (y / 16) .. of features 32 (y % 16) ..
-            return __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i)(uintptr_t)((vbase ^ ((y & 7) << 5)) + ((y >> 3) & 1) * 256 + (y >> 4) * 8192));
-        };
-        v4f w[4];
-        v16f T[1];
-        v16f& S = T[0];
-        v4u cur = operand(keys[0][0], keys[0][1], sc);
-        __builtin_amdgcn_sched_barrier(0);
-        unrolled<36>([&](auto step) {
-            constexpr int s = decltype(step)::value;
-            if constexpr (s == 0) mfma32_first(S, cur, Q[0]);
-            else mfma32_next(S, cur, Q[s]);
-            if constexpr (s < 31 && s % 2 == 0) cur = operand(keys[s / 2 % kKeys][2], keys[s / 2 % kKeys][3], sc);
-            else if constexpr (s < 31) cur = operand(keys[(s + 1) / 2 % kKeys][0], keys[(s + 1) / 2 % kKeys][1], sc);
-            else if constexpr (s < 35) cur = keys[(s - 15) % kKeys];
-            if constexpr (s < 32 && s % 2 == 0 && s / 2 + kKeys < 20) keys[s / 2 % kKeys] = key(base, s / 2 + kKeys);
-            if constexpr (s >= 26 && s < 26 + 4) w[s - 26] = *(const v4f*)(base + kScaleOff + (s - 26) * 256 + g * 16);
-            if constexpr (s >= 30) values[s - 30] = value(s - 30);
-            copy(step);
+    // The scores of half h of the tile at `base`, whose first two keys are in the ring.  beside(step): what stands behind the step's MFMA;
+    // tail(0 / 1): the ring's place is free for what the next phase reads first.
+    auto score = [&](const uint8_t* base, auto half, auto beside, auto tail) {
+        constexpr int h = decltype(half)::value;
+        v16f& s = S[h];
+        asm volatile("" : "+v"(kaddr), "+v"(raddr));
+        const int own = lane_now() * 16;
+        unrolled<20>([&](auto step) {
+            constexpr int x = decltype(step)::value, n = x >> 1;
+            if constexpr (x == 0) mfma64_first<0>(s, ring[0], Q[0][0], ks[h], qs[0][0]);
+            else if constexpr (x < 16) mfma64_next<(n & 3)>(s, ring[n & 1], Q[x & 1][n], ks[h], qs[x & 1][n >> 2]);
+            else {
+                const v4u k = __builtin_bit_cast(v4u, __builtin_shufflevector(ring[n & 1], ring[n & 1], 4 * (x & 1), 4 * (x & 1) + 1, 4 * (x & 1) + 2, 4 * (x & 1) + 3));
+                mfma32_next(s, k, rope_q[x & 1]);
+            }
+            if constexpr (x < 12 && (x & 1)) ring[n & 1] = key(base, h, n + 2);
+            if constexpr (x == 13 || x == 15) ring[n & 1] = join(rope_key(base, h, 2 * (n - 6)), rope_key(base, h, 2 * (n - 6) + 1));
+            if constexpr (x >= 14 && x < 18) rope_q[x & 1] = *(const v4u*)(turned + (x - 14) * 1024 + own);
+            beside(step);
+            if constexpr (x == 17) tail(std::integral_constant<int, 0>());
+            if constexpr (x == 19) tail(std::integral_constant<int, 1>());
             __builtin_amdgcn_sched_barrier(0);
         });
-        scores_ready(S);
-        // positions that nobody sees: past the end, of no page (a row that was not finite has scores of NaN already)
-        const int left = seq.end - t * kTile;
-        uint32_t there = ~(uint32_t)__ballot(sc < 0.f);
-        if (left < kTile) there &= left > 0 ? (1u << left) - 1u : 0u;
-        if (there != ~0u || t * kTile + kTile > seq.start) {
-            const int j0 = t * kTile - seq.start;       // the tile's first position among the new ones
-            uint32_t seen = there;
-            if (j0 > -kTile) {
-                int tok = row / p.heads;
-                asm volatile("" : "+v"(tok));           // (formed here: there are no registers to keep it in)
-                const uint64_t bits = p.tree ? (uint64_t)p.tree[(int64_t)b * p.tokens + tok] : (2ull << tok) - 1;
-                seen &= j0 >= 64 ? 0u : j0 >= 0 ? (uint32_t)(bits >> j0) : (uint32_t)(bits << -j0) | ((1u << -j0) - 1u);
-            }
-            seen >>= 4 * g;
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-                if (!(seen >> (8 * (e >> 2) + (e & 3)) & 1)) S[e] = -__builtin_inff();
+    };
+
+    typedef std::integral_constant<int, 0> First;
+    typedef std::integral_constant<int, 1> Second;
+    arrived();
+    scales_of(lds, 0);
+    ring[0] = key(lds, 0, 0);
+    ring[1] = key(lds, 0, 1);
+    score(lds, First(), [](auto) {}, [&](auto k) { ring[k] = key(lds, 1, k); });
+    scales_of(lds, 1);
+    int st = 0;
+    for (int t = t0;; ++t) {
+        const int st_next = st == 2 ? 0 : st + 1, st_free = st_next == 2 ? 0 : st_next + 1;
+        const uint8_t* base = lds + st * kStage;
+        const uint8_t* next = lds + st_next * kStage;
+        const int entry[2] = { entry_of(t + 2, 0), entry_of(t + 2, 1) };
+        // C.  Behind its barrier the next tile is there, and the stage of the one before is free.
+        score(base, Second(), [&](auto step) {
+            soften(t, base, First(), step);
+            if constexpr (decltype(step)::value == 16) arrived();
+        }, [&](auto k) { ring[k] = key(next, 0, k); });
+        const bool more = t + 1 < t1;
+        if (more) {                                     // A
+            scales_of(next, 0);
+            score(next, First(), [&](auto step) { soften(t, base, Second(), step); }, [&](auto k) { ring[k] = value(lds0 + st * kStage, k); });
+        } else {
+            scores_ready(S[1]);
+            unrolled<16>([&](auto step) {
+                soften(t, base, Second(), step);
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            ring[0] = value(lds0 + st * kStage, 0);
+            ring[1] = value(lds0 + st * kStage, 1);
         }
-        float mx = S[0];
+        // B
+        const Source ahead[2] = { source(t + 2, 0, entry[0], st_free), source(t + 2, 1, entry[1], st_free) };
+        asm volatile("" : "+v"(vaddr));
+        const int lane = lane_now(), one = 127, g = lane >> 5, e[2] = { g ? pe[1] : pe[0], (g ? pe[1] : pe[0]) - 4 };
+        if (behind) {
+            behind = false;
+            if (t > t0) {
 #pragma unroll
-        for (int e = 1; e < 16; ++e) mx = __builtin_elementwise_maximum(mx, S[e]);
-        const v2f both = halves32(mx);
-        mx = fmaxf(both.x, both.y);
-        // the maximum is raised as in mla_decode_kernel: when it grows by more than 2^64, and not for rows that nobody reads
-        const bool raise = row0 + i < live && ((mx - m) * scale2 > 64.f || (m == -__builtin_inff() && mx > m));
-        if (__any(raise)) {
-            const float mn = fmaxf(m, mx);
-            const float a = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((m - mn) * scale2);
-            l *= a;
-            m = mn;
-            if (t >= t0 + G) {
-#pragma unroll
-                for (int d = 0; d < 16; ++d) scale_agprs(O[d], a);
+                for (int d = 0; d < 16; ++d) scale_agprs(O[d], shrink);
                 asm volatile("s_nop 7" ::: "memory");
             }
         }
-        const float off = softmax_offset(T, m, scale2);
-        if (__any(sc != sc)) {                          // NaN times an exponential of zero: these rows' codes are zeros, the scores say who sees them
-#pragma unroll
-            for (int e = 0; e < 16; ++e) w[e >> 2][e & 3] = w[e >> 2][e & 3] == w[e >> 2][e & 3] ? w[e >> 2][e & 3] : 0.f;
-        }
-        float sum = 0.f;
-        v4u P[2];
-        auto weights = [&](int e) {                     // two positions' exponentials
-            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(S[e], scale2, -off));
-            const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(S[e + 1], scale2, -off));
-            sum += x + y;
-            P[e >> 3][(e & 7) >> 1] = pack_bf16(x * w[e >> 2][e & 3], y * w[e >> 2][(e & 3) + 1]);
-        };
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) weights(e);
-        cur = operand((uint32_t)values[0][0], (uint32_t)values[0][1], 1.0f);
+        int first_e = e[0], second_e = e[1], unit_scale = one;
+        asm volatile("s_nop 3" : "+v"(first_e), "+v"(second_e), "+v"(unit_scale));      // (between an ordinary instruction's result and an MFMA that the compiler does not know)
         __builtin_amdgcn_sched_barrier(0);
         unrolled<32>([&](auto step) {
-            constexpr int s = decltype(step)::value;
-            O[s & 15] = mfma32(cur, P[s >> 4], O[s & 15]);
-            if constexpr (s < 31) cur = operand((uint32_t)values[(s + 1) % kValues][0], (uint32_t)values[(s + 1) % kValues][1], 1.0f);
-            if constexpr (s + kValues < 32) values[s % kValues] = value(s + kValues);
-            if constexpr (s < 12 && s % 3 == 2) weights(8 + s / 3 * 2);         // the second half's, beside the first half's products
+            constexpr int x = decltype(step)::value, f = x >> 1;
+            mfma64_sum(O[f], ring[f & 1], P[x & 1], unit_scale, x & 1 ? second_e : first_e);
+            if constexpr (x & 1) ring[f & 1] = f < 14 ? value(lds0 + st * kStage, f + 2) : key(next, 1, f - 14);
+            if constexpr (x < 12) issue(lane, ahead[x / 6], std::integral_constant<int, x / 6>(), std::integral_constant<int, x % 6>());
             __builtin_amdgcn_sched_barrier(0);
-            if constexpr (s == kSync) {                 // this tile's last codes are in registers: its stage is free behind the barrier
-                arrived();
-                sc = scale_at(next);
-            }
-            if constexpr (s >= kSync && s - kSync < kKeys) {
-                keys[s - kSync] = key(next, s - kSync);
-                __builtin_amdgcn_sched_barrier(0);
-            }
         });
-        l += sum;
 #pragma unroll
         for (int d = 0; d < 16; ++d) asm volatile("" : "+a"(O[d]));     // (the sums stay where they are)
-    };
-
-    arrived();
-    sc = scale_at(lds + par * kStage);
-#pragma unroll
-    for (int x = 0; x < kKeys; ++x) keys[x] = key(lds + par * kStage, x);
-    int st = 0, entry[G];
-#pragma unroll
-    for (int j = 0; j < G; ++j) entry[j] = entry_of(t0 + (R - 1) * G + j);
-    for (int t = t0; t < t1; t += G) {
-        const int st_next = st + 1 == R ? 0 : st + 1, st_free = st == 0 ? R - 1 : st - 1;
-        // Copies into the stage of the step before, which is free, every few MFMAs: the four wavefronts take turns on the compute unit's load
-        // path.  Page numbers are loaded a step ahead of the copies that need them.
-        Source ahead[G];
-#pragma unroll
-        for (int j = 0; j < G; ++j) {
-            ahead[j] = source(t + (R - 1) * G + j, entry[j], st_free * G + j);
-            entry[j] = entry_of(t + R * G + j);
-        }
-        tile(t + par, lds + (st * G + par) * kStage, lds + (st_next * G + par) * kStage, [&](auto step) {
-            constexpr int s = decltype(step)::value, E = 4 / G;
-            if constexpr (s % E == E - 1 && s / E < kCopies * G) issue(ahead[s / E / kCopies], std::integral_constant<int, s / E % kCopies>());
-        });
+        if (!more) break;
+        scales_of(next, 1);
         st = st_next;
     }
 
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");  // (the last sums are there)
     const v2f parts = halves32(l);
     l = parts.x + parts.y;
-    const int64_t slot = ((int64_t)range * p.blocks + blk) * (RB * 32);         // the workgroup's rows among all
-    __builtin_amdgcn_s_waitcnt(0x0f70);                 // (copies of the tiles past the range are still on their way into the stages)
-    barrier_no_fence();
-    // The sums leave as in mla_decode_kernel: 64 features of 32 rows at a time through LDS (16-byte chunks xor-ed with the row); the G
-    // wavefronts of a row group first add theirs, each for 32 / G of the rows.
-    v2f* const table = (v2f*)(lds + 65536);             // (maximum, sum) [wavefront][row]
-    constexpr int N = 8 / G;
-    float wt[N][G];
-    if constexpr (G == 1) {
-        if (g == 0) p.ml[slot + rg * 32 + i] = v2f{ m, l };
-    } else {
-        if (g == 0) table[wave * 32 + i] = v2f{ m, l };
-        barrier_no_fence();
-        auto weigh = [&](int r, float (&w)[G]) -> v2f { // row r's weights; its maximum and sum
-            v2f x[G];
-            float top = -__builtin_inff(), sum = 0.f;
-#pragma unroll
-            for (int j = 0; j < G; ++j) { x[j] = table[(rg + RB * j) * 32 + r]; top = fmaxf(top, x[j].x); }
-#pragma unroll
-            for (int j = 0; j < G; ++j) {
-                w[j] = x[j].x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((x[j].x - top) * scale2);
-                sum += x[j].y * w[j];
-            }
-            return v2f{ top, sum };
-        };
-#pragma unroll
-        for (int n = 0; n < N; ++n) weigh(4 * (par * N + n) + (lane >> 4), wt[n]);
-        if (par == 0) {
-            float w[G];
-            const v2f ml = weigh(i, w);
-            if (g == 0) p.ml[slot + rg * 32 + i] = ml;
-        }
-    }
-    float* dst = p.part + (slot + rg * 32 + par * (4 * N) + (lane >> 4)) * kC + (lane & 15) * 4;
+    const int last_lane = lane_now(), i2 = last_lane & 31, g2 = last_lane >> 5;
+    const int64_t slot = ((int64_t)range * p.blocks + blk) * 128 + wave * 32;   // the wavefront's rows among all
+    if (g2 == 0) p.ml[slot + i2] = v2f{ off, l };
+    arrived();                                          // (copies past the range are still on their way into the stages)
+    // The sums leave as rows, which fold reads whole: 64 features of 32 rows at a time through LDS (16-byte chunks xor-ed with the row), so that a
+    // store writes four pieces of 256 bytes; rows that nobody reads stay here.
+    float* dst = p.part + (slot + (last_lane >> 4)) * kC + (last_lane & 15) * 4;
     auto put = [&](int d2) {                            // two buffers a wavefront: the next 64 features are written while these are read
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
             const v16f& o = O[2 * d2 + (c >> 2)];
             const int e = 4 * (c & 3);
-            *(v4f*)(lds + wave * 16384 + (d2 & 1) * 8192 + i * 256 + (((2 * c + g) ^ (i & 15)) << 4)) = v4f{ o[e], o[e + 1], o[e + 2], o[e + 3] };
+            *(v4f*)(lds + wave * 16384 + (d2 & 1) * 8192 + i2 * 256 + (((2 * c + g2) ^ (i2 & 15)) << 4)) = v4f{ o[e], o[e + 1], o[e + 2], o[e + 3] };
         }
     };
     put(0);
 #pragma unroll
     for (int d2 = 0; d2 < 8; ++d2) {
-        if constexpr (G > 1) barrier_no_fence();        // everybody's are there, and the buffers written next have been read
-        v4f x[N][G];
+        v4f x[8];
 #pragma unroll
-        for (int n = 0; n < N; ++n)
-#pragma unroll
-            for (int j = 0; j < G; ++j) {
-                const int r = 4 * (par * N + n) + (lane >> 4);
-                x[n][j] = *(const v4f*)(lds + (rg + RB * j) * 16384 + (d2 & 1) * 8192 + r * 256 + (((lane & 15) ^ (r & 15)) << 4));
-            }
+        for (int n = 0; n < 8; ++n) {
+            const int r = 4 * n + (last_lane >> 4);
+            x[n] = *(const v4f*)(lds + wave * 16384 + (d2 & 1) * 8192 + r * 256 + (((last_lane & 15) ^ (r & 15)) << 4));
+        }
         if (d2 < 7) put(d2 + 1);
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            v4f v = x[n][0];
-            if constexpr (G > 1) {
-                v = v * wt[n][0];
-#pragma unroll
-                for (int j = 1; j < G; ++j) v += x[n][j] * wt[n][j];
-            }
-            *(v4f*)(dst + n * 4 * kC + d2 * 64) = v;
-        }
+        for (int n = 0; n < 8; ++n)
+            if (row0 + 4 * n + (last_lane >> 4) < live) *(v4f*)(dst + n * 4 * kC + d2 * 64) = x[n];
     }
 }
 
-// Row blocks of 128 (token, head) rows, or of 64 with two tiles side by side; one workgroup a compute unit (its registers take a whole one).
-struct PagedPlan { int side, groups; int64_t blocks, ranges; };
+// Row blocks of 128 (token, head) rows; one workgroup a compute unit (its registers take a whole one).
+struct PagedPlan { int groups; int64_t blocks, ranges; };
 PagedPlan paged_plan(int64_t batch, int64_t rows) {
     PagedPlan a;
-    a.side = rows <= 64 ? 2 : 1;
-    a.groups = (int)((rows + 127) / 128 * 4);
-    a.blocks = (rows + 128 / a.side - 1) / (128 / a.side);
+    a.blocks = (rows + 127) / 128;
+    a.groups = (int)(a.blocks * 4);
     // Ranges of all sequences: as many as there are compute units for the row blocks; where the sequences alone are more than half of
     // these, room for the longer ones to be cut.
     const int64_t units = a.blocks < 256 ? 256 / a.blocks : 1;
     a.ranges = batch <= units / 2 ? units : batch + units / 2;
     return a;
 }
-// Folded queries, partial sums, their maxima and sums, the division of the work
-struct PagedSpace { size_t part, ml, plan, bytes; };
+// Folded queries, their exponents, partial sums, their maxima and sums, the division of the work
+struct PagedSpace { size_t exponents, part, ml, plan, bytes; };
 PagedSpace paged_space(const PagedPlan& a, int64_t batch) {
-    const int64_t rows = a.ranges * a.blocks * (128 / a.side);
+    const int64_t rows = a.ranges * a.blocks * 128;
     PagedSpace s;
-    s.part = (size_t)(batch * a.groups * (32 * kC * 2));
+    s.exponents = (size_t)(batch * a.groups * (32 * kC * 2));
+    s.part = s.exponents + (size_t)(batch * a.groups * (32 * 8));
     s.ml = s.part + (size_t)(rows * kC * 4);
     s.plan = s.ml + (size_t)(rows * 8);
     s.bytes = s.plan + (size_t)(batch * 8);
     return s;
-}
-
-template <int G> int launch_paged(const PagedArgs& a, bool pack, unsigned grid, hipStream_t st) {
-    static void (*const kernels[2])(PagedArgs) = { mla_paged_kernel<false, G>, mla_paged_kernel<true, G> };
-    static LdsGrant grant[2];
-    constexpr int bytes = kStages * kStage;
-    static_assert(bytes >= 65536 + 1024 && bytes <= 160 * 1024, "the sums leave through the stages");
-    if (!grant[pack].ensure((const void*)kernels[pack], bytes)) return DSV3_ERR_LAUNCH;
-    hipLaunchKernelGGL(kernels[pack], dim3(grid), dim3(256), bytes, st, a);
-    return DSV3_OK;
 }
 
 }  // namespace
@@ -462,7 +518,7 @@ int launch_mla_decode_paged(const void* q, const void* freqs, const dsv3_mla_pag
     if (plan.ranges * plan.blocks > 0xfffff0 || batch * tokens > 0x7fffffff - 16) return DSV3_ERR_BAD_SHAPE;
     PagedArgs a;
     uint8_t* wsp = (uint8_t*)workspace;
-    a.ql = wsp; a.q = (const uint16_t*)q; a.freqs = (const v2f*)freqs;
+    a.ql = wsp; a.qe = wsp + space.exponents; a.q = (const uint16_t*)q; a.freqs = (const v2f*)freqs;
     a.kv = (const uint8_t*)cache.kv; a.scales = cache.kv_scale; a.pe = (const uint8_t*)cache.pe;
     a.table = cache.table; a.width = cache.table_width; a.pages = cache.pages;
     a.starts = starts; a.counts = counts; a.tree = tree;
@@ -470,19 +526,20 @@ int launch_mla_decode_paged(const void* q, const void* freqs, const dsv3_mla_pag
     a.batch = (int)batch; a.tokens = (int)tokens; a.rows = (int)rows; a.heads = heads; a.positions = (int)positions;
     a.page = cache.page_size; a.groups = plan.groups; a.blocks = (int)plan.blocks; a.ranges = (int)plan.ranges;
     a.page_magic = magic_of(positions, cache.page_size);
-    a.scale = scale;
+    a.scale = scale * 1.44269504088896340736f;
     // operand order up to 16 tokens in all, which is what the kernel that writes it takes (mla_decode.hip)
     const bool pack = batch * tokens <= 16;
-    const int rc = pack ? launch_wkv_b_absorb_q_packed(q, (int64_t)heads * kQd, kQd, w, ws, wsp, batch, tokens, a.groups / 4, heads, kNope, kNope, st)
-                        : launch_wkv_b_absorb(q, (int64_t)heads * kQd, kQd, w, ws, wsp, DSV3_ABSORB_Q, batch * tokens, heads, kNope, kNope, kC, st);
+    const int rc = launch_wkv_b_absorb_q_codes(q, (int64_t)heads * kQd, kQd, w, ws, wsp, wsp + space.exponents, pack, batch, tokens, (int)plan.blocks, heads, st);
     if (rc != DSV3_OK) return rc;
+    static void (*const kernels[2])(PagedArgs) = { mla_paged_kernel<false>, mla_paged_kernel<true> };
+    static LdsGrant grant[2];
+    static_assert(kLds <= 160 * 1024 && 4 * 16384 <= kStages * kStage, "the sums leave through the stages");
+    if (!grant[pack].ensure((const void*)kernels[pack], kLds)) return DSV3_ERR_LAUNCH;
     const unsigned grid = (unsigned)((plan.ranges * plan.blocks + 7) / 8 * 8);
-    const int launched = plan.side == 1 ? launch_paged<1>(a, pack, grid, st) : launch_paged<2>(a, pack, grid, st);
-    if (launched != DSV3_OK) return launched;
+    hipLaunchKernelGGL(kernels[pack], dim3(grid), dim3(256), kLds, st, a);
     FoldArgs f = {};
     f.part = a.part; f.ml = a.ml; f.plan = a.plan; f.counts = counts; f.w = (const uint8_t*)w; f.ws = ws; f.y = y; f.ys = ys;
-    f.tokens = (int)(batch * tokens); f.per_seq = (int)tokens; f.heads = heads; f.rows = 128 / plan.side; f.blocks = a.blocks;
-    f.scale = scale;
+    f.tokens = (int)(batch * tokens); f.per_seq = (int)tokens; f.heads = heads; f.rows = 128; f.blocks = a.blocks;
     return launch_fold<true>(f, st);
 }
 

@@ -51,6 +51,7 @@ struct AbsorbArgs {
     int slabs;              // feature slabs per head (side Q: C/128, side V: v/32)
     int subtiles;           // ceil(tokens / 16)
     int per_seq, blocks;    // (packed side Q) tokens and 128-row blocks per sequence
+    uint8_t* exponents;     // (side Q in codes) of blocks of 64 features, [tokens, heads, 8]
 };
 
 // Where the 16-byte piece of features f .. f + 7 of (token, head h) goes on side Q.  PACK: in the order in which the attention
@@ -62,6 +63,21 @@ __device__ __forceinline__ v4u* q_piece(const AbsorbArgs& p, int64_t tok, int h,
     const int t = (int)tok, b = t / p.per_seq, row = (t - b * p.per_seq) * p.heads + h;
     const int64_t rows32 = ((int64_t)b * p.blocks + (row >> 7)) * 4 + ((row >> 5) & 3);
     return (v4u*)p.y + (rows32 * (p.n_out / 16) + (f >> 4)) * 64 + ((f >> 3) & 1) * 32 + (row & 31);
+}
+
+// Side Q as two e4m3 codes a feature (split_codes): where the eight codes of features f .. f + 7 go, the second ones `second` bytes behind the first.
+// Rows of 512 + 512 bytes, or in the order in which the attention on a cache of codes (mla_paged_decode.hip) reads its operands: [sequence]
+// [block of 128 (token, head) rows][32 rows][first, second][K step of 64 features][half of 16 of 32][lane: features' half of 64, row].
+template <bool PACK>
+__device__ __forceinline__ uint8_t* q_codes(const AbsorbArgs& p, int64_t tok, int h, int f, int& second) {
+    if (!PACK) {
+        second = 512;
+        return (uint8_t*)p.y + (tok * p.heads + h) * 1024 + f;
+    }
+    const int t = (int)tok, b = t / p.per_seq, row = (t - b * p.per_seq) * p.heads + h;
+    const int64_t rows32 = ((int64_t)b * p.blocks + (row >> 7)) * 4 + ((row >> 5) & 3);
+    second = 16384;
+    return (uint8_t*)p.y + rows32 * 32768 + (((f >> 6) * 2 + ((f >> 4) & 1)) * 64 + ((f >> 5) & 1) * 32 + (row & 31)) * 16 + (f & 8);
 }
 
 // 8 fp8 bytes -> 8 binary32
@@ -389,7 +405,8 @@ __global__ __launch_bounds__(256) void absorb_v_staged_kernel(AbsorbArgs p) {
 // still formed by one wavefront over the whole K range in the same order, so the results are those of the kernels
 // above bit for bit.
 // PACK: the pieces of eight consecutive heads fill a line, so that these heads (a run of heads / 8) are given to one XCD.
-template <int KS, int PF, bool PACK = false>
+// CODES: two e4m3 codes a feature (q_codes), which share an exponent in blocks of 64, eight lanes.
+template <int KS, int PF, bool PACK = false, bool CODES = false>
 __global__ __launch_bounds__(256) void absorb_q_shared_kernel(AbsorbArgs p) {
     __shared__ v4u frag[KS * 8 * 64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -460,10 +477,33 @@ __global__ __launch_bounds__(256) void absorb_q_shared_kernel(AbsorbArgs p) {
         for (int j = 0; j < 4; ++j) {
             int64_t tok = (int64_t)ms * 16 + g * 4 + j;
             tok = tok < last ? tok : last;
-            v4u o;
+            if constexpr (CODES) {
+                uint32_t largest = 0u;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) o[q] = pack_bf16(acc[2 * q][j], acc[2 * q + 1][j]);
-            *q_piece<PACK>(p, tok, h, c0 + i * 8) = o;
+                for (int t = 0; t < 8; ++t) largest = umax_u32(largest, abs_bits(acc[t][j]));
+                largest = dpp_umax<0xb1>(largest);      // quad_perm 1 0 3 2, 2 3 0 1, row_half_mirror
+                largest = dpp_umax<0x4e>(largest);
+                largest = dpp_umax<0x141>(largest);
+                const int e = split_exponent(largest);
+                const float scale = u32_as_f32((uint32_t)e << 23), rest = u32_as_f32((uint32_t)(e - 4) << 23);
+                v2u first, second;
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    uint32_t x, y;
+                    split_codes(acc[4 * q][j], acc[4 * q + 1][j], acc[4 * q + 2][j], acc[4 * q + 3][j], scale, rest, x, y);
+                    first[q] = x; second[q] = y;
+                }
+                int behind;
+                uint8_t* dst = q_codes<PACK>(p, tok, h, c0 + i * 8, behind);
+                *(v2u*)dst = first;
+                *(v2u*)(dst + behind) = second;
+                if ((i & 7) == 0) p.exponents[(tok * p.heads + h) * 8 + slab * 2 + (i >> 3)] = (uint8_t)e;
+            } else {
+                v4u o;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) o[q] = pack_bf16(acc[2 * q][j], acc[2 * q + 1][j]);
+                *q_piece<PACK>(p, tok, h, c0 + i * 8) = o;
+            }
         }
     }
 }
@@ -653,6 +693,31 @@ int launch_wkv_b_absorb_q_packed(const void* x, int64_t x_ts, int64_t x_hs, cons
     p.y = (uint16_t*)y; p.tokens = batch * per_seq; p.heads = heads; p.head_rows = nope + v; p.nope = nope;
     p.subtiles = 1; p.n_out = 512; p.slabs = 4; p.per_seq = (int)per_seq; p.blocks = blocks;
     hipLaunchKernelGGL((absorb_q_shared_kernel<4, 1, true>), dim3(heads, p.slabs), dim3(256), 0, st, p);
+    return launch_status();
+}
+
+// Side Q of C == 512 and nope == 128 as two e4m3 codes a feature (q_codes), for the attention on a cache of codes: y as many bytes as bf16 rows would
+// be, exponents [batch * per_seq, heads, 8].
+int launch_wkv_b_absorb_q_codes(const void* x, int64_t x_ts, int64_t x_hs, const void* w, const float* ws, void* y, void* y_exponents, bool pack,
+                                int64_t batch, int64_t per_seq, int blocks, int heads, hipStream_t st) {
+    if (pack && batch * per_seq > 16) return DSV3_ERR_BAD_SHAPE;
+    AbsorbArgs p;
+    p.x = (const uint16_t*)x; p.x_ts = x_ts; p.x_hs = x_hs;
+    p.w = (const uint8_t*)w; p.ws = ws; p.w_cols = 512; p.ws_cols = 4;
+    p.y = (uint16_t*)y; p.exponents = (uint8_t*)y_exponents; p.tokens = batch * per_seq; p.heads = heads; p.head_rows = 256; p.nope = 128;
+    p.subtiles = (int)((p.tokens + 15) / 16); p.n_out = 512; p.slabs = 4; p.per_seq = (int)per_seq; p.blocks = blocks;
+    if (pack) {
+        hipLaunchKernelGGL((absorb_q_shared_kernel<4, 1, true, true>), dim3(heads, p.slabs), dim3(256), 0, st, p);
+        return launch_status();
+    }
+    // a slab per workgroup, its sub-tiles dealt over (gridDim.z, wavefront), as in launch_wkv_b_absorb; one kernel for any number of tokens
+    int gz = (p.subtiles + 3) / 4;
+    const int cap = 512 / (4 * heads);
+    gz = gz > cap ? cap : gz;
+    gz = gz < 1 ? 1 : gz;
+    const dim3 grid(heads, p.slabs, gz), block(256);
+    if ((p.subtiles + 4 * gz - 1) / (4 * gz) <= 1) hipLaunchKernelGGL((absorb_q_shared_kernel<4, 1, false, true>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((absorb_q_shared_kernel<4, 2, false, true>), grid, block, 0, st, p);
     return launch_status();
 }
 

@@ -279,7 +279,7 @@ def _attention_case(b, s, h, context, page, kind, seed):
 
 
 def _attention_reference(args, seen):
-    """Binary64 with the absorbed form's roundings to bf16: weights, rotated and folded query, latent sum."""
+    """Binary64 with the roundings to bf16 that the weights and the rotated query have."""
     q, freqs, kv, scale, pe, table, starts, counts, _, w8, ws, positions, softmax_scale = args
     b, s, h, _ = q.shape
     pages, page = scale.shape
@@ -305,18 +305,19 @@ def _attention_reference(args, seen):
         turned = _rotated(q[i, :n, :, NOPE:], freqs[i, :n, None]).bfloat16().double()
         visible = visible.cuda()
         for a in range(h):
-            folded = (q[i, :n, a, :NOPE].double() @ w[a, :NOPE]).bfloat16().double()
+            folded = q[i, :n, a, :NOPE].double() @ w[a, :NOPE]
             score = (folded @ c.T + turned[:, a] @ k.T) * softmax_scale
             p = score.masked_fill(~visible, float("-inf")).softmax(-1).masked_fill(~visible, 0)
             for t in range(n):              # (a product with a weight of zero would bring in what the token does not see)
                 if bool(visible[t].any()):
-                    out[i, t, a] = (p[t, visible[t]] @ c[visible[t]]).bfloat16().double() @ w[a, NOPE:].T
+                    out[i, t, a] = (p[t, visible[t]] @ c[visible[t]]) @ w[a, NOPE:].T
     return out
 
 
 def _close(got, ref):
-    # the latent sum and the result round to bf16 (2^-8 of the value at most each), the exponentials too; in the value product of 512 terms
-    # these errors average out against a result of the same size: 2^-7 of the row's norm
+    # The latent sum and the result round to bf16 (2^-8 of the value at most each: 2^-8 of the norm for the result, as much for the sum, whose errors
+    # a random product of 512 terms carries over in proportion); folded queries and exponentials are pairs of codes, 2^-9 at most, which
+    # average out over 512 features and the positions: 2^-7 of the row's norm
     return ((got - ref).norm(dim=-1) <= 2.0 ** -7 * ref.norm(dim=-1)).all()
 
 
