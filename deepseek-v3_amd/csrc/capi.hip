@@ -471,7 +471,7 @@ int dsv3_mla_latent_gemm(const void* x, const float* x_s, const void* w, const f
 // What the functions of the paged cache share (no GPU call).
 static int mla_pages_validate(const dsv3_mla_pages* cache, int64_t batch) {
     if (!cache) return DSV3_ERR_NULL_POINTER;
-    if (cache->pages < 1 || cache->pages > 0x7fffffff || cache->page_size < 8 || cache->page_size > 65536 || cache->page_size % 8 != 0 ||
+    if (cache->pages < 1 || cache->pages > 0x7fffffff || cache->page_size < 8 || cache->page_size > 16384 || cache->page_size % 8 != 0 ||
         cache->table_width < 1 || cache->table_width > 0x7fffffff || batch < 0 || batch > 65535)
         return DSV3_ERR_BAD_SHAPE;
     if (batch == 0) return DSV3_OK;

@@ -9,6 +9,9 @@ namespace {
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) void* lptr_t;
 typedef __attribute__((address_space(3))) v2i* lds_v2i;
+typedef __attribute__((address_space(3))) v4u* lds_v4u;
+typedef __attribute__((address_space(3))) v4f* lds_v4f;
+typedef __attribute__((address_space(3))) float* lds_f32;
 
 __device__ __forceinline__ v16f mfma32(v4u a, v4u b, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);

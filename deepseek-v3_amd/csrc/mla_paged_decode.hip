@@ -19,8 +19,7 @@ constexpr int kRopeOff = kTile * kC;                    // a stage: 64 rows of 5
 constexpr int kScaleOff = kRopeOff + kTile * kRope * 2;
 constexpr int kStage = kScaleOff + 8 * 256;
 constexpr int kStages = 3;                              // tiles in LDS: the one whose values and the one whose keys are read, one on its way
-constexpr int kQueryOff = kStages * kStage;             // behind them the wavefronts' rotary queries, 4 KiB each
-constexpr int kLds = kQueryOff + 4 * 4096;
+constexpr int kLds = kStages * kStage;
 
 struct PagedArgs {
     const uint8_t* ql;                                  // folded queries in codes [batch][rows][first, second][512], rows = tokens * heads, or in operand order
@@ -35,17 +34,18 @@ struct PagedArgs {
     v2f* ml;                                            // [range][row block][row] (maximum, sum)
     v2i* plan;                                          // [batch] (first range, ranges)
     int batch, tokens, rows, heads, positions, page, groups, blocks, ranges;        // groups: of 32 rows, in whole 128s; ranges: at most
-    uint32_t page_magic;                                // for quotient()
+    uint32_t page_magic;                                // 2^31 / (page / 8) rounded up: pos / page = (pos / 8 * page_magic) / 2^31 for the positions that there are
     float scale;                                        // of the softmax, times log2 e
 };
 
-// Rows that are no page's: zeros, with a scale that no row has.
+// Rows that are no page's: zeros, with a scale that no row has (positive: exponentials times it keep their sign).
+constexpr float kNothing = 0x1p-126f;
 struct alignas(16) Nothing { uint8_t kv[8 * kC]; uint8_t pe[8 * kRope * 2]; float scale[8]; };
-__device__ const Nothing nothing = { {}, {}, { -1.f, -1.f, -1.f, -1.f, -1.f, -1.f, -1.f, -1.f } };
+__device__ const Nothing nothing = { {}, {}, { kNothing, kNothing, kNothing, kNothing, kNothing, kNothing, kNothing, kNothing } };
 
 // Loads that the compiler may make scalar: `p` is written by nobody while the kernel runs.
 typedef const __attribute__((address_space(4))) int32_t* const_ints;
-__device__ __forceinline__ int scalar_load(const int32_t* p, int64_t at) { return ((const_ints)(uintptr_t)p)[at]; }
+__device__ __forceinline__ int scalar_load(const int32_t* p, uint32_t at) { return ((const_ints)(uintptr_t)p)[at]; }
 
 template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_add(int v) { return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
 // sums of lanes 0 .. l
@@ -106,16 +106,16 @@ template <class F> __device__ __forceinline__ Share share_of(const PagedArgs& p,
 // Bytes 0 .. 15 of both lane halves share the scale that the low lanes hold, bytes 16 .. 31 that of the high lanes.  (As a builtin with a sum of zero
 // the compiler puts the result over the operands, which are still being read.)
 template <int B> __device__ __forceinline__ void mfma64_first(v16f& d, v8i a, v8i b, int sa, int sb) {
-    asm volatile("s_nop 3\n\tv_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, 0, %3, %4 op_sel:[0,%5,0] op_sel_hi:[0,%6,0] cbsz:0 blgp:0"
+    asm volatile("s_nop 1\n\tv_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, 0, %3, %4 op_sel:[0,%5,0] op_sel_hi:[0,%6,0] cbsz:0 blgp:0"
                  : "=&v"(d) : "v"(a), "v"(b), "v"(sa), "v"(sb), "n"(B & 1), "n"(B >> 1));
 }
 template <int B> __device__ __forceinline__ void mfma64_next(v16f& d, v8i a, v8i b, int sa, int sb) {
-    asm volatile("v_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[0,%5,0] op_sel_hi:[0,%6,0] cbsz:0 blgp:0"
+    asm volatile("s_nop 1\n\tv_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[0,%5,0] op_sel_hi:[0,%6,0] cbsz:0 blgp:0"
                  : "+v"(d) : "v"(a), "v"(b), "v"(sa), "v"(sb), "n"(B & 1), "n"(B >> 1));
 }
 // the same with its sum in accumulation registers, byte 0 of both scales
 __device__ __forceinline__ void mfma64_sum(v16f& d, v8i a, v8i b, int sa, int sb) {
-    asm volatile("v_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:0 blgp:0" : "+a"(d) : "v"(a), "v"(b), "v"(sa), "v"(sb));
+    asm volatile("s_nop 1\n\tv_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:0 blgp:0" : "+a"(d) : "v"(a), "v"(b), "v"(sa), "v"(sb));
 }
 // a * b, and zero where a or b is: also beside a scale of NaN (the codes of such a row are zeros, the scores say who sees it)
 __device__ __forceinline__ float times(float a, float b) {
@@ -170,19 +170,21 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     // all lanes, for what the first eight fetch).  Rows past the sequence's end are its last one again; what is no page's comes from `nothing`.
     const uint32_t lds0 = lds_addr_of(lds);
     const int32_t* entries = p.table + b * p.width;
+    struct Place { int entry, rest; };                  // page number, row in the page
     struct Source { const uint8_t* kv; const uint8_t* pe; const float* scales; int last; uint32_t at; };
-    auto entry_of = [&](int t, int h) -> int {          // the page number of group h of the wavefront's rows of tile t (past the end: of the last ones)
-        return scalar_load(entries, quotient(min(t * kTile + wave * 16 + h * 8, seq.end - 1), p.page, p.page_magic));
+    auto place_of = [&](int t, int h) -> Place {        // of group h of the wavefront's rows of tile t (past the end: of the last group)
+        const uint32_t pos = min(t * kTile + wave * 16 + h * 8, (seq.end - 1) & ~7), k = __umulhi(pos >> 2, p.page_magic);
+        return Place{ scalar_load(entries, k), (int)(pos - k * p.page) };
     };
-    auto source = [&](int t, int h, int entry, int stage) -> Source {
-        const int pos = t * kTile + wave * 16 + h * 8;
+    auto source = [&](int t, int h, Place at, int stage) -> Source {
+        const int left = min(seq.end, t1 * kTile) - (t * kTile + wave * 16 + h * 8);
         Source s = { nothing.kv, nothing.pe, nothing.scale, 0, lds0 + stage * kStage };
-        if (t < t1 && pos < seq.end && (uint32_t)entry < (uint64_t)p.pages) {
-            const int64_t r = (int64_t)entry * p.page + (pos - quotient(pos, p.page, p.page_magic) * p.page);
+        if (left > 0 && (uint32_t)at.entry < (uint32_t)p.pages) {
+            const uint64_t r = (uint64_t)(uint32_t)at.entry * (uint32_t)p.page + (uint32_t)at.rest;
             s.kv = p.kv + r * kC;
             s.pe = p.pe + r * (kRope * 2);
             s.scales = p.scales + r;
-            s.last = min(7, seq.end - 1 - pos);
+            s.last = min(7, left - 1);
         }
         return s;
     };
@@ -199,7 +201,7 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     };
     auto copy_tile = [&](int t, int stage) {
         unrolled<2>([&](auto h) {
-            const Source s = source(t, h, entry_of(t, h), stage);
+            const Source s = source(t, h, place_of(t, h), stage);
             unrolled<6>([&](auto n) { issue(lane, s, h, n); });
         });
     };
@@ -223,7 +225,7 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
 
     v8i Q[2][8];                                        // first and second codes; K step n: features 64 n + 32 g .. + 31
     int qs[2][2];                                       // their scales, K steps 0 .. 3 and 4 .. 7
-    uint8_t* const turned = lds + kQueryOff + wave * 4096;                      // rotary query, a lane's 16 bytes of K step s of 16 at s KiB
+    v4u turned[4];                                      // rotary query, K steps of 16
     {
         // (packed, a last block's missing rows hold anything; nobody reads their results)
         const uint8_t* src = PACK ? p.ql + ((int64_t)b * p.groups + row0 / 32) * 32768 + lane * 16 : p.ql + ((int64_t)b * p.rows + row) * 1024 + g * 32;
@@ -247,27 +249,26 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
                 const float re = bf16lo_to_f32(x[e]), im = bf16hi_to_f32(x[e]);
                 x[e] = pack_bf16(re * cs.x - im * cs.y, re * cs.y + im * cs.x);
             }
-            *(v4u*)(turned + s * 1024 + lane * 16) = x;
+            turned[s] = x;
         }
     }
 
-    // (opaque again in every phase, below: formed ahead of the loop, what the reads' places xor to would take the registers that there are not)
-    uint32_t kaddr = i * kC + (((2 * g) ^ (i & 15)) << 4);                // K step n: ^ (4 n mod 16) << 4
-    uint32_t raddr = kRopeOff + i * 128 + ((g ^ ((i >> 1) & 7)) << 4);    // ^ 2 s << 4
+    const uint32_t kaddr = i * kC + (((2 * g) ^ (i & 15)) << 4);                // K step n: ^ (4 n mod 16) << 4
+    const uint32_t raddr = kRopeOff + i * 128 + ((g ^ ((i >> 1) & 7)) << 4);    // ^ 2 s << 4
     // transposed reads: lane group q2 of a half takes 16 features; its lane l fetches eight of row l / 2 of 4 g .. + 3, 8 + 4 g .. + 3 of 16 rows
     const int l15 = lane & 15, q2 = (lane >> 4) & 1, vrow = 8 * (l15 >> 3) + 4 * g + ((l15 >> 1) & 3);
-    uint32_t vaddr = vrow * kC + ((q2 ^ vrow) << 4) + 8 * (l15 & 1);
-    auto key = [&](const uint8_t* base, int half, int n) -> v8i {
-        const uint8_t* at = base + half * (32 * kC) + (n >> 2) * 256;
-        return join(*(const v4u*)(at + (kaddr ^ ((n & 3) << 6))), *(const v4u*)(at + (kaddr ^ ((n & 3) << 6 | 16))));
+    const uint32_t vaddr = vrow * kC + ((q2 ^ vrow) << 4) + 8 * (l15 & 1);
+    // `at`: a stage's address, a multiple of a KiB, with the lane's place added, so that constants can be xor-ed to the sum
+    auto read16 = [](uint32_t at) -> v4u { return *(lds_v4u)(uintptr_t)at; };
+    auto key = [&](uint32_t at, int half, int n) -> v8i {
+        return join(read16((at ^ ((n & 3) << 6)) + half * (32 * kC) + (n >> 2) * 256), read16((at ^ ((n & 3) << 6 | 16)) + half * (32 * kC) + (n >> 2) * 256));
     };
-    auto rope_key = [&](const uint8_t* base, int half, int s) -> v4u { return *(const v4u*)(base + half * (32 * kRope * 2) + (raddr ^ (s << 5))); };
-    auto value = [&](uint32_t stage, int f) -> v8i {    // features 32 f .. of all 64 positions
-        const uint32_t at = stage + (vaddr ^ ((f & 7) << 5)) + (f >> 3) * 256;
+    auto rope_key = [&](uint32_t at, int half, int s) -> v4u { return read16((at ^ (s << 5)) + half * (32 * kRope * 2)); };
+    auto value = [&](uint32_t at, int f) -> v8i {       // features 32 f .. of all 64 positions
         v8i v;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const v2i x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i)(uintptr_t)(at + k * (16 * kC)));
+            const v2i x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i)(uintptr_t)((at ^ ((f & 7) << 5)) + (f >> 3) * 256 + k * (16 * kC)));
             v[2 * k] = x[0];
             v[2 * k + 1] = x[1];
         }
@@ -277,27 +278,28 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     v16f O[16] = {};
     v16f S[2];
     v8i ring[2];                                        // keys of two K steps, or values of 64 features: read two to four MFMAs ahead
-    v4u rope_q[2];
+    v4u rope[4];                                        // rotary keys
     v8i P[2];                                           // exponentials, first and second codes; dwords 4 h .. of half h
     int pe[2];                                          // their exponents, by halves
     float off = -__builtin_inff(), l = 0.f;             // exponentials are of 2^(score - off), off a whole number; this lane's share of their sum
     int ks[2];                                          // scale byte of position i, by halves
     uint32_t none[2];                                   // positions that nobody sees for want of a page, by halves
-    auto scales_of = [&](const uint8_t* base, int half) {
+    auto scales_of = [&](uint32_t stage, int half) {
         const int i = lane_now() & 31;
-        const float sc = *(const float*)(base + kScaleOff + (4 * half + (i >> 3)) * 256 + (i & 7) * 4);
+        const float sc = *(lds_f32)(uintptr_t)(stage + (i >> 3) * 256 + (i & 7) * 4 + kScaleOff + half * 1024);
         ks[half] = (int)(f32_as_u32(sc) >> 23 & 0xff);  // (NaN: 255, which makes the products NaN)
-        none[half] = (uint32_t)__ballot(sc < 0.f);
+        none[half] = (uint32_t)__ballot(sc == kNothing);
     };
 
-    // The exponentials of half h, in 16 steps that stand beside the MFMAs of 20.
+    // The exponentials of half h, in 17 steps that stand beside the MFMAs of 20.
     v4f w[4];
-    float pm = 0.f, offu = 0.f, shrink = 1.f;
+    uint32_t largest = 0u;                              // bits of the largest exponential times its scale
+    float pm = 0.f, offu = 0.f, shrink = 1.f, ex[2];
     bool behind = false;                                // the sums are still to be multiplied with `shrink`
-    auto soften = [&](int t, const uint8_t* base, auto half, auto step) {
+    auto soften = [&](int t, uint32_t stage, auto half, auto step) {
         constexpr int h = decltype(half)::value, x = decltype(step)::value;
         v16f& s = S[h];
-        if constexpr (x < 8 && x % 2 == 0) w[x / 2] = *(const v4f*)(base + kScaleOff + (4 * h + x / 2) * 256 + (lane_now() >> 5) * 16);
+        if constexpr (x < 8 && x % 2 == 0) w[x / 2] = *(lds_v4f)(uintptr_t)(stage + (lane_now() >> 5) * 16 + kScaleOff + (4 * h + x / 2) * 256);
         if constexpr (x == 1) {
             asm volatile("" : "+v"(s));                 // (behind two more MFMAs: the scores are there)
             const int at = t * kTile + 32 * h, left = seq.end - at;
@@ -337,50 +339,53 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
                 behind = true;
             }
             offu = off == -__builtin_inff() ? 0.f : off;
-            pm = 0.f;
+            largest = 0u;
+        }
+        if constexpr (x >= 4 && x < 12) {               // (a step behind their exponentials: those results take a while)
+            constexpr int e = 2 * (x - 4);
+            l += ex[0];
+            l += ex[1];
+            s[e] = times(ex[0], w[e >> 2][e & 3]);
+            s[e + 1] = times(ex[1], w[e >> 2][(e & 3) + 1]);
+            largest = umax_u32(largest, umax_u32(f32_as_u32(s[e]), f32_as_u32(s[e + 1])));
+            asm volatile("" : "+v"(l), "+v"(largest));                          // (here, not where they are next looked at)
         }
         if constexpr (x >= 3 && x < 11) {
 #pragma unroll
-            for (int e = 2 * (x - 3); e < 2 * (x - 3) + 2; ++e) {
-                const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], p.scale, -offu));
-                l += v;
-                s[e] = times(v, w[e >> 2][e & 3]);
-            }
-            pm = __builtin_elementwise_max(pm, __builtin_elementwise_max(s[2 * (x - 3)], s[2 * (x - 3) + 1]));
+            for (int e = 0; e < 2; ++e) ex[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * (x - 3) + e], p.scale, -offu));
         }
-        if constexpr (x == 11) {
-            const v2f both = halves32(pm);              // (the halves' bytes share a scale)
-            pe[h] = split_exponent(f32_as_u32(fmaxf(both.x, both.y)));
+        if constexpr (x == 12) {                        // (the halves' bytes share a scale)
+            const v2u both = __builtin_amdgcn_permlane32_swap(largest, largest, false, false);
+            pe[h] = split_exponent(umax_u32(both[0], both[1]));
         }
-        if constexpr (x >= 12 && x < 16) {
-            constexpr int k = x - 12;
+        if constexpr (x >= 13 && x < 17) {
+            constexpr int k = x - 13;
             uint32_t first, second;
             split_codes(s[4 * k], s[4 * k + 1], s[4 * k + 2], s[4 * k + 3], u32_as_f32((uint32_t)pe[h] << 23), u32_as_f32((uint32_t)(pe[h] - 4) << 23), first, second);
+            asm volatile("" : "+v"(first), "+v"(second));                       // (made here, not where they are used)
             P[0][4 * h + k] = (int)first;
             P[1][4 * h + k] = (int)second;
         }
     };
-    // The scores of half h of the tile at `base`, whose first two keys are in the ring.  beside(step): what stands behind the step's MFMA;
+    // The scores of half h of the tile at `stage`, whose first two keys are in the ring.  beside(step): what stands behind the step's MFMA;
     // tail(0 / 1): the ring's place is free for what the next phase reads first.
-    auto score = [&](const uint8_t* base, auto half, auto beside, auto tail) {
+    auto score = [&](uint32_t stage, auto half, auto beside, auto tail) {
         constexpr int h = decltype(half)::value;
         v16f& s = S[h];
-        asm volatile("" : "+v"(kaddr), "+v"(raddr));
-        const int own = lane_now() * 16;
+        uint32_t keys = kaddr, ropes = raddr;
+        asm volatile("" : "+v"(keys), "+v"(ropes));     // (formed ahead of the loop, what the reads' places xor to would take the registers that there are not)
+        keys += stage;
+        ropes += stage;
         unrolled<20>([&](auto step) {
             constexpr int x = decltype(step)::value, n = x >> 1;
             if constexpr (x == 0) mfma64_first<0>(s, ring[0], Q[0][0], ks[h], qs[0][0]);
             else if constexpr (x < 16) mfma64_next<(n & 3)>(s, ring[n & 1], Q[x & 1][n], ks[h], qs[x & 1][n >> 2]);
-            else {
-                const v4u k = __builtin_bit_cast(v4u, __builtin_shufflevector(ring[n & 1], ring[n & 1], 4 * (x & 1), 4 * (x & 1) + 1, 4 * (x & 1) + 2, 4 * (x & 1) + 3));
-                mfma32_next(s, k, rope_q[x & 1]);
-            }
-            if constexpr (x < 12 && (x & 1)) ring[n & 1] = key(base, h, n + 2);
-            if constexpr (x == 13 || x == 15) ring[n & 1] = join(rope_key(base, h, 2 * (n - 6)), rope_key(base, h, 2 * (n - 6) + 1));
-            if constexpr (x >= 14 && x < 18) rope_q[x & 1] = *(const v4u*)(turned + (x - 14) * 1024 + own);
+            else mfma32_next(s, rope[x - 16], turned[x - 16]);
+            if constexpr (x < 12 && (x & 1)) ring[n & 1] = key(keys, h, n + 2);
+            if constexpr (x >= 12 && x < 16) rope[x - 12] = rope_key(ropes, h, x - 12);
             beside(step);
             if constexpr (x == 17) tail(std::integral_constant<int, 0>());
-            if constexpr (x == 19) tail(std::integral_constant<int, 1>());
+            if constexpr (x == 18) tail(std::integral_constant<int, 1>());
             __builtin_amdgcn_sched_barrier(0);
         });
     };
@@ -388,38 +393,29 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     typedef std::integral_constant<int, 0> First;
     typedef std::integral_constant<int, 1> Second;
     arrived();
-    scales_of(lds, 0);
-    ring[0] = key(lds, 0, 0);
-    ring[1] = key(lds, 0, 1);
-    score(lds, First(), [](auto) {}, [&](auto k) { ring[k] = key(lds, 1, k); });
-    scales_of(lds, 1);
+    scales_of(lds0, 0);
+    ring[0] = key(lds0 + kaddr, 0, 0);
+    ring[1] = key(lds0 + kaddr, 0, 1);
+    score(lds0, First(), [](auto) {}, [&](auto k) { ring[k] = key(lds0 + kaddr, 1, k); });
+    scales_of(lds0, 1);
     int st = 0;
     for (int t = t0;; ++t) {
         const int st_next = st == 2 ? 0 : st + 1, st_free = st_next == 2 ? 0 : st_next + 1;
-        const uint8_t* base = lds + st * kStage;
-        const uint8_t* next = lds + st_next * kStage;
-        const int entry[2] = { entry_of(t + 2, 0), entry_of(t + 2, 1) };
+        const uint32_t base = lds0 + st * kStage, next = lds0 + st_next * kStage;
+        const Place places[2] = { place_of(t + 2, 0), place_of(t + 2, 1) };
         // C.  Behind its barrier the next tile is there, and the stage of the one before is free.
         score(base, Second(), [&](auto step) {
             soften(t, base, First(), step);
             if constexpr (decltype(step)::value == 16) arrived();
-        }, [&](auto k) { ring[k] = key(next, 0, k); });
-        const bool more = t + 1 < t1;
-        if (more) {                                     // A
-            scales_of(next, 0);
-            score(next, First(), [&](auto step) { soften(t, base, Second(), step); }, [&](auto k) { ring[k] = value(lds0 + st * kStage, k); });
-        } else {
-            scores_ready(S[1]);
-            unrolled<16>([&](auto step) {
-                soften(t, base, Second(), step);
-                __builtin_amdgcn_sched_barrier(0);
-            });
-            ring[0] = value(lds0 + st * kStage, 0);
-            ring[1] = value(lds0 + st * kStage, 1);
-        }
+        }, [&](auto k) { ring[k] = key(next + kaddr, 0, k); });
+        // A, also behind the last tile (of zeros: a path without it would let the compiler copy scores before they are there)
+        scales_of(next, 0);
+        score(next, First(), [&](auto step) { soften(t, base, Second(), step); }, [&](auto k) { ring[k] = value(base + vaddr, k); });
         // B
-        const Source ahead[2] = { source(t + 2, 0, entry[0], st_free), source(t + 2, 1, entry[1], st_free) };
-        asm volatile("" : "+v"(vaddr));
+        const Source ahead[2] = { source(t + 2, 0, places[0], st_free), source(t + 2, 1, places[1], st_free) };
+        uint32_t values = vaddr;
+        asm volatile("" : "+v"(values));
+        values += base;
         const int lane = lane_now(), one = 127, g = lane >> 5, e[2] = { g ? pe[1] : pe[0], (g ? pe[1] : pe[0]) - 4 };
         if (behind) {
             behind = false;
@@ -429,19 +425,17 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
                 asm volatile("s_nop 7" ::: "memory");
             }
         }
-        int first_e = e[0], second_e = e[1], unit_scale = one;
-        asm volatile("s_nop 3" : "+v"(first_e), "+v"(second_e), "+v"(unit_scale));      // (between an ordinary instruction's result and an MFMA that the compiler does not know)
         __builtin_amdgcn_sched_barrier(0);
         unrolled<32>([&](auto step) {
             constexpr int x = decltype(step)::value, f = x >> 1;
-            mfma64_sum(O[f], ring[f & 1], P[x & 1], unit_scale, x & 1 ? second_e : first_e);
-            if constexpr (x & 1) ring[f & 1] = f < 14 ? value(lds0 + st * kStage, f + 2) : key(next, 1, f - 14);
+            mfma64_sum(O[f], ring[f & 1], P[x & 1], one, e[x & 1]);
+            if constexpr (x & 1) ring[f & 1] = f < 14 ? value(values, f + 2) : key(next + kaddr, 1, f - 14);
             if constexpr (x < 12) issue(lane, ahead[x / 6], std::integral_constant<int, x / 6>(), std::integral_constant<int, x % 6>());
             __builtin_amdgcn_sched_barrier(0);
         });
 #pragma unroll
         for (int d = 0; d < 16; ++d) asm volatile("" : "+a"(O[d]));     // (the sums stay where they are)
-        if (!more) break;
+        if (t + 1 == t1) break;
         scales_of(next, 1);
         st = st_next;
     }
@@ -525,7 +519,7 @@ int launch_mla_decode_paged(const void* q, const void* freqs, const dsv3_mla_pag
     a.part = (float*)(wsp + space.part); a.ml = (v2f*)(wsp + space.ml); a.plan = (v2i*)(wsp + space.plan);
     a.batch = (int)batch; a.tokens = (int)tokens; a.rows = (int)rows; a.heads = heads; a.positions = (int)positions;
     a.page = cache.page_size; a.groups = plan.groups; a.blocks = (int)plan.blocks; a.ranges = (int)plan.ranges;
-    a.page_magic = magic_of(positions, cache.page_size);
+    a.page_magic = (uint32_t)(((1ll << 31) + cache.page_size / 8 - 1) / (cache.page_size / 8));
     a.scale = scale * 1.44269504088896340736f;
     // operand order up to 16 tokens in all, which is what the kernel that writes it takes (mla_decode.hip)
     const bool pack = batch * tokens <= 16;

@@ -338,7 +338,7 @@ dsv3_mla_pages checked_pages(const char* what, const Tensor& kv, const Tensor& s
                 what, ": kv_scale must be a contiguous fp32 [pages, page]");
     TORCH_CHECK(pe.dim() == 3 && pe.scalar_type() == at::kBFloat16 && pe.is_contiguous() && pe.size(0) == kv.size(0) && pe.size(1) == kv.size(1),
                 what, ": pe_pages must be a contiguous bf16 [pages, page, rope]");
-    TORCH_CHECK(kv.size(1) >= 8 && kv.size(1) <= 65536 && kv.size(1) % 8 == 0, what, ": a page must have a multiple of 8 positions, up to 65536, got ", kv.size(1));
+    TORCH_CHECK(kv.size(1) >= 8 && kv.size(1) <= 16384 && kv.size(1) % 8 == 0, what, ": a page must have a multiple of 8 positions, up to 16384, got ", kv.size(1));
     TORCH_CHECK(kv.size(2) == 512 && pe.size(2) == 64, what, ": latents of 512 and rotary keys of 64 are implemented, got ", kv.size(2), " and ", pe.size(2));
     TORCH_CHECK(table.dim() == 2 && table.scalar_type() == at::kInt && table.is_contiguous() && table.size(0) == batch && table.size(1) > 0,
                 what, ": page_table must be a contiguous int32 [batch, width]");

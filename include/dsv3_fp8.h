@@ -404,7 +404,7 @@ int dsv3_mla_latent_gemm(const void* x, const float* x_s, const void* w, const f
  * ---- The latent cache of the attention layer in pages, in eight bits ----
  *
  * The reference keeps one dense bf16 cache per layer with a place for every position of every sequence (inference/model.py:443-444).
- * Here sequences share pages of page_size positions (a multiple of 8, up to 65536): row j of a sequence is row
+ * Here sequences share pages of page_size positions (a multiple of 8, up to 16384): row j of a sequence is row
  * table[b][j / page_size] * page_size + j % page_size of three arrays,
  *     kv       e4m3 [pages, page_size, 512]     the latent's codes (16-byte aligned)
  *     kv_scale binary32 [pages, page_size]      a power of two: latent = code * scale, a bf16 number (4-byte aligned)
