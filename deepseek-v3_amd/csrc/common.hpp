@@ -63,11 +63,13 @@ __device__ __forceinline__ int split_exponent(uint32_t largest) {       // from 
 }
 __device__ __forceinline__ void split_codes(float a, float b, float c, float d, float scale, float rest, uint32_t& first, uint32_t& second) {
     typedef short v2s __attribute__((ext_vector_type(2)));
-    v2s r = {};
+    v2s r;
+    asm("" : "=v"(r));                                  // (any: both halves are written)
     r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, a, b, scale, false);
     r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, c, d, scale, true);
     first = __builtin_bit_cast(uint32_t, r);
     const v2f lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(first, scale, false), hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(first, scale, true);
+    asm("" : "=v"(r));
     r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, a - lo.x, b - lo.y, rest, false);
     r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, c - hi.x, d - hi.y, rest, true);
     second = __builtin_bit_cast(uint32_t, r);

@@ -40,6 +40,7 @@ struct PagedArgs {
 
 // Rows that are no page's: zeros, with a scale that no row has (positive: exponentials times it keep their sign).
 constexpr float kNothing = 0x1p-126f;
+constexpr float kNoScore = -0x1p100f;                   // the exponents' offset in front of a row's first score
 struct alignas(16) Nothing { uint8_t kv[8 * kC]; uint8_t pe[8 * kRope * 2]; float scale[8]; };
 __device__ const Nothing nothing = { {}, {}, { kNothing, kNothing, kNothing, kNothing, kNothing, kNothing, kNothing, kNothing } };
 
@@ -117,12 +118,8 @@ template <int B> __device__ __forceinline__ void mfma64_next(v16f& d, v8i a, v8i
 __device__ __forceinline__ void mfma64_sum(v16f& d, v8i a, v8i b, int sa, int sb) {
     asm volatile("s_nop 1\n\tv_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:0 blgp:0" : "+a"(d) : "v"(a), "v"(b), "v"(sa), "v"(sb));
 }
-// a * b, and zero where a or b is: also beside a scale of NaN (the codes of such a row are zeros, the scores say who sees it)
-__device__ __forceinline__ float times(float a, float b) {
-    float r;
-    asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
-    return r;
-}
+// a * b, and zero where a or b is (v_mul_legacy_f32): also beside a scale of NaN (the codes of such a row are zeros, the scores say who sees it)
+extern "C" __device__ float dsv3_mul_legacy(float, float) __asm("llvm.amdgcn.fmul.legacy");
 // the lane's number, formed where it is needed: nothing that goes by it stays in a register for the loop
 __device__ __forceinline__ int lane_now() {
     int l = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
@@ -281,7 +278,7 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     v4u rope[4];                                        // rotary keys
     v8i P[2];                                           // exponentials, first and second codes; dwords 4 h .. of half h
     int pe[2];                                          // their exponents, by halves
-    float off = -__builtin_inff(), l = 0.f;             // exponentials are of 2^(score - off), off a whole number; this lane's share of their sum
+    float off = kNoScore, l = 0.f;                      // exponentials are of 2^(score - off), off a whole number; this lane's share of their sum
     int ks[2];                                          // scale byte of position i, by halves
     uint32_t none[2];                                   // positions that nobody sees for want of a page, by halves
     auto scales_of = [&](uint32_t stage, int half) {
@@ -294,20 +291,22 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     // The exponentials of half h, in 17 steps that stand beside the MFMAs of 20.
     v4f w[4];
     uint32_t largest = 0u;                              // bits of the largest exponential times its scale
-    float pm = 0.f, offu = 0.f, shrink = 1.f, ex[2];
+    float pm = 0.f, shrink = 1.f, ex[2];
+    uint32_t scales_at = 0u;
+    const uint64_t alive = __ballot(row0 + i < live);
     bool behind = false;                                // the sums are still to be multiplied with `shrink`
     auto soften = [&](int t, uint32_t stage, auto half, auto step) {
         constexpr int h = decltype(half)::value, x = decltype(step)::value;
         v16f& s = S[h];
-        if constexpr (x < 8 && x % 2 == 0) w[x / 2] = *(lds_v4f)(uintptr_t)(stage + (lane_now() >> 5) * 16 + kScaleOff + (4 * h + x / 2) * 256);
+        if constexpr (x == 0) scales_at = stage + (lane_now() >> 5) * 16 + kScaleOff;
+        if constexpr (x < 8 && x % 2 == 0) w[x / 2] = *(lds_v4f)(uintptr_t)(scales_at + (4 * h + x / 2) * 256);
         if constexpr (x == 1) {
             asm volatile("" : "+v"(s));                 // (behind two more MFMAs: the scores are there)
-            const int at = t * kTile + 32 * h, left = seq.end - at;
-            uint32_t there = ~none[h];
-            if (left < 32) there &= left > 0 ? (1u << left) - 1u : 0u;
-            if (there != ~0u || at + 32 > seq.start) {
-                const int j0 = at - seq.start;          // the first position among the new ones
-                uint32_t seen = there;
+            const int at = t * kTile + 32 * h;
+            if (none[h] || at + 32 > seq.start) {       // (the sequence's end lies behind its start)
+                const int left = seq.end - at, j0 = at - seq.start;            // j0: the first position among the new ones
+                uint32_t seen = ~none[h];
+                if (left < 32) seen &= left > 0 ? (1u << left) - 1u : 0u;
                 if (j0 > -32) {
                     const int tok = min(row0 + (lane_now() & 31), p.rows - 1) / p.heads;
                     const uint64_t bits = p.tree ? (uint64_t)p.tree[(int64_t)b * p.tokens + tok] : (2ull << tok) - 1;
@@ -328,31 +327,30 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
             // `off` is only raised when a score passes it by more than 2^64: exponentials and sums have room for that in binary32, and so the 256
             // multiplications are needed in the rarest of cases.  By whole powers of two: the first half's codes change their exponent only.
             // (Rows that nobody reads do not ask for it.)
-            const bool raise = row0 + (lane_now() & 31) < live && (top - off > 64.f || (off == -__builtin_inff() && top > off));
-            if (__any(raise)) {
-                const float on = raise ? __builtin_ceilf(top) : off;
-                const float a = !raise ? 1.f : off == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(off - on);
+            const uint64_t raise = __ballot(top - off > 64.f) & alive;
+            if (raise) {
+                const bool mine = raise >> lane_now() & 1;
+                const float on = mine ? __builtin_ceilf(top) : off, a = __builtin_amdgcn_exp2f(off - on);
                 l *= a;
-                if constexpr (h == 1) pe[0] = max(5, pe[0] - (raise ? (int)fminf(on - off, 300.f) : 0));
+                if constexpr (h == 1) pe[0] = max(5, pe[0] - (int)fminf(on - off, 300.f));
                 off = on;
                 shrink = behind ? shrink * a : a;       // (the sums follow in front of phase B)
                 behind = true;
             }
-            offu = off == -__builtin_inff() ? 0.f : off;
             largest = 0u;
         }
         if constexpr (x >= 4 && x < 12) {               // (a step behind their exponentials: those results take a while)
             constexpr int e = 2 * (x - 4);
             l += ex[0];
             l += ex[1];
-            s[e] = times(ex[0], w[e >> 2][e & 3]);
-            s[e + 1] = times(ex[1], w[e >> 2][(e & 3) + 1]);
+            s[e] = dsv3_mul_legacy(ex[0], w[e >> 2][e & 3]);
+            s[e + 1] = dsv3_mul_legacy(ex[1], w[e >> 2][(e & 3) + 1]);
             largest = umax_u32(largest, umax_u32(f32_as_u32(s[e]), f32_as_u32(s[e + 1])));
             asm volatile("" : "+v"(l), "+v"(largest));                          // (here, not where they are next looked at)
         }
         if constexpr (x >= 3 && x < 11) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) ex[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * (x - 3) + e], p.scale, -offu));
+            for (int e = 0; e < 2; ++e) ex[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * (x - 3) + e], p.scale, -off));
         }
         if constexpr (x == 12) {                        // (the halves' bytes share a scale)
             const v2u both = __builtin_amdgcn_permlane32_swap(largest, largest, false, false);
