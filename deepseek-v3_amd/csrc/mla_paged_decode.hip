@@ -44,6 +44,10 @@ constexpr float kNoScore = -0x1p100f;                   // the exponents' offset
 struct alignas(16) Nothing { uint8_t kv[8 * kC]; uint8_t pe[8 * kRope * 2]; float scale[8]; };
 __device__ const Nothing nothing = { {}, {}, { kNothing, kNothing, kNothing, kNothing, kNothing, kNothing, kNothing, kNothing } };
 
+// Row r's chunk c of 16 bytes of a latent lies at c ^ swz(r).  Sixteen rows read at the same c (the scores) hit sixteen different chunks, and so do the
+// eight rows of two neighbouring chunks that half a wavefront's transposed read takes (0 .. 3 and 8 .. 11, or 4 .. 7 and 12 .. 15 of sixteen).
+__device__ __forceinline__ int swz(int r) { return ((r & 3) << 1) | (r & 8) | ((r >> 2) & 1); }
+
 // Loads that the compiler may make scalar: `p` is written by nobody while the kernel runs.
 typedef const __attribute__((address_space(4))) int32_t* const_ints;
 __device__ __forceinline__ int scalar_load(const int32_t* p, uint32_t at) { return ((const_ints)(uintptr_t)p)[at]; }
@@ -167,17 +171,18 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     // all lanes, for what the first eight fetch).  Rows past the sequence's end are its last one again; what is no page's comes from `nothing`.
     const uint32_t lds0 = lds_addr_of(lds);
     const int32_t* entries = p.table + b * p.width;
-    struct Place { int entry, rest; };                  // page number, row in the page
     struct Source { const uint8_t* kv; const uint8_t* pe; const float* scales; int last; uint32_t at; };
-    auto place_of = [&](int t, int h) -> Place {        // of group h of the wavefront's rows of tile t (past the end: of the last group)
-        const uint32_t pos = min(t * kTile + wave * 16 + h * 8, (seq.end - 1) & ~7), k = __umulhi(pos >> 2, p.page_magic);
-        return Place{ scalar_load(entries, k), (int)(pos - k * p.page) };
+    auto first_of = [&](int t, int h) -> uint32_t {     // group h of the wavefront's rows of tile t (past the end: the last group)
+        return min(t * kTile + wave * 16 + h * 8, (seq.end - 1) & ~7);
     };
-    auto source = [&](int t, int h, Place at, int stage) -> Source {
-        const int left = min(seq.end, t1 * kTile) - (t * kTile + wave * 16 + h * 8);
+    // page number of group `lane % 2`, as a load of vectors: one by scalars would make every wait for LDS behind it wait for it as well
+    auto page_of = [&](int t) -> int { return entries[__umulhi(first_of(t, lane_now() & 1) >> 2, p.page_magic)]; };
+    auto source = [&](int t, int h, int page, int stage) -> Source {
+        const int entry = __builtin_amdgcn_readlane(page, h), left = min(seq.end, t1 * kTile) - (t * kTile + wave * 16 + h * 8);
         Source s = { nothing.kv, nothing.pe, nothing.scale, 0, lds0 + stage * kStage };
-        if (left > 0 && (uint32_t)at.entry < (uint32_t)p.pages) {
-            const uint64_t r = (uint64_t)(uint32_t)at.entry * (uint32_t)p.page + (uint32_t)at.rest;
+        if (left > 0 && (uint32_t)entry < (uint32_t)p.pages) {
+            const uint32_t pos = first_of(t, h);
+            const uint64_t r = (uint64_t)(uint32_t)entry * (uint32_t)p.page + (pos - __umulhi(pos >> 2, p.page_magic) * p.page);
             s.kv = p.kv + r * kC;
             s.pe = p.pe + r * (kRope * 2);
             s.scales = p.scales + r;
@@ -187,9 +192,9 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     };
     auto issue = [&](int lane, const Source& s, auto group, auto which) {
         constexpr int n = decltype(which)::value, h = decltype(group)::value;
-        if constexpr (n < 4) {                          // row r's chunk c of 16 bytes lies at c ^ r (low four bits)
-            const uint32_t chunk = ((lane & 31) ^ (lane >> 5)) << 4;
-            copy16(s.kv, min(2 * n + (lane >> 5), s.last) * kC + (chunk ^ ((8 * h + 2 * n) << 4)), s.at + (wave * 16 + 8 * h + 2 * n) * kC);
+        if constexpr (n < 4) {                          // (swz of row 8 h + 2 n + lane / 32 of sixteen, the lane's part first)
+            const uint32_t chunk = ((lane & 31) ^ ((lane >> 5) << 1)) << 4;
+            copy16(s.kv, min(2 * n + (lane >> 5), s.last) * kC + (chunk ^ ((8 * h | (n & 1) << 2 | n >> 1) << 4)), s.at + (wave * 16 + 8 * h + 2 * n) * kC);
         } else if constexpr (n == 4) {                  // a key's chunk c at c ^ r / 2 (low three bits)
             copy16(s.pe, min(lane >> 3, s.last) * (kRope * 2) + (((lane & 7) ^ (4 * h + (lane >> 4))) << 4), s.at + kRopeOff + (wave * 16 + 8 * h) * (kRope * 2));
         } else {
@@ -197,8 +202,9 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
         }
     };
     auto copy_tile = [&](int t, int stage) {
+        const int page = page_of(t);
         unrolled<2>([&](auto h) {
-            const Source s = source(t, h, place_of(t, h), stage);
+            const Source s = source(t, h, page, stage);
             unrolled<6>([&](auto n) { issue(lane, s, h, n); });
         });
     };
@@ -250,11 +256,11 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
         }
     }
 
-    const uint32_t kaddr = i * kC + (((2 * g) ^ (i & 15)) << 4);                // K step n: ^ (4 n mod 16) << 4
+    const uint32_t kaddr = i * kC + (((2 * g) ^ swz(i & 15)) << 4);             // K step n: ^ (4 n mod 16) << 4
     const uint32_t raddr = kRopeOff + i * 128 + ((g ^ ((i >> 1) & 7)) << 4);    // ^ 2 s << 4
     // transposed reads: lane group q2 of a half takes 16 features; its lane l fetches eight of row l / 2 of 4 g .. + 3, 8 + 4 g .. + 3 of 16 rows
     const int l15 = lane & 15, q2 = (lane >> 4) & 1, vrow = 8 * (l15 >> 3) + 4 * g + ((l15 >> 1) & 3);
-    const uint32_t vaddr = vrow * kC + ((q2 ^ vrow) << 4) + 8 * (l15 & 1);
+    const uint32_t vaddr = vrow * kC + ((q2 ^ swz(vrow)) << 4) + 8 * (l15 & 1);
     // `at`: a stage's address, a multiple of a KiB, with the lane's place added, so that constants can be xor-ed to the sum
     auto read16 = [](uint32_t at) -> v4u { return *(lds_v4u)(uintptr_t)at; };
     auto key = [&](uint32_t at, int half, int n) -> v8i {
@@ -281,9 +287,12 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     float off = kNoScore, l = 0.f;                      // exponentials are of 2^(score - off), off a whole number; this lane's share of their sum
     int ks[2];                                          // scale byte of position i, by halves
     uint32_t none[2];                                   // positions that nobody sees for want of a page, by halves
-    auto scales_of = [&](uint32_t stage, int half) {
+    float sc;                                           // the scale that the next scores need
+    auto scale_at = [&](uint32_t stage, int half) -> float {
         const int i = lane_now() & 31;
-        const float sc = *(lds_f32)(uintptr_t)(stage + (i >> 3) * 256 + (i & 7) * 4 + kScaleOff + half * 1024);
+        return *(lds_f32)(uintptr_t)(stage + (i >> 3) * 256 + (i & 7) * 4 + kScaleOff + half * 1024);
+    };
+    auto look_at_scale = [&](int half) {
         ks[half] = (int)(f32_as_u32(sc) >> 23 & 0xff);  // (NaN: 255, which makes the products NaN)
         none[half] = (uint32_t)__ballot(sc == kNothing);
     };
@@ -382,35 +391,42 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
             if constexpr (x < 12 && (x & 1)) ring[n & 1] = key(keys, h, n + 2);
             if constexpr (x >= 12 && x < 16) rope[x - 12] = rope_key(ropes, h, x - 12);
             beside(step);
-            if constexpr (x == 17) tail(std::integral_constant<int, 0>());
-            if constexpr (x == 18) tail(std::integral_constant<int, 1>());
+            if constexpr (x == 14) tail(std::integral_constant<int, 0>());
+            if constexpr (x == 16) tail(std::integral_constant<int, 1>());
             __builtin_amdgcn_sched_barrier(0);
         });
     };
 
     typedef std::integral_constant<int, 0> First;
     typedef std::integral_constant<int, 1> Second;
+    int page = page_of(t0 + 2);
     arrived();
-    scales_of(lds0, 0);
+    sc = scale_at(lds0, 0);
     ring[0] = key(lds0 + kaddr, 0, 0);
     ring[1] = key(lds0 + kaddr, 0, 1);
+    look_at_scale(0);
+    sc = scale_at(lds0, 1);
     score(lds0, First(), [](auto) {}, [&](auto k) { ring[k] = key(lds0 + kaddr, 1, k); });
-    scales_of(lds0, 1);
+    look_at_scale(1);
     int st = 0;
     for (int t = t0;; ++t) {
         const int st_next = st == 2 ? 0 : st + 1, st_free = st_next == 2 ? 0 : st_next + 1;
         const uint32_t base = lds0 + st * kStage, next = lds0 + st_next * kStage;
-        const Place places[2] = { place_of(t + 2, 0), place_of(t + 2, 1) };
+        const int page_now = page;
         // C.  Behind its barrier the next tile is there, and the stage of the one before is free.
         score(base, Second(), [&](auto step) {
             soften(t, base, First(), step);
-            if constexpr (decltype(step)::value == 16) arrived();
+            if constexpr (decltype(step)::value == 13) {
+                arrived();
+                page = page_of(t + 3);
+                sc = scale_at(next, 0);
+            }
         }, [&](auto k) { ring[k] = key(next + kaddr, 0, k); });
         // A, also behind the last tile (of zeros: a path without it would let the compiler copy scores before they are there)
-        scales_of(next, 0);
+        look_at_scale(0);
         score(next, First(), [&](auto step) { soften(t, base, Second(), step); }, [&](auto k) { ring[k] = value(base + vaddr, k); });
         // B
-        const Source ahead[2] = { source(t + 2, 0, places[0], st_free), source(t + 2, 1, places[1], st_free) };
+        const Source ahead[2] = { source(t + 2, 0, page_now, st_free), source(t + 2, 1, page_now, st_free) };
         uint32_t values = vaddr;
         asm volatile("" : "+v"(values));
         values += base;
@@ -428,13 +444,14 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
             constexpr int x = decltype(step)::value, f = x >> 1;
             mfma64_sum(O[f], ring[f & 1], P[x & 1], one, e[x & 1]);
             if constexpr (x & 1) ring[f & 1] = f < 14 ? value(values, f + 2) : key(next + kaddr, 1, f - 14);
+            if constexpr (x == 20) sc = scale_at(next, 1);
             if constexpr (x < 12) issue(lane, ahead[x / 6], std::integral_constant<int, x / 6>(), std::integral_constant<int, x % 6>());
             __builtin_amdgcn_sched_barrier(0);
         });
 #pragma unroll
         for (int d = 0; d < 16; ++d) asm volatile("" : "+a"(O[d]));     // (the sums stay where they are)
         if (t + 1 == t1) break;
-        scales_of(next, 1);
+        look_at_scale(1);
         st = st_next;
     }
 
