@@ -36,6 +36,11 @@ template <int IMM> __device__ __forceinline__ void copy16_buffer(v4i buffer, uin
     asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
                  :: "v"(lane_off), "s"(buffer), "s"(lds_addr), "n"(IMM) : "memory", "m0", "scc");
 }
+// the same from lane_off + off
+__device__ __forceinline__ void copy16_buffer_at(v4i buffer, uint32_t lane_off, uint32_t off, uint32_t lds_addr) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %3 offen lds"
+                 :: "v"(lane_off), "s"(buffer), "s"(lds_addr), "s"(off) : "memory", "m0");
+}
 // f(integral_constant 0), .., f(integral_constant N - 1)
 template <int N, int I = 0, class F> __device__ __forceinline__ void unrolled(F f) {
     if constexpr (I < N) {

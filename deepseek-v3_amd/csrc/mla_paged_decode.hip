@@ -15,7 +15,15 @@ namespace dsv3 {
 namespace {
 
 constexpr int kTile = 64;                               // positions per tile
-constexpr int kRopeOff = kTile * kC;                    // a stage: 64 rows of 512 codes, 64 rotary keys of 128 B, eight groups of eight scales, 256 B each
+// A stage: 64 rows of 512 codes, 64 rotary keys of 128 B, eight groups of eight scales, 256 B each.  Two neighbouring rows are a KiB, as they are
+// copied, the odd one with its chunks of 16 bytes c at c ^ 4; the eight pairs of 16 rows stand 32 bytes further apart than that, pairs 2, 3, 6 and 7
+// another 16.  Sixteen rows read at the same place (the scores) then hit sixteen different chunks of 256 bytes, and so do the eight rows of two
+// neighbouring chunks that half a wavefront's transposed read takes (0 .. 3 and 8 .. 11, or 4 .. 7 and 12 .. 15 of sixteen), all from a few
+// addresses a phase with constants added.
+constexpr int kPair = 2 * kC + 32, kRows16 = 34 * 256;
+constexpr int pair_off(int p) { return p * kPair + ((p >> 1) & 1) * 16; }       // of 0 .. 7
+static_assert(pair_off(7) + 2 * kC <= kRows16, "16 rows");
+constexpr int kRopeOff = 4 * kRows16;
 constexpr int kScaleOff = kRopeOff + kTile * kRope * 2;
 constexpr int kStage = kScaleOff + 8 * 256;
 constexpr int kStages = 3;                              // tiles in LDS: the one whose values and the one whose keys are read, one on its way
@@ -38,15 +46,10 @@ struct PagedArgs {
     float scale;                                        // of the softmax, times log2 e
 };
 
-// Rows that are no page's: zeros, with a scale that no row has (positive: exponentials times it keep their sign).
+// The scale of rows that are no page's, which no row has (positive: exponentials times it keep their sign).
 constexpr float kNothing = 0x1p-126f;
 constexpr float kNoScore = -0x1p100f;                   // the exponents' offset in front of a row's first score
-struct alignas(16) Nothing { uint8_t kv[8 * kC]; uint8_t pe[8 * kRope * 2]; float scale[8]; };
-__device__ const Nothing nothing = { {}, {}, { kNothing, kNothing, kNothing, kNothing, kNothing, kNothing, kNothing, kNothing } };
-
-// Row r's chunk c of 16 bytes of a latent lies at c ^ swz(r).  Sixteen rows read at the same c (the scores) hit sixteen different chunks, and so do the
-// eight rows of two neighbouring chunks that half a wavefront's transposed read takes (0 .. 3 and 8 .. 11, or 4 .. 7 and 12 .. 15 of sixteen).
-__device__ __forceinline__ int swz(int r) { return ((r & 3) << 1) | (r & 8) | ((r >> 2) & 1); }
+__device__ const float nothing[8] = { kNothing, kNothing, kNothing, kNothing, kNothing, kNothing, kNothing, kNothing };
 
 // Loads that the compiler may make scalar: `p` is written by nobody while the kernel runs.
 typedef const __attribute__((address_space(4))) int32_t* const_ints;
@@ -104,7 +107,9 @@ template <class F> __device__ __forceinline__ Share share_of(const PagedArgs& p,
         }
         base = __builtin_amdgcn_readlane(upto, 63);
     }
-    return s;
+    // (uniform, which the compiler does not see)
+    return Share{ __builtin_amdgcn_readfirstlane(s.b), __builtin_amdgcn_readfirstlane(s.first), __builtin_amdgcn_readfirstlane(s.ranges),
+                  __builtin_amdgcn_readfirstlane(s.per), s.used };
 }
 
 // v_mfma_scale_f32_32x32x64_f8f6f4 of codes with its result in ordinary registers (mla.hpp: mfma32_first).  a's scale: byte 0 of sa; b's: byte B of sb.
@@ -168,10 +173,11 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     const int row = min(row0 + i, p.rows - 1);          // rows past the end repeat the last one; fold leaves them out
 
     // A wavefront copies two groups of eight rows of a tile, of which each lies in one page: four KiB of latents, a KiB of rotary keys, the scales (by
-    // all lanes, for what the first eight fetch).  Rows past the sequence's end are its last one again; what is no page's comes from `nothing`.
+    // all lanes, for what the first eight fetch).  A group is a buffer of the rows that it has: rows past the sequence's end, and all that
+    // is no page's, are zeros; the scales of the latter come from `nothing`.
     const uint32_t lds0 = lds_addr_of(lds);
     const int32_t* entries = p.table + b * p.width;
-    struct Source { const uint8_t* kv; const uint8_t* pe; const float* scales; int last; uint32_t at; };
+    struct Source { v4i kv, pe; const float* scales; int last; uint32_t at; };
     auto first_of = [&](int t, int h) -> uint32_t {     // group h of the wavefront's rows of tile t (past the end: the last group)
         return min(t * kTile + wave * 16 + h * 8, (seq.end - 1) & ~7);
     };
@@ -179,33 +185,34 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     auto page_of = [&](int t) -> int { return entries[__umulhi(first_of(t, lane_now() & 1) >> 2, p.page_magic)]; };
     auto source = [&](int t, int h, int page, int stage) -> Source {
         const int entry = __builtin_amdgcn_readlane(page, h), left = min(seq.end, t1 * kTile) - (t * kTile + wave * 16 + h * 8);
-        Source s = { nothing.kv, nothing.pe, nothing.scale, 0, lds0 + stage * kStage };
-        if (left > 0 && (uint32_t)entry < (uint32_t)p.pages) {
-            const uint32_t pos = first_of(t, h);
-            const uint64_t r = (uint64_t)(uint32_t)entry * (uint32_t)p.page + (pos - __umulhi(pos >> 2, p.page_magic) * p.page);
-            s.kv = p.kv + r * kC;
-            s.pe = p.pe + r * (kRope * 2);
-            s.scales = p.scales + r;
-            s.last = min(7, left - 1);
-        }
-        return s;
+        // without branches, which would part the products that this stands beside (an empty buffer's address is not looked at)
+        const int64_t some = -(int64_t)((left > 0) & ((uint32_t)entry < (uint32_t)p.pages));
+        const uint32_t pos = first_of(t, h);
+        const uint64_t r = (uint64_t)(uint32_t)entry * (uint32_t)p.page + (pos - __umulhi(pos >> 2, p.page_magic) * p.page);
+        const int rows = min(8, left) & (int)some;
+        const uint64_t scales = (((uint64_t)(uintptr_t)p.scales + r * 4) & some) | ((uint64_t)(uintptr_t)nothing & ~some);
+        return Source{ buffer_of(p.kv + r * kC, rows * kC), buffer_of(p.pe + r * (kRope * 2), rows * (kRope * 2)), (const float*)(uintptr_t)scales,
+                       max(rows, 1) - 1, lds0 + stage * kStage };
     };
-    auto issue = [&](int lane, const Source& s, auto group, auto which) {
+    // where a lane reads of two rows of latents
+    auto latent_off = [&]() -> uint32_t { const int lane = lane_now(); return (lane >> 5) * kC + (((lane & 31) ^ (lane >> 5 << 2)) << 4); };
+    auto issue = [&](const Source& s, uint32_t latents, auto group, auto which) {
         constexpr int n = decltype(which)::value, h = decltype(group)::value;
-        if constexpr (n < 4) {                          // (swz of row 8 h + 2 n + lane / 32 of sixteen, the lane's part first)
-            const uint32_t chunk = ((lane & 31) ^ ((lane >> 5) << 1)) << 4;
-            copy16(s.kv, min(2 * n + (lane >> 5), s.last) * kC + (chunk ^ ((8 * h | (n & 1) << 2 | n >> 1) << 4)), s.at + (wave * 16 + 8 * h + 2 * n) * kC);
+        if constexpr (n < 4) {
+            copy16_buffer_at(s.kv, latents, n * (2 * kC), s.at + wave * kRows16 + pair_off(4 * h + n));
         } else if constexpr (n == 4) {                  // a key's chunk c at c ^ r / 2 (low three bits)
-            copy16(s.pe, min(lane >> 3, s.last) * (kRope * 2) + (((lane & 7) ^ (4 * h + (lane >> 4))) << 4), s.at + kRopeOff + (wave * 16 + 8 * h) * (kRope * 2));
+            const int lane = lane_now();
+            copy16_buffer_at(s.pe, (lane >> 3) * (kRope * 2) + (((lane & 7) ^ (4 * h + (lane >> 4))) << 4), 0, s.at + kRopeOff + (wave * 16 + 8 * h) * (kRope * 2));
         } else {
-            copy4(s.scales, min(lane & 7, s.last) * 4, s.at + kScaleOff + (wave * 2 + h) * 256);
+            copy4(s.scales, min(lane_now() & 7, s.last) * 4, s.at + kScaleOff + (wave * 2 + h) * 256);
         }
     };
     auto copy_tile = [&](int t, int stage) {
         const int page = page_of(t);
         unrolled<2>([&](auto h) {
             const Source s = source(t, h, page, stage);
-            unrolled<6>([&](auto n) { issue(lane, s, h, n); });
+            const uint32_t latents = latent_off();
+            unrolled<6>([&](auto n) { issue(s, latents, h, n); });
         });
     };
     // this wavefront's copies have landed, and everybody's
@@ -256,22 +263,29 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
         }
     }
 
-    const uint32_t kaddr = i * kC + (((2 * g) ^ swz(i & 15)) << 4);             // K step n: ^ (4 n mod 16) << 4
+    const auto row_off = [](int r) { return (r >> 1) * kPair + ((r >> 2) & 1) * 16 + (r & 1) * kC; };      // of 0 .. 15
+    // K step n is 64 bytes; of an odd row, steps n and n + 1 of even n are exchanged.  Values: 32 bytes for 32 features, in odd rows two and two exchanged.
+    const uint32_t kaddr = (i >> 4) * kRows16 + row_off(i & 15) + 32 * g;
     const uint32_t raddr = kRopeOff + i * 128 + ((g ^ ((i >> 1) & 7)) << 4);    // ^ 2 s << 4
     // transposed reads: lane group q2 of a half takes 16 features; its lane l fetches eight of row l / 2 of 4 g .. + 3, 8 + 4 g .. + 3 of 16 rows
     const int l15 = lane & 15, q2 = (lane >> 4) & 1, vrow = 8 * (l15 >> 3) + 4 * g + ((l15 >> 1) & 3);
-    const uint32_t vaddr = vrow * kC + ((q2 ^ swz(vrow)) << 4) + 8 * (l15 & 1);
-    // `at`: a stage's address, a multiple of a KiB, with the lane's place added, so that constants can be xor-ed to the sum
+    const uint32_t vaddr = row_off(vrow) + 16 * q2 + 8 * (l15 & 1);
+    const uint32_t kodd = (i & 1) * 64, vodd = (vrow & 1) * 64;
     auto read16 = [](uint32_t at) -> v4u { return *(lds_v4u)(uintptr_t)at; };
-    auto key = [&](uint32_t at, int half, int n) -> v8i {
-        return join(read16((at ^ ((n & 3) << 6)) + half * (32 * kC) + (n >> 2) * 256), read16((at ^ ((n & 3) << 6 | 16)) + half * (32 * kC) + (n >> 2) * 256));
+    // `at`: a stage's address with the lane's place, the even and the odd ones of what an odd row exchanges
+    struct Two { uint32_t at[2]; };
+    auto keys_at = [&](uint32_t stage) -> Two { return Two{ { stage + kaddr + kodd, stage + kaddr - kodd } }; };
+    auto values_at = [&](uint32_t stage) -> Two { return Two{ { stage + vaddr + vodd, stage + vaddr - vodd } }; };
+    auto key = [&](const Two& a, int half, int n) -> v8i {
+        const uint32_t at = a.at[n & 1] + half * (2 * kRows16) + n * 64;
+        return join(read16(at), read16(at + 16));
     };
     auto rope_key = [&](uint32_t at, int half, int s) -> v4u { return read16((at ^ (s << 5)) + half * (32 * kRope * 2)); };
-    auto value = [&](uint32_t at, int f) -> v8i {       // features 32 f .. of all 64 positions
+    auto value = [&](const Two& a, int f) -> v8i {      // features 32 f .. of all 64 positions
         v8i v;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const v2i x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i)(uintptr_t)((at ^ ((f & 7) << 5)) + (f >> 3) * 256 + k * (16 * kC)));
+            const v2i x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i)(uintptr_t)(a.at[(f >> 1) & 1] + f * 32 + k * kRows16));
             v[2 * k] = x[0];
             v[2 * k + 1] = x[1];
         }
@@ -379,10 +393,10 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     auto score = [&](uint32_t stage, auto half, auto beside, auto tail) {
         constexpr int h = decltype(half)::value;
         v16f& s = S[h];
-        uint32_t keys = kaddr, ropes = raddr;
-        asm volatile("" : "+v"(keys), "+v"(ropes));     // (formed ahead of the loop, what the reads' places xor to would take the registers that there are not)
-        keys += stage;
+        uint32_t ropes = raddr;
+        asm volatile("" : "+v"(ropes));                 // (formed ahead of the loop, what the reads' places xor to would take the registers that there are not)
         ropes += stage;
+        const Two keys = keys_at(stage);
         unrolled<20>([&](auto step) {
             constexpr int x = decltype(step)::value, n = x >> 1;
             if constexpr (x == 0) mfma64_first<0>(s, ring[0], Q[0][0], ks[h], qs[0][0]);
@@ -402,11 +416,11 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     int page = page_of(t0 + 2);
     arrived();
     sc = scale_at(lds0, 0);
-    ring[0] = key(lds0 + kaddr, 0, 0);
-    ring[1] = key(lds0 + kaddr, 0, 1);
+    ring[0] = key(keys_at(lds0), 0, 0);
+    ring[1] = key(keys_at(lds0), 0, 1);
     look_at_scale(0);
     sc = scale_at(lds0, 1);
-    score(lds0, First(), [](auto) {}, [&](auto k) { ring[k] = key(lds0 + kaddr, 1, k); });
+    score(lds0, First(), [](auto) {}, [&](auto k) { ring[k] = key(keys_at(lds0), 1, k); });
     look_at_scale(1);
     int st = 0;
     for (int t = t0;; ++t) {
@@ -421,16 +435,15 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
                 page = page_of(t + 3);
                 sc = scale_at(next, 0);
             }
-        }, [&](auto k) { ring[k] = key(next + kaddr, 0, k); });
+        }, [&](auto k) { ring[k] = key(keys_at(next), 0, k); });
         // A, also behind the last tile (of zeros: a path without it would let the compiler copy scores before they are there)
         look_at_scale(0);
-        score(next, First(), [&](auto step) { soften(t, base, Second(), step); }, [&](auto k) { ring[k] = value(base + vaddr, k); });
+        score(next, First(), [&](auto step) { soften(t, base, Second(), step); }, [&](auto k) { ring[k] = value(values_at(base), k); });
         // B
-        const Source ahead[2] = { source(t + 2, 0, page_now, st_free), source(t + 2, 1, page_now, st_free) };
-        uint32_t values = vaddr;
-        asm volatile("" : "+v"(values));
-        values += base;
-        const int lane = lane_now(), one = 127, g = lane >> 5, e[2] = { g ? pe[1] : pe[0], (g ? pe[1] : pe[0]) - 4 };
+        const Two values = values_at(base);
+        Source ahead;
+        uint32_t latents;
+        const int one = 127, g = lane_now() >> 5, e[2] = { g ? pe[1] : pe[0], (g ? pe[1] : pe[0]) - 4 };
         if (behind) {
             behind = false;
             if (t > t0) {
@@ -443,9 +456,15 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
         unrolled<32>([&](auto step) {
             constexpr int x = decltype(step)::value, f = x >> 1;
             mfma64_sum(O[f], ring[f & 1], P[x & 1], one, e[x & 1]);
-            if constexpr (x & 1) ring[f & 1] = f < 14 ? value(values, f + 2) : key(next + kaddr, 1, f - 14);
+            if constexpr (x & 1) ring[f & 1] = f < 14 ? value(values, f + 2) : key(keys_at(next), 1, f - 14);
+            // copies of the tile after the next, one behind a product
+            if constexpr (x == 0 || x == 8) {
+                ahead = source(t + 2, x / 8, page_now, st_free);
+                latents = latent_off();
+            }
+            if constexpr (x >= 1 && x < 7) issue(ahead, latents, First(), std::integral_constant<int, x - 1>());
+            if constexpr (x >= 9 && x < 15) issue(ahead, latents, Second(), std::integral_constant<int, x - 9>());
             if constexpr (x == 20) sc = scale_at(next, 1);
-            if constexpr (x < 12) issue(lane, ahead[x / 6], std::integral_constant<int, x / 6>(), std::integral_constant<int, x % 6>());
             __builtin_amdgcn_sched_barrier(0);
         });
 #pragma unroll
