@@ -234,6 +234,32 @@ _mla_query = torch.ops.dsv3fp8.mla_query.default
 _mla_output = torch.ops.dsv3fp8.mla_output.default
 
 
+class LatentPages:
+    """The cache of one attention layer in pages of e4m3 rows, for ``MLA.forward_paged``: ``kv`` [pages, page_size, 512] codes, ``scale``
+    [pages, page_size] one power of two a row, ``pe`` [pages, page_size, 64] rotary keys in bf16; 644 bytes a position where ``kv_cache`` and
+    ``pe_cache`` take 1152.  Sequence i's position t lies in page ``page_table[i, t // page_size]`` (int32; an entry that is no page of the
+    pool stands for none: nothing is written there, and nobody sees it).  Which page belongs to whom is the program's business; two
+    sequences may share the pages of a common beginning as long as neither writes into them.  ``page_size``: a multiple of 8 up to 16384."""
+
+    def __init__(self, pages: int, page_size: int, device=None):
+        if pages < 1 or page_size % 8 or not 8 <= page_size <= 16384:
+            raise ValueError(f"LatentPages: {pages} pages of {page_size} rows; a page has a multiple of 8, 8 to 16384")
+        device = device if device is not None else torch.get_default_device()
+        self.kv = torch.zeros(pages, page_size, 512, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+        self.scale = torch.ones(pages, page_size, dtype=torch.float32, device=device)
+        self.pe = torch.zeros(pages, page_size, 64, dtype=torch.bfloat16, device=device)
+
+    def read(self, page_table: torch.Tensor, lengths: torch.Tensor, positions: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Latents [b, positions, 512] and rotary keys [b, positions, 64] in bf16, as ``kv_cache`` and ``pe_cache`` hold them; zeros from
+        a sequence's length on."""
+        return torch.ops.dsv3fp8.mla_cache_read(self.kv, self.scale, self.pe, page_table, lengths, positions)
+
+    def keep(self, page_table: torch.Tensor, starts: torch.Tensor, path: torch.Tensor, kept: torch.Tensor) -> None:
+        """After a step with a tree of drafted tokens: row ``starts + path[:, j]`` moves to ``starts + j`` for the first ``kept`` nodes of
+        each sequence's accepted path (ascending, ``path`` [b, most] and ``kept`` [b] int32)."""
+        torch.ops.dsv3fp8.mla_cache_keep(self.kv, self.scale, self.pe, page_table, starts, path, kept)
+
+
 class MLA(nn.Module):
     """Multi-head latent attention (model.py:395-497).
 
@@ -473,6 +499,54 @@ class MLA(nn.Module):
         out = self._absorb(torch.einsum("bsht,btc->bshc", probs, latent), ops._lib.ABSORB_V, wkv_b)
         return self.wo(out.flatten(2))
 
+
+    def _paged_ok(self, x, freqs_cis) -> bool:
+        """What ``forward_paged`` asks of the layer beside ``_latent_kernel_ok``; the operators check their own arguments."""
+        wo, w = self.wo, self.wkv_b.weight
+        return (not torch.is_grad_enabled() and gemm_impl == "fp8" and block_size == 128 and world_size == 1 and x.is_cuda and x.dtype == torch.bfloat16
+                and x.dim() == 3 and x.numel() > 0 and torch.get_default_dtype() == torch.bfloat16
+                and (self.qk_nope_head_dim, self.qk_rope_head_dim, self.v_head_dim, self.kv_lora_rank) == (128, 64, 128, 512)
+                and w.element_size() == 1 and w.device == x.device and _plain(wo, RowParallelLinear) and wo.weight.element_size() == 1 and wo.bias is None
+                and freqs_cis.dtype == torch.complex64 and freqs_cis.shape == (x.size(0), x.size(1), self.qk_rope_head_dim // 2))
+
+    def forward_paged(self, x: torch.Tensor, cache: LatentPages, page_table: torch.Tensor, starts: torch.Tensor, counts: torch.Tensor,
+                      freqs_cis: torch.Tensor, positions: int, tree: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``forward`` on a cache in pages, for sequences of different lengths: sequence i has ``starts[i]`` positions in the cache and takes
+        ``counts[i]`` (up to s) new tokens behind them, x [b, s, dim].  ``starts``, ``counts`` and ``page_table`` (int32) stay on the device, so that
+        a captured step serves every length; ``positions`` is what the longest sequence has at most after the step.  ``freqs_cis`` [b, s, 32]: each
+        new token's rotation.  ``tree`` (int64 [b, s], s <= 64): bit j of token i says that it sees new token j; without one a token sees those in
+        front of it and itself.  Rows of tokens that a sequence does not have are zeros.
+
+        Up to 64 new tokens, wkv_b is folded into queries and outputs and the codes are read as they lie.  More (a prompt) go through keys and
+        values per head of the rows read back, sequence by sequence: at 128 heads 1 x 128 tokens at 1024 positions take 123 us so and
+        156 folded in two pieces, 1 x 4096 at 4096 910 and 4937; only few new tokens far into a long context lose (1 x 128 at 8192: 523 and 357).
+
+        There is no slower path behind the kernels: a layer or call that they do not take raises."""
+        latent = self._latent_kernel_ok(x) if self._paged_ok(x, freqs_cis) else None
+        if latent is None:
+            raise RuntimeError("MLA.forward_paged needs an FP8 layer of the 671B head dimensions with a low-rank query and plain submodules, bf16 input [b, s, dim] "
+                               "on the GPU, gemm_impl 'fp8', no gradients, and freqs_cis complex64 [b, s, 32]")
+        b, s = x.size(0), x.size(1)
+        if s > 64 and tree is not None:
+            raise ValueError(f"MLA.forward_paged: a tree has up to 64 tokens, not {s}")
+        q_norm, kv_norm, q_eps, kv_eps, wq = latent
+        w, w_scale, wo = self.wkv_b.weight, self.wkv_b.scale, self.wo.weight
+        qq, qs = torch.ops.dsv3fp8.mla_latent_paged(linear(x, self._wa, None, self.wq_a.scale_fmt), q_norm, kv_norm, freqs_cis, cache.kv, cache.scale,
+                                                    cache.pe, page_table, starts, counts, q_eps, kv_eps)
+        q = fp8_gemm(qq, qs, wq, self.wq_b.scale).unflatten(-1, (self.n_local_heads, self.qk_head_dim))
+        if s <= 64:
+            yq, ys = torch.ops.dsv3fp8.mla_decode_paged_quant(q, freqs_cis, cache.kv, cache.scale, cache.pe, page_table, starts, counts, tree, w, w_scale,
+                                                              positions, self.softmax_scale)
+            return fp8_gemm(yq, ys, wo, wo.scale)
+        kv, pe = cache.read(page_table, starts + counts, positions)
+        new, at, parts = torch.arange(s, device=x.device), torch.arange(positions, device=x.device), []
+        for i in range(b):
+            mask = torch.zeros(s, positions, dtype=torch.bfloat16, device=x.device).masked_fill_(at > (starts[i] + new)[:, None], float("-inf"))
+            parts.append(torch.ops.dsv3fp8.mla_prefill(q[i:i + 1], freqs_cis[i], kv[i:i + 1], pe[i:i + 1], w, w_scale, mask, positions, self.softmax_scale))
+        yq, ys = (torch.cat([part[k].view(torch.uint8) if k == 0 else part[k] for part in parts]) for k in (0, 1))
+        y = fp8_gemm(yq.view(torch.float8_e4m3fn), ys, wo, wo.scale)
+        there = (new < counts[:, None]) & (starts >= 0)[:, None]
+        return y.masked_fill_(~there.unsqueeze(-1), 0)
 
     def _forward_naive(self, x, q, kva, start_pos: int, freqs_cis, mask):
         """Per-head key / value caches (model.py:470-479, 488-490): the new positions' latents go through wkv_b as a

@@ -1,0 +1,94 @@
+"""MLA.forward_paged and LatentPages on the host: what they refuse, and which operators a call consists of (no kernel runs)."""
+import pytest
+import torch
+
+from test_mla_dispatch import FP8, _OnGpu, layer  # noqa: F401  (layer: a fixture)
+
+
+@pytest.mark.parametrize("pages,page", [(0, 64), (-1, 64), (4, 0), (4, 7), (4, 12), (4, 16392), (4, -8)])
+def test_pools_that_there_are_not(pages, page):
+    from dsv3fp8.model import LatentPages
+    with pytest.raises(ValueError):
+        LatentPages(pages, page)
+
+
+def test_pool():
+    from dsv3fp8.model import LatentPages
+    c = LatentPages(3, 24)
+    assert c.kv.shape == (3, 24, 512) and c.kv.dtype == FP8 and c.scale.shape == (3, 24) and c.scale.dtype == torch.float32
+    assert c.pe.shape == (3, 24, 64) and c.pe.dtype == torch.bfloat16
+    assert (c.kv.float() == 0).all() and (c.scale == 1).all()
+
+
+def _arguments(b, s):
+    from dsv3fp8.model import LatentPages
+    x = torch.zeros(b, s, 256, dtype=torch.bfloat16).as_subclass(_OnGpu)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    return [x, LatentPages(4, 64), torch.zeros(b, 2, dtype=torch.int32), i32(*[0] * b), i32(*[s] * b), torch.ones(b, s, 32, dtype=torch.complex64), 128]
+
+
+@pytest.fixture
+def calls(layer, monkeypatch):  # noqa: F811
+    """The operators in front of and behind the attention as stand-ins that note their arguments."""
+    from dsv3fp8 import model
+    monkeypatch.setattr(model, "gemm_impl", "fp8")
+    layer.qk_nope_head_dim, layer.qk_rope_head_dim, layer.v_head_dim, layer.kv_lora_rank = 128, 64, 128, 512
+    layer.qk_head_dim, out = 192, []
+
+    def note(name, result):
+        return lambda *a: (out.append((name, a)), result(*a))[1]
+    ops = torch.ops.dsv3fp8
+    monkeypatch.setattr(model, "linear", lambda x, *a: x)
+    monkeypatch.setattr(model, "fp8_gemm", note("gemm", lambda a, s, w, ws: torch.zeros(*a.shape[:-1], w.size(0), dtype=torch.bfloat16)))
+    pair = lambda a, n: (torch.zeros(*a.shape[:2], n, dtype=FP8), torch.zeros(*a.shape[:2], 1))  # noqa: E731
+    monkeypatch.setattr(ops, "mla_latent_paged", note("latent", lambda a, *r: pair(a, 128)))
+    monkeypatch.setattr(ops, "mla_decode_paged_quant", note("decode", lambda q, *r: pair(q, 256)))
+    monkeypatch.setattr(ops, "mla_prefill", note("prefill", lambda q, *r: pair(q, 256)))
+    monkeypatch.setattr(ops, "mla_cache_read", note("read", lambda kv, sc, pe, table, n, t: (torch.zeros(table.size(0), t, 512), torch.zeros(table.size(0), t, 64))))
+    return out
+
+
+@pytest.mark.parametrize("b,s", [(2, 1), (1, 64), (3, 65)])
+def test_operators_of_a_call(layer, calls, b, s):  # noqa: F811
+    args = _arguments(b, s)
+    tree = torch.ones(b, s, dtype=torch.int64) if s <= 64 else None
+    with torch.no_grad():
+        y = layer.forward_paged(*args, tree)
+    assert y.shape == (b, s, 256)
+    assert [c[0] for c in calls] == (["latent", "gemm", "decode", "gemm"] if s <= 64 else ["latent", "gemm", "read"] + ["prefill"] * b + ["gemm"])
+    latent = calls[0][1]
+    assert latent[1] is layer.q_norm.weight and latent[2] is layer.kv_norm.weight and latent[4] is args[1].kv and latent[7] is args[2]
+    if s <= 64:
+        decode = calls[2][1]
+        assert decode[2] is args[1].kv and decode[5] is args[2] and decode[8] is tree and decode[9] is layer.wkv_b.weight and decode[11] == 128
+
+
+@pytest.mark.parametrize("what", ["grad", "dtype", "shape", "freqs", "freqs shape", "wo", "wo hook", "norm", "dims", "gemm", "empty", "tree"])
+def test_calls_that_are_refused(layer, calls, monkeypatch, what):  # noqa: F811
+    from dsv3fp8 import model
+    args, tree = _arguments(2, 3), None
+    if what == "dtype":
+        args[0] = args[0].float()
+    elif what == "shape":
+        args[0] = args[0][0]
+    elif what == "freqs":
+        args[5] = args[5].to(torch.complex128)
+    elif what == "freqs shape":
+        args[5] = args[5][0]
+    elif what == "wo":
+        layer.wo = torch.nn.Linear(256, 256)
+    elif what == "wo hook":
+        layer.wo.register_forward_hook(lambda *a: None)
+    elif what == "norm":
+        layer.kv_norm.eps = None
+    elif what == "dims":
+        layer.v_head_dim = 64
+    elif what == "gemm":
+        monkeypatch.setattr(model, "gemm_impl", "bf16")
+    elif what == "empty":
+        args = _arguments(2, 0)
+    elif what == "tree":
+        args, tree = _arguments(2, 65), torch.ones(2, 65, dtype=torch.int64)
+    with torch.set_grad_enabled(what == "grad"), pytest.raises((RuntimeError, ValueError)):
+        layer.forward_paged(*args, tree)
+    assert not calls
