@@ -28,6 +28,10 @@ constexpr int kScaleOff = kRopeOff + kTile * kRope * 2;
 constexpr int kStage = kScaleOff + 8 * 256;
 constexpr int kStages = 3;                              // tiles in LDS: the one whose values and the one whose keys are read, one on its way
 constexpr int kLds = kStages * kStage;
+// A stage of a wavefront by itself: the rotary keys of its last 32 rows only, the others come into registers.
+constexpr int kFewScaleOff = kRopeOff + kTile / 2 * kRope * 2;
+constexpr int kFewStage = kFewScaleOff + 8 * 256;
+constexpr int kFewLds = 4 * kFewStage;
 
 struct PagedArgs {
     const uint8_t* ql;                                  // folded queries in codes [batch][rows][first, second][512], rows = tokens * heads, or in operand order
@@ -50,6 +54,7 @@ struct PagedArgs {
 constexpr float kNothing = 0x1p-126f;
 constexpr float kNoScore = -0x1p100f;                   // the exponents' offset in front of a row's first score
 __device__ const float nothing[8] = { kNothing, kNothing, kNothing, kNothing, kNothing, kNothing, kNothing, kNothing };
+__device__ const v4u nothing_key[kRope / 8] = {};
 
 // Loads that the compiler may make scalar: `p` is written by nobody while the kernel runs.
 typedef const __attribute__((address_space(4))) int32_t* const_ints;
@@ -68,9 +73,9 @@ __device__ __forceinline__ int wave_scan(int v) {
 __device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
 
 // Which positions a workgroup takes.  The lengths are on the device, so every workgroup divides the work by itself: `per` tiles a
-// range, the fewest with which all sequences' ranges are at most p.ranges, ranges numbered through the sequences.
+// range, the fewest with which all sequences' ranges are at most p.ranges, ranges numbered through the sequences; then rounded up to a MULTIPLE.
 struct Share { int b, first, ranges, per, used; };      // sequence (-1: none), its first range and ranges, tiles a range, ranges of all
-template <class F> __device__ __forceinline__ Share share_of(const PagedArgs& p, int lane, F which, bool write_plan) {
+template <int MULTIPLE, class F> __device__ __forceinline__ Share share_of(const PagedArgs& p, int lane, F which, bool write_plan) {
     auto tiles = [&](int b) -> int {
         if (b >= p.batch) return 0;
         const SeqSpan s = seq_span(p.starts[b], p.counts[b], p.tokens, p.positions);
@@ -91,6 +96,10 @@ template <class F> __device__ __forceinline__ Share share_of(const PagedArgs& p,
         // a sequence's last range is half full on average: what these take off the ranges does not change with `per`
         const int lost = s.used - all / per, left = max(1, p.ranges - lost);
         s.per = max(per + 1, min(all / left, per + per / 4));
+    }
+    if constexpr (MULTIPLE > 1) {
+        const int per = s.per = (s.per + MULTIPLE - 1) / MULTIPLE * MULTIPLE;
+        s.used = sum([per](int t) { return (t + per - 1) / per; });
     }
     const int range = which(s.used);
     int base = 0;
@@ -151,14 +160,14 @@ __device__ __forceinline__ v8i join(v4u a, v4u b) {
 //   A  scores of the next tile's first half | exponentials of the second half
 //   B  weighted sums of the tile      | copies of the tile after the next
 // Measured (us, the form before): one sequence of 61 tokens x 128 heads at 32768 positions 542 -> ...
-template <bool PACK>
+template <bool PACK, bool FEW>
 __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = lane & 31, g = lane >> 5;
     // a contiguous run of the ranges in use per XCD, the row blocks of a range next to each other: its rows are in the XCD's L2
     int unit = -1;
-    const Share mine = share_of(p, lane, [&](int used) -> int {
+    const Share mine = share_of<FEW ? 4 : 1>(p, lane, [&](int used) -> int {
         const int T = used * p.blocks, q = T / 8, r = T % 8, x = blockIdx.x % 8, k = blockIdx.x / 8;
         if (k < q + (x < r)) unit = x * q + min(x, r) + k;
         return unit < 0 ? -1 : unit / p.blocks;
@@ -169,7 +178,7 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     const int live = seq.count * p.heads;               // rows behind these are of tokens that the sequence does not have
     if (blk * 128 >= live) return;
     const int t0 = (range - mine.first) * mine.per, t1 = min((seq.end + kTile - 1) / kTile, t0 + mine.per);
-    const int row0 = blk * 128 + wave * 32;
+    const int row0 = FEW ? 0 : blk * 128 + wave * 32;
     const int row = min(row0 + i, p.rows - 1);          // rows past the end repeat the last one; fold leaves them out
 
     // A wavefront copies two groups of eight rows of a tile, of which each lies in one page: four KiB of latents, a KiB of rotary keys, the scales (by
@@ -178,38 +187,43 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     const uint32_t lds0 = lds_addr_of(lds);
     const int32_t* entries = p.table + b * p.width;
     struct Source { v4i kv, pe; const float* scales; int last; uint32_t at; };
+    constexpr int kScaleAt = FEW ? kFewScaleOff : kScaleOff, kGroups = FEW ? 8 : 2;
+    const int first_row = FEW ? 0 : wave * 16;          // the wavefront's rows in a tile
     auto first_of = [&](int t, int h) -> uint32_t {     // group h of the wavefront's rows of tile t (past the end: the last group)
-        return min(t * kTile + wave * 16 + h * 8, (seq.end - 1) & ~7);
+        return min(t * kTile + first_row + h * 8, (seq.end - 1) & ~7);
     };
-    // page number of group `lane % 2`, as a load of vectors: one by scalars would make every wait for LDS behind it wait for it as well
-    auto page_of = [&](int t) -> int { return entries[__umulhi(first_of(t, lane_now() & 1) >> 2, p.page_magic)]; };
-    auto source = [&](int t, int h, int page, int stage) -> Source {
-        const int entry = __builtin_amdgcn_readlane(page, h), left = min(seq.end, t1 * kTile) - (t * kTile + wave * 16 + h * 8);
+    auto row_of = [&](uint32_t entry, uint32_t pos) -> uint64_t {       // where position pos, whose page is `entry`, lies in the pool
+        return (uint64_t)entry * (uint32_t)p.page + (pos - __umulhi((pos & ~7u) >> 2, p.page_magic) * p.page);
+    };
+    // page number of group `lane % kGroups`, as a load of vectors: one by scalars would make every wait for LDS behind it wait for it as well
+    auto page_of = [&](int t) -> int { return entries[__umulhi(first_of(t, lane_now() & (kGroups - 1)) >> 2, p.page_magic)]; };
+    auto source = [&](int t, int h, int page, uint32_t stage) -> Source {
+        const int entry = __builtin_amdgcn_readlane(page, h), left = min(seq.end, t1 * kTile) - (t * kTile + first_row + h * 8);
         // without branches, which would part the products that this stands beside (an empty buffer's address is not looked at)
         const int64_t some = -(int64_t)((left > 0) & ((uint32_t)entry < (uint32_t)p.pages));
-        const uint32_t pos = first_of(t, h);
-        const uint64_t r = (uint64_t)(uint32_t)entry * (uint32_t)p.page + (pos - __umulhi(pos >> 2, p.page_magic) * p.page);
+        const uint64_t r = row_of(entry, first_of(t, h));
         const int rows = min(8, left) & (int)some;
         const uint64_t scales = (((uint64_t)(uintptr_t)p.scales + r * 4) & some) | ((uint64_t)(uintptr_t)nothing & ~some);
         return Source{ buffer_of(p.kv + r * kC, rows * kC), buffer_of(p.pe + r * (kRope * 2), rows * (kRope * 2)), (const float*)(uintptr_t)scales,
-                       max(rows, 1) - 1, lds0 + stage * kStage };
+                       max(rows, 1) - 1, stage };
     };
     // where a lane reads of two rows of latents
     auto latent_off = [&]() -> uint32_t { const int lane = lane_now(); return (lane >> 5) * kC + (((lane & 31) ^ (lane >> 5 << 2)) << 4); };
     auto issue = [&](const Source& s, uint32_t latents, auto group, auto which) {
         constexpr int n = decltype(which)::value, h = decltype(group)::value;
         if constexpr (n < 4) {
-            copy16_buffer_at(s.kv, latents, n * (2 * kC), s.at + wave * kRows16 + pair_off(4 * h + n));
+            copy16_buffer_at(s.kv, latents, n * (2 * kC), s.at + (FEW ? h >> 1 : wave) * kRows16 + pair_off(4 * (h & 1) + n));
         } else if constexpr (n == 4) {                  // a key's chunk c at c ^ r / 2 (low three bits)
             const int lane = lane_now();
-            copy16_buffer_at(s.pe, (lane >> 3) * (kRope * 2) + (((lane & 7) ^ (4 * h + (lane >> 4))) << 4), 0, s.at + kRopeOff + (wave * 16 + 8 * h) * (kRope * 2));
+            if constexpr (!FEW || h >= 4)
+                copy16_buffer_at(s.pe, (lane >> 3) * (kRope * 2) + (((lane & 7) ^ (4 * (h & 1) + (lane >> 4))) << 4), 0,
+                                 s.at + kRopeOff + (FEW ? 8 * (h - 4) : wave * 16 + 8 * h) * (kRope * 2));
         } else {
-            copy4(s.scales, min(lane_now() & 7, s.last) * 4, s.at + kScaleOff + (wave * 2 + h) * 256);
+            copy4(s.scales, min(lane_now() & 7, s.last) * 4, s.at + kScaleAt + (FEW ? h : wave * 2 + h) * 256);
         }
     };
-    auto copy_tile = [&](int t, int stage) {
-        const int page = page_of(t);
-        unrolled<2>([&](auto h) {
+    auto copy_tile = [&](int t, uint32_t stage, int page) {
+        unrolled<kGroups>([&](auto h) {
             const Source s = source(t, h, page, stage);
             const uint32_t latents = latent_off();
             unrolled<6>([&](auto n) { issue(s, latents, h, n); });
@@ -220,17 +234,23 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
         __builtin_amdgcn_s_waitcnt(0x0f70);             // vmcnt(0)
         barrier_no_fence();
     };
-    copy_tile(t0, 0);
-    copy_tile(t0 + 1, 1);
-
-    if (row0 >= live) {                                 // no rows: the others' copies
-        arrived();
-        for (int t = t0, st = 2; t < t1; ++t, st = st == 2 ? 0 : st + 1) {
+    uint32_t own = lds0 + wave * kFewStage;             // FEW: the wavefront's stage
+    int page = 0;
+    if constexpr (FEW) {
+        page = page_of(t0 + wave);
+        if (t0 + wave < t1) copy_tile(t0 + wave, own, page);
+    } else {
+        copy_tile(t0, lds0, page_of(t0));
+        copy_tile(t0 + 1, lds0 + kStage, page_of(t0 + 1));
+        if (row0 >= live) {                             // no rows: the others' copies
             arrived();
-            copy_tile(t + 2, st);
+            for (int t = t0, st = 2; t < t1; ++t, st = st == 2 ? 0 : st + 1) {
+                arrived();
+                copy_tile(t + 2, lds0 + st * kStage, page_of(t + 2));
+            }
+            arrived();
+            return;
         }
-        arrived();
-        return;
     }
 
     v8i Q[2][8];                                        // first and second codes; K step n: features 64 n + 32 g .. + 31
@@ -266,7 +286,7 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     const auto row_off = [](int r) { return (r >> 1) * kPair + ((r >> 2) & 1) * 16 + (r & 1) * kC; };      // of 0 .. 15
     // K step n is 64 bytes; of an odd row, steps n and n + 1 of even n are exchanged.  Values: 32 bytes for 32 features, in odd rows two and two exchanged.
     const uint32_t kaddr = (i >> 4) * kRows16 + row_off(i & 15) + 32 * g;
-    const uint32_t raddr = kRopeOff + i * 128 + ((g ^ ((i >> 1) & 7)) << 4);    // ^ 2 s << 4
+    const uint32_t raddr = kRopeOff - (FEW ? 32 * kRope * 2 : 0) + i * 128 + ((g ^ ((i >> 1) & 7)) << 4);    // ^ 2 s << 4
     // transposed reads: lane group q2 of a half takes 16 features; its lane l fetches eight of row l / 2 of 4 g .. + 3, 8 + 4 g .. + 3 of 16 rows
     const int l15 = lane & 15, q2 = (lane >> 4) & 1, vrow = 8 * (l15 >> 3) + 4 * g + ((l15 >> 1) & 3);
     const uint32_t vaddr = row_off(vrow) + 16 * q2 + 8 * (l15 & 1);
@@ -304,7 +324,7 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     float sc;                                           // the scale that the next scores need
     auto scale_at = [&](uint32_t stage, int half) -> float {
         const int i = lane_now() & 31;
-        return *(lds_f32)(uintptr_t)(stage + (i >> 3) * 256 + (i & 7) * 4 + kScaleOff + half * 1024);
+        return *(lds_f32)(uintptr_t)(stage + (i >> 3) * 256 + (i & 7) * 4 + kScaleAt + half * 1024);
     };
     auto look_at_scale = [&](int half) {
         ks[half] = (int)(f32_as_u32(sc) >> 23 & 0xff);  // (NaN: 255, which makes the products NaN)
@@ -321,7 +341,7 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     auto soften = [&](int t, uint32_t stage, auto half, auto step) {
         constexpr int h = decltype(half)::value, x = decltype(step)::value;
         v16f& s = S[h];
-        if constexpr (x == 0) scales_at = stage + (lane_now() >> 5) * 16 + kScaleOff;
+        if constexpr (x == 0) scales_at = stage + (lane_now() >> 5) * 16 + kScaleAt;
         if constexpr (x < 8 && x % 2 == 0) w[x / 2] = *(lds_v4f)(uintptr_t)(scales_at + (4 * h + x / 2) * 256);
         if constexpr (x == 1) {
             asm volatile("" : "+v"(s));                 // (behind two more MFMAs: the scores are there)
@@ -403,7 +423,7 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
             else if constexpr (x < 16) mfma64_next<(n & 3)>(s, ring[n & 1], Q[x & 1][n], ks[h], qs[x & 1][n >> 2]);
             else mfma32_next(s, rope[x - 16], turned[x - 16]);
             if constexpr (x < 12 && (x & 1)) ring[n & 1] = key(keys, h, n + 2);
-            if constexpr (x >= 12 && x < 16) rope[x - 12] = rope_key(ropes, h, x - 12);
+            if constexpr (x >= 12 && x < 16 && !(FEW && h == 0)) rope[x - 12] = rope_key(ropes, h, x - 12);
             beside(step);
             if constexpr (x == 14) tail(std::integral_constant<int, 0>());
             if constexpr (x == 16) tail(std::integral_constant<int, 1>());
@@ -411,42 +431,13 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
         });
     };
 
-    typedef std::integral_constant<int, 0> First;
-    typedef std::integral_constant<int, 1> Second;
-    int page = page_of(t0 + 2);
-    arrived();
-    sc = scale_at(lds0, 0);
-    ring[0] = key(keys_at(lds0), 0, 0);
-    ring[1] = key(keys_at(lds0), 0, 1);
-    look_at_scale(0);
-    sc = scale_at(lds0, 1);
-    score(lds0, First(), [](auto) {}, [&](auto k) { ring[k] = key(keys_at(lds0), 1, k); });
-    look_at_scale(1);
-    int st = 0;
-    for (int t = t0;; ++t) {
-        const int st_next = st == 2 ? 0 : st + 1, st_free = st_next == 2 ? 0 : st_next + 1;
-        const uint32_t base = lds0 + st * kStage, next = lds0 + st_next * kStage;
-        const int page_now = page;
-        // C.  Behind its barrier the next tile is there, and the stage of the one before is free.
-        score(base, Second(), [&](auto step) {
-            soften(t, base, First(), step);
-            if constexpr (decltype(step)::value == 13) {
-                arrived();
-                page = page_of(t + 3);
-                sc = scale_at(next, 0);
-            }
-        }, [&](auto k) { ring[k] = key(keys_at(next), 0, k); });
-        // A, also behind the last tile (of zeros: a path without it would let the compiler copy scores before they are there)
-        look_at_scale(0);
-        score(next, First(), [&](auto step) { soften(t, base, Second(), step); }, [&](auto k) { ring[k] = value(values_at(base), k); });
-        // B
+    // The weighted sums of the tile at `base`, whose first two values are in the ring
+    auto weigh = [&](bool first, uint32_t base, auto beside) {
         const Two values = values_at(base);
-        Source ahead;
-        uint32_t latents;
         const int one = 127, g = lane_now() >> 5, e[2] = { g ? pe[1] : pe[0], (g ? pe[1] : pe[0]) - 4 };
         if (behind) {
             behind = false;
-            if (t > t0) {
+            if (!first) {
 #pragma unroll
                 for (int d = 0; d < 16; ++d) scale_agprs(O[d], shrink);
                 asm volatile("s_nop 7" ::: "memory");
@@ -456,55 +447,169 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
         unrolled<32>([&](auto step) {
             constexpr int x = decltype(step)::value, f = x >> 1;
             mfma64_sum(O[f], ring[f & 1], P[x & 1], one, e[x & 1]);
-            if constexpr (x & 1) ring[f & 1] = f < 14 ? value(values, f + 2) : key(keys_at(next), 1, f - 14);
-            // copies of the tile after the next, one behind a product
-            if constexpr (x == 0 || x == 8) {
-                ahead = source(t + 2, x / 8, page_now, st_free);
-                latents = latent_off();
-            }
-            if constexpr (x >= 1 && x < 7) issue(ahead, latents, First(), std::integral_constant<int, x - 1>());
-            if constexpr (x >= 9 && x < 15) issue(ahead, latents, Second(), std::integral_constant<int, x - 9>());
-            if constexpr (x == 20) sc = scale_at(next, 1);
+            if constexpr ((x & 1) && f < 14) ring[f & 1] = value(values, f + 2);
+            beside(step);
             __builtin_amdgcn_sched_barrier(0);
         });
 #pragma unroll
         for (int d = 0; d < 16; ++d) asm volatile("" : "+a"(O[d]));     // (the sums stay where they are)
-        if (t + 1 == t1) break;
+    };
+
+    typedef std::integral_constant<int, 0> First;
+    typedef std::integral_constant<int, 1> Second;
+    if constexpr (FEW) {
+        // A wavefront by itself takes every fourth tile, from its own stage, without barriers: the scores of the first half, those of the second
+        // beside the first's exponentials, the second's exponentials, the weighted sums.
+        for (int t = t0 + wave; t < t1; t += 4) {
+            asm volatile("" : "+s"(own));               // (what is formed from it is not kept through the loop: there are no registers for that)
+            {
+                const int lane = lane_now(), i = lane & 31, entry = __shfl(page, i >> 3);
+                const uint32_t pos = t * kTile + i;
+                const bool there = (int)pos < seq.end && (uint32_t)entry < (uint32_t)p.pages;
+                const v4u* src = there ? (const v4u*)(p.pe + row_of(entry, pos) * (kRope * 2)) : nothing_key;
+#pragma unroll
+                for (int s = 0; s < 4; ++s) rope[s] = src[2 * s + (lane >> 5)];
+            }
+            page = page_of(t + 4);
+            __builtin_amdgcn_s_waitcnt(0x0f70);         // vmcnt(0)
+            asm volatile("" ::: "memory");
+            sc = scale_at(own, 0);
+            ring[0] = key(keys_at(own), 0, 0);
+            ring[1] = key(keys_at(own), 0, 1);
+            look_at_scale(0);
+            sc = scale_at(own, 1);
+            score(own, First(), [](auto) {}, [&](auto k) { ring[k] = key(keys_at(own), 1, k); });
+            look_at_scale(1);
+            score(own, Second(), [&](auto step) { soften(t, own, First(), step); }, [&](auto k) { ring[k] = value(values_at(own), k); });
+            scores_ready(S[1]);
+            scores_ready(S[1]);
+            unrolled<17>([&](auto step) {
+                soften(t, own, Second(), step);
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            weigh(t == t0 + wave, own, [](auto) {});
+            if (t + 4 < t1) copy_tile(t + 4, own, page);                // (every read of the stage has been used)
+        }
+    } else {
+        page = page_of(t0 + 2);
+        arrived();
+        sc = scale_at(lds0, 0);
+        ring[0] = key(keys_at(lds0), 0, 0);
+        ring[1] = key(keys_at(lds0), 0, 1);
+        look_at_scale(0);
+        sc = scale_at(lds0, 1);
+        score(lds0, First(), [](auto) {}, [&](auto k) { ring[k] = key(keys_at(lds0), 1, k); });
         look_at_scale(1);
-        st = st_next;
+        int st = 0;
+        for (int t = t0;; ++t) {
+            const int st_next = st == 2 ? 0 : st + 1, st_free = st_next == 2 ? 0 : st_next + 1;
+            const uint32_t base = lds0 + st * kStage, next = lds0 + st_next * kStage;
+            const int page_now = page;
+            // C.  Behind its barrier the next tile is there, and the stage of the one before is free.
+            score(base, Second(), [&](auto step) {
+                soften(t, base, First(), step);
+                if constexpr (decltype(step)::value == 13) {
+                    arrived();
+                    page = page_of(t + 3);
+                    sc = scale_at(next, 0);
+                }
+            }, [&](auto k) { ring[k] = key(keys_at(next), 0, k); });
+            // A, also behind the last tile (of zeros: a path without it would let the compiler copy scores before they are there)
+            look_at_scale(0);
+            score(next, First(), [&](auto step) { soften(t, base, Second(), step); }, [&](auto k) { ring[k] = value(values_at(base), k); });
+            // B
+            Source ahead;
+            uint32_t latents;
+            weigh(t == t0, base, [&](auto step) {
+                constexpr int x = decltype(step)::value;
+                if constexpr (x == 29 || x == 31) ring[x >> 1 & 1] = key(keys_at(next), 1, (x >> 1) - 14);
+                // copies of the tile after the next, one behind a product
+                if constexpr (x == 0 || x == 8) {
+                    ahead = source(t + 2, x / 8, page_now, lds0 + st_free * kStage);
+                    latents = latent_off();
+                }
+                if constexpr (x >= 1 && x < 7) issue(ahead, latents, First(), std::integral_constant<int, x - 1>());
+                if constexpr (x >= 9 && x < 15) issue(ahead, latents, Second(), std::integral_constant<int, x - 9>());
+                if constexpr (x == 20) sc = scale_at(next, 1);
+            });
+            if (t + 1 == t1) break;
+            look_at_scale(1);
+            st = st_next;
+        }
     }
 
     asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");  // (the last sums are there)
+#pragma unroll
+    for (int d = 0; d < 16; ++d) asm volatile("" : "+a"(O[d]));
     const v2f parts = halves32(l);
     l = parts.x + parts.y;
     const int last_lane = lane_now(), i2 = last_lane & 31, g2 = last_lane >> 5;
-    const int64_t slot = ((int64_t)range * p.blocks + blk) * 128 + wave * 32;   // the wavefront's rows among all
-    if (g2 == 0) p.ml[slot + i2] = v2f{ off, l };
-    arrived();                                          // (copies past the range are still on their way into the stages)
+    const int64_t slot = ((int64_t)range * p.blocks + blk) * 128 + (FEW ? 0 : wave * 32);       // the wavefront's rows among all
+    float factor = 1.f;                                 // FEW: to the wavefronts' common offset
+    if constexpr (FEW) {
+        __syncthreads();                                // the stages are free
+        v2f* stats = (v2f*)lds;
+        if (g2 == 0) stats[wave * 32 + i2] = v2f{ off, l };
+        __syncthreads();
+        float top = kNoScore, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) top = fmaxf(top, stats[w * 32 + i2].x);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) sum += stats[w * 32 + i2].y * __builtin_amdgcn_exp2f(stats[w * 32 + i2].x - top);
+        factor = __builtin_amdgcn_exp2f(off - top);
+        if (wave == 0 && g2 == 0) p.ml[slot + i2] = v2f{ top, sum };
+    } else {
+        if (g2 == 0) p.ml[slot + i2] = v2f{ off, l };
+        arrived();                                      // (copies past the range are still on their way into the stages)
+    }
     // The sums leave as rows, which fold reads whole: 64 features of 32 rows at a time through LDS (16-byte chunks xor-ed with the row), so that a
     // store writes four pieces of 256 bytes; rows that nobody reads stay here.
-    float* dst = p.part + (slot + (last_lane >> 4)) * kC + (last_lane & 15) * 4;
-    auto put = [&](int d2) {                            // two buffers a wavefront: the next 64 features are written while these are read
+    auto put = [&](int d2, uint8_t* at) {
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
             const v16f& o = O[2 * d2 + (c >> 2)];
             const int e = 4 * (c & 3);
-            *(v4f*)(lds + wave * 16384 + (d2 & 1) * 8192 + i2 * 256 + (((2 * c + g2) ^ (i2 & 15)) << 4)) = v4f{ o[e], o[e + 1], o[e + 2], o[e + 3] };
+            v4f x = { o[e], o[e + 1], o[e + 2], o[e + 3] };
+            if constexpr (FEW) x *= factor;
+            *(v4f*)(at + i2 * 256 + (((2 * c + g2) ^ (i2 & 15)) << 4)) = x;
         }
     };
-    put(0);
+    auto taken = [&](const uint8_t* at, int r, int c) -> v4f { return *(const v4f*)(at + r * 256 + ((c ^ (r & 15)) << 4)); };
+    if constexpr (FEW) {                                // the four wavefronts' sums meet there
+        const int r0 = wave * 4 + (last_lane >> 4), c = last_lane & 15;
+        float* dst = p.part + (slot + r0) * kC + c * 4;
+        uint8_t* sums = lds + 4096;
+        put(0, sums + wave * 8192);
 #pragma unroll
-    for (int d2 = 0; d2 < 8; ++d2) {
-        v4f x[8];
+        for (int d2 = 0; d2 < 8; ++d2) {                // two buffers a wavefront: the next 64 features are written while these are read
+            const uint8_t* at = sums + (d2 & 1) * 32768;
+            __syncthreads();
+            v4f x[2];
 #pragma unroll
-        for (int n = 0; n < 8; ++n) {
-            const int r = 4 * n + (last_lane >> 4);
-            x[n] = *(const v4f*)(lds + wave * 16384 + (d2 & 1) * 8192 + r * 256 + (((last_lane & 15) ^ (r & 15)) << 4));
+            for (int n = 0; n < 2; ++n) {
+                x[n] = taken(at, r0 + 16 * n, c);
+#pragma unroll
+                for (int w = 1; w < 4; ++w) x[n] += taken(at + w * 8192, r0 + 16 * n, c);
+            }
+            if (d2 < 7) put(d2 + 1, sums + (~d2 & 1) * 32768 + wave * 8192);
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+                if (r0 + 16 * n < live) *(v4f*)(dst + n * 16 * kC + d2 * 64) = x[n];
         }
-        if (d2 < 7) put(d2 + 1);
+    } else {
+        float* dst = p.part + (slot + (last_lane >> 4)) * kC + (last_lane & 15) * 4;
+        uint8_t* at = lds + wave * 16384;
+        put(0, at);
 #pragma unroll
-        for (int n = 0; n < 8; ++n)
-            if (row0 + 4 * n + (last_lane >> 4) < live) *(v4f*)(dst + n * 4 * kC + d2 * 64) = x[n];
+        for (int d2 = 0; d2 < 8; ++d2) {
+            v4f x[8];
+#pragma unroll
+            for (int n = 0; n < 8; ++n) x[n] = taken(at + (d2 & 1) * 8192, 4 * n + (last_lane >> 4), last_lane & 15);
+            if (d2 < 7) put(d2 + 1, at + (~d2 & 1) * 8192);
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+                if (row0 + 4 * n + (last_lane >> 4) < live) *(v4f*)(dst + n * 4 * kC + d2 * 64) = x[n];
+        }
     }
 }
 
@@ -560,12 +665,15 @@ int launch_mla_decode_paged(const void* q, const void* freqs, const dsv3_mla_pag
     const bool pack = batch * tokens <= 16;
     const int rc = launch_wkv_b_absorb_q_codes(q, (int64_t)heads * kQd, kQd, w, ws, wsp, wsp + space.exponents, pack, batch, tokens, (int)plan.blocks, heads, st);
     if (rc != DSV3_OK) return rc;
-    static void (*const kernels[2])(PagedArgs) = { mla_paged_kernel<false>, mla_paged_kernel<true> };
-    static LdsGrant grant[2];
-    static_assert(kLds <= 160 * 1024 && 4 * 16384 <= kStages * kStage, "the sums leave through the stages");
-    if (!grant[pack].ensure((const void*)kernels[pack], kLds)) return DSV3_ERR_LAUNCH;
+    const bool few = rows <= 32;
+    static void (*const kernels[2][2])(PagedArgs) = { { mla_paged_kernel<false, false>, mla_paged_kernel<true, false> },
+                                                      { mla_paged_kernel<false, true>, mla_paged_kernel<true, true> } };
+    static LdsGrant grant[2][2];
+    static_assert(kLds <= 160 * 1024 && kFewLds <= 160 * 1024 && 4 * 16384 <= kStages * kStage && 4096 + 2 * 32768 <= kFewLds, "the sums leave through the stages");
+    const int lds = few ? kFewLds : kLds;
+    if (!grant[few][pack].ensure((const void*)kernels[few][pack], lds)) return DSV3_ERR_LAUNCH;
     const unsigned grid = (unsigned)((plan.ranges * plan.blocks + 7) / 8 * 8);
-    hipLaunchKernelGGL(kernels[pack], dim3(grid), dim3(256), kLds, st, a);
+    hipLaunchKernelGGL(kernels[few][pack], dim3(grid), dim3(256), lds, st, a);
     FoldArgs f = {};
     f.part = a.part; f.ml = a.ml; f.plan = a.plan; f.counts = counts; f.w = (const uint8_t*)w; f.ws = ws; f.y = y; f.ys = ys;
     f.tokens = (int)(batch * tokens); f.per_seq = (int)tokens; f.heads = heads; f.rows = 128; f.blocks = a.blocks;

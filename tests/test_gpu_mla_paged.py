@@ -329,6 +329,11 @@ ATTEND = [(1, 1, 1, 1, 8, None), (1, 1, 128, 31, 64, None), (2, 1, 128, 33, 8, N
           (9, 2, 64, 333, 16, "tree"), (20, 1, 16, 3000, 32, None), (130, 3, 64, 200, 64, "tree"), (1, 2, 32, 64, 64, None)]
 
 
+# up to 32 (token, head) rows a sequence, whose positions the wavefronts share: none for some of them, many, several tokens, heads that do not divide 32
+ATTEND += [(2, 8, 4, 300, 24, "tree"), (3, 16, 2, 700, 64, "any"), (2, 32, 1, 130, 8, "tree"), (1, 1, 32, 128, 16, None), (1, 1, 32, 129, 16, None),
+           (4, 2, 16, 5000, 40, None), (7, 3, 10, 260, 64, "any"), (1, 1, 33, 500, 64, None), (600, 1, 16, 40, 8, None), (2, 1, 16, 20000, 64, None)]
+
+
 @pytest.mark.parametrize("grow", [False, True])
 @pytest.mark.parametrize("b,s,h,context,page,kind", ATTEND)
 def test_attention(b, s, h, context, page, kind, grow):
