@@ -1,6 +1,6 @@
 // Attention of MLA.forward for one new token or a tree of drafted ones per sequence (reference: inference/model.py:480-497), on the cache
 // in pages of e4m3 rows (mla_paged.hip), in the absorbed form of mla_decode.hip: behind the query's fold through wkv_b
-//   attend   one range of a sequence's positions for 128 or 64 of its (token, head) rows: scores, softmax, weighted sum; binary32 partial sums
+//   attend   one range of a sequence's positions for 128 of its (token, head) rows: scores, softmax, weighted sum; binary32 partial sums
 //   fold     mla_fold.hpp
 // The matrix cores take the codes as they are.  What meets them is two codes an element as well (split_codes), with scales of powers of two that
 // the products apply: the folded query, split by the kernel that folds it (wkv_b_absorb.hip), and the exponentials times their
@@ -73,9 +73,9 @@ __device__ __forceinline__ int wave_scan(int v) {
 __device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
 
 // Which positions a workgroup takes.  The lengths are on the device, so every workgroup divides the work by itself: `per` tiles a
-// range, the fewest with which all sequences' ranges are at most p.ranges, ranges numbered through the sequences; then rounded up to a MULTIPLE.
+// range, the fewest with which all sequences' ranges are at most p.ranges, ranges numbered through the sequences.
 struct Share { int b, first, ranges, per, used; };      // sequence (-1: none), its first range and ranges, tiles a range, ranges of all
-template <int MULTIPLE, class F> __device__ __forceinline__ Share share_of(const PagedArgs& p, int lane, F which, bool write_plan) {
+template <class F> __device__ __forceinline__ Share share_of(const PagedArgs& p, int lane, F which, bool write_plan) {
     auto tiles = [&](int b) -> int {
         if (b >= p.batch) return 0;
         const SeqSpan s = seq_span(p.starts[b], p.counts[b], p.tokens, p.positions);
@@ -96,10 +96,6 @@ template <int MULTIPLE, class F> __device__ __forceinline__ Share share_of(const
         // a sequence's last range is half full on average: what these take off the ranges does not change with `per`
         const int lost = s.used - all / per, left = max(1, p.ranges - lost);
         s.per = max(per + 1, min(all / left, per + per / 4));
-    }
-    if constexpr (MULTIPLE > 1) {
-        const int per = s.per = (s.per + MULTIPLE - 1) / MULTIPLE * MULTIPLE;
-        s.used = sum([per](int t) { return (t + per - 1) / per; });
     }
     const int range = which(s.used);
     int base = 0;
@@ -159,7 +155,16 @@ __device__ __forceinline__ v8i join(v4u a, v4u b) {
 //   C  scores of the second half      | exponentials of the first half
 //   A  scores of the next tile's first half | exponentials of the second half
 //   B  weighted sums of the tile      | copies of the tile after the next
-// Measured (us, the form before): one sequence of 61 tokens x 128 heads at 32768 positions 542 -> ...
+// Measured: one sequence of 61 tokens x 128 heads at 32768 positions 410 us, 1.28 PFLOP/s of the bf16 products that the pairs stand for (the form
+// before: 542); the matrix cores are busy 2/3 of the time.  Without the copies of all but the first rows it would be 40 us less wherever they
+// are issued, without the exponentials and their codes 65.  A compute unit that does one tile takes 12 us: 1.2 to find it, 3.2 until it is there with
+// the queries, 4 for the products, 3.2 for writing 128 x 512 sums.
+//
+// FEW (up to 32 rows a sequence, 16 heads of one token say): the wavefronts share the positions in place of the rows, each with a stage for
+// itself and no barrier; the products of one stand beside the copies and exponentials of the others, and the four sums meet in LDS.  64
+// sequences x 16 heads at up to 8192 positions (147 MB): 50 us, three quarters of what the memory gives; with one wavefront at work
+// and the others copying for it 61.  Blocks of 32 rows do not pay where there are more: 32 sequences x 128 heads at up to 4096 positions 57.4 us for the
+// whole call and 56.5 with blocks of 128, one sequence at 700 26.6 and 26.3.
 template <bool PACK, bool FEW>
 __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
@@ -167,7 +172,7 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     const int i = lane & 31, g = lane >> 5;
     // a contiguous run of the ranges in use per XCD, the row blocks of a range next to each other: its rows are in the XCD's L2
     int unit = -1;
-    const Share mine = share_of<FEW ? 4 : 1>(p, lane, [&](int used) -> int {
+    const Share mine = share_of(p, lane, [&](int used) -> int {
         const int T = used * p.blocks, q = T / 8, r = T % 8, x = blockIdx.x % 8, k = blockIdx.x / 8;
         if (k < q + (x < r)) unit = x * q + min(x, r) + k;
         return unit < 0 ? -1 : unit / p.blocks;
