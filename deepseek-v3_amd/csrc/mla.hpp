@@ -22,9 +22,10 @@ __device__ __forceinline__ void copy16(const void* base, uint32_t lane_off, uint
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
                  :: "v"(lane_off), "s"(base), "s"(lds_addr) : "memory", "m0");
 }
-// 256 bytes global -> LDS: lane l's four at base + lane_off land at lds_addr + 4 l
+// 256 bytes global -> LDS: lane l's four at base + lane_off land at lds_addr + 4 l.  (Here and in copy16_buffer_at the wait is as long as one on scalar
+// registers that a vector instruction has just written has to be: the compiler does not look into the block.)
 __device__ __forceinline__ void copy4(const void* base, uint32_t lane_off, uint32_t lds_addr) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1"
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dword %0, %1"
                  :: "v"(lane_off), "s"(base), "s"(lds_addr) : "memory", "m0");
 }
 // copy16 through a buffer descriptor (the range check answers requests past its end with zeros), into LDS at lds_addr + IMM
@@ -36,9 +37,9 @@ template <int IMM> __device__ __forceinline__ void copy16_buffer(v4i buffer, uin
     asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
                  :: "v"(lane_off), "s"(buffer), "s"(lds_addr), "n"(IMM) : "memory", "m0", "scc");
 }
-// the same from lane_off + off
+// the same from lane_off + off, which the range check takes together
 __device__ __forceinline__ void copy16_buffer_at(v4i buffer, uint32_t lane_off, uint32_t off, uint32_t lds_addr) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %3 offen lds"
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dwordx4 %0, %1, %3 offen lds"
                  :: "v"(lane_off), "s"(buffer), "s"(lds_addr), "s"(off) : "memory", "m0");
 }
 // f(integral_constant 0), .., f(integral_constant N - 1)
