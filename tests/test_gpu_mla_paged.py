@@ -367,7 +367,7 @@ def test_attention_quantised_is_the_rounded_result_quantised(b, s, h, context, p
     assert torch.equal(_bits(y), _bits(torch.ops.dsv3fp8.mla_decode_paged(*args)))          # and the same again
 
 
-@pytest.mark.parametrize("h,page", [(128, 64), (6, 24)])
+@pytest.mark.parametrize("h,page", [(128, 64), (6, 24), (2, 40)])
 def test_rows_that_are_not_finite_reach_those_who_see_them(h, page):
     """A latent of NaN (stored as zeros and a scale of NaN) and a key of NaN or infinity, in a drafted branch: the tokens of other branches do
     not notice; then one in the context, which everybody sees."""
@@ -398,14 +398,15 @@ def test_rows_that_are_not_finite_reach_those_who_see_them(h, page):
     assert torch.isnan(got[0]).all() and torch.equal(_bits(got[1]), _bits(clean[1]))
 
 
+@pytest.mark.parametrize("h", [20, 8])
 @pytest.mark.parametrize("page", [8, 40, 64])
-def test_attention_skips_what_is_no_page(page):
-    args, seen = _attention_case(3, 4, 20, 230, page, "tree", 2)
+def test_attention_skips_what_is_no_page(page, h):
+    args, seen = _attention_case(3, 4, h, 230, page, "tree", 2)
     pages = args[3].size(0)
     for i, k, entry in ((0, 1, -1), (0, 2, pages), (2, 0, 2 ** 31 - 1), (1, 0, -7)):
         if k < args[5].size(1):
             args[5][i, k] = entry
-    got = torch.ops.dsv3fp8.mla_decode_paged(*args).view(3, 4, 20, V).double()
+    got = torch.ops.dsv3fp8.mla_decode_paged(*args).view(3, 4, h, V).double()
     assert torch.isfinite(got).all() and _close(got, _attention_reference(args, seen))
 
 
@@ -427,7 +428,7 @@ def test_attention_of_nobody():
     assert torch.ops.dsv3fp8.mla_decode_paged(*args).shape == (0, 1, 16 * V)
 
 
-@pytest.mark.parametrize("b,s,h,context", [(3, 1, 128, 500), (2, 20, 16, 300)])
+@pytest.mark.parametrize("b,s,h,context", [(3, 1, 128, 500), (2, 20, 16, 300), (3, 2, 16, 700)])
 def test_a_step_captured_and_replayed(b, s, h, context):
     """Rows written, attended to and kept in one graph, on a stream of its own; two graphs; lengths, pages and queries change between replays."""
     cases = [_attention_case(b, s, h, context, 24, "tree" if s > 1 else None, seed)[0] for seed in (1, 2, 3)]
@@ -502,9 +503,10 @@ def test_two_streams_at_once():
             assert torch.equal(_bits(y), _bits(want[k]))
 
 
-def test_attention_past_32_bits_of_bytes():
+@pytest.mark.parametrize("h", [16, 8])
+def test_attention_past_32_bits_of_bytes(h):
     page, pages = 4096, 2200
-    args, seen = _attention_case(2, 3, 16, 9000, page, "tree", 6)
+    args, seen = _attention_case(2, 3, h, 9000, page, "tree", 6)
     small = args[3].size(0)
     kv = torch.zeros(pages, page, C, dtype=torch.uint8, device="cuda")
     scale, pe = torch.ones(pages, page, device="cuda"), torch.zeros(pages, page, ROPE, device="cuda").bfloat16()
@@ -512,4 +514,4 @@ def test_attention_past_32_bits_of_bytes():
     kv[pages - small:], scale[pages - small:], pe[pages - small:] = args[2].view(torch.uint8), args[3], args[4]
     table = torch.where((args[5] >= 0) & (args[5] < small), args[5] + (pages - small), -1).int()
     got = torch.ops.dsv3fp8.mla_decode_paged(*args[:2], kv.view(FP8), scale, pe, table, *args[6:])
-    assert torch.equal(_bits(got), _bits(want)) and _close(got.view(2, 3, 16, V).double(), _attention_reference(args, seen))
+    assert torch.equal(_bits(got), _bits(want)) and _close(got.view(2, 3, h, V).double(), _attention_reference(args, seen))
