@@ -23,9 +23,10 @@ struct FoldArgs {
 // the four K blocks' results meet in LDS (absorb_v_ksplit_kernel's maps, wkv_b_absorb.hip).  The 128 features
 // of a (token, head) are one quantisation block of the output projection's input.
 // Three launches were in its place (combine 5 .. 13.7 us, the product 4.5 .. 7.5, act_quant 4.2).
-// PAGED: the latents go into the product as two bf16 each, whose rounding would be as large as the result's own: the relative error (rms) of the
-// whole attention at 4096 positions is 0.0025 so and 0.0030 with one (0.0017 is the rounding of its result), and it costs 1 us of 120.  Every sequence has ranges of its own, [range][row block][row]; a row that saw no position, and one of a token that its sequence does
-// not have, gives zeros (else NaN, as softmax does).
+// PAGED: every sequence has ranges of its own, [range][row block][row]; a row that saw no position, and one of a token that its sequence does
+// not have, gives zeros (else NaN, as softmax does).  The latents go into the product as two bf16 each: rounded to one, they would be off by as
+// much as the result's own rounding.  The relative error (rms) of the whole attention at 4096 positions is 0.0025 so, 0.0030 with one (0.0017: the
+// rounding of the result alone); it costs 1 us of 120.
 template <bool QUANT, bool PAGED>
 __global__ __launch_bounds__(512, 4) void mla_fold_kernel(FoldArgs p) {
     __shared__ __attribute__((aligned(1024))) uint8_t lat[(PAGED ? 2 : 1) * 16 * 1024];         // chunk c of row r at c ^ r (low four bits); then what bf16 leaves
