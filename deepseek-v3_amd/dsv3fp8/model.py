@@ -278,6 +278,7 @@ class MLA(nn.Module):
     conditions are ``_kernels_ok``, ``_latent_kernel_ok`` and ``_attention_kernels_ok``).  Other calls run the scores, the
     softmax and the weighted sum as bf16 torch operations between the two products; ``MLA.fused = False`` takes
     the dequantise-then-einsum sequence for the products too.  Parameter names are the checkpoint's.
+    ``forward_paged`` is the layer on a cache in pages (``LatentPages``) for sequences of different lengths and drafted trees.
 
     ``wq_a`` and ``wkv_a`` read the same input.  With FP8 weights (and ``q_lora_rank`` a multiple of the block size,
     so that both keep their own scale blocks) ``stack_a()`` lays them out as one ``[q_lora_rank + kv_lora_rank +
