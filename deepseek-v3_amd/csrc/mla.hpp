@@ -23,7 +23,8 @@ __device__ __forceinline__ void copy16(const void* base, uint32_t lane_off, uint
                  :: "v"(lane_off), "s"(base), "s"(lds_addr) : "memory", "m0");
 }
 // 256 bytes global -> LDS: lane l's four at base + lane_off land at lds_addr + 4 l.  (Here and in copy16_buffer_at the wait is as long as one on scalar
-// registers that a vector instruction has just written has to be: the compiler does not look into the block.)
+// registers that a vector instruction has just written has to be, five states: the compiler does not look into the block.  copy16 and copy16_buffer wait for
+// m0 alone: scalar instructions write what they read, in all kernels of the build (tests/test_wait_states.py).)
 __device__ __forceinline__ void copy4(const void* base, uint32_t lane_off, uint32_t lds_addr) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dword %0, %1"
                  :: "v"(lane_off), "s"(base), "s"(lds_addr) : "memory", "m0");
