@@ -502,20 +502,21 @@ class MLA(nn.Module):
 
 
     def _paged_ok(self, x, freqs_cis) -> bool:
-        """What ``forward_paged`` asks of the layer beside ``_latent_kernel_ok``; the operators check their own arguments."""
+        """What ``forward_paged`` asks of the layer beside ``_latent_kernel_ok``.  The first operator, which writes the new rows, checks the cache and
+        the sequences; what only those behind it would refuse is looked at here and in ``forward_paged``."""
         wo, w = self.wo, self.wkv_b.weight
         return (not torch.is_grad_enabled() and gemm_impl == "fp8" and block_size == 128 and world_size == 1 and x.is_cuda and x.dtype == torch.bfloat16
                 and x.dim() == 3 and x.numel() > 0 and torch.get_default_dtype() == torch.bfloat16
                 and (self.qk_nope_head_dim, self.qk_rope_head_dim, self.v_head_dim, self.kv_lora_rank) == (128, 64, 128, 512)
-                and w.element_size() == 1 and w.device == x.device and _plain(wo, RowParallelLinear) and wo.weight.element_size() == 1 and wo.bias is None
+                and 1e-30 < self.softmax_scale < 1e30 and w.element_size() == 1 and w.device == x.device and _plain(wo, RowParallelLinear) and wo.weight.element_size() == 1 and wo.bias is None
                 and freqs_cis.dtype == torch.complex64 and freqs_cis.shape == (x.size(0), x.size(1), self.qk_rope_head_dim // 2))
 
     def forward_paged(self, x: torch.Tensor, cache: LatentPages, page_table: torch.Tensor, starts: torch.Tensor, counts: torch.Tensor,
                       freqs_cis: torch.Tensor, positions: int, tree: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``forward`` on a cache in pages, for sequences of different lengths: sequence i has ``starts[i]`` positions in the cache and takes
         ``counts[i]`` (up to s) new tokens behind them, x [b, s, dim].  ``starts``, ``counts`` and ``page_table`` (int32) stay on the device, so that
-        a captured step serves every length; ``positions`` is what the longest sequence has at most after the step.  ``freqs_cis`` [b, s, 32]: each
-        new token's rotation.  ``tree`` (int64 [b, s], s <= 64): bit j of token i says that it sees new token j; without one a token sees those in
+        a captured step serves every length; ``positions`` is what the longest sequence has at most after the step, up to what ``page_table`` has
+        room for (and 2^23 - 1).  ``freqs_cis`` [b, s, 32]: each new token's rotation.  ``tree`` (int64 [b, s], s <= 64): bit j of token i says that it sees new token j; without one a token sees those in
         front of it and itself.  Rows of tokens that a sequence does not have are zeros.
 
         Up to 64 new tokens, wkv_b is folded into queries and outputs and the codes are read as they lie.  More (a prompt) go through keys and
@@ -530,6 +531,13 @@ class MLA(nn.Module):
         b, s = x.size(0), x.size(1)
         if s > 64 and tree is not None:
             raise ValueError(f"MLA.forward_paged: a tree has up to 64 tokens, not {s}")
+        if page_table.dim() != 2 or page_table.size(0) != b:
+            raise ValueError(f"MLA.forward_paged: page_table must have a row for each of {b} sequences, got {tuple(page_table.shape)}")
+        room = min(page_table.size(1) * cache.kv.size(1), 0x7fffff)
+        if not 1 <= positions <= room:
+            raise ValueError(f"MLA.forward_paged: positions must be 1 to the {room} that page_table has room for, got {positions}")
+        if tree is not None and (tree.shape != (b, s) or tree.dtype != torch.int64 or tree.device != x.device or not tree.is_contiguous()):
+            raise ValueError(f"MLA.forward_paged: tree must be a contiguous int64 [{b}, {s}] on {x.device}")
         q_norm, kv_norm, q_eps, kv_eps, wq = latent
         w, w_scale, wo = self.wkv_b.weight, self.wkv_b.scale, self.wo.weight
         qq, qs = torch.ops.dsv3fp8.mla_latent_paged(linear(x, self._wa, None, self.wq_a.scale_fmt), q_norm, kv_norm, freqs_cis, cache.kv, cache.scale,

@@ -92,3 +92,41 @@ def test_calls_that_are_refused(layer, calls, monkeypatch, what):  # noqa: F811
     with torch.set_grad_enabled(what == "grad"), pytest.raises((RuntimeError, ValueError)):
         layer.forward_paged(*args, tree)
     assert not calls
+
+
+@pytest.mark.parametrize("s", [1, 3, 64, 65, 200])
+@pytest.mark.parametrize("positions", [0, -1, 129, 1 << 23, 2 ** 40])
+def test_positions_that_the_table_has_no_room_for(layer, calls, s, positions):  # noqa: F811
+    """Two pages of 64 a sequence; refused before a row is written, whatever the number of tokens."""
+    args = _arguments(2, s)
+    args[6] = positions
+    if positions >= 1 << 23:                                # a table that would have room: more than the kernels count to
+        args[2] = torch.zeros(1, 1, dtype=torch.int32).expand(2, positions // 64 + 1)
+    with torch.no_grad(), pytest.raises(ValueError, match="positions"):
+        layer.forward_paged(*args)
+    assert not calls
+
+
+@pytest.mark.parametrize("s", [3, 65])
+def test_tables_of_another_shape(layer, calls, s):  # noqa: F811
+    args = _arguments(2, s)
+    args[2] = args[2][0]
+    with torch.no_grad(), pytest.raises(ValueError, match="page_table"):
+        layer.forward_paged(*args)
+    assert not calls
+
+
+@pytest.mark.parametrize("tree", [torch.ones(2, 3), torch.ones(2, 3, dtype=torch.int32), torch.ones(3, dtype=torch.int64), torch.ones(2, 4, dtype=torch.int64),
+                                  torch.ones(1, 3, dtype=torch.int64), torch.ones(3, 2, dtype=torch.int64).t(), torch.ones(2, 3, dtype=torch.int64, device="meta")])
+def test_trees_that_are_refused_before_a_row_is_written(layer, calls, tree):  # noqa: F811
+    with torch.no_grad(), pytest.raises(ValueError, match="tree"):
+        layer.forward_paged(*_arguments(2, 3), tree)
+    assert not calls
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1, 1e-40, float("inf"), float("nan")])
+def test_scales_that_are_refused_before_a_row_is_written(layer, calls, scale):  # noqa: F811
+    layer.softmax_scale = scale
+    with torch.no_grad(), pytest.raises(RuntimeError, match="forward_paged"):
+        layer.forward_paged(*_arguments(2, 3))
+    assert not calls
