@@ -548,14 +548,19 @@ class MLA(nn.Module):
                                                               positions, self.softmax_scale)
             return fp8_gemm(yq, ys, wo, wo.scale)
         kv, pe = cache.read(page_table, starts + counts, positions)
-        new, at, parts = torch.arange(s, device=x.device), torch.arange(positions, device=x.device), []
+        at = torch.arange(max(s, positions), device=x.device)
+        new, at, pages, page = at[:s], at[:positions], *cache.scale.shape
+        # What a position adds to the scores of those who see it: nothing, or -inf where it lies in no page (its row was read as zeros).  Position 0 gets the
+        # lowest number then: beside any other its weight is zero, and who sees no other (who sees one has position 0 in a page or another) gets that row of zeros.
+        entries = page_table[:, :-(-positions // page)]
+        adds = torch.where(entries.remainder(pages) == entries, 0.0, float("-inf")).repeat_interleave(page, 1)[:, :positions]
+        adds[:, 0].clamp_(min=torch.finfo(adds.dtype).min)
+        last, parts = starts.unsqueeze(-1) + new, []        # what token t sees, itself
         for i in range(b):
-            mask = torch.zeros(s, positions, dtype=torch.bfloat16, device=x.device).masked_fill_(at > (starts[i] + new)[:, None], float("-inf"))
+            mask = torch.where(at <= last[i].unsqueeze(-1), adds[i], float("-inf"))
             parts.append(torch.ops.dsv3fp8.mla_prefill(q[i:i + 1], freqs_cis[i], kv[i:i + 1], pe[i:i + 1], w, w_scale, mask, positions, self.softmax_scale))
-        yq, ys = (torch.cat([part[k].view(torch.uint8) if k == 0 else part[k] for part in parts]) for k in (0, 1))
-        y = fp8_gemm(yq.view(torch.float8_e4m3fn), ys, wo, wo.scale)
-        there = (new < counts[:, None]) & (starts >= 0)[:, None]
-        return y.masked_fill_(~there.unsqueeze(-1), 0)
+        yq, ys = parts[0] if b == 1 else (torch.cat([part[0].view(torch.uint8) for part in parts]).view(torch.float8_e4m3fn), torch.cat([part[1] for part in parts]))
+        return fp8_gemm(yq, ys, wo, wo.scale).masked_fill_(((new >= counts.unsqueeze(-1)) | (starts < 0).unsqueeze(-1)).unsqueeze(-1), 0)
 
     def _forward_naive(self, x, q, kva, start_pos: int, freqs_cis, mask):
         """Per-head key / value caches (model.py:470-479, 488-490): the new positions' latents go through wkv_b as a

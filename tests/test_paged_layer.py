@@ -130,3 +130,31 @@ def test_scales_that_are_refused_before_a_row_is_written(layer, calls, scale):  
     with torch.no_grad(), pytest.raises(RuntimeError, match="forward_paged"):
         layer.forward_paged(*_arguments(2, 3))
     assert not calls
+
+
+def _masks(calls):
+    return [c[1][6] for c in calls if c[0] == "prefill"]
+
+
+@pytest.mark.parametrize("page,positions", [(64, 300), (8, 300), (24, 290), (512, 100), (16, 320)])
+def test_prompts_do_not_see_what_lies_in_no_page(layer, calls, page, positions):  # noqa: F811
+    """Position 0 in no page has the lowest number: nothing beside any other, a row of zeros for who sees no other."""
+    from dsv3fp8.model import LatentPages
+    width = -(-positions // page) + 1
+    args, pages = _arguments(3, 70), 2 * width
+    args[1], args[6] = LatentPages(pages, page), positions
+    table = torch.randint(0, pages, (3, width), generator=torch.Generator().manual_seed(page)).int()
+    table[0, 0], table[1, width // 2], table[1, width - 2], table[2, 0] = pages, -1, 2 ** 31 - 1, -2 ** 31
+    args[2], args[3] = table, torch.tensor([5, 0, positions - 70], dtype=torch.int32)
+    with torch.no_grad():
+        layer.forward_paged(*args)
+    masks = _masks(calls)
+    assert len(masks) == 3
+    at = torch.arange(positions)
+    for i, mask in enumerate(masks):
+        entry = table[i].long()[at // page]
+        want = torch.zeros(70, positions).masked_fill((entry < 0) | (entry >= pages), float("-inf"))
+        if not 0 <= entry[0] < pages:
+            want[:, 0] = torch.finfo(torch.bfloat16).min
+        want[at > args[3][i] + torch.arange(70)[:, None]] = float("-inf")
+        assert mask.dtype == torch.bfloat16 and mask.is_contiguous() and torch.equal(mask.float(), want)
