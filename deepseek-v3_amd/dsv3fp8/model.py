@@ -517,7 +517,8 @@ class MLA(nn.Module):
         ``counts[i]`` (up to s) new tokens behind them, x [b, s, dim].  ``starts``, ``counts`` and ``page_table`` (int32) stay on the device, so that
         a captured step serves every length; ``positions`` is what the longest sequence has at most after the step, up to what ``page_table`` has
         room for (and 2^23 - 1).  ``freqs_cis`` [b, s, 32]: each new token's rotation.  ``tree`` (int64 [b, s], s <= 64): bit j of token i says that it sees new token j; without one a token sees those in
-        front of it and itself.  Rows of tokens that a sequence does not have are zeros.
+        front of it and itself.  Rows of tokens that a sequence does not have, and of those that see nothing, are zeros.  A cached row that is not finite makes NaN
+        of the tokens that see it and of no others (up to 64 new tokens, an infinite score of the wrong sign only leaves that row out).
 
         Up to 64 new tokens, wkv_b is folded into queries and outputs and the codes are read as they lie.  More (a prompt) go through keys and
         values per head of the rows read back, sequence by sequence: at 128 heads 1 x 128 tokens at 1024 positions take 123 us so and
@@ -555,6 +556,11 @@ class MLA(nn.Module):
         entries = page_table[:, :-(-positions // page)]
         adds = torch.where(entries.remainder(pages) == entries, 0.0, float("-inf")).repeat_interleave(page, 1)[:, :positions]
         adds[:, 0].clamp_(min=torch.finfo(adds.dtype).min)
+        # A row that is not finite: zeros, so that it reaches nobody through a score that is hidden or a weight of zero, and NaN for those who see it
+        # (a latent that is not finite is NaN in all elements)
+        adds = adds.add(torch.linalg.vector_norm(pe, float("inf"), -1).add_(kv[..., 0]), alpha=0)
+        kv.nan_to_num_(0.0, 0.0, 0.0)
+        pe.nan_to_num_(0.0, 0.0, 0.0)
         last, parts = starts.unsqueeze(-1) + new, []        # what token t sees, itself
         for i in range(b):
             mask = torch.where(at <= last[i].unsqueeze(-1), adds[i], float("-inf"))

@@ -108,3 +108,51 @@ def test_prompts_over_pages_that_there_are_not(M, s, page, starts):
     for y in _both(*args):
         assert torch.isfinite(y).all() and (y[nothing] == 0).all()
         _check(y, ref)
+
+
+@pytest.mark.parametrize("what", ["token", "latent", "nan key", "inf key"])
+def test_rows_that_are_not_finite_reach_the_tokens_that_see_them(M, what):
+    """A new token of NaN in the middle of a block; rows of the prefix and of other sequences' pages likewise.  The others get the bits that they get without."""
+    s, starts = 130, (40, 0, 100)
+    layer, cache, table, x, freqs = _case(M, 7, 3, s, 24, 10, starts)
+    args = (table, _ints(*starts), _ints(s, s, 90), freqs, 230)
+    with torch.inference_mode():
+        clean = layer.forward_paged(x, _copy(cache), *args)
+    bad = [(0, 40 + 37), (1, 101)] if what == "token" else [(0, 33), (2, 99)]          # sequence, position
+    for i, at in bad:
+        row = int(table[i, at // 24]), at % 24
+        if what == "token":
+            x[i, at - starts[i], 5] = float("nan")
+        elif what == "latent":
+            cache.kv.view(torch.uint8)[row], cache.scale[row] = 0, float("nan")
+        else:
+            cache.pe[row][3] = float("nan" if what == "nan key" else "inf")
+    nan = torch.zeros(3, s, dtype=torch.bool, device="cuda")
+    for i, at in bad:
+        nan[i, max(0, at - starts[i]):] = True
+    nan[2, 90:] = False
+    for n, y in enumerate(_both(layer, x, cache, *args)):
+        if n == 0:
+            assert torch.isnan(y[nan]).all() and torch.equal(y[~nan].view(torch.int16), clean[~nan].view(torch.int16))
+        else:
+            assert torch.isfinite(y[~nan]).all()
+            assert what == "inf key" or torch.isnan(y[nan]).all()
+
+
+def test_rows_behind_a_sequence_reach_nobody(M):
+    """NaN in codes, scales and keys of all that no sequence has, as a page leaves them whose owner was another; fewer tokens than the widest sequence's."""
+    s, starts = 70, (30, 0, 65)
+    layer, cache, table, x, freqs = _case(M, 9, 3, s, 16, 10, starts)
+    counts = (s, 66, 5)
+    args = (table, _ints(*starts), _ints(*counts), freqs, 150)
+    with torch.inference_mode():
+        clean = layer.forward_paged(x, _copy(cache), *args)
+    used = torch.zeros(*cache.scale.shape, dtype=torch.bool, device="cuda")
+    for i, n in enumerate(starts):
+        for at in range(n + counts[i]):
+            used[int(table[i, at // 16]), at % 16] = True
+    cache.kv.view(torch.uint8)[~used], cache.scale[~used], cache.pe[~used] = 0x7f, float("nan"), float("nan")
+    for i, n in enumerate(counts):
+        x[i, n:] = float("nan")
+    y, pieces = _both(layer, x, cache, *args)
+    assert torch.equal(y.view(torch.int16), clean.view(torch.int16)) and torch.isfinite(pieces).all()

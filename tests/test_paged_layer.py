@@ -158,3 +158,29 @@ def test_prompts_do_not_see_what_lies_in_no_page(layer, calls, page, positions):
             want[:, 0] = torch.finfo(torch.bfloat16).min
         want[at > args[3][i] + torch.arange(70)[:, None]] = float("-inf")
         assert mask.dtype == torch.bfloat16 and mask.is_contiguous() and torch.equal(mask.float(), want)
+
+
+def test_prompts_see_rows_that_are_not_finite_and_no_others_do(layer, calls, monkeypatch):  # noqa: F811
+    """Such rows go into the attention as zeros, with NaN in the mask for those who see them."""
+    args, s, positions = _arguments(2, 70), 70, 128
+    args[3] = torch.tensor([50, 0], dtype=torch.int32)
+    kv, pe = torch.randn(2, positions, 512).bfloat16(), torch.randn(2, positions, 64).bfloat16()
+    kv[0, 7], kv[1, 40] = float("nan"), float("nan")
+    pe[0, 60, 3], pe[1, 41, 5], pe[1, 69, 63], pe[1, 100] = float("nan"), float("inf"), float("-inf"), float("nan")
+    pe[0, 1, 2], kv[0, 2, 5] = torch.finfo(torch.bfloat16).max, torch.finfo(torch.bfloat16).min
+    read = kv.clone(), pe.clone()
+    monkeypatch.setattr(torch.ops.dsv3fp8, "mla_cache_read", lambda *a: read)
+    with torch.no_grad():
+        layer.forward_paged(*args)
+    masks = _masks(calls)
+    given = [c[1] for c in calls if c[0] == "prefill"]
+    at, token = torch.arange(positions), torch.arange(s)[:, None]
+    for i, bad in enumerate(([7, 60], [40, 41, 69, 100])):
+        want = torch.zeros(s, positions)
+        want[:, bad] = float("nan")
+        want[at > args[3][i] + token] = float("-inf")
+        assert torch.equal(masks[i].isnan(), want.isnan()) and torch.equal(masks[i][~want.isnan()].float(), want[~want.isnan()].float())
+        good = torch.ones(positions, dtype=torch.bool)
+        good[bad] = False
+        for got, clean in zip(given[i][2:4], (kv[i:i + 1], pe[i:i + 1])):
+            assert got.isfinite().all() and torch.equal(got[:, good], clean[:, good])
