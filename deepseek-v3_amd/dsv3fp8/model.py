@@ -548,7 +548,7 @@ class MLA(nn.Module):
             yq, ys = torch.ops.dsv3fp8.mla_decode_paged_quant(q, freqs_cis, cache.kv, cache.scale, cache.pe, page_table, starts, counts, tree, w, w_scale,
                                                               positions, self.softmax_scale)
             return fp8_gemm(yq, ys, wo, wo.scale)
-        kv, pe = cache.read(page_table, starts + counts, positions)
+        kv, pe = cache.read(page_table, torch.full_like(starts, positions), positions)         # (what lies behind a sequence is hidden from its tokens)
         at = torch.arange(max(s, positions), device=x.device)
         new, at, pages, page = at[:s], at[:positions], *cache.scale.shape
         # What a position adds to the scores of those who see it: nothing, or -inf where it lies in no page (its row was read as zeros).  Position 0 gets the

@@ -156,3 +156,19 @@ def test_rows_behind_a_sequence_reach_nobody(M):
         x[i, n:] = float("nan")
     y, pieces = _both(layer, x, cache, *args)
     assert torch.equal(y.view(torch.int16), clean.view(torch.int16)) and torch.isfinite(pieces).all()
+
+
+def test_starts_and_counts_out_of_range(M):
+    """Counts above the rows are all rows, negative ones and those of a negative start none; a start behind the stated positions sees these and writes nothing."""
+    s, starts = 70, (60, 0, 5, 44)
+    layer, cache, table, x, freqs = _case(M, 11, 4, s, 24, 6, starts)
+    most = 2 ** 31 - 1
+    with torch.inference_mode():
+        want = layer.forward_paged(x, _copy(cache), table, _ints(*starts), _ints(s, s, s, s), freqs, 140)
+    y, pieces = _both(layer, x, cache, table, _ints(60, 0, 5, -1), _ints(most, s + 1, -most - 1, s), freqs, 140)
+    assert torch.equal(y[:2].view(torch.int16), want[:2].view(torch.int16)) and (y[2:] == 0).all()
+    assert torch.isfinite(pieces).all() and (pieces[2:] == 0).all()
+    args = (layer, x, cache, table, _ints(most, most - 69, most - 1, 44), _ints(s, s, most, s), freqs, 44)
+    ref = _reference(*args)
+    for got in _both(*args):
+        _check(got, ref)

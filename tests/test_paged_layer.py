@@ -184,3 +184,18 @@ def test_prompts_see_rows_that_are_not_finite_and_no_others_do(layer, calls, mon
         good[bad] = False
         for got, clean in zip(given[i][2:4], (kv[i:i + 1], pe[i:i + 1])):
             assert got.isfinite().all() and torch.equal(got[:, good], clean[:, good])
+
+
+@pytest.mark.parametrize("start,count", [(50, 2 ** 31 - 1), (2 ** 31 - 1, 70), (2 ** 31 - 60, 2 ** 31 - 1), (0, 71), (127, -2 ** 31), (-5, -2 ** 31)])
+def test_prompts_with_starts_and_counts_out_of_range(layer, calls, start, count):  # noqa: F811
+    """A count above the rows is all rows; positions behind the stated ones are none: what a token sees has been read, and nothing else is in its mask."""
+    args = _arguments(1, 70)
+    args[3][0], args[4][0] = start, count
+    with torch.no_grad():
+        y = layer.forward_paged(*args)
+    lengths, mask = next(c[1][4] for c in calls if c[0] == "read"), _masks(calls)[0]
+    token, at = torch.arange(70)[:, None], torch.arange(128)
+    mine = torch.arange(70) < count
+    sees = at <= start + token
+    assert lengths.dtype == torch.int32 and torch.equal(mask == 0, sees) and y.shape == (1, 70, 256)
+    assert (not mine.any() or start < 0 or int(lengths[0]) > int(sees[mine].nonzero()[:, 1].max()))
