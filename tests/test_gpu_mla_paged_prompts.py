@@ -172,3 +172,35 @@ def test_starts_and_counts_out_of_range(M):
     ref = _reference(*args)
     for got in _both(*args):
         _check(got, ref)
+
+
+def test_a_prompt_captured_and_replayed(M):
+    """One graph of a prompt's step, replayed after lengths, tables, inputs and rows that are not finite have changed on the device."""
+    s = 70
+    layer, cache, table, x, freqs = _case(M, 13, 2, s, 16, 9, (60, 20))
+    start_cache, g = _copy(cache), torch.Generator().manual_seed(3)
+    starts, counts = _ints(60, 20), _ints(s, s)
+    with torch.inference_mode():
+        layer.forward_paged(x, _copy(cache), table, starts, counts, freqs, 140)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = layer.forward_paged(x, cache, table, starts, counts, freqs, 140)
+        for step in range(6):
+            x.copy_(torch.randn(x.shape, generator=g).bfloat16())
+            if step % 2:
+                x[0, 33, 5] = float("nan")
+            starts.copy_(_ints(60 - 7 * step, 20 + step))
+            counts.copy_(_ints(s - step, s))
+            table.copy_(torch.randperm(18, generator=g).view(2, 9).int())
+            if step > 2:
+                table[1, step - 3] = -1
+            for mine, theirs in ((cache.kv.view(torch.uint8), start_cache.kv.view(torch.uint8)), (cache.scale, start_cache.scale), (cache.pe, start_cache.pe)):
+                mine.copy_(theirs)
+            other = _copy(cache)
+            graph.replay()
+            want = layer.forward_paged(x, other, table, starts, counts, freqs, 140)
+            torch.cuda.synchronize()
+            for a, c in ((y, want), (cache.pe, other.pe)):
+                assert torch.equal(a.view(torch.int16), c.view(torch.int16))
+            assert torch.isnan(want[0, 33:s - step]).all() == bool(step % 2) and torch.isfinite(want[0, :33]).all()
