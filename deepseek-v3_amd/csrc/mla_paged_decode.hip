@@ -52,7 +52,7 @@ struct PagedArgs {
 
 // The scale of rows that are no page's, which no row has (positive: exponentials times it keep their sign).
 constexpr float kNothing = 0x1p-126f;
-constexpr float kNoScore = -0x1p100f;                   // the exponents' offset in front of a row's first score
+constexpr float kNoScore = -0x1.fffffep127f;            // the exponents' offset in front of a row's first score
 __device__ const float nothing[8] = { kNothing, kNothing, kNothing, kNothing, kNothing, kNothing, kNothing, kNothing };
 __device__ const v4u nothing_key[kRope / 8] = {};
 
@@ -339,10 +339,10 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     // The exponentials of half h, in 17 steps that stand beside the MFMAs of 20.
     v4f w[4];
     uint32_t largest = 0u;                              // bits of the largest exponential times its scale
-    float pm = 0.f, shrink = 1.f, ex[2];
+    float pm = 0.f, shrink = 1.f, ex[2], times = 0.f, less = 0.f;       // exponentials are of 2^(score * times - less)
     uint32_t scales_at = 0u;
     const uint64_t alive = __ballot(row0 + i < live);
-    bool behind = false;                                // the sums are still to be multiplied with `shrink`
+    bool behind = false, far = false;                   // the sums are still to be multiplied with `shrink`; some row's offset is beyond 2^24
     auto soften = [&](int t, uint32_t stage, auto half, auto step) {
         constexpr int h = decltype(half)::value, x = decltype(step)::value;
         v16f& s = S[h];
@@ -384,6 +384,20 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
                 off = on;
                 shrink = behind ? shrink * a : a;       // (the sums follow in front of phase B)
                 behind = true;
+                far = __ballot(__builtin_fabsf(off) > 0x1p24f && off != kNoScore) & alive;
+            }
+            times = p.scale;
+            less = off;
+            if (far) {
+                // `off` is a rounded score: up to 2^24 it is a whole number that a fused product minus it differs from by 1 at most, but far beyond, the
+                // difference would be any power of two.  There the score's product is rounded as the offset was, so that the largest exponential is 1.
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float x = s[e] * p.scale;
+                    s[e] = __builtin_fabsf(off) > 0x1p24f ? x - off : __builtin_fmaf(s[e], p.scale, -off);
+                }
+                times = 1.f;
+                less = 0.f;
             }
             largest = 0u;
         }
@@ -398,7 +412,7 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
         }
         if constexpr (x >= 3 && x < 11) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) ex[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * (x - 3) + e], p.scale, -off));
+            for (int e = 0; e < 2; ++e) ex[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * (x - 3) + e], times, -less));
         }
         if constexpr (x == 12) {                        // (the halves' bytes share a scale)
             const v2u both = __builtin_amdgcn_permlane32_swap(largest, largest, false, false);

@@ -515,3 +515,30 @@ def test_attention_past_32_bits_of_bytes(h):
     table = torch.where((args[5] >= 0) & (args[5] < small), args[5] + (pages - small), -1).int()
     got = torch.ops.dsv3fp8.mla_decode_paged(*args[:2], kv.view(FP8), scale, pe, table, *args[6:])
     assert torch.equal(_bits(got), _bits(want)) and _close(got.view(2, 3, h, V).double(), _attention_reference(args, seen))
+
+
+@pytest.mark.parametrize("order", ["any", "rising", "late"])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("power", [17, 25, 60, 118])
+@pytest.mark.parametrize("b,s,h,context", [(2, 1, 128, 700), (2, 1, 16, 1500), (1, 9, 40, 300)])
+def test_attention_of_scores_of_any_size(b, s, h, context, power, sign, order):
+    """Scores of whole numbers times 2^power, formed exactly, up to 2^125: the largest one's positions have all the weight, those of equal ones in equal parts."""
+    args, seen = _attention_case(b, s, h, context, 64, "tree" if s > 1 else None, 31)
+    args[0].zero_()
+    args[0][..., NOPE] = 2.0 ** min(power, 60)
+    args[1].fill_(1)
+    g = torch.Generator().manual_seed(power)
+    for i in range(b):
+        n = int(args[6][i] + args[7][i])
+        rows = _rows(args[5].cpu(), 64, args[3].size(0), i, range(n)).cuda()
+        v = torch.randint(1, 200, (n,), generator=g).float() * sign
+        if order == "rising":
+            v = v.sort().values
+        v *= 2.0 ** max(0, power - 60)
+        if order == "late":
+            v[:n // 2] *= 2.0 ** -40                             # ordinary scores, then large ones
+        args[4].view(-1, ROPE)[rows] = 0
+        args[4].view(-1, ROPE)[rows, 0] = v.bfloat16().cuda()
+    args[12] = 0.5
+    got = torch.ops.dsv3fp8.mla_decode_paged(*args).view(b, s, h, V).double()
+    assert torch.isfinite(got).all() and _close(got, _attention_reference(args, seen))
