@@ -55,8 +55,8 @@ __device__ __forceinline__ v2f fp8x2_lo_to_f32(uint32_t p) { return __builtin_am
 __device__ __forceinline__ v2f fp8x2_hi_to_f32(uint32_t p) { return __builtin_amdgcn_cvt_pk_f32_fp8((int)p, true); }
 
 // Four binary32 as the sum of two e4m3 codes each, of scales 2^(e - 127) and a sixteenth of it (e from split_exponent): what the first code
-// leaves off, at most half a step of 2^-3, is the second's.  Off by 2^-9 of the value at most, half of what bf16 is, down to 2^-14 of the largest of
-// the values that share the scale; below that by 2^-23 of that largest one.
+// leaves off, at most half a step of 2^-3, is the second's.  Off by 2^-9 of the value at most, half of what bf16 is, down to 2^-12 of the largest of
+// the values that share the scale, below which the second code is subnormal; there by 2^-21 of that largest one (half a step of 2^-9, of a sixteenth of the scale).
 __device__ __forceinline__ int split_exponent(uint32_t largest) {       // from the largest |value|'s bits: it becomes 128 .. 256
     const int e = (int)(largest >> 23) - 7;
     return e < 5 ? 5 : e > 247 ? 247 : e;

@@ -2,7 +2,7 @@
 // rows moved to the front.  (Reference: the caches of inference/model.py:443-444 and what fills them, :457-466, :480-483; it keeps them dense and in bf16.)
 // A row is 512 latents as e4m3 codes, one binary32 power of two that multiplies them, 64 rotary elements in bf16: 644 bytes for 1152.
 // One scale a row: the codes' own exponents span 2^-9 .. 448, so that an element is off by half a step of 2^-3 (a sixteenth of its
-// value) down to 2^-15 of the row's largest; a scale per 128 would move that limit and nothing else.  A power of two: code times
+// value) down to 2^-13.8 of the row's largest (2^-6, the smallest normal code, where that is 224 .. 448); a scale per 128 would move that limit and nothing else.  A power of two: code times
 // scale is a bf16 number, so that reading rounds nothing.
 #include "mla.hpp"
 #include "paged.hpp"

@@ -4,7 +4,8 @@
 //   fold     mla_fold.hpp
 // The matrix cores take the codes as they are.  What meets them is two codes an element as well (split_codes), with scales of powers of two that
 // the products apply: the folded query, split by the kernel that folds it (wkv_b_absorb.hip), and the exponentials times their
-// position's scale, split here.  A pair of codes is off by 2^-9 of the value at most, where bf16 would be by 2^-8; scores and sums are binary32.
+// position's scale, split here.  A pair of codes is off by 2^-9 of the value, where bf16 would be by 2^-8, and of the smallest values by
+// 2^-21 of the largest beside them.  Scores and sums are binary32.
 #include <type_traits>
 
 #include "mla.hpp"
@@ -260,7 +261,7 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
 
     v8i Q[2][8];                                        // first and second codes; K step n: features 64 n + 32 g .. + 31
     int qs[2][2];                                       // their scales, K steps 0 .. 3 and 4 .. 7
-    v4u turned[4];                                      // rotary query, K steps of 16
+    v4u turned[4];                                      // rotary query, K steps of 16: rounded to bf16, as apply_rotary_emb leaves it and as its keys are
     {
         // (packed, a last block's missing rows hold anything; nobody reads their results)
         const uint8_t* src = PACK ? p.ql + ((int64_t)b * p.groups + row0 / 32) * 32768 + lane * 16 : p.ql + ((int64_t)b * p.rows + row) * 1024 + g * 32;

@@ -207,3 +207,42 @@ def test_shapes_without_a_device(name):
     shapes = {"mla_latent_paged": [(2, 3, 128), (2, 3, 1)], "mla_cache_read": [(2, 20, 512), (2, 20, 64)], "mla_cache_keep": [], "mla_decode_paged": [(2, 3, 512)], "mla_decode_paged_quant": [(2, 3, 512), (2, 3, 4)]}[name]
     got = (got,) if isinstance(got, torch.Tensor) else got
     assert [tuple(t.shape) for t in got or ()] == shapes
+
+
+def _e4m3(x):
+    """The nearest e4m3 values, ties to even."""
+    return x.float().to(FP8).double()
+
+
+def _spread(g, octaves):
+    """Rows of 32 values over so many powers of two below the largest, which is any of its binade; every eighth next to a tie of three or seven bits."""
+    v = torch.exp2(-octaves * torch.rand(40000, 32, generator=g, dtype=torch.float64)) * (1 + torch.rand(40000, 1, generator=g, dtype=torch.float64))
+    mantissa, exponent = torch.frexp(v)
+    tie = torch.ldexp((mantissa * 16).round() / 16 + 2.0 ** -5 + 2.0 ** -20 * torch.randn(v.shape, generator=g), exponent)
+    v[:, 1::8] = tie[:, 1::8]
+    v[:, 0] = v.amax(-1)
+    return v.float().double()
+
+
+def test_two_codes_a_value():
+    """What the comment at split_codes (csrc/common.hpp) states of it: off by 2^-9 of the value down to 2^-12 of the largest that shares the scale, by 2^-21 of
+    that below; and no better limits hold."""
+    v = _spread(torch.Generator().manual_seed(1), 26)
+    largest = v.amax(-1, keepdim=True)
+    scale = torch.exp2(torch.floor(torch.log2(largest)) - 7)                # the largest becomes 128 .. 256
+    first = _e4m3(v / scale) * scale
+    second = _e4m3((v - first) / (scale / 16)) * (scale / 16)
+    error, ratio = (v - first - second).abs(), v / largest
+    assert (error <= torch.where(ratio >= 2.0 ** -12, 2.0 ** -9 * v, 2.0 ** -21 * largest)).all()
+    assert ((error > 2.0 ** -9 * v) & (ratio > 2.0 ** -13.1)).any() and (error > 2.0 ** -22 * largest)[ratio < 2.0 ** -13].any()
+
+
+def test_one_code_an_element():
+    """What the head of csrc/mla_paged.hip states of a row: off by a sixteenth of the element down to 2^-13.8 of the row's largest (2^-6 of 224 scales), by 2^-10
+    of a scale below."""
+    v = _spread(torch.Generator().manual_seed(2), 20)
+    largest = v.amax(-1, keepdim=True)
+    scale = torch.exp2(torch.ceil(torch.log2(largest / 448)))
+    error, limit = (v - _e4m3(v / scale) * scale).abs(), 2.0 ** -6 / 224
+    assert (error <= torch.where(v >= limit * largest, v / 16, 2.0 ** -10 * scale)).all()
+    assert ((error > v / 16) & (v > 2.0 ** -14.2 * largest)).any()
