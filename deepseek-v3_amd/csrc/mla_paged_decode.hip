@@ -74,7 +74,10 @@ __device__ __forceinline__ int wave_scan(int v) {
 __device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
 
 // Which positions a workgroup takes.  The lengths are on the device, so every workgroup divides the work by itself: `per` tiles a
-// range, the fewest with which all sequences' ranges are at most p.ranges, ranges numbered through the sequences.
+// range, with which all sequences' ranges are at most p.ranges, ranges numbered through the sequences.  The search for it goes upwards in steps of up to a
+// quarter and does not go back: with many more ranges than sequences it finds the fewest, with few (8 sequences of 250 .. 2001 positions, 10 ranges) in a fifth
+// of the cases only, elsewhere up to a fifth more.  A range counts for p.blocks workgroups, also where its sequence has fewer rows than the widest; those
+// without any return at once.
 struct Share { int b, first, ranges, per, used; };      // sequence (-1: none), its first range and ranges, tiles a range, ranges of all
 template <class F> __device__ __forceinline__ Share share_of(const PagedArgs& p, int lane, F which, bool write_plan) {
     auto tiles = [&](int b) -> int {
@@ -639,7 +642,7 @@ PagedPlan paged_plan(int64_t batch, int64_t rows) {
     PagedPlan a;
     a.blocks = (rows + 127) / 128;
     a.groups = (int)(a.blocks * 4);
-    // Ranges of all sequences: as many as there are compute units for the row blocks, so that all run at once (8 sequences x 25 tokens x 128
+    // Ranges of all sequences: as many as there are compute units for the row blocks of the widest, so that all run at once (8 sequences x 25 tokens x 128
     // heads, 10 to 2001 positions: 10 ranges of up to 22 tiles 84 us, 13 of up to 18 in two rounds 105); where the sequences alone are
     // more than these, room for the longer ones to be cut.
     const int64_t units = a.blocks < 256 ? 256 / a.blocks : 1;
