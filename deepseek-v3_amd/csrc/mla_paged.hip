@@ -11,6 +11,7 @@ namespace dsv3 {
 namespace {
 
 constexpr int kC = 512, kRope = 64;
+constexpr int64_t kMostItems = 0xffffffff;              // of a launch
 
 struct WriteArgs {
     const uint16_t* a; int64_t a_stride;                // bf16 rows [q_rank | 512 | 64], stride in elements
@@ -220,8 +221,10 @@ int launch_mla_latent_paged(const void* a, int64_t a_stride, const void* q_w, co
     p.table = cache.table; p.width = cache.table_width; p.pages = cache.pages; p.page = cache.page_size;
     p.starts = starts; p.counts = counts; p.y = (uint8_t*)y; p.ys = ys;
     p.total = batch * rows; p.rows = (int)rows; p.q_rank = q_rank; p.q_eps = q_eps; p.kv_eps = kv_eps;
-    if (q_rank) hipLaunchKernelGGL(mla_write_kernel<true>, dim3((unsigned)p.total), dim3(320), 0, st, p);
-    else hipLaunchKernelGGL(mla_write_kernel<false>, dim3((unsigned)((p.total + 3) / 4)), dim3(256), 0, st, p);
+    const int64_t grid = q_rank ? p.total : (p.total + 3) / 4, threads = q_rank ? 320 : 256;
+    if (grid * threads > kMostItems) return DSV3_ERR_BAD_SHAPE;
+    if (q_rank) hipLaunchKernelGGL(mla_write_kernel<true>, dim3((unsigned)grid), dim3((unsigned)threads), 0, st, p);
+    else hipLaunchKernelGGL(mla_write_kernel<false>, dim3((unsigned)grid), dim3((unsigned)threads), 0, st, p);
     return launch_status();
 }
 
@@ -231,6 +234,7 @@ int launch_mla_cache_read(const dsv3_mla_pages& cache, const int32_t* lengths, v
     p.table = cache.table; p.width = cache.table_width; p.pages = cache.pages; p.page = cache.page_size;
     p.lengths = lengths; p.out = (uint16_t*)kv; p.out_pe = (uint16_t*)pe;
     p.positions = (int)positions; p.per_seq = (int)((positions + 7) / 8); p.groups = batch * p.per_seq;
+    if ((p.groups + 3) / 4 * 256 > kMostItems) return DSV3_ERR_BAD_SHAPE;
     hipLaunchKernelGGL(mla_read_kernel, dim3((unsigned)((p.groups + 3) / 4)), dim3(256), 0, st, p);
     return launch_status();
 }

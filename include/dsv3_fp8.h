@@ -431,7 +431,8 @@ typedef struct dsv3_mla_pages {
  * at row starts[b] + i of sequence b, i < counts[b]; y, s as dsv3_mla_latent.  The norms' sums are binary64 here.  A latent that holds a
  * NaN or an infinity is stored as zeros with a scale of NaN.  q_rank 0: no query latent (q_norm, y and s are not looked at).
  * freqs: binary32 (cos, sin) pairs [batch, rows, 32], each row's own.  A negative start: none of the sequence's rows is written.
- * Two rows that the table sends to one place leave either's values there, or parts of both.
+ * Two rows that the table sends to one place leave either's values there, or parts of both.  Up to 13421772 rows in all, without a query
+ * latent 67108860 (what a launch holds).
  */
 int dsv3_mla_latent_paged(const void* a, int64_t a_stride, const void* q_norm, const void* kv_norm, const float* freqs,
                           const dsv3_mla_pages* cache, const int32_t* starts, const int32_t* counts, void* y, float* s, int64_t batch,
@@ -440,6 +441,7 @@ int dsv3_mla_latent_paged(const void* a, int64_t a_stride, const void* q_norm, c
 /*
  * The first `positions` rows of every sequence as dense bf16 arrays, kv [batch, positions, 512] and pe [batch, positions, 64]: what
  * dsv3_mla_prefill takes as caches.  Rows from lengths[b] (int32 [batch], device) on are zeros.
+ * Up to 67108860 groups of eight positions in all.
  */
 int dsv3_mla_cache_read(const dsv3_mla_pages* cache, const int32_t* lengths, void* kv, void* pe, int64_t batch, int64_t positions,
                         void* stream);

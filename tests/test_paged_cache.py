@@ -246,3 +246,16 @@ def test_one_code_an_element():
     error, limit = (v - _e4m3(v / scale) * scale).abs(), 2.0 ** -6 / 224
     assert (error <= torch.where(v >= limit * largest, v / 16, 2.0 ** -10 * scale)).all()
     assert ((error > v / 16) & (v > 2.0 ** -14.2 * largest)).any()
+
+
+# a launch has fewer than 2^32 work-items: a workgroup of 320 a row with a query latent, 256 for four rows without one and for 32 positions read back
+def test_sizes_that_no_launch_holds(L):
+    def write(b, rows, qr):
+        return L.lib.dsv3_mla_latent_paged(A16, 2112, A16, A16, A16, _cache(L), A16, A16, A16, A16, b, rows, qr, 512, 64, 1e-6, 1e-6, None)
+
+    def read(b, positions):
+        return L.lib.dsv3_mla_cache_read(_cache(L), A16, A16, A16, b, positions, None)
+    for rows in (13421773 // 3 + 1, 0x7fffff):
+        assert write(3, rows, 1536) == 2
+    assert write(9, 67108863 // 9 + 1, 0) == 2 and write(255, 0x7fffff, 0) == 2
+    assert read(65, 0x7fffff) == 2 and read(65535, 8193) == 2
