@@ -38,17 +38,17 @@ namespace pingpong {
 // One global -> LDS copy of 16 (or 4) bytes per lane: uniform 64-bit base in scalar registers, 32-bit lane offset,
 // uniform LDS address through M0 (lane l lands at lds_addr + 16 l).  Written out because the compiler otherwise
 // forms a 64-bit address per lane with vector ALU instructions in front of every copy.
-// A memory instruction needs five wait states behind a vector instruction that wrote its scalars, and the compiler, which does not look into
-// the blocks, keeps the scales' base of the persistent kernel in lanes of a vector register and reads it back right in front of copy4:
-// copy4 waits for that.  copy16, of which there are eight a K block, waits for M0 alone: no kernel of the build writes its scalars so (tests/test_wait_states.py).
+// WAIT + 1 wait states in front of the copy.  M0 needs one.  A memory instruction needs five behind a vector instruction that wrote its scalars, and the
+// compiler, which does not look into the blocks, keeps the scales' base of the persistent kernel in lanes of a vector register and reads it back right in
+// front of the copy: that one takes WAIT = 4.  No other copy of the build has its scalars from there (tests/test_wait_states.py).
 __device__ __forceinline__ uint32_t lds_addr_of(const void* p) { return (uint32_t)(uintptr_t)(lptr_t)p; }
 __device__ __forceinline__ void copy16(const void* base, uint32_t lane_off, uint32_t lds_addr) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
                  :: "v"(lane_off), "s"(base), "s"(lds_addr) : "memory", "m0");
 }
-__device__ __forceinline__ void copy4(const void* base, uint32_t lane_off, uint32_t lds_addr) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dword %0, %1"
-                 :: "v"(lane_off), "s"(base), "s"(lds_addr) : "memory", "m0");
+template <int WAIT> __device__ __forceinline__ void copy4(const void* base, uint32_t lane_off, uint32_t lds_addr) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop %3\n\tglobal_load_lds_dword %0, %1"
+                 :: "v"(lane_off), "s"(base), "s"(lds_addr), "n"(WAIT) : "memory", "m0");
 }
 
 // SM: 16-row sub-tiles per wavefront.  4: the 256-row tile described above.  2: a 128-row tile (32 x 128 per
@@ -251,8 +251,8 @@ __device__ __forceinline__ void tile(
         }
         if constexpr (PS) {
             const bool nx = tail && kb >= KB;
-            copy4((nx ? nxt.sc : cur.sc) + (uint32_t)(nx ? kb - KB : kb), sc_off * 4u, lds_addr_of(lds + LDS_SC + slot * SC_SLOT + wave * 256));
-        } else copy4(sc_base + (uint32_t)kb, sc_off * 4u, lds_addr_of(lds + LDS_SC + slot * SC_SLOT + wave * 256));
+            copy4<4>((nx ? nxt.sc : cur.sc) + (uint32_t)(nx ? kb - KB : kb), sc_off * 4u, lds_addr_of(lds + LDS_SC + slot * SC_SLOT + wave * 256));
+        } else copy4<0>(sc_base + (uint32_t)kb, sc_off * 4u, lds_addr_of(lds + LDS_SC + slot * SC_SLOT + wave * 256));
     };
 
     // ---- fragment addresses: lane reads row (lane & 15) of a 16-row sub-tile, K bytes 32 (lane >> 4) .. + 31
