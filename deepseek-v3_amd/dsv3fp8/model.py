@@ -558,8 +558,8 @@ class MLA(nn.Module):
         adds[:, 0].clamp_(min=torch.finfo(adds.dtype).min)
         # A row that is not finite: zeros, so that it reaches nobody through a score that is hidden or a weight of zero, and NaN for those who see it
         # (a latent that is not finite is NaN in all elements)
-        adds = adds.add(torch.linalg.vector_norm(pe, float("inf"), -1).add_(kv[..., 0]), alpha=0)
-        kv.nan_to_num_(0.0, 0.0, 0.0)
+        adds = adds.add(torch.linalg.vector_norm(pe, float("inf"), -1), alpha=0).add_(kv[..., 0], alpha=0)
+        kv.nan_to_num_(0.0, float("inf"), float("-inf"))
         pe.nan_to_num_(0.0, 0.0, 0.0)
         last, parts = starts.unsqueeze(-1) + new, []        # what token t sees, itself
         for i in range(b):

@@ -167,7 +167,7 @@ def test_prompts_see_rows_that_are_not_finite_and_no_others_do(layer, calls, mon
     kv, pe = torch.randn(2, positions, 512).bfloat16(), torch.randn(2, positions, 64).bfloat16()
     kv[0, 7], kv[1, 40] = float("nan"), float("nan")
     pe[0, 60, 3], pe[1, 41, 5], pe[1, 69, 63], pe[1, 100] = float("nan"), float("inf"), float("-inf"), float("nan")
-    pe[0, 1, 2], kv[0, 2, 5] = torch.finfo(torch.bfloat16).max, torch.finfo(torch.bfloat16).min
+    pe[0, 1, 2], kv[0, 1:3, 0] = torch.finfo(torch.bfloat16).max, torch.finfo(torch.bfloat16).max       # (whose sum would be none)
     read = kv.clone(), pe.clone()
     monkeypatch.setattr(torch.ops.dsv3fp8, "mla_cache_read", lambda *a: read)
     with torch.no_grad():
