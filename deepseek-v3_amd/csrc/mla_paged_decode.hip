@@ -159,8 +159,8 @@ __device__ __forceinline__ v8i join(v4u a, v4u b) {
 //   C  scores of the second half      | exponentials of the first half
 //   A  scores of the next tile's first half | exponentials of the second half
 //   B  weighted sums of the tile      | copies of the tile after the next
-// Measured: one sequence of 61 tokens x 128 heads at 32768 positions 410 us, 1.28 PFLOP/s of the bf16 products that the pairs stand for (the form
-// before: 542); the matrix cores are busy 2/3 of the time.  Without the copies of all but the first rows it would be 40 us less wherever they
+// Measured: one sequence of 61 tokens x 128 heads at 32768 positions 403 .. 435 us by card, up to 1.29 PFLOP/s of the bf16 products that the pairs stand for in
+// the whole call (the form before: 542); the matrix cores are busy 57 .. 64 % of the time.  Without the copies of all but the first rows it would be 40 us less wherever they
 // are issued, without the exponentials and their codes 65.  A compute unit that does one tile takes 12 us: 1.2 to find it, 3.2 until it is there with
 // the queries, 4 for the products, 3.2 for writing 128 x 512 sums.
 //

@@ -516,13 +516,15 @@ class MLA(nn.Module):
         """``forward`` on a cache in pages, for sequences of different lengths: sequence i has ``starts[i]`` positions in the cache and takes
         ``counts[i]`` (up to s) new tokens behind them, x [b, s, dim].  ``starts``, ``counts`` and ``page_table`` (int32) stay on the device, so that
         a captured step serves every length; ``positions`` is what the longest sequence has at most after the step, up to what ``page_table`` has
-        room for (and 2^23 - 1).  ``freqs_cis`` [b, s, 32]: each new token's rotation.  ``tree`` (int64 [b, s], s <= 64): bit j of token i says that it sees new token j; without one a token sees those in
-        front of it and itself.  Rows of tokens that a sequence does not have, and of those that see nothing, are zeros.  A cached row that is not finite makes NaN
-        of the tokens that see it and of no others (up to 64 new tokens, an infinite score of the wrong sign only leaves that row out).
+        room for (and 2^23 - 1).  ``freqs_cis`` [b, s, 32]: each new token's rotation.  ``tree`` (int64 [b, s], s <= 64): bit j of token i says
+        that it sees new token j; without one a token sees those in front of it and itself.  Rows of tokens that a sequence does not have, and of
+        those that see nothing, are zeros.  A cached row that is not finite makes NaN of the tokens that see it and of no others (with up to 64 new
+        tokens, a score of -inf only leaves its row out).
 
         Up to 64 new tokens, wkv_b is folded into queries and outputs and the codes are read as they lie.  More (a prompt) go through keys and
-        values per head of the rows read back, sequence by sequence: at 128 heads 1 x 128 tokens at 1024 positions take 123 us so and
-        156 folded in two pieces, 1 x 4096 at 4096 910 and 4937; only few new tokens far into a long context lose (1 x 128 at 8192: 523 and 357).
+        values per head of the rows read back, sequence by sequence: a layer of 128 heads takes 239 us for 1 x 128 tokens at 1024 positions so and
+        245 in two pieces of 64, 1616 and 8345 for 1 x 4096; few new tokens on their own (1 x 70: 230 and 183, bound by the host) or far into a long
+        context (1 x 128 at 8192: 626 and 400) lose.
 
         There is no slower path behind the kernels: a layer or call that they do not take raises."""
         latent = self._latent_kernel_ok(x) if self._paged_ok(x, freqs_cis) else None

@@ -455,7 +455,8 @@ int dsv3_mla_cache_read(const dsv3_mla_pages* cache, const int32_t* lengths, voi
  * `positions`: no sequence has more (what lies behind is not seen); at most table_width * page_size.  It and the other sizes are all that
  * the host knows: lengths are read on the device, the work is divided there.
  * q: bf16 [batch, rows, heads, 192], its last 64 elements not yet rotated; freqs: binary32 (cos, sin) pairs [batch, rows, 32], each
- * row's own; wkv_b, wkv_b_scale, softmax_scale as dsv3_mla_decode (the scale between 1e-30 and 1e30); y: bf16 [batch, rows, heads * 128].
+ * row's own, and the rotated elements round to bf16 (as apply_rotary_emb leaves them, model.py:375-392); wkv_b, wkv_b_scale, softmax_scale as dsv3_mla_decode
+ * (the scale between 1e-30 and 1e30); y: bf16 [batch, rows, heads * 128].
  * workspace: 256-byte aligned, dsv3_mla_decode_paged_workspace_bytes() bytes.
  */
 size_t dsv3_mla_decode_paged_workspace_bytes(int64_t batch, int64_t rows, int heads);
