@@ -542,3 +542,18 @@ def test_attention_of_scores_of_any_size(b, s, h, context, power, sign, order):
     args[12] = 0.5
     got = torch.ops.dsv3fp8.mla_decode_paged(*args).view(b, s, h, V).double()
     assert torch.isfinite(got).all() and _close(got, _attention_reference(args, seen))
+
+
+@pytest.mark.parametrize("s,h", [(3, 40), (4, 8)])
+def test_counts_out_of_range(s, h):
+    """A count above the rows is all rows, a negative one none."""
+    args, seen = _attention_case(4, s, h, 200, 24, None, 17)
+    args[0] = args[0].nan_to_num(1.0)
+    most = 2 ** 31 - 1
+    first = args[6].tolist()
+    args[6] = torch.tensor([first[0], 0, first[2], most], dtype=torch.int32, device="cuda")
+    args[7] = torch.tensor([s, s, 0, s], dtype=torch.int32, device="cuda")
+    want = torch.ops.dsv3fp8.mla_decode_paged(*args)
+    args[7] = torch.tensor([most, s + 1, -most - 1, most], dtype=torch.int32, device="cuda")
+    got = torch.ops.dsv3fp8.mla_decode_paged(*args)
+    assert torch.equal(_bits(got), _bits(want)) and (got[2] == 0).all()
