@@ -522,9 +522,9 @@ class MLA(nn.Module):
         tokens, a score of -inf only leaves its row out).
 
         Up to 64 new tokens, wkv_b is folded into queries and outputs and the codes are read as they lie.  More (a prompt) go through keys and
-        values per head of the rows read back, sequence by sequence: a layer of 128 heads takes 239 us for 1 x 128 tokens at 1024 positions so and
-        245 in two pieces of 64, 1616 and 8345 for 1 x 4096; few new tokens on their own (1 x 70: 230 and 183, bound by the host) or far into a long
-        context (1 x 128 at 8192: 626 and 400) lose.
+        values per head of the rows read back, sequence by sequence: a layer of 128 heads takes 235 us for 1 x 128 tokens at 1024 positions so and
+        246 in two pieces of 64, 1610 and 8510 for 1 x 4096; few new tokens on their own (1 x 70: 220 and 182, bound by the host) or far into a long
+        context (1 x 128 at 8192: 624 and 398) lose.
 
         There is no slower path behind the kernels: a layer or call that they do not take raises."""
         latent = self._latent_kernel_ok(x) if self._paged_ok(x, freqs_cis) else None
@@ -556,16 +556,16 @@ class MLA(nn.Module):
         # What a position adds to the scores of those who see it: nothing, or -inf where it lies in no page (its row was read as zeros).  Position 0 gets the
         # lowest number then: beside any other its weight is zero, and who sees no other (who sees one has position 0 in a page or another) gets that row of zeros.
         entries = page_table[:, :-(-positions // page)]
-        adds = torch.where(entries.remainder(pages) == entries, 0.0, float("-inf")).repeat_interleave(page, 1)[:, :positions]
+        adds = (entries.remainder(pages) == entries).log().repeat_interleave(page, 1)[:, :positions]       # (of one and zero)
         adds[:, 0].clamp_(min=torch.finfo(adds.dtype).min)
         # A row that is not finite: zeros, so that it reaches nobody through a score that is hidden or a weight of zero, and NaN for those who see it
         # (a latent that is not finite is NaN in all elements)
         adds = adds.add(torch.linalg.vector_norm(pe, float("inf"), -1), alpha=0).add_(kv[..., 0], alpha=0)
         kv.nan_to_num_(0.0, float("inf"), float("-inf"))
         pe.nan_to_num_(0.0, 0.0, 0.0)
-        last, parts = starts.unsqueeze(-1) + new, []        # what token t sees, itself
+        last, hidden, parts = starts.unsqueeze(-1) + new, adds.new_full((), float("-inf")), []         # last: what token t sees, itself
         for i in range(b):
-            mask = torch.where(at <= last[i].unsqueeze(-1), adds[i], float("-inf"))
+            mask = torch.where(at <= last[i].unsqueeze(-1), adds[i], hidden)
             parts.append(torch.ops.dsv3fp8.mla_prefill(q[i:i + 1], freqs_cis[i], kv[i:i + 1], pe[i:i + 1], w, w_scale, mask, positions, self.softmax_scale))
         yq, ys = parts[0] if b == 1 else (torch.cat([part[0].view(torch.uint8) for part in parts]).view(torch.float8_e4m3fn), torch.cat([part[1] for part in parts]))
         return fp8_gemm(yq, ys, wo, wo.scale).masked_fill_(((new >= counts.unsqueeze(-1)) | (starts < 0).unsqueeze(-1)).unsqueeze(-1), 0)
