@@ -92,6 +92,50 @@ int dsv3_weight_quant(const void* w, int w_dtype, void* y, float* s,
     return launch_weight_quant(w, w_dtype, y, s, m, n, scale_fmt, (hipStream_t)stream);
 }
 
+// What both directions of the 4-bit format check; `wide` has 16 bits an element or more.
+static int mx4_validate(const void* codes, const void* s, const void* wide, int dtype, int64_t numel, int64_t last_dim) {
+    if (!valid_dtype(dtype)) return DSV3_ERR_BAD_DTYPE;
+    if (numel < 0 || last_dim < 0 || last_dim % 32 != 0 || numel > (int64_t)1 << 37) return DSV3_ERR_BAD_SHAPE;
+    if (numel == 0) return DSV3_OK;
+    if (last_dim == 0 || numel % last_dim != 0) return DSV3_ERR_BAD_SHAPE;
+    if (!codes || !s || !wide) return DSV3_ERR_NULL_POINTER;
+    if (!aligned(codes, 4) || !aligned(wide, 16)) return DSV3_ERR_MISALIGNED;
+    return DSV3_OK;
+}
+
+int dsv3_mx4_quant(const void* x, int x_dtype, void* y, void* s, int64_t numel, int64_t last_dim, void* stream) {
+    const int rc = mx4_validate(y, s, x, x_dtype, numel, last_dim);
+    if (rc != DSV3_OK || numel == 0) return rc;
+    return launch_mx4_quant(x, x_dtype, y, s, numel, (hipStream_t)stream);
+}
+
+int dsv3_mx4_dequant(const void* x, const void* s, void* y, int y_dtype, int64_t numel, int64_t last_dim, void* stream) {
+    const int rc = mx4_validate(x, s, y, y_dtype, numel, last_dim);
+    if (rc != DSV3_OK || numel == 0) return rc;
+    return launch_mx4_dequant(x, s, y, y_dtype, numel, (hipStream_t)stream);
+}
+
+static bool mx4_gemm_sizes_ok(int64_t m, int64_t n, int64_t k) {
+    return m >= 0 && n >= 0 && k >= 0 && k % 128 == 0 && m <= 0x7fffffff && n <= 0x7fffffff && k <= 0x7fffffff;
+}
+
+size_t dsv3_mx4_gemm_workspace_bytes(int a_kind, int64_t m, int64_t n, int64_t k) {
+    if ((a_kind != DSV3_MX4 && a_kind != DSV3_E4M3) || !mx4_gemm_sizes_ok(m, n, k) || m == 0 || n == 0 || k == 0) return 0;
+    return mx4_gemm_workspace_bytes(a_kind == DSV3_E4M3, m, n, k);
+}
+
+int dsv3_mx4_gemm(const void* a, const void* a_s, int a_kind, const void* b, const void* b_s, void* c, int c_dtype,
+                  int64_t m, int64_t n, int64_t k, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!valid_dtype(c_dtype) || (a_kind != DSV3_MX4 && a_kind != DSV3_E4M3)) return DSV3_ERR_BAD_DTYPE;
+    if (!mx4_gemm_sizes_ok(m, n, k)) return DSV3_ERR_BAD_SHAPE;
+    if (m == 0 || n == 0) return DSV3_OK;
+    if (!c || (k > 0 && (!a || !a_s || !b || !b_s))) return DSV3_ERR_NULL_POINTER;
+    if (!aligned(a, 16) || !aligned(b, 16) || !aligned(c, 16) || !aligned(a_s, 4) || !aligned(b_s, 4)) return DSV3_ERR_MISALIGNED;
+    const size_t need = dsv3_mx4_gemm_workspace_bytes(a_kind, m, n, k);
+    if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 256))) return DSV3_ERR_WORKSPACE;
+    return launch_mx4_gemm(a, a_s, a_kind == DSV3_E4M3, b, b_s, c, c_dtype, m, n, k, workspace, (hipStream_t)stream);
+}
+
 size_t dsv3_fp8_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k) {
     if (m <= 0 || n <= 0 || k <= 0 || k % 128 != 0) return 0;
     return fp8_gemm_workspace_bytes(m, n, k);

@@ -23,7 +23,7 @@ using at::Tensor;
 using std::tuple;
 typedef c10::optional<Tensor> OptTensor;
 
-constexpr auto kFp8 = at::kFloat8_e4m3fn;
+constexpr auto kFp8 = at::kFloat8_e4m3fn, kFp4 = at::kFloat4_e2m1fn_x2, kE8m0 = at::kFloat8_e8m0fnu;
 
 int dtype_code(at::ScalarType t) {
     switch (t) {
@@ -184,6 +184,61 @@ tuple<Tensor, Tensor> swiglu_quant(const Tensor& h, int64_t block, int64_t fmt) 
     check(dsv3_swiglu_quant(h.data_ptr(), code, y.data_ptr(), (float*)s.data_ptr(), rows, inter, bs, (int)fmt, on.stream),
           "dsv3_swiglu_quant");
     return {y, s};
+}
+
+// Microscaled 4-bit numbers: codes [.., k / 2], two a byte, and a byte per 32 [.., k / 32]
+void check_mx4(const char* what, const char* name, const Tensor& codes, const Tensor& s) {
+    TORCH_CHECK(codes.scalar_type() == kFp4 && s.scalar_type() == kE8m0, what, ": ", name, " must be float4_e2m1fn_x2 codes with float8_e8m0fnu scales, got ",
+                codes.scalar_type(), " and ", s.scalar_type());
+    TORCH_CHECK(codes.dim() > 0 && codes.dim() == s.dim() && codes.is_contiguous() && s.is_contiguous() && codes.size(-1) == s.size(-1) * 16 &&
+                codes.sizes().slice(0, codes.dim() - 1) == s.sizes().slice(0, s.dim() - 1), what, ": ", name, " must be contiguous, with a scale per 32 elements, got ",
+                codes.sizes(), " and ", s.sizes());
+}
+
+tuple<Tensor, Tensor> mx4_quant(const Tensor& x) {
+    const int code = dtype_code(x.scalar_type());
+    TORCH_CHECK(x.dim() > 0 && x.is_contiguous() && x.size(-1) % 32 == 0, "mx4_quant: x must be contiguous, its last dimension a multiple of 32, got ", x.sizes());
+    on_one_gpu("mx4_quant", x, {});
+    Tensor y = with_last(x, x.size(-1) / 2, kFp4), s = with_last(x, x.size(-1) / 32, kE8m0);
+    On on(x);
+    check(dsv3_mx4_quant(x.data_ptr(), code, y.data_ptr(), s.data_ptr(), x.numel(), x.size(-1), on.stream), "dsv3_mx4_quant");
+    return {y, s};
+}
+
+Tensor mx4_dequant(const Tensor& x, const Tensor& s, int64_t out) {
+    check_mx4("mx4_dequant", "x", x, s);
+    on_one_gpu("mx4_dequant", x, { &s });
+    Tensor y = with_last(x, x.size(-1) * 2, dtype_of(out));
+    On on(x);
+    check(dsv3_mx4_dequant(x.data_ptr(), s.data_ptr(), y.data_ptr(), (int)out, y.numel(), y.size(-1), on.stream), "dsv3_mx4_dequant");
+    return y;
+}
+
+Tensor mx4_gemm(const Tensor& a, const Tensor& a_s, const Tensor& b, const Tensor& b_s, int64_t out) {
+    const char* what = "mx4_gemm";
+    check_mx4(what, "b", b, b_s);
+    TORCH_CHECK(b.dim() == 2 && a.dim() > 0, what, ": b must be a matrix, and a one or rows of one, got ", b.sizes(), " and ", a.sizes());
+    const int64_t n = b.size(0), k = b.size(1) * 2;
+    const bool a8 = a.scalar_type() == kFp8;
+    if (a8) {
+        TORCH_CHECK(a.is_contiguous() && a_s.scalar_type() == at::kFloat && a_s.is_contiguous() && a_s.dim() == a.dim() && a.size(-1) == a_s.size(-1) * 128 &&
+                    a.sizes().slice(0, a.dim() - 1) == a_s.sizes().slice(0, a.dim() - 1), what, ": e4m3 activations must be contiguous, with fp32 scales per 128 elements, got ",
+                    a.sizes(), " and ", a_s.sizes());
+    } else {
+        check_mx4(what, "a", a, a_s);
+    }
+    TORCH_CHECK(a.size(-1) * (a8 ? 1 : 2) == k && k % 128 == 0, what, ": a and b must share a last dimension that is a multiple of 128 elements, got ", a.size(-1) * (a8 ? 1 : 2), " and ", k);
+    on_one_gpu(what, a, { &a_s, &b, &b_s });
+    const int kind = a8 ? DSV3_E4M3 : DSV3_MX4;
+    int64_t m = 1;
+    for (int64_t d = 0; d + 1 < a.dim(); ++d) m *= a.size(d);
+    On on(a);
+    const size_t need = dsv3_mx4_gemm_workspace_bytes(kind, m, n, k);
+    const Tensor ws = need ? scratch(a, need) : Tensor();
+    Tensor c = with_last(a, n, dtype_of(out));
+    check(dsv3_mx4_gemm(a.data_ptr(), a_s.data_ptr(), kind, b.data_ptr(), b_s.data_ptr(), c.data_ptr(), (int)out, m, n, k, need ? ws.data_ptr() : nullptr,
+                        need, on.stream), "dsv3_mx4_gemm");
+    return c;
 }
 
 void check_caches(const Tensor& kv, const Tensor& pe, int64_t batch, int64_t positions) {
@@ -473,6 +528,9 @@ TORCH_LIBRARY_IMPL(dsv3fp8, CUDA, m) {
     m.impl("fp8_gemm_pow2", fp8_gemm_pow2);
     m.impl("linear_fp8", linear_fp8);
     m.impl("swiglu_quant", swiglu_quant);
+    m.impl("mx4_quant", mx4_quant);
+    m.impl("mx4_dequant", mx4_dequant);
+    m.impl("mx4_gemm", mx4_gemm);
     m.impl("mla_prefill", mla_prefill);
     m.impl("mla_decode", mla_decode);
     m.impl("mla_decode_quant", mla_decode_quant);

@@ -12,11 +12,12 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent.parent / "lib" / "libdsv3fp8.so"
 TORCH_LIB_PATH = LIB_PATH.with_name("libdsv3torch.so")      # the operators' native implementations, on top of it
 
-# enum dsv3_dtype / dsv3_scale_fmt / dsv3_status (include/dsv3_fp8.h)
+# enum dsv3_dtype / dsv3_scale_fmt / .. / dsv3_mx4_operand / dsv3_status (include/dsv3_fp8.h)
 BF16, F16, F32 = 0, 1, 2
 SCALE_FMT_NONE, SCALE_FMT_UE8M0 = 0, 1
 ABSORB_Q, ABSORB_V = 0, 1
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+MX4, E4M3 = 0, 1
 OK = 0
 
 
@@ -33,6 +34,11 @@ EXPORTS = {
     "dsv3_act_quant": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_void_p]),
     "dsv3_weight_dequant": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int, c_void_p]),
     "dsv3_weight_quant": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_void_p]),
+    "dsv3_mx4_quant": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int64, c_void_p]),
+    "dsv3_mx4_dequant": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_void_p]),
+    "dsv3_mx4_gemm_workspace_bytes": (c_size_t, [c_int, c_int64, c_int64, c_int64]),
+    "dsv3_mx4_gemm": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int,
+                              c_int64, c_int64, c_int64, c_void_p, c_size_t, c_void_p]),
     "dsv3_fp8_gemm": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
                               c_int64, c_int64, c_int64, c_void_p, c_size_t, c_void_p]),
     "dsv3_fp8_gemm_pow2": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,

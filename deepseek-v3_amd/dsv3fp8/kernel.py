@@ -64,3 +64,28 @@ def fp8_gemm_f32(a: torch.Tensor, a_s: torch.Tensor, b: torch.Tensor, b_s: torch
     assert a.is_contiguous() and b.is_contiguous(), 'Input tensors must be contiguous'
     assert a_s.is_contiguous() and b_s.is_contiguous(), 'Scaling factor tensors must be contiguous'
     return torch.ops.dsv3fp8.fp8_gemm(a, a_s, b, b_s, _lib.F32)
+
+
+def mx4_quant(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``x`` in microscaled 4-bit numbers (not in the reference): ``(y, s)``, two e2m1 codes a byte in ``torch.float4_e2m1fn_x2``
+    ``[*x.shape[:-1], x.size(-1) // 2]`` and one power of two per 32 elements in ``torch.float8_e8m0fnu`` ``[*x.shape[:-1], x.size(-1) // 32]``, the
+    smallest of which no element is more than six times (``act_quant``'s ``scale_fmt="ue8m0"`` rule for these codes).  A block that holds
+    a NaN or an infinity becomes NaN throughout.  For activations and for weights ``[out, in]``."""
+    assert x.is_contiguous(), 'Input tensor must be contiguous'
+    assert x.size(-1) % 32 == 0, 'Last dimension size must be divisible by 32'
+    return torch.ops.dsv3fp8.mx4_quant(x)
+
+
+def mx4_dequant(x: torch.Tensor, s: torch.Tensor) -> torch.Tensor:
+    """The values of ``mx4_quant``'s codes and scales, in the default dtype: exact in fp32 and bf16."""
+    assert x.is_contiguous() and s.is_contiguous(), 'Input tensors must be contiguous'
+    return torch.ops.dsv3fp8.mx4_dequant(x, s, ops.dtype_code(torch.get_default_dtype()))
+
+
+def mx4_gemm(a: torch.Tensor, a_s: torch.Tensor, b: torch.Tensor, b_s: torch.Tensor) -> torch.Tensor:
+    """``c = a @ b.T`` with a weight ``b`` of microscaled 4-bit numbers, in the default dtype (not in the reference).  ``a`` is of such numbers
+    too, or e4m3 with a power of two per 128 elements: ``act_quant(x, 128, "ue8m0")``, whose scales the caller vouches for as in
+    ``fp8_gemm_pow2``.  The matrix instruction takes both formats and the scales as they are."""
+    assert a.is_contiguous() and b.is_contiguous(), 'Input tensors must be contiguous'
+    assert a_s.is_contiguous() and b_s.is_contiguous(), 'Scaling factor tensors must be contiguous'
+    return torch.ops.dsv3fp8.mx4_gemm(a, a_s, b, b_s, ops.dtype_code(torch.get_default_dtype()))

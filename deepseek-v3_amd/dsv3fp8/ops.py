@@ -1,6 +1,7 @@
 """PyTorch-ROCm custom ops over the C ABI.
 
-``torch.ops.dsv3fp8.{act_quant, weight_dequant, weight_quant, fp8_gemm}`` and the grouped
+``torch.ops.dsv3fp8.{act_quant, weight_dequant, weight_quant, fp8_gemm}``, the ones on microscaled 4-bit numbers
+``{mx4_quant, mx4_dequant, mx4_gemm}``, the grouped
 mixture-of-experts ops ``{gate_route, group_tiles, moe_route, fp8_gemm_grouped, swiglu_quant, moe_combine}`` and the
 attention ops ``{wkv_b_absorb, mla_latent, mla_decode, mla_decode_quant, mla_prefill, mla_query, mla_output}`` and the
 ones on a cache in pages ``{mla_latent_paged, mla_decode_paged, mla_decode_paged_quant, mla_cache_read,
@@ -18,7 +19,7 @@ from . import _lib
 
 _DTYPE_CODE = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16, torch.float32: _lib.F32}
 _CODE_DTYPE = {v: k for k, v in _DTYPE_CODE.items()}
-FP8 = torch.float8_e4m3fn
+FP8, FP4, E8M0 = torch.float8_e4m3fn, torch.float4_e2m1fn_x2, torch.float8_e8m0fnu
 
 _libdef = torch.library.Library("dsv3fp8", "DEF")
 _libdef.define("act_quant(Tensor x, int block_size, int scale_fmt) -> (Tensor, Tensor)")
@@ -27,6 +28,9 @@ _libdef.define("weight_quant(Tensor w, int block_size, int scale_fmt) -> (Tensor
 _libdef.define("fp8_gemm(Tensor a, Tensor a_s, Tensor b, Tensor b_s, int out_dtype) -> Tensor")
 _libdef.define("fp8_gemm_pow2(Tensor a, Tensor a_s, Tensor b, Tensor b_s, int out_dtype) -> Tensor")
 _libdef.define("linear_fp8(Tensor x, Tensor b, Tensor b_s, int scale_fmt, int out_dtype) -> Tensor")
+_libdef.define("mx4_quant(Tensor x) -> (Tensor, Tensor)")
+_libdef.define("mx4_dequant(Tensor x, Tensor s, int out_dtype) -> Tensor")
+_libdef.define("mx4_gemm(Tensor a, Tensor a_s, Tensor b, Tensor b_s, int out_dtype) -> Tensor")
 _libdef.define("group_tiles(Tensor counts, int max_tiles) -> (Tensor, Tensor, Tensor)")
 _libdef.define("moe_route(Tensor indices, Tensor weights, int experts, bool shared_group) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)")
 _libdef.define("fp8_gemm_grouped(Tensor a, Tensor a_s, Tensor? a_rows, Tensor b, Tensor b_s, int rows, "
@@ -89,6 +93,14 @@ def _weight_quant_meta(w, block_size, scale_fmt):
 
 def _fp8_gemm_meta(a, a_s, b, b_s, out_dtype):
     return a.new_empty(*a.size()[:-1], b.size(0), dtype=_CODE_DTYPE[out_dtype])
+
+
+def _mx4_quant_meta(x):
+    return x.new_empty(*x.size()[:-1], x.size(-1) // 2, dtype=FP4), x.new_empty(*x.size()[:-1], x.size(-1) // 32, dtype=E8M0)
+
+
+def _mx4_dequant_meta(x, s, out_dtype):
+    return x.new_empty(*x.size()[:-1], x.size(-1) * 2, dtype=_CODE_DTYPE[out_dtype])
 
 
 def linear_fp8_fused(m: int, n: int, k: int) -> bool:
@@ -344,6 +356,7 @@ for _name, _dev in (("wkv_b_absorb", _wkv_b_absorb_dev), ("gate_route", _gate_ro
     _libimpl.impl(_name, _dev, "CUDA")
 for _name, _meta in (("act_quant", _act_quant_meta), ("weight_dequant", _weight_dequant_meta),
                      ("weight_quant", _weight_quant_meta), ("fp8_gemm", _fp8_gemm_meta), ("fp8_gemm_pow2", _fp8_gemm_meta),
+                     ("mx4_quant", _mx4_quant_meta), ("mx4_dequant", _mx4_dequant_meta), ("mx4_gemm", _fp8_gemm_meta),
                      ("linear_fp8", _linear_fp8_meta), ("swiglu_quant", _swiglu_quant_meta),
                      ("mla_prefill", _mla_prefill_meta), ("mla_decode", _mla_decode_meta), ("mla_decode_quant", _mla_prefill_meta), ("mla_latent", _mla_latent_meta),
                      ("mla_query", _mla_query_meta), ("mla_output", _mla_output_meta),

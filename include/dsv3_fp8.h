@@ -62,6 +62,12 @@ typedef enum dsv3_scale_fmt {
     DSV3_SCALE_FMT_UE8M0 = 1
 } dsv3_scale_fmt;
 
+/* What the activations of dsv3_mx4_gemm are. */
+typedef enum dsv3_mx4_operand {
+    DSV3_MX4 = 0,        /* e2m1 codes, an e8m0 byte per 32                     */
+    DSV3_E4M3 = 1        /* e4m3 codes, a binary32 power of two per 128         */
+} dsv3_mx4_operand;
+
 /* Which of the two wkv_b products of the absorbed attention dsv3_wkv_b_absorb computes. */
 typedef enum dsv3_absorb_side {
     DSV3_ABSORB_Q = 0,   /* "bshd,hdc->bshc" with wkv_b[:, :nope]   (inference/model.py:483) */
@@ -182,6 +188,43 @@ size_t dsv3_fp8_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k);
 size_t dsv3_fp8_gemm_static_max_bytes(void);
 int dsv3_fp8_gemm_static(const void* a, const float* a_s, const void* b, const float* b_s,
                          void* c, int c_dtype, int64_t m, int64_t n, int64_t k, void* stream);
+
+/*
+ * ---- Microscaled 4-bit numbers ----
+ *
+ * Codes e2m1 (0, 1/2, 1, 3/2, 2, 3, 4, 6 and their negatives; bit 3 is the sign), two to a byte, the even element in the low half; for every 32
+ * elements along the last dimension one e8m0 byte, the power of two 2^(byte - 127) that multiplies them, 255 for NaN.  The reference has no
+ * such format; a linear layer's weight takes 17/32 bytes an element in it where block-scaled e4m3 takes one.
+ */
+
+/*
+ * Into the format: per 32 elements
+ *     byte - 127 = the smallest e in [-127, 126] with max|x| <= 6 * 2^e,   code = e2m1( x / 2^e )   (round to nearest, ties to the even code)
+ * so that nothing is cut off at 6.  A block that holds a NaN or an infinity gets byte 255 and codes of zero: it is NaN throughout.
+ * x: [numel] of x_dtype, y: [numel / 2] bytes, s: [numel / 32] bytes.  `last_dim` is x.size(-1), a multiple of 32, numel a multiple of it.
+ * x 16-byte aligned, y 4-byte.  numel == 0 is a no-op.  Up to 2^37 elements (what a launch holds).
+ */
+int dsv3_mx4_quant(const void* x, int x_dtype, void* y, void* s, int64_t numel, int64_t last_dim, void* stream);
+
+/*
+ * And back: y[i] = y_dtype( code * 2^(byte - 127) ), exact in binary32 and bf16 wherever their exponents reach, rounded in fp16.
+ * x 4-byte aligned, y 16-byte; sizes as dsv3_mx4_quant.
+ */
+int dsv3_mx4_dequant(const void* x, const void* s, void* y, int y_dtype, int64_t numel, int64_t last_dim, void* stream);
+
+/*
+ * The product with a weight of such numbers:
+ *     c[i, j] = c_dtype( sum_k a[i, k] * b[j, k] )
+ * b: codes [n, k / 2] and bytes [n, k / 32]; a: the same, [m, k / 2] and [m, k / 32], for a_kind DSV3_MX4, or e4m3 codes [m, k] and binary32
+ * scales [m, k / 128] for DSV3_E4M3, powers of two as dsv3_act_quant's DSV3_SCALE_FMT_UE8M0 makes them (the caller's guarantee; of any other scale its
+ * exponent alone counts).  k a multiple of 128; any m, n >= 0; k == 0 gives zeros.  Products are exact, sums binary32 in an order of the kernels' own, the same
+ * for the same sizes.  A NaN scale makes NaN of the results that its row takes part in, and of no others.
+ * a, b and c 16-byte aligned, a_s and b_s 4-byte.  workspace: dsv3_mx4_gemm_workspace_bytes() bytes where that is not 0, 256-byte
+ * aligned; its contents on entry are ignored.  Calls that share a workspace must be ordered on one stream.
+ */
+size_t dsv3_mx4_gemm_workspace_bytes(int a_kind, int64_t m, int64_t n, int64_t k);
+int dsv3_mx4_gemm(const void* a, const void* a_s, int a_kind, const void* b, const void* b_s, void* c, int c_dtype,
+                  int64_t m, int64_t n, int64_t k, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * ---- Mixture-of-experts layer on the same GEMM (inference/model.py:601-633 Expert, :669-693 MoE.forward) ----
