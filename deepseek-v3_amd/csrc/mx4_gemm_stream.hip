@@ -102,8 +102,6 @@ template <bool A8> int launch_a(const Mx4Args& p, int c_dtype, hipStream_t st) {
 
 }  // namespace
 
-bool mx4_stream_takes(int64_t m, int64_t n, int64_t k, bool a8) { return m <= 64; }
-
 int launch_mx4_stream(const Mx4Args& p, bool a8, int c_dtype, hipStream_t st) {
     return a8 ? launch_a<true>(p, c_dtype, st) : launch_a<false>(p, c_dtype, st);
 }

@@ -141,7 +141,8 @@ def operands(g, m, n, k, a8, spread=6):
 
 # rows up to and beyond every kernel's tiles, ragged columns, one to many K blocks, odd numbers of them
 PRODUCTS = [(1, 1, 128), (1, 576, 7168), (2, 17, 256), (16, 100, 384), (17, 48, 2048), (33, 33, 640), (64, 512, 1152), (65, 130, 128), (65, 64, 1024),
-            (100, 257, 896), (128, 128, 512), (129, 300, 2176), (200, 1000, 512), (257, 513, 256), (256, 256, 4096), (300, 2304, 1536), (520, 520, 384), (1030, 1800, 640)]
+            (100, 257, 896), (128, 128, 512), (129, 300, 2176), (200, 1000, 512), (257, 513, 256), (256, 256, 4096), (300, 2304, 1536), (520, 520, 384), (1030, 1800, 640), (1500, 8200, 640),
+            (1537, 8193, 1152), (3000, 4352, 512), (1600, 8448, 128)]
 
 
 @pytest.mark.parametrize("a8", [False, True], ids=["mx4", "e4m3"])
