@@ -37,7 +37,7 @@ void* static_scratch() {
 
 extern "C" {
 
-int dsv3_version(void) { return 100; }
+int dsv3_version(void) { return 200; }
 
 const char* dsv3_status_string(int status) {
     switch (status) {
@@ -518,9 +518,10 @@ static int mla_pages_validate(const dsv3_mla_pages* cache, int64_t batch) {
     if (cache->pages < 1 || cache->pages > 0x7fffffff || cache->page_size < 8 || cache->page_size > 16384 || cache->page_size % 8 != 0 ||
         cache->table_width < 1 || cache->table_width > 0x7fffffff || batch < 0 || batch > 65535)
         return DSV3_ERR_BAD_SHAPE;
+    if (cache->kv_bits != 0 && cache->kv_bits != 8 && cache->kv_bits != 4) return DSV3_ERR_BAD_DTYPE;
     if (batch == 0) return DSV3_OK;
     if (!cache->kv || !cache->kv_scale || !cache->pe || !cache->table) return DSV3_ERR_NULL_POINTER;
-    if (!aligned(cache->kv, 16) || !aligned(cache->kv_scale, 4) || !aligned(cache->pe, 16) || !aligned(cache->table, 4)) return DSV3_ERR_MISALIGNED;
+    if (!aligned(cache->kv, 16) || !aligned(cache->kv_scale, cache->kv_bits == 4 ? 16 : 4) || !aligned(cache->pe, 16) || !aligned(cache->table, 4)) return DSV3_ERR_MISALIGNED;
     return DSV3_OK;
 }
 

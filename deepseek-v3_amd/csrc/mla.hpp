@@ -12,6 +12,7 @@ typedef __attribute__((address_space(3))) v2i* lds_v2i;
 typedef __attribute__((address_space(3))) v4u* lds_v4u;
 typedef __attribute__((address_space(3))) v4f* lds_v4f;
 typedef __attribute__((address_space(3))) float* lds_f32;
+typedef __attribute__((address_space(3))) uint32_t* lds_u32;
 
 __device__ __forceinline__ v16f mfma32(v4u a, v4u b, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
@@ -28,6 +29,10 @@ __device__ __forceinline__ void copy16(const void* base, uint32_t lane_off, uint
 __device__ __forceinline__ void copy4(const void* base, uint32_t lane_off, uint32_t lds_addr) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dword %0, %1"
                  :: "v"(lane_off), "s"(base), "s"(lds_addr) : "memory", "m0");
+}
+// the same from an address of each lane's own
+__device__ __forceinline__ void copy4_from(uint64_t at, uint32_t lds_addr) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 4\n\tglobal_load_lds_dword %0, off" :: "v"(at), "s"(lds_addr) : "memory", "m0");
 }
 // copy16 through a buffer descriptor (the range check answers requests past its end with zeros), into LDS at lds_addr + IMM
 __device__ __forceinline__ v4i buffer_of(const void* base, int bytes) {

@@ -10,6 +10,7 @@
 
 #include "mla.hpp"
 #include "mla_fold.hpp"
+#include "mx4.hpp"
 #include "paged.hpp"
 
 namespace dsv3 {
@@ -33,13 +34,20 @@ constexpr int kLds = kStages * kStage;
 constexpr int kFewScaleOff = kRopeOff + kTile / 2 * kRope * 2;
 constexpr int kFewStage = kFewScaleOff + 8 * 256;
 constexpr int kFewLds = 4 * kFewStage;
+// Rows of four bits come in as they lie, 16 of a wavefront at a time: 4 KiB of codes and 16 scales each, behind the stages; the wavefront writes their e4m3 codes into
+// the stage.  By itself a wavefront has all 64 rows of its tile at the end of where their codes will stand (row r of them is read before anything is written
+// there: 16 (n + 1) rows of 544 bytes end in front of row 16 (n + 1) of those), and their scales behind the 64 of the rows.
+constexpr int kRaw = 16 * (kC / 2) + 16 * 16;
+constexpr int kLds4 = kLds + 4 * kRaw;
+constexpr int kFewRawOff = 4 * kRows16 - kTile * (kC / 2), kFewRawScaleOff = kFewScaleOff + 1024;
+static_assert(kFewRawOff >= 288 * kTile, "rows of four bits are read before they are written over");
 
 struct PagedArgs {
     const uint8_t* ql;                                  // folded queries in codes [batch][rows][first, second][512], rows = tokens * heads, or in operand order
     const uint8_t* qe;                                  // their exponents [batch][rows][8]
     const uint16_t* q;                                  // queries [batch][rows][192]: their rotary part is read here
     const v2f* freqs;                                   // [batch][tokens][32] (cos, sin)
-    const uint8_t* kv; const float* scales; const uint8_t* pe;
+    const uint8_t* kv; const void* scales; const uint8_t* pe;
     const int32_t* table; int64_t width, pages;
     const int32_t* starts; const int32_t* counts;
     const int64_t* tree;                                // [batch][tokens], or nullptr: a token sees those in front of it and itself
@@ -56,6 +64,9 @@ constexpr float kNothing = 0x1p-126f;
 constexpr float kNoScore = -0x1.fffffep127f;            // the exponents' offset in front of a row's first score
 __device__ const float nothing[8] = { kNothing, kNothing, kNothing, kNothing, kNothing, kNothing, kNothing, kNothing };
 __device__ const v4u nothing_key[kRope / 8] = {};
+// the same for the 16 scales of a row of four bits, which no row has
+constexpr uint32_t kNothing4 = 254u;
+__device__ const uint32_t nothing4[4] = { 0xfefefefe, 0xfefefefe, 0xfefefefe, 0xfefefefe };
 
 // Loads that the compiler may make scalar: `p` is written by nobody while the kernel runs.
 typedef const __attribute__((address_space(4))) int32_t* const_ints;
@@ -169,7 +180,7 @@ __device__ __forceinline__ v8i join(v4u a, v4u b) {
 // sequences x 16 heads at up to 8192 positions (147 MB): 50 us, 2.9 TB/s; with one wavefront at work
 // and the others copying for it 61.  Blocks of 32 rows do not pay where there are more: 32 sequences x 128 heads at up to 4096 positions 57.4 us for the
 // whole call and 56.5 with blocks of 128, one sequence at 700 26.6 and 26.3.
-template <bool PACK, bool FEW>
+template <bool PACK, bool FEW, bool FOUR>
 __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -197,6 +208,8 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     const int32_t* entries = p.table + b * p.width;
     struct Source { v4i kv, pe; const float* scales; int last; uint32_t at; };
     constexpr int kScaleAt = FEW ? kFewScaleOff : kScaleOff, kGroups = FEW ? 8 : 2;
+    constexpr int kScales8 = FOUR ? 32 : 256;           // bytes from one group's scales to the next one's
+    constexpr int kCodes = FOUR ? kC / 2 : kC;          // bytes of a row's codes
     const int first_row = FEW ? 0 : wave * 16;          // the wavefront's rows in a tile
     auto first_of = [&](int t, int h) -> uint32_t {     // group h of the wavefront's rows of tile t (past the end: the last group)
         return min(t * kTile + first_row + h * 8, (seq.end - 1) & ~7);
@@ -212,9 +225,9 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
         const int64_t some = -(int64_t)((left > 0) & ((uint32_t)entry < (uint32_t)p.pages));
         const uint64_t r = row_of(entry, first_of(t, h));
         const int rows = min(8, left) & (int)some;
-        const uint64_t scales = (((uint64_t)(uintptr_t)p.scales + r * 4) & some) | ((uint64_t)(uintptr_t)nothing & ~some);
-        return Source{ buffer_of(p.kv + r * kC, rows * kC), buffer_of(p.pe + r * (kRope * 2), rows * (kRope * 2)), (const float*)(uintptr_t)scales,
-                       max(rows, 1) - 1, stage };
+        const uint64_t scales = (((uint64_t)(uintptr_t)p.scales + r * (FOUR ? kC / 32 : 4)) & some) | ((uint64_t)(uintptr_t)nothing & ~some);
+        return Source{ buffer_of(p.kv + r * kCodes, rows * kCodes), buffer_of(p.pe + r * (kRope * 2), rows * (kRope * 2)), (const float*)(uintptr_t)scales,
+                       FOUR ? rows : max(rows, 1) - 1, stage };
     };
     // where a lane reads of two rows of latents
     auto latent_off = [&]() -> uint32_t { const int lane = lane_now(); return (lane >> 5) * kC + (((lane & 31) ^ (lane >> 5 << 2)) << 4); };
@@ -231,7 +244,92 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
             copy4(s.scales, min(lane_now() & 7, s.last) * 4, s.at + kScaleAt + (FEW ? h : wave * 2 + h) * 256);
         }
     };
+    // Rows of four bits: the codes of 16 rows as they lie (eight of `a`, eight of `b`) to `codes`, their scales to `scales`; rows that are not there have none
+    // that a row has.
+    auto issue_raw = [&](const Source& a, const Source& b, uint32_t codes, uint32_t scales, auto which) {
+        constexpr int n = decltype(which)::value;
+        if constexpr (n < 4) {
+            copy16_buffer_at(n < 2 ? a.kv : b.kv, lane_now() * 16, (n & 1) * 1024, codes + n * 1024);
+        } else {
+            const int lane = lane_now(), row = (lane >> 2) & 7, rows = lane < 32 ? a.last : b.last;
+            const uint64_t at = lane < 32 ? (uint64_t)(uintptr_t)a.scales : (uint64_t)(uintptr_t)b.scales;
+            copy4_from(row < rows ? at + row * (kC / 32) + (lane & 3) * 4 : (uint64_t)(uintptr_t)nothing4 + (lane & 3) * 4, scales);
+        }
+    };
+    // ... and as e4m3 codes of one scale a row.  Lane l has blocks 4 (l % 4) .. + 3 of row l / 4, the n-th in an order by the row with which few lanes meet in
+    // one bank (none in these reads but two of the rows' four, two in each write).
+    struct Widening { uint32_t bytes, codes, to; int turn; int top; };
+    auto widen_scales = [&](uint32_t codes, uint32_t scales, uint32_t to, uint32_t to_scales) -> Widening {
+        const int lane = lane_now(), row = lane >> 2, q = lane & 3;
+        Widening w;
+        w.bytes = *(lds_u32)(uintptr_t)(scales + lane * 4);
+        const uint32_t two = pk_umax_u16(w.bytes & 0x00ff00ffu, w.bytes >> 8 & 0x00ff00ffu);
+        uint32_t top = umax_u32(two & 0xffu, two >> 16);
+        top = dpp_umax<0xb1>(top);
+        top = dpp_umax<0x4e>(top);
+        const uint32_t row_top = umax_u32(top, 8u);     // (a row's scale is 2^-6 times the largest of its blocks', and above that of no row)
+        const float scale = top == kMx4Nan ? u32_as_f32(0x7fc00000u) : top == kNothing4 ? kNothing : u32_as_f32((row_top - 6u) << 23);
+        if (q == 0) *(lds_f32)(uintptr_t)(to_scales + row * 4) = scale;
+        w.turn = 0x1c >> (2 * (row & 3)) & 3;
+        w.codes = codes + row * (kC / 2) + q * 64;
+        w.to = to + (row >> 1) * kPair + (row >> 2 & 1) * 16 + (row & 1) * kC;
+        w.top = (int)(row_top - 133u);
+        return w;
+    };
+    // block n: the dwords of its codes, then eight of e4m3 codes
+    auto widen_read = [&](const Widening& w, auto n) -> v4u {
+        return *(lds_v4u)(uintptr_t)(w.codes + ((decltype(n)::value + w.turn & 3) << 4));
+    };
+    auto widen_scale = [&](const Widening& w, auto n) -> float {        // 2^6 times the block's part of the row's largest scale
+        const int byte = w.bytes >> (8 * (decltype(n)::value + w.turn & 3)) & 0xff;
+        return u32_as_f32((uint32_t)max(byte - (int)w.top, 119) << 23);
+    };
+    auto widen_one = [&](uint32_t codes, float scale) -> v2u {
+        const v2f a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 1);
+        const v2f c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 3);
+        return v2u{ pack_fp8x4(a.x, a.y, b.x, b.y), pack_fp8x4(c.x, c.y, d.x, d.y) };
+    };
+    auto widen_write = [&](const Widening& w, auto n, v4u lo, v4u hi) {
+        const int lane = lane_now(), row = lane >> 2, q = lane & 3, c = 8 * q + 2 * (decltype(n)::value + w.turn & 3) ^ (row & 1) << 2;
+        *(lds_v4u)(uintptr_t)(w.to + c * 16) = lo;
+        *(lds_v4u)(uintptr_t)(w.to + c * 16 + 16) = hi;
+    };
+    auto widen = [&](uint32_t codes, uint32_t scales, uint32_t to, uint32_t to_scales) {
+        const Widening w = widen_scales(codes, scales, to, to_scales);
+        v4u raw[4];
+        unrolled<4>([&](auto n) { raw[decltype(n)::value] = widen_read(w, n); });
+        unrolled<4>([&](auto n) {
+            const v4u x = raw[decltype(n)::value];
+            const float scale = widen_scale(w, n);
+            const v2u a = widen_one(x[0], scale), b = widen_one(x[1], scale), c = widen_one(x[2], scale), d = widen_one(x[3], scale);
+            widen_write(w, n, v4u{ a[0], a[1], b[0], b[1] }, v4u{ c[0], c[1], d[0], d[1] });
+        });
+    };
+    const uint32_t raw0 = lds0 + kLds + wave * kRaw;    // (wavefronts that share a tile)
+    auto copy_raw = [&](int t, uint32_t at, int page) {
+        const Source a = source(t, 0, page, 0), b = source(t, 1, page, 0);
+        unrolled<5>([&](auto n) { issue_raw(a, b, at, at + 16 * (kC / 2), n); });
+    };
+    auto copy_keys = [&](int t, uint32_t stage, int page) {
+        const uint32_t none = 0;
+        unrolled<2>([&](auto h) { issue(source(t, decltype(h)::value, page, stage), none, h, std::integral_constant<int, 4>()); });
+    };
+    auto widen_tile = [&](uint32_t at, uint32_t stage) {
+        widen(at, at + 16 * (kC / 2), stage + wave * kRows16, stage + kScaleAt + wave * 2 * kScales8);
+    };
     auto copy_tile = [&](int t, uint32_t stage, int page) {
+        if constexpr (FOUR) {                           // (a wavefront by itself)
+            unrolled<4>([&](auto i) {
+                constexpr int n = decltype(i)::value;
+                const Source a = source(t, 2 * n, page, stage), b = source(t, 2 * n + 1, page, stage);
+                unrolled<5>([&](auto k) { issue_raw(a, b, stage + kFewRawOff + n * 16 * (kC / 2), stage + kFewRawScaleOff + n * 256, k); });
+                if constexpr (n >= 2) {
+                    issue(a, 0u, std::integral_constant<int, 2 * n>(), std::integral_constant<int, 4>());
+                    issue(b, 0u, std::integral_constant<int, 2 * n + 1>(), std::integral_constant<int, 4>());
+                }
+            });
+            return;
+        }
         unrolled<kGroups>([&](auto h) {
             const Source s = source(t, h, page, stage);
             const uint32_t latents = latent_off();
@@ -245,9 +343,39 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     };
     uint32_t own = lds0 + wave * kFewStage;             // FEW: the wavefront's stage
     int page = 0;
+    int page_keys = 0;                                  // FOUR: of the tile before the one of `page`
     if constexpr (FEW) {
         page = page_of(t0 + wave);
         if (t0 + wave < t1) copy_tile(t0 + wave, own, page);
+    } else if constexpr (FOUR) {
+        // the first two tiles at once, the second one's rows by way of the third stage
+        const int pages[2] = { page_of(t0), page_of(t0 + 1) };
+        page = page_of(t0 + 2);
+        copy_raw(t0, raw0, pages[0]);
+        copy_raw(t0 + 1, lds0 + 2 * kStage + wave * kRaw, pages[1]);
+        copy_keys(t0, lds0, pages[0]);
+        copy_keys(t0 + 1, lds0 + kStage, pages[1]);
+        __builtin_amdgcn_s_waitcnt(0x0f70);             // vmcnt(0)
+        asm volatile("" ::: "memory");
+        widen_tile(raw0, lds0);
+        widen_tile(lds0 + 2 * kStage + wave * kRaw, lds0 + kStage);
+        __builtin_amdgcn_s_waitcnt(0xc07f);             // lgkmcnt(0): the rows have been read
+        copy_raw(t0 + 2, raw0, page);
+        page_keys = page;
+        if (row0 >= live) {                             // no rows: the others' copies
+            barrier_no_fence();
+            for (int t = t0, st = 2; t < t1; ++t, st = st == 2 ? 0 : st + 1) {
+                arrived();                              // (rows of tile t + 2 and keys of tile t + 1)
+                const int next = page_of(t + 3);
+                copy_keys(t + 2, lds0 + st * kStage, page_keys);
+                widen_tile(raw0, lds0 + st * kStage);
+                __builtin_amdgcn_s_waitcnt(0xc07f);     // lgkmcnt(0)
+                copy_raw(t + 3, raw0, next);
+                page_keys = next;
+            }
+            arrived();
+            return;
+        }
     } else {
         copy_tile(t0, lds0, page_of(t0));
         copy_tile(t0 + 1, lds0 + kStage, page_of(t0 + 1));
@@ -333,7 +461,7 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     float sc;                                           // the scale that the next scores need
     auto scale_at = [&](uint32_t stage, int half) -> float {
         const int i = lane_now() & 31;
-        return *(lds_f32)(uintptr_t)(stage + (i >> 3) * 256 + (i & 7) * 4 + kScaleAt + half * 1024);
+        return *(lds_f32)(uintptr_t)(stage + (i >> 3) * kScales8 + (i & 7) * 4 + kScaleAt + half * 4 * kScales8);
     };
     auto look_at_scale = [&](int half) {
         ks[half] = (int)(f32_as_u32(sc) >> 23 & 0xff);  // (NaN: 255, which makes the products NaN)
@@ -351,7 +479,7 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
         constexpr int h = decltype(half)::value, x = decltype(step)::value;
         v16f& s = S[h];
         if constexpr (x == 0) scales_at = stage + (lane_now() >> 5) * 16 + kScaleAt;
-        if constexpr (x < 8 && x % 2 == 0) w[x / 2] = *(lds_v4f)(uintptr_t)(scales_at + (4 * h + x / 2) * 256);
+        if constexpr (x < 8 && x % 2 == 0) w[x / 2] = *(lds_v4f)(uintptr_t)(scales_at + (4 * h + x / 2) * kScales8);
         if constexpr (x == 1) {
             asm volatile("" : "+v"(s));                 // (behind two more MFMAs: the scores are there)
             const int at = t * kTile + 32 * h;
@@ -496,6 +624,11 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
             page = page_of(t + 4);
             __builtin_amdgcn_s_waitcnt(0x0f70);         // vmcnt(0)
             asm volatile("" ::: "memory");
+            if constexpr (FOUR)
+                unrolled<4>([&](auto i) {
+                    constexpr int n = decltype(i)::value;
+                    widen(own + kFewRawOff + n * 16 * (kC / 2), own + kFewRawScaleOff + n * 256, own + n * kRows16, own + kScaleAt + n * 2 * kScales8);
+                });
             sc = scale_at(own, 0);
             ring[0] = key(keys_at(own), 0, 0);
             ring[1] = key(keys_at(own), 0, 1);
@@ -514,8 +647,12 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
             if (t + 4 < t1) copy_tile(t + 4, own, page);                // (every read of the stage has been used)
         }
     } else {
-        page = page_of(t0 + 2);
-        arrived();
+        if constexpr (FOUR) {
+            barrier_no_fence();                         // (every wavefront has waited for its own copies)
+        } else {
+            page = page_of(t0 + 2);
+            arrived();
+        }
         sc = scale_at(lds0, 0);
         ring[0] = key(keys_at(lds0), 0, 0);
         ring[1] = key(keys_at(lds0), 0, 1);
@@ -533,7 +670,7 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
                 soften(t, base, First(), step);
                 if constexpr (decltype(step)::value == 13) {
                     arrived();
-                    page = page_of(t + 3);
+                    page = page_of(t + 3);              // (FOUR: its rows are copied in this turn's B, its keys in the next)
                     sc = scale_at(next, 0);
                 }
             }, [&](auto k) { ring[k] = key(keys_at(next), 0, k); });
@@ -543,9 +680,34 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
             // B
             Source ahead;
             uint32_t latents;
+            // Rows of four bits: the keys of the tile after the next; its rows, which have been copied, into the stage, a block in six steps; and in their place
+            // those of the tile behind it
+            Widening wide;
+            v4u raw, out[2];
+            Source ahead2;
             weigh(t == t0, base, [&](auto step) {
                 constexpr int x = decltype(step)::value;
                 if constexpr (x == 29 || x == 31) ring[x >> 1 & 1] = key(keys_at(next), 1, (x >> 1) - 14);
+                if constexpr (FOUR) {
+                    const uint32_t to = lds0 + st_free * kStage;
+                    if constexpr (x < 2) issue(source(t + 2, x, page_keys, to), 0u, step, std::integral_constant<int, 4>());
+                    if constexpr (x == 2) wide = widen_scales(raw0, raw0 + 16 * (kC / 2), to + wave * kRows16, to + kScaleAt + wave * 2 * kScales8);
+                    if constexpr (x >= 3 && x < 27) {
+                        constexpr std::integral_constant<int, (x - 3) / 6> n;
+                        constexpr int k = (x - 3) % 6;
+                        if constexpr (k == 0) raw = widen_read(wide, n);
+                        if constexpr (k >= 1 && k < 5) {
+                            const v2u two = widen_one(raw[k - 1], widen_scale(wide, n));
+                            out[(k - 1) / 2][2 * ((k - 1) & 1)] = two[0];
+                            out[(k - 1) / 2][2 * ((k - 1) & 1) + 1] = two[1];
+                        }
+                        if constexpr (k == 5) widen_write(wide, n, out[0], out[1]);
+                    }
+                    if constexpr (x == 26) { ahead = source(t + 3, 0, page, 0); ahead2 = source(t + 3, 1, page, 0); }
+                    if constexpr (x >= 27) issue_raw(ahead, ahead2, raw0, raw0 + 16 * (kC / 2), std::integral_constant<int, x - 27>());
+                    if constexpr (x == 20) sc = scale_at(next, 1);
+                    return;
+                }
                 // copies of the tile after the next, one behind a product
                 if constexpr (x == 0 || x == 8) {
                     ahead = source(t + 2, x / 8, page_now, lds0 + st_free * kStage);
@@ -555,6 +717,7 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
                 if constexpr (x >= 9 && x < 15) issue(ahead, latents, Second(), std::integral_constant<int, x - 9>());
                 if constexpr (x == 20) sc = scale_at(next, 1);
             });
+            page_keys = page;
             if (t + 1 == t1) break;
             look_at_scale(1);
             st = st_next;
@@ -676,6 +839,7 @@ int launch_mla_decode_paged(const void* q, const void* freqs, const dsv3_mla_pag
     PagedArgs a;
     uint8_t* wsp = (uint8_t*)workspace;
     a.ql = wsp; a.qe = wsp + space.exponents; a.q = (const uint16_t*)q; a.freqs = (const v2f*)freqs;
+    const bool four = cache.kv_bits == 4;
     a.kv = (const uint8_t*)cache.kv; a.scales = cache.kv_scale; a.pe = (const uint8_t*)cache.pe;
     a.table = cache.table; a.width = cache.table_width; a.pages = cache.pages;
     a.starts = starts; a.counts = counts; a.tree = tree;
@@ -689,14 +853,15 @@ int launch_mla_decode_paged(const void* q, const void* freqs, const dsv3_mla_pag
     const int rc = launch_wkv_b_absorb_q_codes(q, (int64_t)heads * kQd, kQd, w, ws, wsp, wsp + space.exponents, pack, batch, tokens, (int)plan.blocks, heads, st);
     if (rc != DSV3_OK) return rc;
     const bool few = rows <= 32;
-    static void (*const kernels[2][2])(PagedArgs) = { { mla_paged_kernel<false, false>, mla_paged_kernel<true, false> },
-                                                      { mla_paged_kernel<false, true>, mla_paged_kernel<true, true> } };
-    static LdsGrant grant[2][2];
-    static_assert(kLds <= 160 * 1024 && kFewLds <= 160 * 1024 && 4 * 16384 <= kStages * kStage && 4096 + 2 * 32768 <= kFewLds, "the sums leave through the stages");
-    const int lds = few ? kFewLds : kLds;
-    if (!grant[few][pack].ensure((const void*)kernels[few][pack], lds)) return DSV3_ERR_LAUNCH;
+    static void (*const kernels[2][2][2])(PagedArgs) = {
+        { { mla_paged_kernel<false, false, false>, mla_paged_kernel<true, false, false> }, { mla_paged_kernel<false, true, false>, mla_paged_kernel<true, true, false> } },
+        { { mla_paged_kernel<false, false, true>, mla_paged_kernel<true, false, true> }, { mla_paged_kernel<false, true, true>, mla_paged_kernel<true, true, true> } } };
+    static LdsGrant grant[2][2][2];
+    static_assert(kLds4 <= 160 * 1024 && kFewLds <= 160 * 1024 && 4 * 16384 <= kStages * kStage && 4096 + 2 * 32768 <= kFewLds, "the sums leave through the stages");
+    const int lds = few ? kFewLds : four ? kLds4 : kLds;
+    if (!grant[four][few][pack].ensure((const void*)kernels[four][few][pack], lds)) return DSV3_ERR_LAUNCH;
     const unsigned grid = (unsigned)((plan.ranges * plan.blocks + 7) / 8 * 8);
-    hipLaunchKernelGGL(kernels[few][pack], dim3(grid), dim3(256), lds, st, a);
+    hipLaunchKernelGGL(kernels[four][few][pack], dim3(grid), dim3(256), lds, st, a);
     FoldArgs f = {};
     f.part = a.part; f.ml = a.ml; f.plan = a.plan; f.counts = counts; f.w = (const uint8_t*)w; f.ws = ws; f.y = y; f.ys = ys;
     f.tokens = (int)(batch * tokens); f.per_seq = (int)tokens; f.heads = heads; f.rows = 128; f.blocks = a.blocks;

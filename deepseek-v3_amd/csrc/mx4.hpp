@@ -7,6 +7,7 @@ namespace dsv3 {
 namespace {
 
 constexpr uint32_t kMx4Nan = 255u;
+constexpr uint32_t kMx4RowSpan = 14u;                   // of a cache row: no scale lies more powers of two below the row's largest
 
 // The smallest power of two of which no element is more than six times, from the bits of the largest |element|: largest = f 2^e with f in [1, 2)
 // is at most 6 2^(e - 2) where f <= 3/2, and 6 2^(e - 1) elsewhere.  Subnormal largest elements are below 6 2^-127.

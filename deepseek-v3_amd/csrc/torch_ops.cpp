@@ -385,19 +385,26 @@ Tensor mla_output(const Tensor& q, const Tensor& freqs, const Tensor& kv, const 
     return fp8_gemm(y, ys, wo, wo_s, DSV3_BF16);
 }
 
-// The paged cache of a layer, as its operators take it: kv e4m3 [pages, page, rank], scale fp32 [pages, page], pe bf16 [pages, page, rope],
-// and the sequences' page numbers, int32 [batch, width]
+// The paged cache of a layer, as its operators take it: kv e4m3 [pages, page, rank] with scales fp32 [pages, page], or e2m1 [pages, page, rank / 2] with e8m0
+// [pages, page, rank / 32]; pe bf16 [pages, page, rope] and the sequences' page numbers, int32 [batch, width]
+constexpr int64_t kRank = 512;
 dsv3_mla_pages checked_pages(const char* what, const Tensor& kv, const Tensor& scale, const Tensor& pe, const Tensor& table, int64_t batch) {
-    TORCH_CHECK(kv.dim() == 3 && kv.scalar_type() == kFp8 && kv.is_contiguous() && kv.size(0) > 0, what, ": kv_pages must be a contiguous e4m3 [pages, page, rank] of one page at least");
-    TORCH_CHECK(scale.dim() == 2 && scale.scalar_type() == at::kFloat && scale.is_contiguous() && scale.size(0) == kv.size(0) && scale.size(1) == kv.size(1),
-                what, ": kv_scale must be a contiguous fp32 [pages, page]");
+    const bool four = kv.scalar_type() == kFp4;
+    TORCH_CHECK(kv.dim() == 3 && (four || kv.scalar_type() == kFp8) && kv.is_contiguous() && kv.size(0) > 0, what, ": kv_pages must be a contiguous e4m3 [pages, page, rank] or float4_e2m1fn_x2 [pages, page, rank / 2] of one page at least");
+    if (four) {
+        TORCH_CHECK(scale.dim() == 3 && scale.scalar_type() == kE8m0 && scale.is_contiguous() && scale.size(0) == kv.size(0) && scale.size(1) == kv.size(1) && scale.size(2) * 16 == kv.size(2),
+                    what, ": kv_scale must be a contiguous float8_e8m0fnu [pages, page, rank / 32]");
+    } else {
+        TORCH_CHECK(scale.dim() == 2 && scale.scalar_type() == at::kFloat && scale.is_contiguous() && scale.size(0) == kv.size(0) && scale.size(1) == kv.size(1),
+                    what, ": kv_scale must be a contiguous fp32 [pages, page]");
+    }
     TORCH_CHECK(pe.dim() == 3 && pe.scalar_type() == at::kBFloat16 && pe.is_contiguous() && pe.size(0) == kv.size(0) && pe.size(1) == kv.size(1),
                 what, ": pe_pages must be a contiguous bf16 [pages, page, rope]");
     TORCH_CHECK(kv.size(1) >= 8 && kv.size(1) <= 16384 && kv.size(1) % 8 == 0, what, ": a page must have a multiple of 8 positions, up to 16384, got ", kv.size(1));
-    TORCH_CHECK(kv.size(2) == 512 && pe.size(2) == 64, what, ": latents of 512 and rotary keys of 64 are implemented, got ", kv.size(2), " and ", pe.size(2));
+    TORCH_CHECK(kv.size(2) == (four ? kRank / 2 : kRank) && pe.size(2) == 64, what, ": latents of 512 and rotary keys of 64 are implemented, got ", kv.size(2) * (four ? 2 : 1), " and ", pe.size(2));
     TORCH_CHECK(table.dim() == 2 && table.scalar_type() == at::kInt && table.is_contiguous() && table.size(0) == batch && table.size(1) > 0,
                 what, ": page_table must be a contiguous int32 [batch, width]");
-    return { kv.data_ptr(), (float*)scale.data_ptr(), pe.data_ptr(), kv.size(0), (int)kv.size(1), (const int32_t*)table.data_ptr(), table.size(1) };
+    return { kv.data_ptr(), scale.data_ptr(), pe.data_ptr(), kv.size(0), (int)kv.size(1), (const int32_t*)table.data_ptr(), table.size(1), four ? 4 : 8 };
 }
 const int32_t* checked_ints(const char* what, const char* name, const Tensor& t, int64_t batch) {
     TORCH_CHECK(t.dim() == 1 && t.scalar_type() == at::kInt && t.is_contiguous() && t.size(0) == batch, what, ": ", name, " must be a contiguous int32 [batch]");
@@ -418,14 +425,14 @@ tuple<Tensor, Tensor> mla_latent_paged(const Tensor& a, const OptTensor& qn, con
     const int32_t* at_start = checked_ints(what, "starts", starts, b);
     const int32_t* count = checked_ints(what, "counts", counts, b);
     check_row_freqs(what, freqs, b, s, pe.size(2));
-    TORCH_CHECK(kn.numel() == kv.size(2) && kn.scalar_type() == at::kBFloat16 && kn.is_contiguous() &&
-                (!qn || (qn->scalar_type() == at::kBFloat16 && qn->is_contiguous() && qr > 0)) && a.size(2) == qr + kv.size(2) + pe.size(2),
+    TORCH_CHECK(kn.numel() == kRank && kn.scalar_type() == at::kBFloat16 && kn.is_contiguous() &&
+                (!qn || (qn->scalar_type() == at::kBFloat16 && qn->is_contiguous() && qr > 0)) && a.size(2) == qr + kRank + pe.size(2),
                 what, ": norm weights do not fit the row");
     on_one_gpu(what, a, { qn ? &*qn : &a, &kn, &freqs, &kv, &scale, &pe, &table, &starts, &counts });
     Tensor y = at::empty({b, s, qr}, a.options().dtype(kFp8)), ys = at::empty({b, s, qr / 128}, a.options().dtype(at::kFloat));
     On on(a);
     check(dsv3_mla_latent_paged(a.data_ptr(), a.size(2), qn ? qn->data_ptr() : nullptr, kn.data_ptr(), (const float*)freqs.data_ptr(), &cache, at_start,
-                                count, y.data_ptr(), (float*)ys.data_ptr(), b, s, qr, kv.size(2), (int)pe.size(2), (float)q_eps, (float)kv_eps,
+                                count, y.data_ptr(), (float*)ys.data_ptr(), b, s, qr, kRank, (int)pe.size(2), (float)q_eps, (float)kv_eps,
                                 on.stream), "dsv3_mla_latent_paged");
     return {y, ys};
 }
@@ -438,7 +445,7 @@ tuple<Tensor, Tensor> mla_cache_read(const Tensor& kv, const Tensor& scale, cons
     const int32_t* length = checked_ints(what, "lengths", lengths, b);
     TORCH_CHECK(positions >= 0 && positions <= 0x7fffff, what, ": positions must be 0 to ", 0x7fffff, ", got ", positions);
     on_one_gpu(what, kv, { &scale, &pe, &table, &lengths });
-    Tensor out = at::empty({b, positions, kv.size(2)}, pe.options()), out_pe = at::empty({b, positions, pe.size(2)}, pe.options());
+    Tensor out = at::empty({b, positions, kRank}, pe.options()), out_pe = at::empty({b, positions, pe.size(2)}, pe.options());
     On on(kv);
     check(dsv3_mla_cache_read(&cache, length, out.data_ptr(), out_pe.data_ptr(), b, positions, on.stream), "dsv3_mla_cache_read");
     return {out, out_pe};
@@ -457,9 +464,9 @@ void attention_paged(const char* what, const Tensor& q, const Tensor& freqs, con
     check_row_freqs(what, freqs, b, s, pe.size(2));
     TORCH_CHECK(s <= 64, what, ": up to 64 new tokens a sequence are implemented, got ", s);
     TORCH_CHECK(q.size(3) == 128 + pe.size(2), what, ": q must have 128 elements and the rotary ones a head, got ", q.size(3));
-    TORCH_CHECK(w.dim() == 2 && w.is_contiguous() && w.scalar_type() == kFp8 && w.size(1) == kv.size(2) && w.size(0) == h * 256, what,
+    TORCH_CHECK(w.dim() == 2 && w.is_contiguous() && w.scalar_type() == kFp8 && w.size(1) == kRank && w.size(0) == h * 256, what,
                 ": wkv_b must be a contiguous fp8 [h * (128 + 128), kv_rank]");
-    TORCH_CHECK(ws.scalar_type() == at::kFloat && ws.dim() == 2 && ws.is_contiguous() && ws.size(0) == h * 2 && ws.size(1) == kv.size(2) / 128, what,
+    TORCH_CHECK(ws.scalar_type() == at::kFloat && ws.dim() == 2 && ws.is_contiguous() && ws.size(0) == h * 2 && ws.size(1) == kRank / 128, what,
                 ": wkv_b's scales must be fp32, one per block of 128 x 128");
     if (tree)
         TORCH_CHECK(tree->dim() == 2 && tree->scalar_type() == at::kLong && tree->is_contiguous() && tree->size(0) == b && tree->size(1) == s, what,

@@ -24,7 +24,7 @@ OK = 0
 class MlaPages(ctypes.Structure):
     """dsv3_mla_pages (include/dsv3_fp8.h)."""
     _fields_ = [("kv", c_void_p), ("kv_scale", c_void_p), ("pe", c_void_p), ("pages", c_int64), ("page_size", c_int),
-                ("table", c_void_p), ("table_width", c_int64)]
+                ("table", c_void_p), ("table_width", c_int64), ("kv_bits", c_int)]
 
 
 _pages_p = ctypes.POINTER(MlaPages)

@@ -235,18 +235,24 @@ _mla_output = torch.ops.dsv3fp8.mla_output.default
 
 
 class LatentPages:
-    """The cache of one attention layer in pages of e4m3 rows, for ``MLA.forward_paged``: ``kv`` [pages, page_size, 512] codes, ``scale``
+    """The cache of one attention layer in pages, for ``MLA.forward_paged``.  ``bits`` 8: ``kv`` [pages, page_size, 512] e4m3 codes, ``scale``
     [pages, page_size] one power of two a row, ``pe`` [pages, page_size, 64] rotary keys in bf16; 644 bytes a position where ``kv_cache`` and
-    ``pe_cache`` take 1152.  Sequence i's position t lies in page ``page_table[i, t // page_size]`` (int32; an entry that is no page of the
+    ``pe_cache`` take 1152.  ``bits`` 4: ``kv`` [pages, page_size, 256] of microscaled 4-bit numbers (``mx4_quant``), ``scale`` [pages, page_size, 16]
+    their powers of two per 32; 400 bytes.  Sequence i's position t lies in page ``page_table[i, t // page_size]`` (int32; an entry that is no page of the
     pool stands for none: nothing is written there, and nobody sees it).  Which page belongs to whom is the program's business; two
     sequences may share the pages of a common beginning as long as neither writes into them.  ``page_size``: a multiple of 8 up to 16384."""
 
-    def __init__(self, pages: int, page_size: int, device=None):
+    def __init__(self, pages: int, page_size: int, device=None, bits: int = 8):
         if pages < 1 or page_size % 8 or not 8 <= page_size <= 16384:
             raise ValueError(f"LatentPages: {pages} pages of {page_size} rows; a page has a multiple of 8, 8 to 16384")
+        if bits not in (4, 8):
+            raise ValueError(f"LatentPages: rows of {bits} bits; 4 and 8 are implemented")
         device = device if device is not None else torch.get_default_device()
-        self.kv = torch.zeros(pages, page_size, 512, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
-        self.scale = torch.ones(pages, page_size, dtype=torch.float32, device=device)
+        self.kv = torch.zeros(pages, page_size, 64 * bits, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn if bits == 8 else torch.float4_e2m1fn_x2)
+        if bits == 8:
+            self.scale = torch.ones(pages, page_size, dtype=torch.float32, device=device)
+        else:
+            self.scale = torch.full((pages, page_size, 16), 127, dtype=torch.uint8, device=device).view(torch.float8_e8m0fnu)
         self.pe = torch.zeros(pages, page_size, 64, dtype=torch.bfloat16, device=device)
 
     def read(self, page_table: torch.Tensor, lengths: torch.Tensor, positions: int) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -552,7 +558,7 @@ class MLA(nn.Module):
             return fp8_gemm(yq, ys, wo, wo.scale)
         kv, pe = cache.read(page_table, torch.full_like(starts, positions), positions)         # (what lies behind a sequence is hidden from its tokens)
         at = torch.arange(max(s, positions), device=x.device)
-        new, at, pages, page = at[:s], at[:positions], *cache.scale.shape
+        new, at, pages, page = at[:s], at[:positions], *cache.scale.shape[:2]
         # What a position adds to the scores of those who see it: nothing, or -inf where it lies in no page (its row was read as zeros).  Position 0 gets the
         # lowest number then: beside any other its weight is zero, and who sees no other (who sees one has position 0 in a page or another) gets that row of zeros.
         entries = page_table[:, :-(-positions // page)]

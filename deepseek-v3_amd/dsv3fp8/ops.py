@@ -330,7 +330,7 @@ def _mla_latent_paged_meta(a, q_norm, kv_norm, freqs, kv_pages, kv_scale, pe_pag
 
 def _mla_cache_read_meta(kv_pages, kv_scale, pe_pages, page_table, lengths, positions):
     b = page_table.size(0)
-    return pe_pages.new_empty(b, positions, kv_pages.size(2)), pe_pages.new_empty(b, positions, pe_pages.size(2))
+    return pe_pages.new_empty(b, positions, kv_pages.size(2) * (2 if kv_pages.dtype == FP4 else 1)), pe_pages.new_empty(b, positions, pe_pages.size(2))
 
 
 def _mla_decode_paged_meta(q, freqs, kv_pages, kv_scale, pe_pages, page_table, starts, counts, tree, wkv_b, scale, positions, softmax_scale):

@@ -444,7 +444,7 @@ int dsv3_mla_latent_gemm(const void* x, const float* x_s, const void* w, const f
                          int rope_dim, float q_eps, float kv_eps, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
- * ---- The latent cache of the attention layer in pages, in eight bits ----
+ * ---- The latent cache of the attention layer in pages, in eight bits or in four ----
  *
  * The reference keeps one dense bf16 cache per layer with a place for every position of every sequence (inference/model.py:443-444).
  * Here sequences share pages of page_size positions (a multiple of 8, up to 16384): row j of a sequence is row
@@ -452,6 +452,10 @@ int dsv3_mla_latent_gemm(const void* x, const float* x_s, const void* w, const f
  *     kv       e4m3 [pages, page_size, 512]     the latent's codes (16-byte aligned)
  *     kv_scale binary32 [pages, page_size]      a power of two: latent = code * scale, a bf16 number (4-byte aligned)
  *     pe       bf16 [pages, page_size, 64]      the rotated key (16-byte aligned)
+ * or, with kv_bits 4, microscaled 4-bit numbers (dsv3_mx4_quant),
+ *     kv       e2m1 [pages, page_size, 256]     two codes a byte (16-byte aligned)
+ *     kv_scale e8m0 [pages, page_size, 16]      a power of two per 32 latents (16-byte aligned), none more than 2^14 below the row's largest
+ * 400 bytes a position where eight bits take 644 and the dense cache 1152.
  * An entry of the table outside [0, pages) names no page: rows there are not written, are read as zeros and seen by no query.
  * The struct lies in host memory and is read during the call; everything it points to is device memory.  Rows that the functions read
  * are those that they have written, or zeros: codes that are NaN by themselves are none of these.
@@ -460,19 +464,21 @@ int dsv3_mla_latent_gemm(const void* x, const float* x_s, const void* w, const f
  */
 typedef struct dsv3_mla_pages {
     void* kv;
-    float* kv_scale;
+    void* kv_scale;
     void* pe;
     int64_t pages;
     int page_size;
     const int32_t* table;       /* int32 [batch, table_width] */
     int64_t table_width;
+    int kv_bits;                /* 8 (or 0): e4m3 codes, one scale a row; 4: see below */
 } dsv3_mla_pages;
 
 /*
  * dsv3_mla_latent whose cache rows go into pages (inference/model.py:457-466, :480-483), for rows a[i] = [ query latent (q_rank) | latent (512) | rotary key (64) ]:
  *     n = bf16( rms_norm(latent) * kv_norm ),  scale = 2^ceil(log2( max(amax n, 1e-4) / 448 )),  kv = e4m3( n / scale ),  pe = bf16( rotated key )
  * at row starts[b] + i of sequence b, i < counts[b]; y, s as dsv3_mla_latent.  The norms' sums are binary64 here.  A latent that holds a
- * NaN or an infinity is stored as zeros with a scale of NaN.  q_rank 0: no query latent (q_norm, y and s are not looked at).
+ * NaN or an infinity is stored as zeros with a scale of NaN.  In four bits: n as dsv3_mx4_quant leaves it, but that no scale is less than 2^-14 times the
+ * row's largest (its block's codes are the smaller for it), and a row that is not finite has codes of zero and scales of NaN throughout.  q_rank 0: no query latent (q_norm, y and s are not looked at).
  * freqs: binary32 (cos, sin) pairs [batch, rows, 32], each row's own.  A negative start: none of the sequence's rows is written.
  * Two rows that the table sends to one place leave either's values there, or parts of both.  Up to 13421772 rows in all, without a query
  * latent 67108860 (what a launch holds).
