@@ -215,12 +215,12 @@ __global__ __launch_bounds__(256, RT * CT >= 16 ? 1 : 2) void mx4_tile_kernel(Ti
             });
         });
     };
-    // (one way out: with several the compiler moves the sums)
-    for (int s = 0;;) {
+    // (one way out, at the end: otherwise the compiler moves the sums)
+    int s = 0;
+    do {
         stage(s, I0(), I0());
         stage(s + 1, I1(), std::integral_constant<int, A8 ? 0 : 1>());
         s += 2;
-        if (s >= stages) break;
         if constexpr (A8) {
 #pragma unroll
             for (int t = 0; t < GA; ++t) sa[0][t] = sa[1][t];
@@ -228,7 +228,7 @@ __global__ __launch_bounds__(256, RT * CT >= 16 ? 1 : 2) void mx4_tile_kernel(Ti
             for (int t = 0; t < GB; ++t) sb[0][t] = sb[1][t];
             load_scales(s / 2 + 1, I1());
         }
-    }
+    } while (s < stages);
     __builtin_amdgcn_s_waitcnt(0x0070);                 // (copies past the end are still on their way into LDS)
     barrier_no_fence();
 
