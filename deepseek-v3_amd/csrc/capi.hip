@@ -116,7 +116,7 @@ int dsv3_mx4_dequant(const void* x, const void* s, void* y, int y_dtype, int64_t
 }
 
 static bool mx4_gemm_sizes_ok(int64_t m, int64_t n, int64_t k) {
-    return m >= 0 && n >= 0 && k >= 0 && k % 128 == 0 && m <= 0x7fffffff && n <= 0x7fffffff && k <= 0x7fffffff;
+    return m >= 0 && n >= 0 && k >= 0 && k % 128 == 0 && m <= 0x7fffff00 && n <= 0x7fffff00 && k <= 1 << 22;     // (offsets in a tile are 32 bits)
 }
 
 size_t dsv3_mx4_gemm_workspace_bytes(int a_kind, int64_t m, int64_t n, int64_t k) {

@@ -14,7 +14,6 @@ struct Mx4Args {
     int64_t m, n, k;
 };
 
-bool mx4_tile_takes(int64_t m, int64_t n, int64_t k);
 int launch_mx4_stream(const Mx4Args& p, bool a8, int c_dtype, hipStream_t st);
 size_t mx4_tile_workspace_bytes(int64_t m, int64_t n, int64_t k, bool a8);
 int launch_mx4_tile(const Mx4Args& p, bool a8, int c_dtype, void* workspace, hipStream_t st);

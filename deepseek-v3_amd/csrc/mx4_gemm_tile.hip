@@ -6,73 +6,100 @@ namespace dsv3 {
 namespace {
 
 typedef const __attribute__((address_space(3))) v4u* lds_read16;
-// the loaded value is looked at here
-__device__ __forceinline__ void there(v2u& x) { asm volatile("" : "+v"(x)); }
+typedef const __attribute__((address_space(3))) v2u* lds_read8;
 
 struct TileArgs {
     const uint8_t* a; const uint8_t* b;
-    const v2u* as; const v2u* bs;                       // scales as the instruction takes them, of 64 rows and 256 along k: a dword per lane for each 32 rows
+    const uint8_t* as; const uint8_t* bs;               // scales as the instruction takes them
     void* c; v4f* part;                                 // results, or sums of slices [slice][tile][wavefront][16-byte pieces][lane]
-    int m, n, k, units, pack_units;                     // units: of 256 along k, the last one may be half; those that there are scales for
-    int tiles_m, tiles_n, per_slice;                    // units of a slice, an even number
+    int m, n, k, steps, pack_cols;                      // steps: of 128 along k; those that there are scales for
+    int tiles_m, tiles_n, per_slice;                    // steps of a slice, an even number
 };
 
-// ---- scales.  A lane (r, g) = (l % 32, l / 32) of v_mfma_scale_f32_32x32x64_f8f6f4 gives the scale of row r's block g of 32.  Four products
-// u = 0 .. 3 take 256 along k; product u multiplies blocks 4 (u / 2) + u % 2 (g = 0) and two further (g = 1), so that its four scales are one dword:
-// bytes 2 g, 2 g + 1 of the first 128 and of the second.  Rows and products that are not there get zeros.
-struct PackArgs { const uint32_t* a; const uint32_t* b; v2u* as; v2u* bs; int64_t a_groups, b_groups; int m, n, cols, units; };
+// ---- scales.  A lane (r, g) = (l % 32, l / 32) of v_mfma_scale_f32_32x32x64_f8f6f4 gives the scale of row r's block g of 32.  Two products
+// u = 0, 1 take 128 along k; product u multiplies blocks u (g = 0) and u + 2 (g = 1), so that a lane's two scales are the bytes 2 g, 2 g + 1 of the row's four.
+// They are laid out for 128 rows and 128 along k as 512 bytes, eight for each lane: two for each 32 rows.  Rows that are not there, and what lies behind k, get zeros.
+struct PackArgs { const uint32_t* a; const uint32_t* b; v2u* as; v2u* bs; int64_t a_groups, b_groups; int m, n, cols, pack_cols; };
 template <bool A8> __global__ __launch_bounds__(256) void mx4_pack_kernel(PackArgs p) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, g = lane >> 5;
+    constexpr int COLS = 16;                            // of a workgroup
+    __shared__ uint32_t rows[128][COLS + 1];
     int64_t group = blockIdx.x;
     const bool of_a = group < p.a_groups;
     if (!of_a) group -= p.a_groups;
     const uint32_t* src = of_a ? p.a : p.b;
-    const int rows = of_a ? p.m : p.n;
-    v2u* dst = (of_a ? p.as : p.bs) + group * p.units * 64 + lane;
-    for (int unit = blockIdx.y * 16 + wave; unit < min(p.units, (int)blockIdx.y * 16 + 16); unit += 4) {
-        v2u w = {};
+    const int64_t have = of_a ? p.m : p.n;
+    const int c0 = blockIdx.y * COLS, t = threadIdx.x;
+    uint32_t x[8];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int64_t row = group * 64 + t * 32 + r;
-            if (row >= rows) continue;
-            const uint32_t* s = src + row * p.cols + 2 * unit;
-            uint32_t lo = 2 * unit < p.cols ? s[0] : 0u, hi = 2 * unit + 1 < p.cols ? s[1] : 0u;
-            if (A8 && of_a) { lo = (lo >> 23 & 0xffu) * 0x01010101u; hi = (hi >> 23 & 0xffu) * 0x01010101u; }
-            w[t] = (lo >> (16 * g) & 0xffffu) | (hi >> (16 * g)) << 16;
-        }
-        dst[(int64_t)unit * 64] = w;
+    for (int i = 0; i < 8; ++i) {                       // 16 rows at a time, a whole piece of each
+        const int64_t row = group * 128 + i * 16 + (t >> 4);
+        const int col = c0 + (t & 15);
+        x[i] = row < have && col < p.cols ? src[row * p.cols + col] : 0u;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) rows[i * 16 + (t >> 4)][t & 15] = A8 && of_a ? (x[i] >> 23 & 0xffu) * 0x01010101u : x[i];
+    __syncthreads();
+    const int lane = t & 63, r = lane & 31, g = lane >> 5;
+    v2u* dst = (of_a ? p.as : p.bs) + (group * p.pack_cols + c0) * 64 + lane;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int c = (t >> 6) + 4 * i;
+        if (c0 + c >= p.pack_cols) break;
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = rows[j * 32 + r][c] >> (16 * g) & 0xffffu;
+        dst[(int64_t)c * 64] = v2u{ w[0] | w[1] << 16, w[2] | w[3] << 16 };
     }
 }
 
 // The product of 32 weight rows and 32 activation rows over 64 along k, onto sums that stay in accumulation registers: as builtins with 16 of them the compiler
 // moves and spills the sums.  It does not know that these are MFMAs, so what it would keep apart stands here: two wait states in front (an ordinary instruction
-// may have written an operand); behind the last one, before a sum is read, sums_there.  SEL: the byte of both scales.
-template <int SEL> __device__ __forceinline__ void mfma_codes(v16f& d, v4u w, v4u a, uint32_t sw, uint32_t sa) {
-    asm volatile("s_nop 1\n\tv_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%5,0] op_sel_hi:[%6,%6,0] cbsz:4 blgp:4"
-                 : "+a"(d) : "v"(w), "v"(a), "v"(sw), "v"(sa), "n"(SEL & 1), "n"(SEL >> 1));
+// may have written an operand); behind the last one, before a sum is read, sums_there.  SW, SA: the bytes of their scales.
+template <int SW, int SA> __device__ __forceinline__ void mfma_codes(v16f& d, v4u w, v4u a, uint32_t sw, uint32_t sa) {
+    asm volatile("s_nop 1\n\tv_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%6,0] op_sel_hi:[%7,%8,0] cbsz:4 blgp:4"
+                 : "+a"(d) : "v"(w), "v"(a), "v"(sw), "v"(sa), "n"(SW & 1), "n"(SA & 1), "n"(SW >> 1), "n"(SA >> 1));
 }
-template <int SEL> __device__ __forceinline__ void mfma_codes(v16f& d, v4u w, v8i a, uint32_t sw, uint32_t sa) {
-    asm volatile("s_nop 1\n\tv_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%5,0] op_sel_hi:[%6,%6,0] cbsz:4 blgp:0"
-                 : "+a"(d) : "v"(w), "v"(a), "v"(sw), "v"(sa), "n"(SEL & 1), "n"(SEL >> 1));
+template <int SW, int SA> __device__ __forceinline__ void mfma_codes(v16f& d, v4u w, v8i a, uint32_t sw, uint32_t sa) {
+    asm volatile("s_nop 1\n\tv_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%6,0] op_sel_hi:[%7,%8,0] cbsz:4 blgp:0"
+                 : "+a"(d) : "v"(w), "v"(a), "v"(sw), "v"(sa), "n"(SW & 1), "n"(SA & 1), "n"(SW >> 1), "n"(SA >> 1));
 }
 __device__ __forceinline__ void sums_there(v16f& d) { asm volatile("s_nop 15\n\ts_nop 15" : "+a"(d)); }
 
-// ---- the product.  Four wavefronts, 2 x 2, each 32 RT activation rows x 32 CT weight rows.  A stage of LDS holds 128 bytes of every activation row
-// (256 codes, or 128 e4m3 ones) and the codes of the weight rows that meet them; chunks of 16 bytes stand at c ^ (row / 2 % 8), in rows of 64 bytes at
-// c ^ (row / 4 % 4), so that 16 rows read at one place hit all banks.
-template <bool A8, int RT, int CT> struct Geo {
+// Two copies of 1 KiB, to lds_addr and the KiB behind it (the second one's offset counts for both its addresses)
+__device__ __forceinline__ void copy16_two(const void* base, uint32_t off, uint32_t off_less_1024, uint32_t lds_addr) {
+    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %2\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024"
+                 :: "v"(off), "v"(off_less_1024), "s"(base), "s"(lds_addr) : "memory", "m0");
+}
+template <int N> __device__ __forceinline__ void wait_copies() {        // all but the N youngest
+    __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4) << 14);
+    asm volatile("" ::: "memory");
+}
+
+// ---- the product.  Four wavefronts, 2 x 2, each 32 RT activation rows x 32 CT weight rows.  A stage of LDS holds 128 along k: rows of 64 bytes, or 128 of
+// e4m3 activations, whose chunks of 16 bytes stand at c ^ (row / 4 % 4) and c ^ (row / 2 % 8), so that 16 rows read at one place hit all banks.
+//
+// D stages, D - 1 on their way.  A compute unit has one tile of 256 x 256, or two of 128 x 128, whose barriers and copies stand beside each other's products.
+//
+// Measured, mx4 x mx4: 4096 x 7168 -> 18432 in 282 .. 292 us by card (3.7 .. 3.8 PFLOP/s), 4096 x 18432 -> 7168 in 262 .. 271 (4.0 .. 4.1); e4m3 x mx4
+// 376 .. 395 and 360 .. 375.  4.5 and 1.75 rounds of tiles cost the first 10 % and the second 12 %.  The products alone, with neither copies nor reads, would take
+// 200 and 180 us at the 1.85 GHz that the chip's power leaves: the copies cost 50 us more, the reads 20.  More stages on their way change nothing there (three
+// or four), nor do stages of twice the length.
+template <bool A8, int RT, int CT, int D> struct Geo {
     static constexpr int TM = 64 * RT, TN = 64 * CT;
-    static constexpr int SUB = A8 ? 2 : 4;              // products along k of a stage
-    static constexpr int WB = A8 ? 64 : 128;            // bytes of a weight row
-    static constexpr int SA = TM * 128, SB = TN * WB;
-    static constexpr int NA = TM / 32, NB = TN * WB / 4096;             // copies of a wavefront
-    static constexpr int LDS = 2 * (SA + SB);
+    static constexpr int AB = A8 ? 128 : 64, WB = 64;   // bytes of a row
+    static constexpr int SA = TM * AB, SB = TN * WB;
+    static constexpr int GA = (TM + 127) / 128, GB = (TN + 127) / 128;  // 128 rows whose scales come in as one
+    static constexpr int SS = (GA + GB) * 512;
+    static constexpr int NA = SA / 4096, NB = SB / 4096, NS = (GA + GB) / 2, NC = NA + NB + NS;         // copies of a wavefront
+    static constexpr int B0 = D * SA, S0 = B0 + D * SB, LDS = S0 + D * SS;
+    static_assert(NA * 4096 == SA && NB * 4096 == SB && NS * 2 == GA + GB, "whole copies for every wavefront");
+    static_assert((D - 1) * NC < 64, "no more copies than can be counted");
 };
 
-template <bool A8, int RT, int CT, int CD, bool SPLIT>
-__global__ __launch_bounds__(256, RT * CT >= 16 ? 1 : 2) void mx4_tile_kernel(TileArgs p) {
-    using G = Geo<A8, RT, CT>;
-    constexpr int SUB = G::SUB, NA = G::NA, NB = G::NB, NC = NA + NB, X = RT * CT;
+template <bool A8, int RT, int CT, int D, int CD, bool SPLIT>
+__global__ __launch_bounds__(256, 1) void mx4_tile_kernel(TileArgs p) {
+    using G = Geo<A8, RT, CT, D>;
+    constexpr int NA = G::NA, NB = G::NB, NC = G::NC, X = RT * CT;
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave & 1, wn = wave >> 1, r = lane & 31, g = lane >> 5;
@@ -86,148 +113,154 @@ __global__ __launch_bounds__(256, RT * CT >= 16 ? 1 : 2) void mx4_tile_kernel(Ti
         m0 = (4 * band + in % rows) * G::TM;
         n0 = in / rows * G::TN;
     }
-    const int u0 = blockIdx.y * p.per_slice, units = min(p.per_slice, p.units - u0);
-    const int steps128 = min(p.k / 128 - 2 * u0, 2 * units);            // of the slice
-    const int last = (A8 ? steps128 : units) - 1, stages = last + 2 & ~1;   // an odd one out is followed by itself, with scales of zero
+    const int k0 = blockIdx.y * p.per_slice, last = min(p.per_slice, p.steps - k0) - 1;
+    const int stages = last + 2 & ~1;                   // an odd one out is followed by itself, with scales of zero
 
     // ---- copies into LDS
     const uint32_t lds0 = lds_addr_of(lds);
     const uint32_t a_row = A8 ? p.k : p.k / 2, b_row = p.k / 2;
-    const uint8_t* a0 = p.a + (int64_t)m0 * a_row + (int64_t)u0 * (A8 ? 256 : 128);
-    const uint8_t* b0 = p.b + (int64_t)n0 * b_row + (int64_t)u0 * 128;
-    uint32_t a_off[NA], b_off[NB];                      // rows past the end repeat the last one
+    // (addresses from 1024 in front, which the second copy of two takes off)
+    const uint8_t* a0 = p.a + (int64_t)m0 * a_row + (int64_t)k0 * G::AB - 1024;
+    const uint8_t* b0 = p.b + (int64_t)n0 * b_row + (int64_t)k0 * G::WB - 1024;
+    constexpr int AR = 1024 / G::AB, BR = 16;           // rows of a copy; those past the end repeat the last one
+    uint32_t a_off[NA], b_off[NB];
 #pragma unroll
     for (int t = 0; t < NA; ++t) {
-        const int row = (wave * NA + t) * 8 + (lane >> 3);
-        a_off[t] = min(row, p.m - 1 - m0) * a_row + (((lane & 7) ^ (row >> 1 & 7)) << 4);
+        const int row = (wave * NA + t) * AR + lane / (64 / AR), c = A8 ? lane & 7 ^ row >> 1 & 7 : lane & 3 ^ row >> 2 & 3;
+        a_off[t] = min(row, p.m - 1 - m0) * a_row + c * 16 + 1024 - (t & 1) * 1024;
     }
 #pragma unroll
     for (int t = 0; t < NB; ++t) {
-        const int row = A8 ? (wave * NB + t) * 16 + (lane >> 2) : (wave * NB + t) * 8 + (lane >> 3);
-        b_off[t] = min(row, p.n - 1 - n0) * b_row + (A8 ? ((lane & 3) ^ (row >> 2 & 3)) << 4 : ((lane & 7) ^ (row >> 1 & 7)) << 4);
+        const int row = (wave * NB + t) * BR + lane / 4, c = lane & 3 ^ row >> 2 & 3;
+        b_off[t] = min(row, p.n - 1 - n0) * b_row + c * 16 + 1024 - (t & 1) * 1024;
     }
-    // a last stage of half the codes: the other half is the first once more, its scales are zeros
-    const int odd = !A8 && (steps128 & 1);
-    auto copy = [&](int s, auto slot, auto which) {
-        constexpr int n = decltype(which)::value, S = decltype(slot)::value;
+    // scales: 512 bytes for each 128 rows, wavefronts 0 and 1 (2 and 3) one group's halves
+    const uint8_t* sc0[G::NS];
+#pragma unroll
+    for (int i = 0; i < G::NS; ++i) {
+        const int group = 2 * i + (wave >> 1);
+        sc0[i] = (group < G::GA ? p.as + ((int64_t)(m0 / 128 + group) * p.pack_cols + k0) * 512 : p.bs + ((int64_t)(n0 / 128 + group - G::GA) * p.pack_cols + k0) * 512) + (wave & 1) * 256;
+    }
+    // requests of a stage: two copies each (or what is left), then the scales
+    constexpr int QA = (NA + 1) / 2, QB = (NB + 1) / 2, NQ = QA + QB + G::NS;
+    auto copy = [&](int s, int slot, auto which) {
+        constexpr int n = decltype(which)::value;
         const int at = min(s, last);
-        uint32_t back = 0u;
-        if constexpr (!A8) {
-            const int t = n < NA ? n : n - NA, row = (wave * (n < NA ? NA : NB) + t) * 8 + (lane >> 3);
-            back = odd && at == last && (((lane & 7) ^ (row >> 1 & 7)) & 4) ? 64u : 0u;
+        if constexpr (n < QA) {
+            const uint32_t to = lds0 + slot * G::SA + (wave * NA + 2 * n) * 1024;
+            if constexpr (2 * n + 1 < NA) copy16_two(a0 + (int64_t)at * G::AB, a_off[2 * n], a_off[2 * n + 1], to);
+            else copy16(a0 + (int64_t)at * G::AB, a_off[2 * n], to);
+        } else if constexpr (n < QA + QB) {
+            constexpr int t = 2 * (n - QA);
+            const uint32_t to = lds0 + G::B0 + slot * G::SB + (wave * NB + t) * 1024;
+            if constexpr (t + 1 < NB) copy16_two(b0 + (int64_t)at * G::WB, b_off[t], b_off[t + 1], to);
+            else copy16(b0 + (int64_t)at * G::WB, b_off[t], to);
+        } else {                                        // (of the stage past an odd one out, zeros)
+            constexpr int i = n - QA - QB;
+            copy4(sc0[i] + (int64_t)min(s, p.pack_cols - 1 - k0) * 512, lane * 4, lds0 + G::S0 + slot * G::SS + i * 1024 + wave * 256);
         }
-        if constexpr (n < NA) copy16(a0 + (int64_t)at * 128, a_off[n] - back, lds0 + S * G::SA + (wave * NA + n) * 1024);
-        else copy16(b0 + (int64_t)at * G::WB, b_off[n - NA] - back, lds0 + 2 * G::SA + S * G::SB + (wave * NB + n - NA) * 1024);
     };
+    // They are spread over the stage's last product and the next stage's first one: this many of them in the former
+    auto early = [](int n) constexpr { return n * 2 * X / NQ < X; };
 
-    // ---- fragments
-    const uint32_t a_rd = lds0 + (wm * 32 * RT + r) * 128, b_rd = lds0 + 2 * G::SA + (wn * 32 * CT + r) * G::WB;
+    // ---- fragments and scales
     auto read16 = [](uint32_t at) -> v4u { return *(lds_read16)(uintptr_t)at; };
-    uint32_t a_ch[4], b_ch[SUB];               // where the lane's chunk of product u lies in its row
+    // where the lane's chunk of product u lies in a stage, beside the wavefront's first row
+    uint32_t a_ch[A8 ? 4 : 2], b_ch[2];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-        // e4m3: halves of blocks u (bytes 32 u + 16 g) and u + 2
-        const int c = A8 ? 2 * (u & 1) + 4 * (u >> 1) + g : 4 * (u >> 1) + 2 * g + (u & 1);
-        a_ch[u] = a_rd + ((c ^ (r >> 1 & 7)) << 4);
-    }
+    for (int u = 0; u < 2; ++u) b_ch[u] = r * 64 + ((2 * g + u ^ r >> 2 & 3) << 4);
 #pragma unroll
-    for (int u = 0; u < SUB; ++u) {
-        const int c = A8 ? 2 * g + u : 4 * (u >> 1) + 2 * g + (u & 1);
-        b_ch[u] = b_rd + (A8 ? ((c ^ (r >> 2 & 3)) << 4) : ((c ^ (r >> 1 & 7)) << 4));
-    }
-    v4u fa[2][RT][A8 ? 2 : 1], fb[2][CT];
-    constexpr int NR = (A8 ? 2 : 1) * RT + CT;          // reads of a product's fragments
-    auto read = [&](auto slot, auto prod, auto buf, auto which) {
-        constexpr int S = decltype(slot)::value, u = decltype(prod)::value, B = decltype(buf)::value, n = decltype(which)::value;
-        if constexpr (n < CT) fb[B][n] = read16(b_ch[u] + S * G::SB + n * 32 * G::WB);
-        else if constexpr (A8) fa[B][(n - CT) / 2][(n - CT) % 2] = read16(a_ch[u + 2 * ((n - CT) % 2)] + S * G::SA + (n - CT) / 2 * 4096);
-        else fa[B][n - CT][0] = read16(a_ch[u] + S * G::SA + (n - CT) * 4096);
-    };
-
-    // ---- scales: of a unit, for 64 rows each
-    constexpr int GA = (RT + 1) / 2, GB = (CT + 1) / 2;
-    const v2u* as = p.as + ((int64_t)((m0 + wm * 32 * RT) / 64) * p.pack_units + u0) * 64 + lane;
-    const v2u* bs = p.bs + ((int64_t)((n0 + wn * 32 * CT) / 64) * p.pack_units + u0) * 64 + lane;
-    v2u sa[2][GA], sb[2][GB];                           // of the unit in use and the next
-    auto load_scales = [&](int unit, auto buf) {
+    for (int u = 0; u < (A8 ? 4 : 2); ++u)              // e4m3: halves g of blocks u and u + 2
+        a_ch[u] = A8 ? r * 128 + ((2 * (u & 1) + 4 * (u >> 1) + g ^ r >> 1 & 7) << 4) : b_ch[u];
+    const uint32_t a_rd = lds0 + wm * 32 * RT * G::AB, b_rd = lds0 + G::B0 + wn * 32 * CT * G::WB;
+    // the wavefront's tiles in a lane's eight bytes of 128 rows (tiles of 64 rows may be the second half of them)
+    const uint32_t as_at = lds0 + G::S0 + (wm * RT / 4) * 512 + ((m0 / 32 + wm * RT) & 3) * 2;
+    const uint32_t bs_at = lds0 + G::S0 + (G::GA + wn * CT / 4) * 512 + ((n0 / 32 + wn * CT) & 3) * 2;
+    // Activations' fragments in two sets, the weight's too where there are few products; else each is read anew behind its last product, RT (CT - 1) of them before
+    // it is needed.
+    constexpr bool ONE = X >= 16;
+    v4u fa[2][RT][A8 ? 2 : 1], fb[ONE ? 1 : 2][CT];
+    uint32_t sa[2][(RT + 1) / 2], sb[2][(CT + 1) / 2];  // of the stage in use and the next, two tiles a dword
+    auto read_scales = [&](int slot, auto buf) {
         constexpr int B = decltype(buf)::value;
-        const int64_t at = (int64_t)min(unit, p.pack_units - 1 - u0) * 64;
-#pragma unroll
-        for (int t = 0; t < GA; ++t) sa[B][t] = as[(int64_t)t * p.pack_units * 64 + at];
-#pragma unroll
-        for (int t = 0; t < GB; ++t) sb[B][t] = bs[(int64_t)t * p.pack_units * 64 + at];
+        auto some = [&](uint32_t at, auto& x, auto tiles) {
+            constexpr int n = decltype(tiles)::value;
+            if constexpr (n == 4) { const v2u v = *(lds_read8)(uintptr_t)at; x[0] = v[0]; x[1] = v[1]; }
+            else if constexpr (n == 2) x[0] = *(lds_u32)(uintptr_t)at;
+            else x[0] = *(const __attribute__((address_space(3))) uint16_t*)(uintptr_t)at;
+        };
+        some(lane * 8 + (as_at + slot * G::SS), sa[B], std::integral_constant<int, RT>());
+        some(lane * 8 + (bs_at + slot * G::SS), sb[B], std::integral_constant<int, CT>());
     };
-    auto scales_there = [&](auto buf) {
-        constexpr int B = decltype(buf)::value;
-#pragma unroll
-        for (int t = 0; t < GA; ++t) there(sa[B][t]);
-#pragma unroll
-        for (int t = 0; t < GB; ++t) there(sb[B][t]);
+    constexpr int NRA = (A8 ? 2 : 1) * RT, NR = NRA + CT;               // reads of a product's fragments
+    auto read = [&](int slot, auto prod, auto buf, auto which) {
+        constexpr int u = decltype(prod)::value, B = decltype(buf)::value, n = decltype(which)::value;
+        if constexpr (n >= NRA) fb[ONE ? 0 : B][n - NRA] = read16(b_ch[u] + (b_rd + slot * G::SB) + (n - NRA) * 32 * G::WB);
+        else if constexpr (A8) fa[B][n / 2][n % 2] = read16(a_ch[u + 2 * (n % 2)] + (a_rd + slot * G::SA) + n / 2 * 32 * G::AB);
+        else fa[B][n][0] = read16(a_ch[u] + (a_rd + slot * G::SA) + n * 32 * G::AB);
     };
+    // behind which product it is read
+    auto read_at = [](int n) constexpr { return ONE ? (n < NRA ? n * 8 / NRA : (n - NRA) * RT + RT - 1) : n * X / NR; };
 
     v16f acc[CT][RT] = {};
     typedef std::integral_constant<int, 0> I0;
     typedef std::integral_constant<int, 1> I1;
-    unrolled<NC>([&](auto n) { copy(0, I0(), n); });
-    load_scales(0, I0());
-    if constexpr (A8) load_scales(1, I1());
-    __builtin_amdgcn_s_waitcnt(0x0f70);                 // vmcnt(0)
-    scales_there(I0());
-    scales_there(I1());
-    unrolled<NC>([&](auto n) { copy(1, I1(), n); });
-    if constexpr (!A8) load_scales(1, I1());
+    unrolled<D>([&](auto d) {
+        constexpr int i = decltype(d)::value;
+        unrolled<NQ>([&](auto n) {
+            if constexpr (i < D - 1 || early(decltype(n)::value)) copy(i, i, n);
+        });
+    });
+    wait_copies<(D - 2) * NC>();                        // (and of the last stage's those that are on their way)
     barrier_no_fence();
-    unrolled<NR>([&](auto n) { read(I0(), I0(), I0(), n); });
+    read_scales(0, I0());
+    unrolled<NR>([&](auto n) { read(0, I0(), I0(), n); });
 
     // One stage.  Its last product's fragments are read during the one before; behind the barrier in front of that product the stage is free and the next
     // one is there.
-    auto stage = [&](int s, auto slot, auto unit_buf) {
-        constexpr int S = decltype(slot)::value, UB = decltype(unit_buf)::value;
-        unrolled<SUB>([&](auto prod) {
+    int slot = 0, before = D - 1;                       // the stage's place and that of the one in front of it
+    auto stage = [&](int s, auto parity) {
+        constexpr int P = decltype(parity)::value;
+        const int next = slot + 1 == D ? 0 : slot + 1;
+        unrolled<2>([&](auto prod) {
             constexpr int u = decltype(prod)::value, B = u & 1;
-            constexpr bool last = u == SUB - 1;
+            constexpr bool last = u == 1;
             if constexpr (last) {
-                __builtin_amdgcn_s_waitcnt(0x0070);     // everything that was read and copied is there
-                asm volatile("s_barrier" ::: "memory");
-                if constexpr (!A8 || S == 0) scales_there(std::integral_constant<int, UB ^ 1>());
+                wait_copies<(D - 2) * NC>();            // the next stage's, of this wavefront
+                barrier_no_fence();                     // and of all; what was read is there
             }
             __builtin_amdgcn_sched_barrier(0);
             unrolled<X>([&](auto step) {
                 constexpr int x = decltype(step)::value, ct = x / RT, rt = (ct & 1) ? RT - 1 - x % RT : x % RT;
-                constexpr int sel = A8 ? 2 * S + u : u;
-                const uint32_t ws = sb[UB][ct / 2][ct % 2], xs = sa[UB][rt / 2][rt % 2];
-                if constexpr (A8) mfma_codes<sel>(acc[ct][rt], fb[B][ct], __builtin_bit_cast(v8i, __builtin_shufflevector(fa[B][rt][0], fa[B][rt][1], 0, 1, 2, 3, 4, 5, 6, 7)), ws, xs);
-                else mfma_codes<sel>(acc[ct][rt], fb[B][ct], fa[B][rt][0], ws, xs);
-                // beside it: the next product's fragments, the copies of the stage after the next
+                const uint32_t ws = sb[P][ct / 2], xs = sa[P][rt / 2];
+                constexpr int ws_at = 2 * (ct & 1) + u, xs_at = 2 * (rt & 1) + u;
+                if constexpr (A8) mfma_codes<ws_at, xs_at>(acc[ct][rt], fb[ONE ? 0 : B][ct], __builtin_bit_cast(v8i, __builtin_shufflevector(fa[B][rt][0], fa[B][rt][1], 0, 1, 2, 3, 4, 5, 6, 7)), ws, xs);
+                else mfma_codes<ws_at, xs_at>(acc[ct][rt], fb[ONE ? 0 : B][ct], fa[B][rt][0], ws, xs);
+                // beside it: the next product's fragments, the copies of the stage that takes this one's place
+                if constexpr (last && x == 0) read_scales(next, std::integral_constant<int, P ^ 1>());
                 unrolled<NR>([&](auto n) {
-                    if constexpr (decltype(n)::value * X / NR == x) {
-                        if constexpr (last) read(std::integral_constant<int, S ^ 1>(), I0(), std::integral_constant<int, B ^ 1>(), n);
+                    if constexpr (read_at(decltype(n)::value) == x) {
+                        if constexpr (last) read(next, I0(), std::integral_constant<int, B ^ 1>(), n);
                         else read(slot, std::integral_constant<int, u + 1>(), std::integral_constant<int, B ^ 1>(), n);
                     }
                 });
-                if constexpr (last) {
-                    unrolled<NC>([&](auto n) {
-                        if constexpr (decltype(n)::value * X / NC == x) copy(s + 2, slot, n);
-                    });
-                    if constexpr (!A8 && x == X - 1) load_scales(s + 2, unit_buf);
-                }
+                unrolled<NQ>([&](auto n) {
+                    constexpr int y = decltype(n)::value * 2 * X / NQ;
+                    if constexpr (last && y == x) copy(s + D, slot, n);
+                    if constexpr (!last && y == X + x) copy(s - 1 + D, before, n);
+                });
                 __builtin_amdgcn_sched_barrier(0);
             });
         });
+        before = slot;
+        slot = next;
     };
     // (one way out, at the end: otherwise the compiler moves the sums)
     int s = 0;
     do {
-        stage(s, I0(), I0());
-        stage(s + 1, I1(), std::integral_constant<int, A8 ? 0 : 1>());
+        stage(s, I0());
+        stage(s + 1, I1());
         s += 2;
-        if constexpr (A8) {
-#pragma unroll
-            for (int t = 0; t < GA; ++t) sa[0][t] = sa[1][t];
-#pragma unroll
-            for (int t = 0; t < GB; ++t) sb[0][t] = sb[1][t];
-            load_scales(s / 2 + 1, I1());
-        }
     } while (s < stages);
     __builtin_amdgcn_s_waitcnt(0x0070);                 // (copies past the end are still on their way into LDS)
     barrier_no_fence();
@@ -298,94 +331,105 @@ __global__ __launch_bounds__(256, RT * CT >= 16 ? 1 : 2) void mx4_tile_kernel(Ti
 // Slices' sums, added in their order: a thread has the four results of a lane's 16 bytes.
 template <int RT, int CT, int CD>
 __global__ __launch_bounds__(256) void mx4_join_kernel(const v4f* part, void* out, int m, int n, int tiles_m, int tiles_n, int slices) {
-    constexpr int X = RT * CT;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tile = blockIdx.x, x = blockIdx.y;      // x: (ct, rt)
+    constexpr int X = RT * CT, MOST = 8;                // loads at once
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tile = blockIdx.x, x = blockIdx.y >> 2, e = blockIdx.y & 3;    // x: (ct, rt)
     const int band = tile / (4 * tiles_n), rows = min(4, tiles_m - 4 * band), in = tile - band * 4 * tiles_n;
     const int m0 = (4 * band + in % rows) * (64 * RT), n0 = in / rows * (64 * CT);
     const int ct = x / RT, rt = x % RT, wm = wave & 1, wn = wave >> 1;
-    const int row = m0 + (wm * RT + rt) * 32 + (lane & 31), col0 = n0 + (wn * CT + ct) * 32 + 4 * (lane >> 5);
-    if (row >= m) return;
+    const int row = m0 + (wm * RT + rt) * 32 + (lane & 31), col = n0 + (wn * CT + ct) * 32 + 8 * e + 4 * (lane >> 5);
+    if (row >= m || col >= n) return;
     const int64_t step = (int64_t)tiles_m * tiles_n * 4 * (X * 4 * 64);
-    const v4f* src = part + ((int64_t)tile * 4 + wave) * (X * 4 * 64) + x * 256 + lane;
-    auto* c = (typename OutT<CD>::type*)out + (int64_t)row * n;
+    const v4f* src = part + ((int64_t)tile * 4 + wave) * (X * 4 * 64) + x * 256 + e * 64 + lane;
+    v4f s = {};
+    for (int k = 0; k < slices; k += MOST) {
+        v4f v[MOST];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const int col = col0 + 8 * e;
-        if (col >= n) break;
-        v4f s = src[e * 64];
-        for (int k = 1; k < slices; ++k) s += src[k * step + e * 64];
+        for (int j = 0; j < MOST; ++j) v[j] = src[min(k + j, slices - 1) * step];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (col + j < n) c[col + j] = cvt_out<CD>(s[j]);
+        for (int j = 0; j < MOST; ++j)
+            if (k + j < slices) s = k + j ? s + v[j] : v[j];
     }
+    auto* c = (typename OutT<CD>::type*)out + (int64_t)row * n + col;
+    if (CD != DSV3_F32 && n % 4 == 0) {
+        *(v2u*)c = CD == DSV3_BF16 ? v2u{ pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3]) } : v2u{ pack_f16(s[0], s[1]), pack_f16(s[2], s[3]) };
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (col + j < n) c[j] = cvt_out<CD>(s[j]);
 }
 
-struct Plan { int rt, ct, tiles_m, tiles_n, slices, per_slice, units, pack_units; };
+struct Plan { int rt, ct, tiles_m, tiles_n, slices, per_slice, steps, pack_cols; };
 Plan plan_of(int64_t m, int64_t n, int64_t k, bool a8) {
     Plan p;
-    p.units = (int)((k + 255) / 256);
-    p.pack_units = p.units + 1 & ~1;
-    const int64_t big = ((m + 255) / 256) * ((n + 255) / 256);
-    p.rt = p.ct = big >= 192 ? 4 : 2;
+    p.steps = (int)(k / 128);
+    p.pack_cols = p.steps + 1 & ~1;
+    // Tiles of 256 where their rounds take less time: a round of one each takes 1.03 us a step (e4m3 1.40), one of two small ones 0.78 (1.0), and where there
+    // are no whole rounds of those the next ones fill them.  2000 x 7168 -> 7168: 61 us with 224 tiles of 256 and 82 with 896 small ones; 1024 x 7168 -> 18432
+    // 113 with 288 and 110 (e4m3: 145 and 128).
+    const int64_t large = ((m + 255) / 256) * ((n + 255) / 256), small = ((m + 127) / 128) * ((n + 127) / 128);
+    const double rounds = (double)((large + 255) / 256), half = small > 512 ? small / 512.0 : 1.0;
+    p.rt = p.ct = rounds * (a8 ? 1.40 : 1.03) < half * (a8 ? 1.0 : 0.78) ? 4 : 2;
+    if (m <= 64) p.rt = 1;
     p.tiles_m = (int)((m + 64 * p.rt - 1) / (64 * p.rt));
     p.tiles_n = (int)((n + 64 * p.ct - 1) / (64 * p.ct));
+    // Slices of k where compute units would have no tile; with more, their sums cost more than two tiles a unit save (128 x 7168 -> 18432 without slices 32.5 us,
+    // with three 39; 500 x 7168 -> 4096 with two 24, with four 28).
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-    int64_t slices = tiles >= 192 ? 1 : 256 / tiles;
-    slices = slices > p.units / 4 ? p.units / 4 : slices;
+    int64_t slices = p.rt == 4 || tiles >= 192 ? 1 : 256 / tiles;
+    slices = slices > p.steps / 8 ? p.steps / 8 : slices;
     if (slices < 1) slices = 1;
-    p.per_slice = (int)((p.units + slices - 1) / slices) + 1 & ~1;
-    p.slices = (p.units + p.per_slice - 1) / p.per_slice;
+    p.per_slice = (int)((p.steps + slices - 1) / slices) + 1 & ~1;
+    p.slices = (p.steps + p.per_slice - 1) / p.per_slice;
     return p;
 }
 struct Space { size_t bs, part, bytes; int64_t a_groups, b_groups; };
 Space space_of(const Plan& p) {
     Space s;
-    s.a_groups = (int64_t)p.tiles_m * p.rt; s.b_groups = (int64_t)p.tiles_n * p.ct;
-    s.bs = (size_t)s.a_groups * p.pack_units * 512;
-    s.part = s.bs + (size_t)s.b_groups * p.pack_units * 512;
+    s.a_groups = ((int64_t)p.tiles_m * p.rt + 1) / 2; s.b_groups = ((int64_t)p.tiles_n * p.ct + 1) / 2;
+    s.bs = (size_t)s.a_groups * p.pack_cols * 512;
+    s.part = s.bs + (size_t)s.b_groups * p.pack_cols * 512;
     s.bytes = s.part + (p.slices > 1 ? (size_t)p.slices * p.tiles_m * p.tiles_n * p.rt * p.ct * 4096 * 4 : 0);
     return s;
 }
 
-template <bool A8, int RT, int CT, int CD> int launch_tiles(const TileArgs& a, const Plan& plan, hipStream_t st) {
-    using G = Geo<A8, RT, CT>;
+template <bool A8, int RT, int CT, int D, int CD> int launch_tiles(const TileArgs& a, const Plan& plan, hipStream_t st) {
+    using G = Geo<A8, RT, CT, D>;
     static_assert(G::LDS <= 160 * 1024 && 4 * 32 * CT * 64 * (RT > 1 ? 2 : 1) <= G::LDS, "the results leave through the stages");
     const unsigned tiles = (unsigned)plan.tiles_m * plan.tiles_n;
     if (plan.slices == 1) {
         static LdsGrant grant;
-        if (!grant.ensure((const void*)mx4_tile_kernel<A8, RT, CT, CD, false>, G::LDS)) return DSV3_ERR_LAUNCH;
-        hipLaunchKernelGGL((mx4_tile_kernel<A8, RT, CT, CD, false>), dim3(tiles), dim3(256), G::LDS, st, a);
+        if (!grant.ensure((const void*)mx4_tile_kernel<A8, RT, CT, D, CD, false>, G::LDS)) return DSV3_ERR_LAUNCH;
+        hipLaunchKernelGGL((mx4_tile_kernel<A8, RT, CT, D, CD, false>), dim3(tiles), dim3(256), G::LDS, st, a);
         return launch_status();
     }
     static LdsGrant grant;
-    if (!grant.ensure((const void*)mx4_tile_kernel<A8, RT, CT, DSV3_F32, true>, G::LDS)) return DSV3_ERR_LAUNCH;
-    hipLaunchKernelGGL((mx4_tile_kernel<A8, RT, CT, DSV3_F32, true>), dim3(tiles, plan.slices), dim3(256), G::LDS, st, a);
-    hipLaunchKernelGGL((mx4_join_kernel<RT, CT, CD>), dim3(tiles, RT * CT), dim3(256), 0, st, (const v4f*)a.part, a.c, a.m, a.n, plan.tiles_m, plan.tiles_n, plan.slices);
+    if (!grant.ensure((const void*)mx4_tile_kernel<A8, RT, CT, D, DSV3_F32, true>, G::LDS)) return DSV3_ERR_LAUNCH;
+    hipLaunchKernelGGL((mx4_tile_kernel<A8, RT, CT, D, DSV3_F32, true>), dim3(tiles, plan.slices), dim3(256), G::LDS, st, a);
+    hipLaunchKernelGGL((mx4_join_kernel<RT, CT, CD>), dim3(tiles, RT * CT * 4), dim3(256), 0, st, (const v4f*)a.part, a.c, a.m, a.n, plan.tiles_m, plan.tiles_n, plan.slices);
     return launch_status();
 }
 template <bool A8, int CD> int launch_cd(const TileArgs& a, const Plan& plan, hipStream_t st) {
-    if (plan.rt == 4) return launch_tiles<A8, 4, 4, CD>(a, plan, st);
-    return launch_tiles<A8, 2, 2, CD>(a, plan, st);
+    if (plan.rt == 4) return launch_tiles<A8, 4, 4, A8 ? 3 : 4, CD>(a, plan, st);
+    if (plan.rt == 1) return launch_tiles<A8, 1, 2, A8 ? 4 : 6, CD>(a, plan, st);
+    return launch_tiles<A8, 2, 2, A8 ? 3 : 4, CD>(a, plan, st);
 }
 
 }  // namespace
-
-bool mx4_tile_takes(int64_t m, int64_t n, int64_t k) {
-    // (offsets in a tile are 32 bits, launches and tiles are counted in 31)
-    return k > 0 && k <= 1 << 22 && ((m + 127) / 128) * ((n + 127) / 128) <= 1 << 22 && (m + n) / 64 + 8 <= 1 << 24;
-}
 
 size_t mx4_tile_workspace_bytes(int64_t m, int64_t n, int64_t k, bool a8) { return space_of(plan_of(m, n, k, a8)).bytes; }
 
 int launch_mx4_tile(const Mx4Args& q, bool a8, int c_dtype, void* workspace, hipStream_t st) {
     const Plan plan = plan_of(q.m, q.n, q.k, a8);
     const Space space = space_of(plan);
+    // (what launches hold)
+    if ((int64_t)plan.tiles_m * plan.tiles_n > 0xffffff || space.a_groups + space.b_groups > 0xffffff) return DSV3_ERR_BAD_SHAPE;
     uint8_t* ws = (uint8_t*)workspace;
-    PackArgs pk = { (const uint32_t*)q.a_s, (const uint32_t*)q.b_s, (v2u*)ws, (v2u*)(ws + space.bs), space.a_groups, space.b_groups, (int)q.m, (int)q.n, (int)(q.k / 128), plan.pack_units };
-    const dim3 grid((unsigned)(space.a_groups + space.b_groups), (unsigned)((plan.pack_units + 15) / 16));
+    PackArgs pk = { (const uint32_t*)q.a_s, (const uint32_t*)q.b_s, (v2u*)ws, (v2u*)(ws + space.bs), space.a_groups, space.b_groups, (int)q.m, (int)q.n, (int)(q.k / 128), plan.pack_cols };
+    const dim3 grid((unsigned)(space.a_groups + space.b_groups), (unsigned)((plan.pack_cols + 15) / 16));
     if (a8) hipLaunchKernelGGL(mx4_pack_kernel<true>, grid, dim3(256), 0, st, pk);
     else hipLaunchKernelGGL(mx4_pack_kernel<false>, grid, dim3(256), 0, st, pk);
-    const TileArgs a = { q.a, q.b, pk.as, pk.bs, q.c, (v4f*)(ws + space.part), (int)q.m, (int)q.n, (int)q.k, plan.units, plan.pack_units, plan.tiles_m, plan.tiles_n, plan.per_slice };
+    const TileArgs a = { q.a, q.b, ws, ws + space.bs, q.c, (v4f*)(ws + space.part), (int)q.m, (int)q.n, (int)q.k, plan.steps, plan.pack_cols, plan.tiles_m, plan.tiles_n, plan.per_slice };
     if (c_dtype == DSV3_BF16) return a8 ? launch_cd<true, DSV3_BF16>(a, plan, st) : launch_cd<false, DSV3_BF16>(a, plan, st);
     if (c_dtype == DSV3_F16) return a8 ? launch_cd<true, DSV3_F16>(a, plan, st) : launch_cd<false, DSV3_F16>(a, plan, st);
     return a8 ? launch_cd<true, DSV3_F32>(a, plan, st) : launch_cd<false, DSV3_F32>(a, plan, st);
@@ -393,7 +437,15 @@ int launch_mx4_tile(const Mx4Args& q, bool a8, int c_dtype, void* workspace, hip
 
 // ---- which kernel takes which sizes
 
-static bool tiles(int64_t m, int64_t n, int64_t k) { return m > 64 && mx4_tile_takes(m, n, k); }
+// Up to 32 rows the weight is streamed, and beyond where that moves little: every workgroup of mx4_stream_kernel reads its weight rows and 32 activation rows (at
+// some 10 TB/s, in 3 us at least), while tiles take a launch for the scales in front and often one for the slices behind, 9 us at least.  64 x 7168 -> 2112:
+// 8.5 us streamed and 13.1 in tiles; 100 x 7168 -> 2112 10 and 14.4; 128 x 7168 -> 576 5.3 and 11.4; 300 x 2048 -> 7168 17.2 and 11.7; 64 x 512 -> 32768, many
+// workgroups, 9.6 and 8.4.
+static bool tiles(int64_t m, int64_t n, int64_t k) {
+    if (m <= 32 || k == 0) return false;
+    const int64_t strip = n >= 6144 ? 32 : 16, groups = (n + strip - 1) / strip * ((m + 31) / 32);
+    return groups > 1024 || groups * (strip + 32) * (k / 2) > 100000000;
+}
 
 size_t mx4_gemm_workspace_bytes(bool a8, int64_t m, int64_t n, int64_t k) { return tiles(m, n, k) ? mx4_tile_workspace_bytes(m, n, k, a8) : 0; }
 

@@ -139,10 +139,12 @@ def operands(g, m, n, k, a8, spread=6):
     return a, a_s, b, b_s, held(a, a_s), held(b, b_s)
 
 
-# rows up to and beyond every kernel's tiles, ragged columns, one to many K blocks, odd numbers of them
-PRODUCTS = [(1, 1, 128), (1, 576, 7168), (2, 17, 256), (16, 100, 384), (17, 48, 2048), (33, 33, 640), (64, 512, 1152), (65, 130, 128), (65, 64, 1024),
-            (100, 257, 896), (128, 128, 512), (129, 300, 2176), (200, 1000, 512), (257, 513, 256), (256, 256, 4096), (300, 2304, 1536), (520, 520, 384), (1030, 1800, 640), (1500, 8200, 640),
-            (1537, 8193, 1152), (3000, 4352, 512), (1600, 8448, 128)]
+# streamed: every count of rows that is copied, narrow and wide weights, one to many chunks of 512, shorter last ones, wavefronts with none and with several
+PRODUCTS = [(1, 1, 128), (1, 576, 7168), (2, 17, 256), (4, 100, 384), (3, 6200, 512), (5, 40, 640), (16, 100, 384), (16, 6145, 1152), (9, 7168, 4096), (17, 48, 2048),
+            (32, 6160, 640), (31, 500, 16384), (33, 33, 640), (64, 512, 1152), (65, 130, 128), (65, 64, 1024), (100, 257, 896), (128, 128, 512), (200, 1000, 512)]
+# tiles of 64, 128 and 256 rows, with and without slices of k, odd numbers of steps, ragged rows and columns, columns that are no whole eights
+PRODUCTS += [(40, 8200, 8192), (64, 8203, 8320), (33, 20000, 1152), (64, 33000, 128), (300, 2304, 7168), (129, 9000, 2176), (257, 3001, 2304), (300, 7300, 384), (520, 6200, 384),
+             (1030, 5000, 640), (1500, 8200, 640), (1537, 8193, 1152), (3000, 4352, 512), (1600, 8448, 128), (513, 2050, 1408)]
 
 
 @pytest.mark.parametrize("a8", [False, True], ids=["mx4", "e4m3"])
@@ -168,7 +170,7 @@ def test_product(K, m, n, k, a8):
 
 
 @pytest.mark.parametrize("a8", [False, True], ids=["mx4", "e4m3"])
-@pytest.mark.parametrize("m,n,k", [(1, 40, 256), (20, 100, 1024), (90, 140, 384), (300, 600, 512)])
+@pytest.mark.parametrize("m,n,k", [(1, 40, 256), (20, 100, 1024), (90, 140, 384), (300, 600, 512), (60, 9000, 7168), (260, 3000, 2560), (1300, 9000, 640)])
 def test_products_of_whole_numbers(K, m, n, k, a8):
     """Whole numbers whose sums binary32 holds come out exactly, whatever the order: codes of 0, 1, 2, 3, 4 and 6, scales of 1, 2 and 4."""
     g = torch.Generator().manual_seed(m + n)
@@ -186,7 +188,7 @@ def test_products_of_whole_numbers(K, m, n, k, a8):
 
 
 @pytest.mark.parametrize("a8", [False, True], ids=["mx4", "e4m3"])
-@pytest.mark.parametrize("m,n", [(3, 50), (80, 300), (300, 700)])
+@pytest.mark.parametrize("m,n", [(3, 50), (80, 300), (300, 7000), (50, 20000), (1500, 9000)])
 def test_a_scale_of_nan_reaches_its_row(K, m, n, a8):
     g = torch.Generator().manual_seed(m)
     k = 640
@@ -219,18 +221,18 @@ def test_shapes(K, m, n, k, lead):
 def test_the_same_sums_in_every_call(K):
     for m in (1, 40, 100, 600):
         g = torch.Generator().manual_seed(m)
-        a, a_s, b, b_s, _, _ = operands(g, m, 700, 4096, m % 3 == 0)
+        a, a_s, b, b_s, _, _ = operands(g, m, 7000, 4096, m % 3 == 0)
         first = K.mx4_gemm(a, a_s, b, b_s)
         for _ in range(3):
             assert torch.equal(K.mx4_gemm(a, a_s, b, b_s), first)
 
 
 @pytest.mark.parametrize("a8", [False, True], ids=["mx4", "e4m3"])
-@pytest.mark.parametrize("m", [1, 50, 200])
+@pytest.mark.parametrize("m", [1, 50, 300])
 def test_captured_and_replayed(K, m, a8):
     """Quantise and multiply in a graph, replayed on new contents between eager calls."""
     g = torch.Generator().manual_seed(m)
-    n, k = 300, 1024
+    n, k = 9000, 4096
     _, _, b, b_s, _, _ = operands(g, m, n, k, a8)
     x = torch.randn(m, k, generator=g, dtype=torch.float32).bfloat16().cuda()
 
@@ -257,7 +259,7 @@ def test_two_streams_at_once(K):
     sets = []
     for seed, m in ((1, 200), (2, 300)):
         g = torch.Generator().manual_seed(seed)
-        a, a_s, b, b_s, _, _ = operands(g, m, 900, 2048, seed == 1)
+        a, a_s, b, b_s, _, _ = operands(g, m, 3000, 4096, seed == 1)
         sets.append((a, a_s, b, b_s))
     want = [K.mx4_gemm(*s) for s in sets]
     torch.cuda.synchronize()
