@@ -24,13 +24,17 @@ from torch import nn
 from torch.nn.modules import module as _modules
 
 from . import ops
-from .kernel import act_quant, fp8_gemm, fp8_gemm_pow2, weight_dequant
+from .kernel import act_quant, fp8_gemm, fp8_gemm_pow2, mx4_dequant, mx4_gemm, mx4_quant, weight_dequant
 
 world_size = 1
 rank = 0
 block_size = 128
 gemm_impl: Literal["bf16", "fp8"] = "bf16"     # the reference's default (model.py:16); set to "fp8" for the FP8 GEMM path
 attn_impl: Literal["naive", "absorb"] = "absorb"   # model.py:17
+# what a linear layer's input becomes in front of a weight of microscaled 4-bit numbers (not in the reference; ``linear``): e4m3 with a power of two per
+# 128, or such numbers too
+mx4_activations: Literal["e4m3", "mx4"] = "e4m3"
+FP4 = ops.FP4
 
 
 @dataclass
@@ -64,6 +68,11 @@ class ModelArgs:
     mscale: float = 1.
 
 
+def _eight_bits(weight: torch.Tensor) -> bool:
+    """Whether a weight is one of e4m3 codes with block scales (one of 4-bit numbers has two elements a byte, and layers of its own)."""
+    return weight.element_size() == 1 and weight.dtype != FP4
+
+
 def _scales_are_powers_of_two(weight: torch.Tensor, scale: Optional[torch.Tensor] = None) -> bool:
     """Whether every block scale of an fp8 weight is a power of two (checkpoints made for ``scale_fmt = "ue8m0"``,
     inference/configs/config_v3.1.json:22, store them that way).  Looked at once per version of the scale tensor
@@ -92,9 +101,23 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
            scale_fmt: Optional[str] = None) -> torch.Tensor:
     """y = x @ weight.T + bias with the reference's three-way dispatch (model.py:153-163): wide weights go to
     ``F.linear``; 1-byte weights are dequantised first when ``gemm_impl == "bf16"``, otherwise the activation
-    is quantised per 1x128 block and multiplied with ``fp8_gemm``.  ``weight.scale`` carries the block scales."""
+    is quantised per 1x128 block and multiplied with ``fp8_gemm``.  ``weight.scale`` carries the block scales.
+
+    A weight of microscaled 4-bit numbers (``mx4_quant``: ``torch.float4_e2m1fn_x2`` ``[out, in / 2]``, ``weight.scale`` e8m0 ``[out, in / 32]``) goes the
+    same ways: dequantised for ``F.linear``, or multiplied with ``mx4_gemm``, the activation quantised as ``mx4_activations`` says (``scale_fmt`` has no say:
+    its scales are powers of two either way)."""
     if weight.element_size() > 1:
         return F.linear(x, weight, bias)
+    if weight.dtype == FP4:
+        if gemm_impl == "bf16":
+            return F.linear(x, mx4_dequant(weight, weight.scale), bias)
+        if mx4_activations not in ("e4m3", "mx4"):
+            raise ValueError(f"mx4_activations must be 'e4m3' or 'mx4', not {mx4_activations!r}")
+        xq, xs = act_quant(x, 128, "ue8m0") if mx4_activations == "e4m3" else mx4_quant(x)
+        y = mx4_gemm(xq, xs, weight, weight.scale)
+        if bias is not None:
+            y += bias
+        return y
     if gemm_impl == "bf16":
         return F.linear(x, weight_dequant(weight, weight.scale), bias)
     if (scale_fmt == "ue8m0" and x.is_cuda and block_size == 128 and x.numel() > 64 * x.size(-1)
@@ -117,7 +140,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
 
 class Linear(nn.Module):
     """Linear layer whose weight may be fp8 with a block-scale tensor attached as ``weight.scale``
-    (shape ``[ceil(out/128), ceil(in/128)]``, fp32), as in model.py:166-205."""
+    (shape ``[ceil(out/128), ceil(in/128)]``, fp32), as in model.py:166-205.  With ``dtype`` ``torch.float4_e2m1fn_x2`` the weight is of microscaled
+    4-bit numbers, ``[out, in / 2]`` with ``scale`` e8m0 ``[out, in / 32]``; ``in`` is a multiple of 128 then."""
     dtype = torch.bfloat16
     scale_fmt: Optional[str] = None
 
@@ -125,8 +149,13 @@ class Linear(nn.Module):
         super().__init__()
         self.in_features = in_features
         self.out_features = out_features
-        self.weight = nn.Parameter(torch.empty(out_features, in_features, dtype=dtype or Linear.dtype))
-        if self.weight.element_size() == 1:
+        dtype = dtype or Linear.dtype
+        if dtype == FP4 and in_features % 128:
+            raise ValueError(f"Linear: weights of 4 bits need a multiple of 128 input features, got {in_features}")
+        self.weight = nn.Parameter(torch.empty(out_features, in_features // 2 if dtype == FP4 else in_features, dtype=dtype))
+        if dtype == FP4:
+            self.weight.scale = self.scale = nn.Parameter(torch.empty(out_features, in_features // 32, dtype=ops.E8M0))
+        elif self.weight.element_size() == 1:
             rows = -(-out_features // block_size)
             cols = -(-in_features // block_size)
             self.weight.scale = self.scale = nn.Parameter(torch.empty(rows, cols, dtype=torch.float32))
@@ -343,7 +372,7 @@ class MLA(nn.Module):
         # microsecond, and a decode step is bound by the host
         qp, kp = qa._parameters, ka._parameters
         qw, kw, qs, ks = qp.get("weight"), kp.get("weight"), qp.get("scale"), kp.get("scale")
-        if qw is None or kw is None or qs is None or ks is None or qw.element_size() != 1 or kw.element_size() != 1 \
+        if qw is None or kw is None or qs is None or ks is None or not _eight_bits(qw) or not _eight_bits(kw) \
                 or qp.get("bias") is not None or kp.get("bias") is not None:
             return False
         wa = self.__dict__.get("_wa")
@@ -385,7 +414,9 @@ class MLA(nn.Module):
     def _dequantised_wkv_b(self, x: torch.Tensor) -> Optional[torch.Tensor]:
         """[h, nope+v, c] weight for the einsum path, or None when the products read the FP8 weight in place."""
         w = self.wkv_b.weight
-        if w.element_size() == 1:
+        if w.dtype == FP4:
+            w = mx4_dequant(w, self.wkv_b.scale)
+        elif w.element_size() == 1:
             if self.fused and x.is_cuda and x.dtype == torch.bfloat16:
                 return None
             w = weight_dequant(w, self.wkv_b.scale, block_size)
@@ -405,7 +436,7 @@ class MLA(nn.Module):
         fits = ((self.qk_nope_head_dim, self.qk_rope_head_dim, self.v_head_dim, self.kv_lora_rank) == (128, 64, 128, 512)
                 and kv.dtype == torch.bfloat16 and pe.dtype == torch.bfloat16 and kv.is_contiguous() and pe.is_contiguous()
                 and 1 <= b <= kv.size(0) and s >= 1 and start_pos >= 0 and start_pos + s <= kv.size(1)
-                and w.element_size() == 1 and _offset_aligned(kv) and _offset_aligned(pe) and _offset_aligned(w)
+                and _eight_bits(w) and _offset_aligned(kv) and _offset_aligned(pe) and _offset_aligned(w)
                 and kv.device == device and pe.device == device and w.device == device and freqs_cis.device == device
                 and freqs_cis.dtype == torch.complex64 and freqs_cis.is_contiguous() and not freqs_cis.is_conj()
                 and freqs_cis.shape == (s, self.qk_rope_head_dim // 2))
@@ -428,7 +459,7 @@ class MLA(nn.Module):
                 return None
             weights.append(w)
         w = wq._parameters.get("weight")
-        if w is None or w.element_size() != 1 or wq._parameters.get("bias") is not None or not self.stack_a():
+        if w is None or not _eight_bits(w) or wq._parameters.get("bias") is not None or not self.stack_a():
             return None
         return (*weights, qn.eps, kn.eps, w)
 
@@ -489,7 +520,7 @@ class MLA(nn.Module):
             explicit = self._explicit_pays(b, s, t)
             # the attention's last kernel quantises for wo, unless wo was exchanged, carries hooks or is no FP8 layer
             wo = self.wo
-            if _plain(wo, RowParallelLinear) and wo.weight.element_size() == 1 and wo.bias is None and wo.weight.is_contiguous():
+            if _plain(wo, RowParallelLinear) and _eight_bits(wo.weight) and wo.bias is None and wo.weight.is_contiguous():
                 return _mla_output(*args, explicit, wo.weight, wo.weight.scale)
             if not explicit:
                 return wo(torch.ops.dsv3fp8.mla_decode(*args))
@@ -514,7 +545,7 @@ class MLA(nn.Module):
         return (not torch.is_grad_enabled() and gemm_impl == "fp8" and block_size == 128 and world_size == 1 and x.is_cuda and x.dtype == torch.bfloat16
                 and x.dim() == 3 and x.numel() > 0 and torch.get_default_dtype() == torch.bfloat16
                 and (self.qk_nope_head_dim, self.qk_rope_head_dim, self.v_head_dim, self.kv_lora_rank) == (128, 64, 128, 512)
-                and 1e-30 < self.softmax_scale < 1e30 and w.element_size() == 1 and w.device == x.device and _plain(wo, RowParallelLinear) and wo.weight.element_size() == 1 and wo.bias is None
+                and 1e-30 < self.softmax_scale < 1e30 and _eight_bits(w) and w.device == x.device and _plain(wo, RowParallelLinear) and _eight_bits(wo.weight) and wo.bias is None
                 and freqs_cis.dtype == torch.complex64 and freqs_cis.shape == (x.size(0), x.size(1), self.qk_rope_head_dim // 2))
 
     def forward_paged(self, x: torch.Tensor, cache: LatentPages, page_table: torch.Tensor, starts: torch.Tensor, counts: torch.Tensor,
@@ -610,7 +641,7 @@ class MLP(nn.Module):
         that both projections of an input are one GEMM.  Returns whether the layers qualify; re-stacks if the
         layers' storage was moved since (MoE.stack_experts does that for its shared expert)."""
         w1, w3 = self.w1, self.w3
-        if w1.weight.element_size() != 1 or w3.weight.element_size() != 1 or w1.out_features % block_size \
+        if not _eight_bits(w1.weight) or not _eight_bits(w3.weight) or w1.out_features % block_size \
                 or w1.in_features % block_size or w1.out_features != w3.out_features:
             return False
         w13 = getattr(self, "_w13", None)
@@ -637,7 +668,7 @@ class MLP(nn.Module):
         stacked projection then starts from it instead of quantising ``x`` once more."""
         if (self.stacked and gemm_impl == "fp8" and world_size == 1 and x.is_cuda and x.dtype == torch.bfloat16
                 and x.is_contiguous() and torch.get_default_dtype() == torch.bfloat16 and block_size == 128
-                and self.w2.bias is None and self.w1.bias is None and self.w3.bias is None and self.stack_13()):
+                and self.w2.bias is None and self.w1.bias is None and self.w3.bias is None and self.w2.weight.dtype != FP4 and self.stack_13()):
             # one GEMM for both projections, SwiGLU fused with the re-quantisation of w2's input: the same
             # arithmetic and roundings as the three linears and two tensor ops below
             h = linear(x, self._w13) if quantised is None else fp8_gemm(quantised[0], quantised[1], self._w13, self._w13.scale)
@@ -717,7 +748,7 @@ class MoE(nn.Module):
     With FP8 experts and ``gemm_impl == "fp8"`` the token lists stay on the device: the routed experts run as
     two grouped GEMMs over expert-sorted rows (w1|w3 stacked, then w2) with SwiGLU and the re-quantisation fused
     between them, and one kernel adds the weighted outputs per token in the order the reference's loop does.
-    ``MoE.grouped = False`` selects the reference's expert-by-expert loop (same kernels, one expert at a time).
+    ``MoE.grouped = False`` selects the reference's expert-by-expert loop (same kernels, one expert at a time), which experts of 4-bit weights take too.
     """
 
     grouped: bool = True
@@ -756,7 +787,7 @@ class MoE(nn.Module):
         assert inter % block_size == 0 and dim % block_size == 0
         dev, fp8 = exs[0].w1.weight.device, exs[0].w1.weight.dtype
         sh = self.shared_experts
-        self._shared_stacked = (sh.w1.out_features == inter and sh.w1.weight.dtype == fp8
+        self._shared_stacked = (sh.w1.out_features == inter and sh.w1.weight.dtype == fp8 and sh.w2.weight.dtype != FP4
                                 and sh.w1.weight.device == dev)
         if self._shared_stacked:
             exs.append(sh)
@@ -784,7 +815,7 @@ class MoE(nn.Module):
         fits = (0 < x.size(0) and self.n_activated_experts <= 16 and pairs * max(inter, self.dim) < 2 ** 32
                 and x.size(0) * self.dim < 2 ** 32)
         return (self.grouped and fits and gemm_impl == "fp8" and world_size == 1 and x.is_cuda
-                and ex.w1.weight.element_size() == 1 and x.dtype == torch.bfloat16
+                and _eight_bits(ex.w1.weight) and ex.w2.weight.dtype != FP4 and x.dtype == torch.bfloat16
                 and torch.get_default_dtype() == torch.bfloat16
                 and ex.w1.out_features % block_size == 0 and self.dim % block_size == 0)
 
