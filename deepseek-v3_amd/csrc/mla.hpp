@@ -9,6 +9,7 @@ namespace {
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) void* lptr_t;
 typedef __attribute__((address_space(3))) v2i* lds_v2i;
+typedef __attribute__((address_space(3))) v2u* lds_v2u;
 typedef __attribute__((address_space(3))) v4u* lds_v4u;
 typedef __attribute__((address_space(3))) v4f* lds_v4f;
 typedef __attribute__((address_space(3))) float* lds_f32;

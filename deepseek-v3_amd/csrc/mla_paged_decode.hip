@@ -38,8 +38,10 @@ constexpr int kFewLds = 4 * kFewStage;
 // the stage.  By itself a wavefront has all 64 rows of its tile at the end of where their codes will stand (row r of them is read before anything is written
 // there: 16 (n + 1) rows of 544 bytes end in front of row 16 (n + 1) of those), and their scales behind the 64 of the rows.
 constexpr int kRaw = 16 * (kC / 2) + 16 * 16;
-constexpr int kLds4 = kLds + 4 * kRaw;
-constexpr int kFewRawOff = 4 * kRows16 - kTile * (kC / 2), kFewRawScaleOff = kFewScaleOff + 1024;
+constexpr int kWide = 15 * 8;                           // a wavefront's table of e4m3 codes (widen)
+constexpr int kLds4 = kLds + 4 * (kRaw + 128);
+constexpr int kFewRawOff = 4 * kRows16 - kTile * (kC / 2), kFewRawScaleOff = kFewScaleOff + 1024, kFewWideOff = kFewScaleOff + 512;
+static_assert(kTile * 4 <= 512 && kWide <= 512, "the scales of 64 rows, the table, the scales as they come");
 static_assert(kFewRawOff >= 288 * kTile, "rows of four bits are read before they are written over");
 
 struct PagedArgs {
@@ -180,6 +182,14 @@ __device__ __forceinline__ v8i join(v4u a, v4u b) {
 // sequences x 16 heads at up to 8192 positions (147 MB): 50 us, 2.9 TB/s; with one wavefront at work
 // and the others copying for it 61.  Blocks of 32 rows do not pay where there are more: 32 sequences x 128 heads at up to 4096 positions 57.4 us for the
 // whole call and 56.5 with blocks of 128, one sequence at 700 26.6 and 26.3.
+//
+// FOUR (rows of four bits): 272 B of codes and scales a position in place of 516, which become e4m3 codes of one scale a row in LDS, so that
+// the products are those above, bit for bit.  With wide blocks each wavefront widens 16 of the tile's 64 rows beside B's products: a lane four blocks of 32, six steps each, of
+// which the reads stand three steps in front of their use.  The products bound those calls, and the widening is 170 more instructions a tile and 70 KB more
+// through LDS beside its 300: one sequence of 61 tokens x 128 heads at 32768 positions 510 us (e4m3: 454), 8 x 25 x 128 at up to 2001 157 (138), 32 x 128 at
+// 4096 62 (59).  Codes through float conversions in place of the table 558, the barrier behind the rows' copies too 535, a block read one step in front 524.
+// Few rows are bound by the three waits before a range's first product and by the fold rather than by the bytes that four bits save: 64 sequences x 16
+// heads at 8192 68 us (65), one sequence at 700 30 (27).  What four bits give is the cache: 400 B a position, with its key, for 644.
 template <bool PACK, bool FEW, bool FOUR>
 __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
@@ -259,6 +269,13 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     // ... and as e4m3 codes of one scale a row.  Lane l has blocks 4 (l % 4) .. + 3 of row l / 4, the n-th in an order by the row with which few lanes meet in
     // one bank (none in these reads but two of the rows' four, two in each write).
     struct Widening { uint32_t bytes, codes, to; int turn; int top; };
+    // The e4m3 codes of the eight magnitudes times 2^6 .. 2^-8, exact all of them (2^-9 is e4m3's smallest number): a code is looked up by v_perm_b32, four at once.
+    const uint32_t table = lds0 + (FEW ? wave * kFewStage + kFewWideOff : kLds + wave * (kRaw + 128) + kRaw);
+    if constexpr (FOUR) {
+        const int lane = threadIdx.x & 63;
+        const float unit = u32_as_f32((uint32_t)(133 - lane) << 23);
+        if (lane < kWide / 8) *(lds_v2u)(uintptr_t)(table + lane * 8) = v2u{ pack_fp8x4(0.f, 0.5f * unit, unit, 1.5f * unit), pack_fp8x4(2.f * unit, 3.f * unit, 4.f * unit, 6.f * unit) };
+    }
     auto widen_scales = [&](uint32_t codes, uint32_t scales, uint32_t to, uint32_t to_scales) -> Widening {
         const int lane = lane_now(), row = lane >> 2, q = lane & 3;
         Widening w;
@@ -273,21 +290,22 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
         w.turn = 0x1c >> (2 * (row & 3)) & 3;
         w.codes = codes + row * (kC / 2) + q * 64;
         w.to = to + (row >> 1) * kPair + (row >> 2 & 1) * 16 + (row & 1) * kC;
-        w.top = (int)(row_top - 133u);
+        w.top = (int)row_top;
         return w;
     };
     // block n: the dwords of its codes, then eight of e4m3 codes
     auto widen_read = [&](const Widening& w, auto n) -> v4u {
         return *(lds_v4u)(uintptr_t)(w.codes + ((decltype(n)::value + w.turn & 3) << 4));
     };
-    auto widen_scale = [&](const Widening& w, auto n) -> float {        // 2^6 times the block's part of the row's largest scale
+    auto widen_codes = [&](const Widening& w, auto n) -> v2u {          // those of the block: its scale is so many powers below the row's largest
         const int byte = w.bytes >> (8 * (decltype(n)::value + w.turn & 3)) & 0xff;
-        return u32_as_f32((uint32_t)max(byte - (int)w.top, 119) << 23);
+        return *(lds_v2u)(uintptr_t)(table + min(w.top - byte, 14) * 8);
     };
-    auto widen_one = [&](uint32_t codes, float scale) -> v2u {
-        const v2f a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 1);
-        const v2f c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 3);
-        return v2u{ pack_fp8x4(a.x, a.y, b.x, b.y), pack_fp8x4(c.x, c.y, d.x, d.y) };
+    auto widen_one = [&](uint32_t x, v2u codes) -> v2u {
+        uint32_t even = __builtin_amdgcn_perm(codes[1], codes[0], x & 0x07070707u), odd = __builtin_amdgcn_perm(codes[1], codes[0], x >> 4 & 0x07070707u);
+        even |= x << 4 & 0x80808080u;
+        odd |= x & 0x80808080u;
+        return v2u{ __builtin_amdgcn_perm(odd, even, 0x05010400u), __builtin_amdgcn_perm(odd, even, 0x07030602u) };
     };
     auto widen_write = [&](const Widening& w, auto n, v4u lo, v4u hi) {
         const int lane = lane_now(), row = lane >> 2, q = lane & 3, c = 8 * q + 2 * (decltype(n)::value + w.turn & 3) ^ (row & 1) << 2;
@@ -300,12 +318,12 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
         unrolled<4>([&](auto n) { raw[decltype(n)::value] = widen_read(w, n); });
         unrolled<4>([&](auto n) {
             const v4u x = raw[decltype(n)::value];
-            const float scale = widen_scale(w, n);
-            const v2u a = widen_one(x[0], scale), b = widen_one(x[1], scale), c = widen_one(x[2], scale), d = widen_one(x[3], scale);
+            const v2u codes = widen_codes(w, n);
+            const v2u a = widen_one(x[0], codes), b = widen_one(x[1], codes), c = widen_one(x[2], codes), d = widen_one(x[3], codes);
             widen_write(w, n, v4u{ a[0], a[1], b[0], b[1] }, v4u{ c[0], c[1], d[0], d[1] });
         });
     };
-    const uint32_t raw0 = lds0 + kLds + wave * kRaw;    // (wavefronts that share a tile)
+    const uint32_t raw0 = lds0 + kLds + wave * (kRaw + 128);            // (wavefronts that share a tile)
     auto copy_raw = [&](int t, uint32_t at, int page) {
         const Source a = source(t, 0, page, 0), b = source(t, 1, page, 0);
         unrolled<5>([&](auto n) { issue_raw(a, b, at, at + 16 * (kC / 2), n); });
@@ -669,7 +687,12 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
             score(base, Second(), [&](auto step) {
                 soften(t, base, First(), step);
                 if constexpr (decltype(step)::value == 13) {
-                    arrived();
+                    if constexpr (FOUR) {               // vmcnt(5): all but the last five copies, of the wavefront's own rows, which B waits for
+                        __builtin_amdgcn_s_waitcnt(0x0f75);
+                        barrier_no_fence();
+                    } else {
+                        arrived();
+                    }
                     page = page_of(t + 3);              // (FOUR: its rows are copied in this turn's B, its keys in the next)
                     sc = scale_at(next, 0);
                 }
@@ -684,22 +707,31 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
             // those of the tile behind it
             Widening wide;
             v4u raw, out[2];
+            v2u codes;
             Source ahead2;
             weigh(t == t0, base, [&](auto step) {
                 constexpr int x = decltype(step)::value;
                 if constexpr (x == 29 || x == 31) ring[x >> 1 & 1] = key(keys_at(next), 1, (x >> 1) - 14);
                 if constexpr (FOUR) {
                     const uint32_t to = lds0 + st_free * kStage;
+                    if constexpr (x == 0) {
+                        __builtin_amdgcn_s_waitcnt(0x0f70);             // vmcnt(0): the rows
+                        asm volatile("" ::: "memory");
+                    }
                     if constexpr (x < 2) issue(source(t + 2, x, page_keys, to), 0u, step, std::integral_constant<int, 4>());
                     if constexpr (x == 2) wide = widen_scales(raw0, raw0 + 16 * (kC / 2), to + wave * kRows16, to + kScaleAt + wave * 2 * kScales8);
                     if constexpr (x >= 3 && x < 27) {
                         constexpr std::integral_constant<int, (x - 3) / 6> n;
                         constexpr int k = (x - 3) % 6;
-                        if constexpr (k == 0) raw = widen_read(wide, n);
+                        if constexpr (x == 3) { raw = widen_read(wide, n); codes = widen_codes(wide, n); }
                         if constexpr (k >= 1 && k < 5) {
-                            const v2u two = widen_one(raw[k - 1], widen_scale(wide, n));
+                            const v2u two = widen_one(raw[k - 1], codes);
                             out[(k - 1) / 2][2 * ((k - 1) & 1)] = two[0];
                             out[(k - 1) / 2][2 * ((k - 1) & 1) + 1] = two[1];
+                        }
+                        if constexpr (k == 4 && n < 3) {                // (the next block's: three steps until they are used)
+                            raw = widen_read(wide, std::integral_constant<int, n + 1>());
+                            codes = widen_codes(wide, std::integral_constant<int, n + 1>());
                         }
                         if constexpr (k == 5) widen_write(wide, n, out[0], out[1]);
                     }
