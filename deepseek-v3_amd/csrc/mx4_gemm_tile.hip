@@ -14,6 +14,7 @@ struct TileArgs {
     void* c; v4f* part;                                 // results, or sums of slices [slice][tile][wavefront][16-byte pieces][lane]
     int m, n, k, steps, pack_cols;                      // steps: of 128 along k; those that there are scales for
     int tiles_m, tiles_n, per_slice;                    // steps of a slice, an even number
+    int whole;                                          // tiles in front of those that two workgroups have
 };
 
 // ---- scales.  A lane (r, g) = (l % 32, l / 32) of v_mfma_scale_f32_32x32x64_f8f6f4 gives the scale of row r's block g of 32.  Two products
@@ -80,8 +81,8 @@ template <int N> __device__ __forceinline__ void wait_copies() {        // all b
 //
 // D stages, D - 1 on their way.  A compute unit has one tile of 256 x 256, or two of 128 x 128, whose barriers and copies stand beside each other's products.
 //
-// Measured, mx4 x mx4: 4096 x 7168 -> 18432 in 282 .. 292 us by card (3.7 .. 3.8 PFLOP/s), 4096 x 18432 -> 7168 in 262 .. 271 (4.0 .. 4.1); e4m3 x mx4
-// 376 .. 395 and 360 .. 375.  4.5 and 1.75 rounds of tiles cost the first 10 % and the second 12 %.  The products alone, with neither copies nor reads, would take
+// Measured, mx4 x mx4: 4096 x 7168 -> 18432 in 272 .. 294 us by card (3.7 .. 4.0 PFLOP/s), 4096 x 18432 -> 7168 in 262 .. 271 (4.0 .. 4.1); e4m3 x mx4
+// 367 .. 389 and 360 .. 375.  1.75 rounds of tiles cost the second 12 %.  The products alone, with neither copies nor reads, would take
 // 200 and 180 us at the 1.85 GHz that the chip's power leaves: the copies cost 50 us more, the reads 20.  More stages on their way change nothing there (three
 // or four), nor do stages of twice the length.
 template <bool A8, int RT, int CT, int D> struct Geo {
@@ -89,15 +90,16 @@ template <bool A8, int RT, int CT, int D> struct Geo {
     static constexpr int AB = A8 ? 128 : 64, WB = 64;   // bytes of a row
     static constexpr int SA = TM * AB, SB = TN * WB;
     static constexpr int GA = (TM + 127) / 128, GB = (TN + 127) / 128;  // 128 rows whose scales come in as one
-    static constexpr int SS = (GA + GB) * 512;
-    static constexpr int NA = SA / 4096, NB = SB / 4096, NS = (GA + GB) / 2, NC = NA + NB + NS;         // copies of a wavefront
+    static constexpr int SS = (GA + GB + 1 & ~1) * 512;
+    static constexpr int NA = SA / 4096, NB = SB / 4096, NS = (GA + GB + 1) / 2, NC = NA + NB + NS;         // copies of a wavefront
     static constexpr int B0 = D * SA, S0 = B0 + D * SB, LDS = S0 + D * SS;
-    static_assert(NA * 4096 == SA && NB * 4096 == SB && NS * 2 == GA + GB, "whole copies for every wavefront");
+    static_assert(NA * 4096 == SA && NB * 4096 == SB, "whole copies for every wavefront");
     static_assert((D - 1) * NC < 64, "no more copies than can be counted");
 };
 
-template <bool A8, int RT, int CT, int D, int CD, bool SPLIT>
-__global__ __launch_bounds__(256, 1) void mx4_tile_kernel(TileArgs p) {
+// One of `blocks` workgroups, PARTS a tile of 64 RT x 64 CT PARTS, from tile `first` on.
+template <bool A8, int RT, int CT, int D, int CD, bool SPLIT, int PARTS>
+__device__ __forceinline__ void mx4_tile(const TileArgs& p, int block, int first, int blocks) {
     using G = Geo<A8, RT, CT, D>;
     constexpr int NA = G::NA, NB = G::NB, NC = G::NC, X = RT * CT;
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
@@ -107,11 +109,12 @@ __global__ __launch_bounds__(256, 1) void mx4_tile_kernel(TileArgs p) {
     // workgroup -> tile: a contiguous run per XCD, in bands of 4 tile rows
     int m0, n0, tile;
     {
-        const int T = p.tiles_m * p.tiles_n, x = blockIdx.x % 8, q = T / 8, rest = T % 8;
-        tile = x * q + min(x, rest) + blockIdx.x / 8;
+        const int x = block % 8, q = blocks / 8, rest = blocks % 8, at = x * q + min(x, rest) + block / 8;
+        tile = first + at / PARTS;
         const int band = tile / (4 * p.tiles_n), rows = min(4, p.tiles_m - 4 * band), in = tile - band * 4 * p.tiles_n;
         m0 = (4 * band + in % rows) * G::TM;
-        n0 = in / rows * G::TN;
+        n0 = (in / rows * PARTS + at % PARTS) * G::TN;
+        if (PARTS > 1 && n0 >= p.n) return;
     }
     const int k0 = blockIdx.y * p.per_slice, last = min(p.per_slice, p.steps - k0) - 1;
     const int stages = last + 2 & ~1;                   // an odd one out is followed by itself, with scales of zero
@@ -138,7 +141,7 @@ __global__ __launch_bounds__(256, 1) void mx4_tile_kernel(TileArgs p) {
     const uint8_t* sc0[G::NS];
 #pragma unroll
     for (int i = 0; i < G::NS; ++i) {
-        const int group = 2 * i + (wave >> 1);
+        const int group = min(2 * i + (wave >> 1), G::GA + G::GB - 1);
         sc0[i] = (group < G::GA ? p.as + ((int64_t)(m0 / 128 + group) * p.pack_cols + k0) * 512 : p.bs + ((int64_t)(n0 / 128 + group - G::GA) * p.pack_cols + k0) * 512) + (wave & 1) * 256;
     }
     // requests of a stage: two copies each (or what is left), then the scales
@@ -328,6 +331,19 @@ __global__ __launch_bounds__(256, 1) void mx4_tile_kernel(TileArgs p) {
     }
 }
 
+template <bool A8, int RT, int CT, int D, int CD, bool SPLIT>
+__global__ __launch_bounds__(256, 1) void mx4_tile_kernel(TileArgs p) {
+    if constexpr (RT == 4) {
+        if ((int)blockIdx.x >= p.whole) {
+            mx4_tile<A8, 4, 2, D, CD, SPLIT, 2>(p, blockIdx.x - p.whole, p.whole, gridDim.x - p.whole);
+            return;
+        }
+        mx4_tile<A8, RT, CT, D, CD, SPLIT, 1>(p, blockIdx.x, 0, p.whole);
+    } else {
+        mx4_tile<A8, RT, CT, D, CD, SPLIT, 1>(p, blockIdx.x, 0, gridDim.x);
+    }
+}
+
 // Slices' sums, added in their order: a thread has the four results of a lane's 16 bytes.
 template <int RT, int CT, int CD>
 __global__ __launch_bounds__(256) void mx4_join_kernel(const v4f* part, void* out, int m, int n, int tiles_m, int tiles_n, int slices) {
@@ -359,20 +375,24 @@ __global__ __launch_bounds__(256) void mx4_join_kernel(const v4f* part, void* ou
         if (col + j < n) c[j] = cvt_out<CD>(s[j]);
 }
 
-struct Plan { int rt, ct, tiles_m, tiles_n, slices, per_slice, steps, pack_cols; };
+struct Plan { int rt, ct, tiles_m, tiles_n, whole, slices, per_slice, steps, pack_cols; };
 Plan plan_of(int64_t m, int64_t n, int64_t k, bool a8) {
     Plan p;
     p.steps = (int)(k / 128);
     p.pack_cols = p.steps + 1 & ~1;
-    // Tiles of 256 where their rounds take less time: a round of one each takes 1.03 us a step (e4m3 1.40), one of two small ones 0.78 (1.0), and where there
-    // are no whole rounds of those the next ones fill them.  2000 x 7168 -> 7168: 61 us with 224 tiles of 256 and 82 with 896 small ones; 1024 x 7168 -> 18432
-    // 113 with 288 and 110 (e4m3: 145 and 128).
-    const int64_t large = ((m + 255) / 256) * ((n + 255) / 256), small = ((m + 127) / 128) * ((n + 127) / 128);
-    const double rounds = (double)((large + 255) / 256), half = small > 512 ? small / 512.0 : 1.0;
-    p.rt = p.ct = rounds * (a8 ? 1.40 : 1.03) < half * (a8 ? 1.0 : 0.78) ? 4 : 2;
+    // Tiles of 256 where their rounds take less time: a round of one each takes 1.03 us a step (e4m3 1.40), one of two small ones 0.78 (1.0), of one half of that,
+    // and where there are no whole rounds of those the next ones fill them.  Of a last round that is half empty each tile goes to two workgroups, 0.58 of the
+    // time: 4096 x 7168 -> 18432 (4.5 rounds) 272 us in place of 284, e4m3 367 for 379, 2304 x 7168 -> 9216 (1.27) 91 for 116.  2000 x 7168 -> 7168: 61 us with 224
+    // tiles of 256 and 82 with 896 small ones; 1024 x 7168 -> 18432 98 with 256 tiles and 32 in halves, 106 with small ones (e4m3: 122 and 130); 2048 x 7168 -> 4096
+    // 43 with 128 in halves and 49; 1024 x 7168 -> 4096 32 with 64 in halves and 25 with 256 small ones.
+    const int64_t large = ((m + 255) / 256) * ((n + 255) / 256), small = ((m + 127) / 128) * ((n + 127) / 128), left = large % 256;
+    const bool halves = left > 0 && left <= 128;
+    const double rounds = (double)((large + 255) / 256) - (halves ? 0.42 : 0.0), some = small > 512 ? small / 512.0 : small > 256 ? 1.0 : 0.5;
+    p.rt = p.ct = rounds * (a8 ? 1.40 : 1.03) < some * (a8 ? 1.0 : 0.78) ? 4 : 2;
     if (m <= 64) p.rt = 1;
     p.tiles_m = (int)((m + 64 * p.rt - 1) / (64 * p.rt));
     p.tiles_n = (int)((n + 64 * p.ct - 1) / (64 * p.ct));
+    p.whole = p.tiles_m * p.tiles_n - (p.rt == 4 && halves ? (int)left : 0);
     // Slices of k where compute units would have no tile; with more, their sums cost more than two tiles a unit save (128 x 7168 -> 18432 without slices 32.5 us,
     // with three 39; 500 x 7168 -> 4096 with two 24, with four 28).
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
@@ -400,13 +420,15 @@ template <bool A8, int RT, int CT, int D, int CD> int launch_tiles(const TileArg
     if (plan.slices == 1) {
         static LdsGrant grant;
         if (!grant.ensure((const void*)mx4_tile_kernel<A8, RT, CT, D, CD, false>, G::LDS)) return DSV3_ERR_LAUNCH;
-        hipLaunchKernelGGL((mx4_tile_kernel<A8, RT, CT, D, CD, false>), dim3(tiles), dim3(256), G::LDS, st, a);
+        hipLaunchKernelGGL((mx4_tile_kernel<A8, RT, CT, D, CD, false>), dim3(2 * tiles - plan.whole), dim3(256), G::LDS, st, a);
         return launch_status();
     }
-    static LdsGrant grant;
-    if (!grant.ensure((const void*)mx4_tile_kernel<A8, RT, CT, D, DSV3_F32, true>, G::LDS)) return DSV3_ERR_LAUNCH;
-    hipLaunchKernelGGL((mx4_tile_kernel<A8, RT, CT, D, DSV3_F32, true>), dim3(tiles, plan.slices), dim3(256), G::LDS, st, a);
-    hipLaunchKernelGGL((mx4_join_kernel<RT, CT, CD>), dim3(tiles, RT * CT * 4), dim3(256), 0, st, (const v4f*)a.part, a.c, a.m, a.n, plan.tiles_m, plan.tiles_n, plan.slices);
+    if constexpr (RT < 4) {
+        static LdsGrant grant;
+        if (!grant.ensure((const void*)mx4_tile_kernel<A8, RT, CT, D, DSV3_F32, true>, G::LDS)) return DSV3_ERR_LAUNCH;
+        hipLaunchKernelGGL((mx4_tile_kernel<A8, RT, CT, D, DSV3_F32, true>), dim3(tiles, plan.slices), dim3(256), G::LDS, st, a);
+        hipLaunchKernelGGL((mx4_join_kernel<RT, CT, CD>), dim3(tiles, RT * CT * 4), dim3(256), 0, st, (const v4f*)a.part, a.c, a.m, a.n, plan.tiles_m, plan.tiles_n, plan.slices);
+    }
     return launch_status();
 }
 template <bool A8, int CD> int launch_cd(const TileArgs& a, const Plan& plan, hipStream_t st) {
@@ -429,7 +451,7 @@ int launch_mx4_tile(const Mx4Args& q, bool a8, int c_dtype, void* workspace, hip
     const dim3 grid((unsigned)(space.a_groups + space.b_groups), (unsigned)((plan.pack_cols + 15) / 16));
     if (a8) hipLaunchKernelGGL(mx4_pack_kernel<true>, grid, dim3(256), 0, st, pk);
     else hipLaunchKernelGGL(mx4_pack_kernel<false>, grid, dim3(256), 0, st, pk);
-    const TileArgs a = { q.a, q.b, ws, ws + space.bs, q.c, (v4f*)(ws + space.part), (int)q.m, (int)q.n, (int)q.k, plan.steps, plan.pack_cols, plan.tiles_m, plan.tiles_n, plan.per_slice };
+    const TileArgs a = { q.a, q.b, ws, ws + space.bs, q.c, (v4f*)(ws + space.part), (int)q.m, (int)q.n, (int)q.k, plan.steps, plan.pack_cols, plan.tiles_m, plan.tiles_n, plan.per_slice, plan.whole };
     if (c_dtype == DSV3_BF16) return a8 ? launch_cd<true, DSV3_BF16>(a, plan, st) : launch_cd<false, DSV3_BF16>(a, plan, st);
     if (c_dtype == DSV3_F16) return a8 ? launch_cd<true, DSV3_F16>(a, plan, st) : launch_cd<false, DSV3_F16>(a, plan, st);
     return a8 ? launch_cd<true, DSV3_F32>(a, plan, st) : launch_cd<false, DSV3_F32>(a, plan, st);

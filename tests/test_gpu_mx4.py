@@ -145,6 +145,8 @@ PRODUCTS = [(1, 1, 128), (1, 576, 7168), (2, 17, 256), (4, 100, 384), (3, 6200, 
 # tiles of 64, 128 and 256 rows, with and without slices of k, odd numbers of steps, ragged rows and columns, columns that are no whole eights
 PRODUCTS += [(40, 8200, 8192), (64, 8203, 8320), (33, 20000, 1152), (64, 33000, 128), (300, 2304, 7168), (129, 9000, 2176), (257, 3001, 2304), (300, 7300, 384), (520, 6200, 384),
              (1030, 5000, 640), (1500, 8200, 640), (1537, 8193, 1152), (3000, 4352, 512), (1600, 8448, 128), (513, 2050, 1408)]
+# a last round of 256 x 256 in halves, the last of which may have no columns: all of them, some; in one and more bands of rows
+PRODUCTS += [(1281, 5200, 640), (1200, 5370, 384), (1800, 9300, 640), (1030, 16500, 256), (4500, 8270, 384)]
 
 
 @pytest.mark.parametrize("a8", [False, True], ids=["mx4", "e4m3"])
@@ -170,7 +172,7 @@ def test_product(K, m, n, k, a8):
 
 
 @pytest.mark.parametrize("a8", [False, True], ids=["mx4", "e4m3"])
-@pytest.mark.parametrize("m,n,k", [(1, 40, 256), (20, 100, 1024), (90, 140, 384), (300, 600, 512), (60, 9000, 7168), (260, 3000, 2560), (1300, 9000, 640)])
+@pytest.mark.parametrize("m,n,k", [(1, 40, 256), (20, 100, 1024), (90, 140, 384), (300, 600, 512), (60, 9000, 7168), (260, 3000, 2560), (1300, 9000, 640), (1900, 8330, 384)])
 def test_products_of_whole_numbers(K, m, n, k, a8):
     """Whole numbers whose sums binary32 holds come out exactly, whatever the order: codes of 0, 1, 2, 3, 4 and 6, scales of 1, 2 and 4."""
     g = torch.Generator().manual_seed(m + n)
@@ -188,7 +190,7 @@ def test_products_of_whole_numbers(K, m, n, k, a8):
 
 
 @pytest.mark.parametrize("a8", [False, True], ids=["mx4", "e4m3"])
-@pytest.mark.parametrize("m,n", [(3, 50), (80, 300), (300, 7000), (50, 20000), (1500, 9000)])
+@pytest.mark.parametrize("m,n", [(3, 50), (80, 300), (300, 7000), (50, 20000), (1500, 9000), (1900, 8330)])
 def test_a_scale_of_nan_reaches_its_row(K, m, n, a8):
     g = torch.Generator().manual_seed(m)
     k = 640
