@@ -38,10 +38,11 @@ constexpr int kFewLds = 4 * kFewStage;
 // the stage.  By itself a wavefront has all 64 rows of its tile at the end of where their codes will stand (row r of them is read before anything is written
 // there: 16 (n + 1) rows of 544 bytes end in front of row 16 (n + 1) of those), and their scales behind the 64 of the rows.
 constexpr int kRaw = 16 * (kC / 2) + 16 * 16;
-constexpr int kWide = 15 * 8;                           // a wavefront's table of e4m3 codes (widen)
-constexpr int kLds4 = kLds + 4 * (kRaw + 128);
+constexpr int kFurthest = 19;                           // powers of two below a row's largest scale from which on its e4m3 codes are zeros
+constexpr int kTable = 256;                             // a wavefront's codes for 0 .. kFurthest (widen)
+constexpr int kLds4 = kLds + 4 * (kRaw + kTable);
 constexpr int kFewRawOff = 4 * kRows16 - kTile * (kC / 2), kFewRawScaleOff = kFewScaleOff + 1024, kFewWideOff = kFewScaleOff + 512;
-static_assert(kTile * 4 <= 512 && kWide <= 512, "the scales of 64 rows, the table, the scales as they come");
+static_assert(kTile * 4 <= 512 && (kFurthest + 1) * 8 <= kTable && kLds4 <= 160 * 1024, "the scales of 64 rows, the table, the scales as they come");
 static_assert(kFewRawOff >= 288 * kTile, "rows of four bits are read before they are written over");
 
 struct PagedArgs {
@@ -269,12 +270,13 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     // ... and as e4m3 codes of one scale a row.  Lane l has blocks 4 (l % 4) .. + 3 of row l / 4, the n-th in an order by the row with which few lanes meet in
     // one bank (none in these reads but two of the rows' four, two in each write).
     struct Widening { uint32_t bytes, codes, to; int turn; int top; };
-    // The e4m3 codes of the eight magnitudes times 2^6 .. 2^-8, exact all of them (2^-9 is e4m3's smallest number): a code is looked up by v_perm_b32, four at once.
-    const uint32_t table = lds0 + (FEW ? wave * kFewStage + kFewWideOff : kLds + wave * (kRaw + 128) + kRaw);
+    // The e4m3 codes of the eight magnitudes times 2^6 .. 2^-13, of which a code is looked up by v_perm_b32, four at once.  Down to 2^-8, which is as far as rows
+    // written here go, they are exact (2^-9 is e4m3's smallest number); of rows from elsewhere, blocks below that are rounded to its multiples.
+    const uint32_t table = lds0 + (FEW ? wave * kFewStage + kFewWideOff : kLds + wave * (kRaw + kTable) + kRaw);
     if constexpr (FOUR) {
         const int lane = threadIdx.x & 63;
         const float unit = u32_as_f32((uint32_t)(133 - lane) << 23);
-        if (lane < kWide / 8) *(lds_v2u)(uintptr_t)(table + lane * 8) = v2u{ pack_fp8x4(0.f, 0.5f * unit, unit, 1.5f * unit), pack_fp8x4(2.f * unit, 3.f * unit, 4.f * unit, 6.f * unit) };
+        if (lane <= kFurthest) *(lds_v2u)(uintptr_t)(table + lane * 8) = v2u{ pack_fp8x4(0.f, 0.5f * unit, unit, 1.5f * unit), pack_fp8x4(2.f * unit, 3.f * unit, 4.f * unit, 6.f * unit) };
     }
     auto widen_scales = [&](uint32_t codes, uint32_t scales, uint32_t to, uint32_t to_scales) -> Widening {
         const int lane = lane_now(), row = lane >> 2, q = lane & 3;
@@ -299,7 +301,7 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     };
     auto widen_codes = [&](const Widening& w, auto n) -> v2u {          // those of the block: its scale is so many powers below the row's largest
         const int byte = w.bytes >> (8 * (decltype(n)::value + w.turn & 3)) & 0xff;
-        return *(lds_v2u)(uintptr_t)(table + min(w.top - byte, 14) * 8);
+        return *(lds_v2u)(uintptr_t)(table + min(w.top - byte, kFurthest) * 8);
     };
     auto widen_one = [&](uint32_t x, v2u codes) -> v2u {
         uint32_t even = __builtin_amdgcn_perm(codes[1], codes[0], x & 0x07070707u), odd = __builtin_amdgcn_perm(codes[1], codes[0], x >> 4 & 0x07070707u);
@@ -323,7 +325,7 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
             widen_write(w, n, v4u{ a[0], a[1], b[0], b[1] }, v4u{ c[0], c[1], d[0], d[1] });
         });
     };
-    const uint32_t raw0 = lds0 + kLds + wave * (kRaw + 128);            // (wavefronts that share a tile)
+    const uint32_t raw0 = lds0 + kLds + wave * (kRaw + kTable);            // (wavefronts that share a tile)
     auto copy_raw = [&](int t, uint32_t at, int page) {
         const Source a = source(t, 0, page, 0), b = source(t, 1, page, 0);
         unrolled<5>([&](auto n) { issue_raw(a, b, at, at + 16 * (kC / 2), n); });

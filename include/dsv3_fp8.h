@@ -202,7 +202,7 @@ int dsv3_fp8_gemm_static(const void* a, const float* a_s, const void* b, const f
  *     byte - 127 = the smallest e in [-127, 126] with max|x| <= 6 * 2^e,   code = e2m1( x / 2^e )   (round to nearest, ties to the even code)
  * so that nothing is cut off at 6.  A block that holds a NaN or an infinity gets byte 255 and codes of zero: it is NaN throughout.
  * x: [numel] of x_dtype, y: [numel / 2] bytes, s: [numel / 32] bytes.  `last_dim` is x.size(-1), a multiple of 32, numel a multiple of it.
- * x 16-byte aligned, y 4-byte.  numel == 0 is a no-op.  Up to 2^37 elements (what a launch holds).
+ * x 16-byte aligned, y 4-byte.  numel == 0 is a no-op.  Fewer than 2^37 - 2^13 elements (what a launch holds).
  */
 int dsv3_mx4_quant(const void* x, int x_dtype, void* y, void* s, int64_t numel, int64_t last_dim, void* stream);
 
@@ -217,8 +217,9 @@ int dsv3_mx4_dequant(const void* x, const void* s, void* y, int y_dtype, int64_t
  *     c[i, j] = c_dtype( sum_k a[i, k] * b[j, k] )
  * b: codes [n, k / 2] and bytes [n, k / 32]; a: the same, [m, k / 2] and [m, k / 32], for a_kind DSV3_MX4, or e4m3 codes [m, k] and binary32
  * scales [m, k / 128] for DSV3_E4M3, powers of two as dsv3_act_quant's DSV3_SCALE_FMT_UE8M0 makes them (the caller's guarantee; of any other scale its
- * exponent alone counts).  k a multiple of 128 up to 2^22; any m, n >= 0 whose tiles a launch holds (2^24 of 128 x 128); k == 0 gives zeros.  Products are exact, sums binary32 in an order of the kernels' own, the same
- * for the same sizes.  A NaN scale makes NaN of the results that its row takes part in, and of no others.
+ * exponent alone counts).  k a multiple of 128 up to 2^22; any m, n >= 0 whose tiles a launch holds (2^24 of 128 x 128); k == 0 gives zeros.
+ * Products of 4-bit activations are exact; of e4m3 ones the matrix cores cut off what lies more than 2^13 below the largest of eight.  Sums are binary32, in an
+ * order of the kernels' own, the same for the same sizes.  A NaN scale makes NaN of the results that its row takes part in, and of no others.
  * a, b and c 16-byte aligned, a_s and b_s 4-byte.  workspace: dsv3_mx4_gemm_workspace_bytes() bytes where that is not 0, 256-byte
  * aligned; its contents on entry are ignored.  Calls that share a workspace must be ordered on one stream.
  */
@@ -454,8 +455,9 @@ int dsv3_mla_latent_gemm(const void* x, const float* x_s, const void* w, const f
  *     pe       bf16 [pages, page_size, 64]      the rotated key (16-byte aligned)
  * or, with kv_bits 4, microscaled 4-bit numbers (dsv3_mx4_quant),
  *     kv       e2m1 [pages, page_size, 256]     two codes a byte (16-byte aligned)
- *     kv_scale e8m0 [pages, page_size, 16]      a power of two per 32 latents (16-byte aligned), none more than 2^14 below the row's largest
- * 400 bytes a position where eight bits take 644 and the dense cache 1152.
+ *     kv_scale e8m0 [pages, page_size, 16]      a power of two per 32 latents (16-byte aligned), byte 253 the largest
+ * 400 bytes a position where eight bits take 644 and the dense cache 1152.  The attention takes latents as they are down to 2^-15 of their row's
+ * largest scale, and rounds to multiples of that where rows from elsewhere than dsv3_mla_latent_paged have smaller ones.
  * An entry of the table outside [0, pages) names no page: rows there are not written, are read as zeros and seen by no query.
  * The struct lies in host memory and is read during the call; everything it points to is device memory.  Rows that the functions read
  * are those that they have written, or zeros: codes that are NaN by themselves are none of these.
@@ -470,7 +472,7 @@ typedef struct dsv3_mla_pages {
     int page_size;
     const int32_t* table;       /* int32 [batch, table_width] */
     int64_t table_width;
-    int kv_bits;                /* 8 (or 0): e4m3 codes, one scale a row; 4: see below */
+    int kv_bits;                /* 8 (or 0): e4m3 codes, one scale a row; 4: see above */
 } dsv3_mla_pages;
 
 /*
@@ -478,7 +480,8 @@ typedef struct dsv3_mla_pages {
  *     n = bf16( rms_norm(latent) * kv_norm ),  scale = 2^ceil(log2( max(amax n, 1e-4) / 448 )),  kv = e4m3( n / scale ),  pe = bf16( rotated key )
  * at row starts[b] + i of sequence b, i < counts[b]; y, s as dsv3_mla_latent.  The norms' sums are binary64 here.  A latent that holds a
  * NaN or an infinity is stored as zeros with a scale of NaN.  In four bits: n as dsv3_mx4_quant leaves it, but that no scale is less than 2^-14 times the
- * row's largest (its block's codes are the smaller for it), and a row that is not finite has codes of zero and scales of NaN throughout.  q_rank 0: no query latent (q_norm, y and s are not looked at).
+ * row's largest (its block's codes are the smaller for it), and a row that is not finite has codes of zero and scales of NaN throughout.
+ * q_rank 0: no query latent (q_norm, y and s are not looked at).
  * freqs: binary32 (cos, sin) pairs [batch, rows, 32], each row's own.  A negative start: none of the sequence's rows is written.
  * Two rows that the table sends to one place leave either's values there, or parts of both.  Up to 13421772 rows in all, without a query
  * latent 67108860 (what a launch holds).

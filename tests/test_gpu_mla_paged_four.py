@@ -260,6 +260,24 @@ def test_rows_of_the_smallest_and_largest_scales(h):
             assert (got.abs() < 1e-30).all()
 
 
+@pytest.mark.parametrize("s,h", [(1, 20), (2, 6), (3, 128)])
+def test_rows_whose_scales_lie_far_apart(s, h):
+    """Rows from elsewhere, up to 60 powers of two between a row's scales: read back as they are; attended to as the e4m3 numbers, of 2^6 for the largest scale,
+    that are nearest to them."""
+    four, eight, _ = _case(2, s, h, 200, 24, None, 31)
+    four[4].nan_to_num_(0.0)
+    scale = torch.randint(60, 121, four[3].shape, generator=torch.Generator().manual_seed(s)).to(torch.uint8)
+    scale[..., 3:9] = torch.randint(100, 121, scale[..., 3:9].shape, generator=torch.Generator().manual_seed(h)).to(torch.uint8)
+    four[3] = scale.cuda().view(E8M0)
+    top = scale.int().amax(-1)
+    value = held(four[2].cpu(), four[3].cpu())
+    codes = (value * torch.exp2((133 - top).double())[..., None]).float().to(FP8)
+    same = [*four[:2], codes.cuda(), torch.exp2((top - 133).double()).float().cuda(), *four[4:]]
+    assert torch.equal(_bits(torch.ops.dsv3fp8.mla_decode_paged(*four)), _bits(torch.ops.dsv3fp8.mla_decode_paged(*same)))
+    kv, _ = torch.ops.dsv3fp8.mla_cache_read(*four[2:5], torch.arange(four[2].size(0), dtype=torch.int32).cuda()[:, None], torch.full((four[2].size(0),), 24, dtype=torch.int32).cuda(), 24)
+    assert torch.equal(kv.cpu(), value.bfloat16())
+
+
 def test_attention_past_the_stated_positions_and_negative_starts():
     four, eight, _ = _case(4, 3, 16, 200, 16, None, 4)
     for args in (four, eight):
