@@ -189,8 +189,10 @@ __device__ __forceinline__ v8i join(v4u a, v4u b) {
 // which the reads stand three steps in front of their use.  The products bound those calls, and the widening is 170 more instructions a tile and 70 KB more
 // through LDS beside its 300: one sequence of 61 tokens x 128 heads at 32768 positions 510 us (e4m3: 454), 8 x 25 x 128 at up to 2001 157 (138), 32 x 128 at
 // 4096 62 (59).  Codes through float conversions in place of the table 558, the barrier behind the rows' copies too 535, a block read one step in front 524.
-// Few rows are bound by the three waits before a range's first product and by the fold rather than by the bytes that four bits save: 64 sequences x 16
-// heads at 8192 68 us (65), one sequence at 700 30 (27).  What four bits give is the cache: 400 B a position, with its key, for 644.
+// A wavefront by itself widens all 64 rows, the last 32 beside the first half's scores: 64 sequences x 16 heads at 8192 66.3 us (65.9; all in front of the
+// scores 70.5; with the next tile's rows fetched into L2 meanwhile 69.3), 4 x 4 heads at 20000 35.0 (32.8).  Few rows are bound by the waits before a range's first
+// product and by the fold rather than by the bytes that four bits save; one sequence at 700 takes 30 us (27).  What four bits give is the cache: 400 B a
+// position, with its key, for 644.
 template <bool PACK, bool FEW, bool FOUR>
 __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
@@ -645,7 +647,7 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
             __builtin_amdgcn_s_waitcnt(0x0f70);         // vmcnt(0)
             asm volatile("" ::: "memory");
             if constexpr (FOUR)
-                unrolled<4>([&](auto i) {
+                unrolled<2>([&](auto i) {
                     constexpr int n = decltype(i)::value;
                     widen(own + kFewRawOff + n * 16 * (kC / 2), own + kFewRawScaleOff + n * 256, own + n * kRows16, own + kScaleAt + n * 2 * kScales8);
                 });
@@ -653,8 +655,38 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
             ring[0] = key(keys_at(own), 0, 0);
             ring[1] = key(keys_at(own), 0, 1);
             look_at_scale(0);
-            sc = scale_at(own, 1);
-            score(own, First(), [](auto) {}, [&](auto k) { ring[k] = key(keys_at(own), 1, k); });
+            if constexpr (FOUR) {                       // rows 32 .. 63 beside the first half's scores
+                Widening w[2];
+                unrolled<2>([&](auto i) {
+                    constexpr int n = decltype(i)::value + 2;
+                    w[n - 2] = widen_scales(own + kFewRawOff + n * 16 * (kC / 2), own + kFewRawScaleOff + n * 256, own + n * kRows16, own + kScaleAt + n * 2 * kScales8);
+                });
+                sc = scale_at(own, 1);
+                v4u raw[4], out[2];
+                v2u codes[2];
+                raw[0] = widen_read(w[0], First());
+                codes[0] = widen_codes(w[0], First());
+                score(own, First(), [&](auto step) {
+                    constexpr int x = decltype(step)::value;
+                    unrolled<2>([&](auto i) {
+                        constexpr int d = x < 12 ? x * 2 + decltype(i)::value : x + 12, j = d >> 2, k = d & 3;      // dword k of block j
+                        if constexpr (x < 12 || decltype(i)::value == 0) {
+                            if constexpr (k == 0 && j < 7) codes[(j + 1) & 1] = widen_codes(w[(j + 1) >> 2], std::integral_constant<int, (j + 1) & 3>());
+                            if constexpr (k == 0 && j < 4) raw[(j + 1) & 3] = widen_read(w[(j + 1) >> 2], std::integral_constant<int, (j + 1) & 3>());
+                            if constexpr (k < 3 && j == 4) raw[k + 1] = widen_read(w[1], std::integral_constant<int, k + 1>());     // (before they are written over)
+                            const v2u two = widen_one(raw[j & 3][k], codes[j & 1]);
+                            out[k >> 1][2 * (k & 1)] = two[0];
+                            out[k >> 1][2 * (k & 1) + 1] = two[1];
+                            if constexpr (k == 3) widen_write(w[j >> 2], std::integral_constant<int, j & 3>(), out[0], out[1]);
+                        }
+                    });
+                }, [](auto) {});
+                ring[0] = key(keys_at(own), 1, 0);
+                ring[1] = key(keys_at(own), 1, 1);
+            } else {
+                sc = scale_at(own, 1);
+                score(own, First(), [](auto) {}, [&](auto k) { ring[k] = key(keys_at(own), 1, k); });
+            }
             look_at_scale(1);
             score(own, Second(), [&](auto step) { soften(t, own, First(), step); }, [&](auto k) { ring[k] = value(values_at(own), k); });
             scores_ready(S[1]);
