@@ -208,7 +208,7 @@ int dsv3_mx4_quant(const void* x, int x_dtype, void* y, void* s, int64_t numel, 
 
 /*
  * And back: y[i] = y_dtype( code * 2^(byte - 127) ), exact in binary32 and bf16 wherever their exponents reach, rounded in fp16.
- * x 4-byte aligned, y 16-byte; sizes as dsv3_mx4_quant.
+ * x 4-byte aligned, y 16-byte; sizes as dsv3_mx4_quant, of binary32 up to half of its limit.
  */
 int dsv3_mx4_dequant(const void* x, const void* s, void* y, int y_dtype, int64_t numel, int64_t last_dim, void* stream);
 

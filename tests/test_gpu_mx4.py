@@ -127,6 +127,22 @@ def test_back(K, shape):
     assert torch.equal(K.mx4_dequant(y, s).cpu(), held(y, s).bfloat16())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_more_than_the_caches_hold(K, dtype):
+    """Large tensors go past the caches: what comes out is what their rows give in smaller calls."""
+    torch.set_default_dtype(dtype)
+    x = (torch.randn(9401, 7200, device="cuda", dtype=torch.float32) * torch.rand(9401, 1, device="cuda", dtype=torch.float32)).to(dtype)
+    x[77, 5], x[9400, 7199] = float("nan"), float("inf")
+    assert x.numel() * x.element_size() > 128 << 20
+    y, s = K.mx4_quant(x)
+    v = K.mx4_dequant(y, s)
+    for i in range(0, 9401, 1000):
+        part, scale = K.mx4_quant(x[i:i + 1000])
+        assert torch.equal(y.view(torch.uint8)[i:i + 1000], part.view(torch.uint8)) and torch.equal(s.view(torch.uint8)[i:i + 1000], scale.view(torch.uint8))
+        back = K.mx4_dequant(part, scale)
+        assert torch.equal(v[i:i + 1000].isnan(), back.isnan()) and torch.equal(v[i:i + 1000].nan_to_num(7.0), back.nan_to_num(7.0))
+
+
 def operands(g, m, n, k, a8, spread=6):
     """Random numbers of all sizes, and their values in 64 bits."""
     b, b_s = numbers(torch.randint(0, 16, (n, k), generator=g), torch.randint(127 - spread, 127 + spread, (n, k // 32), generator=g))
