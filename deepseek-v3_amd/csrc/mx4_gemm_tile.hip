@@ -85,22 +85,25 @@ template <int N> __device__ __forceinline__ void wait_copies() {        // all b
 // 367 .. 389 and 360 .. 375.  1.75 rounds of tiles cost the second 12 %.  The products alone, with neither copies nor reads, would take
 // 200 and 180 us at the 1.85 GHz that the chip's power leaves: the copies cost 50 us more, the reads 20.  More stages on their way change nothing there (three
 // or four), nor do stages of twice the length.
-template <bool A8, int RT, int CT, int D> struct Geo {
+// LAID: scales as mx4_pack_kernel lays them out; else a wavefront fetches four bytes of each of 64 rows a stage.
+template <bool A8, int RT, int CT, int D, bool LAID> struct Geo {
     static constexpr int TM = 64 * RT, TN = 64 * CT;
     static constexpr int AB = A8 ? 128 : 64, WB = 64;   // bytes of a row
     static constexpr int SA = TM * AB, SB = TN * WB;
     static constexpr int GA = (TM + 127) / 128, GB = (TN + 127) / 128;  // 128 rows whose scales come in as one
-    static constexpr int SS = (GA + GB + 1 & ~1) * 512;
-    static constexpr int NA = SA / 4096, NB = SB / 4096, NS = (GA + GB + 1) / 2, NC = NA + NB + NS;         // copies of a wavefront
+    static constexpr int SS = LAID ? (GA + GB + 1 & ~1) * 512 : 1024;
+    static constexpr int NA = SA / 4096, NB = SB / 4096, NS = LAID ? (GA + GB + 1) / 2 : 1, NC = NA + NB + NS;         // copies of a wavefront
     static constexpr int B0 = D * SA, S0 = B0 + D * SB, LDS = S0 + D * SS;
     static_assert(NA * 4096 == SA && NB * 4096 == SB, "whole copies for every wavefront");
     static_assert((D - 1) * NC < 64, "no more copies than can be counted");
 };
 
+__device__ const uint32_t no_scale = 0u;
+
 // One of `blocks` workgroups, PARTS a tile of 64 RT x 64 CT PARTS, from tile `first` on.
-template <bool A8, int RT, int CT, int D, int CD, bool SPLIT, int PARTS>
+template <bool A8, int RT, int CT, int D, bool LAID, int CD, bool SPLIT, int PARTS>
 __device__ __forceinline__ void mx4_tile(const TileArgs& p, int block, int first, int blocks) {
-    using G = Geo<A8, RT, CT, D>;
+    using G = Geo<A8, RT, CT, D, LAID>;
     constexpr int NA = G::NA, NB = G::NB, NC = G::NC, X = RT * CT;
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -137,12 +140,19 @@ __device__ __forceinline__ void mx4_tile(const TileArgs& p, int block, int first
         const int row = (wave * NB + t) * BR + lane / 4, c = lane & 3 ^ row >> 2 & 3;
         b_off[t] = min(row, p.n - 1 - n0) * b_row + c * 16 + 1024 - (t & 1) * 1024;
     }
-    // scales: 512 bytes for each 128 rows, wavefronts 0 and 1 (2 and 3) one group's halves
+    // scales: 512 bytes for each 128 rows, wavefronts 0 and 1 (2 and 3) one group's halves; or four bytes of each of a wavefront's 64 rows, activations' first
     const uint8_t* sc0[G::NS];
+    uint64_t sc_row = 0;
+    if constexpr (LAID) {
 #pragma unroll
-    for (int i = 0; i < G::NS; ++i) {
-        const int group = min(2 * i + (wave >> 1), G::GA + G::GB - 1);
-        sc0[i] = (group < G::GA ? p.as + ((int64_t)(m0 / 128 + group) * p.pack_cols + k0) * 512 : p.bs + ((int64_t)(n0 / 128 + group - G::GA) * p.pack_cols + k0) * 512) + (wave & 1) * 256;
+        for (int i = 0; i < G::NS; ++i) {
+            const int group = min(2 * i + (wave >> 1), G::GA + G::GB - 1);
+            sc0[i] = (group < G::GA ? p.as + ((int64_t)(m0 / 128 + group) * p.pack_cols + k0) * 512 : p.bs + ((int64_t)(n0 / 128 + group - G::GA) * p.pack_cols + k0) * 512) + (wave & 1) * 256;
+        }
+    } else {
+        const bool of_a = wave < RT;
+        const int row = of_a ? min(m0 + wave * 64 + lane, p.m - 1) : min(n0 + min(wave - RT, CT - 1) * 64 + lane, p.n - 1);
+        sc_row = (uint64_t)(uintptr_t)(of_a ? p.as : p.bs) + (int64_t)row * (p.k / 32) + (int64_t)k0 * 4;
     }
     // requests of a stage: two copies each (or what is left), then the scales
     constexpr int QA = (NA + 1) / 2, QB = (NB + 1) / 2, NQ = QA + QB + G::NS;
@@ -160,7 +170,8 @@ __device__ __forceinline__ void mx4_tile(const TileArgs& p, int block, int first
             else copy16(b0 + (int64_t)at * G::WB, b_off[t], to);
         } else {                                        // (of the stage past an odd one out, zeros)
             constexpr int i = n - QA - QB;
-            copy4(sc0[i] + (int64_t)min(s, p.pack_cols - 1 - k0) * 512, lane * 4, lds0 + G::S0 + slot * G::SS + i * 1024 + wave * 256);
+            if constexpr (!LAID) copy4_from(s <= last ? sc_row + (uint64_t)s * 4 : (uint64_t)(uintptr_t)&no_scale, lds0 + G::S0 + slot * G::SS + wave * 256);
+            else copy4(sc0[i] + (int64_t)min(s, p.pack_cols - 1 - k0) * 512, lane * 4, lds0 + G::S0 + slot * G::SS + i * 1024 + wave * 256);
         }
     };
     // They are spread over the stage's last product and the next stage's first one: this many of them in the former
@@ -176,24 +187,36 @@ __device__ __forceinline__ void mx4_tile(const TileArgs& p, int block, int first
     for (int u = 0; u < (A8 ? 4 : 2); ++u)              // e4m3: halves g of blocks u and u + 2
         a_ch[u] = A8 ? r * 128 + ((2 * (u & 1) + 4 * (u >> 1) + g ^ r >> 1 & 7) << 4) : b_ch[u];
     const uint32_t a_rd = lds0 + wm * 32 * RT * G::AB, b_rd = lds0 + G::B0 + wn * 32 * CT * G::WB;
-    // the wavefront's tiles in a lane's eight bytes of 128 rows (tiles of 64 rows may be the second half of them)
-    const uint32_t as_at = lds0 + G::S0 + (wm * RT / 4) * 512 + ((m0 / 32 + wm * RT) & 3) * 2;
-    const uint32_t bs_at = lds0 + G::S0 + (G::GA + wn * CT / 4) * 512 + ((n0 / 32 + wn * CT) & 3) * 2;
+    // the wavefront's tiles in a lane's eight bytes of 128 rows (tiles of 64 rows may be the second half of them), or its rows' four bytes
+    const uint32_t as_at = lds0 + G::S0 + (LAID ? (wm * RT / 4) * 512 + ((m0 / 32 + wm * RT) & 3) * 2 + lane * 8 : (wm * RT * 32 + r) * 4);
+    const uint32_t bs_at = lds0 + G::S0 + (LAID ? (G::GA + wn * CT / 4) * 512 + ((n0 / 32 + wn * CT) & 3) * 2 + lane * 8 : (64 * RT + wn * CT * 32 + r) * 4);
     // Activations' fragments in two sets, the weight's too where there are few products; else each is read anew behind its last product, RT (CT - 1) of them before
     // it is needed.
     constexpr bool ONE = X >= 16;
     v4u fa[2][RT][A8 ? 2 : 1], fb[ONE ? 1 : 2][CT];
-    uint32_t sa[2][(RT + 1) / 2], sb[2][(CT + 1) / 2];  // of the stage in use and the next, two tiles a dword
+    constexpr int PER = LAID ? 2 : 1;                // tiles a dword of scales
+    uint32_t sa[2][(RT + PER - 1) / PER], sb[2][(CT + PER - 1) / PER];  // of the stage in use and the next
     auto read_scales = [&](int slot, auto buf) {
         constexpr int B = decltype(buf)::value;
         auto some = [&](uint32_t at, auto& x, auto tiles) {
             constexpr int n = decltype(tiles)::value;
-            if constexpr (n == 4) { const v2u v = *(lds_read8)(uintptr_t)at; x[0] = v[0]; x[1] = v[1]; }
+            if constexpr (!LAID) unrolled<n>([&](auto t) { x[decltype(t)::value] = *(lds_u32)(uintptr_t)(at + decltype(t)::value * 128); });
+            else if constexpr (n == 4) { const v2u v = *(lds_read8)(uintptr_t)at; x[0] = v[0]; x[1] = v[1]; }
             else if constexpr (n == 2) x[0] = *(lds_u32)(uintptr_t)at;
             else x[0] = *(const __attribute__((address_space(3))) uint16_t*)(uintptr_t)at;
         };
-        some(lane * 8 + (as_at + slot * G::SS), sa[B], std::integral_constant<int, RT>());
-        some(lane * 8 + (bs_at + slot * G::SS), sb[B], std::integral_constant<int, CT>());
+        some(as_at + slot * G::SS, sa[B], std::integral_constant<int, RT>());
+        some(bs_at + slot * G::SS, sb[B], std::integral_constant<int, CT>());
+    };
+    // (what is read as it lies: the lane's two bytes of four, the exponent of a binary32)
+    auto turn_scales = [&](auto buf) {
+        constexpr int B = decltype(buf)::value;
+        if constexpr (!LAID) {
+#pragma unroll
+            for (int t = 0; t < RT; ++t) sa[B][t] = A8 ? sa[B][t] >> 23 & 0xffu : sa[B][t] >> (16 * g);
+#pragma unroll
+            for (int t = 0; t < CT; ++t) sb[B][t] >>= 16 * g;
+        }
     };
     constexpr int NRA = (A8 ? 2 : 1) * RT, NR = NRA + CT;               // reads of a product's fragments
     auto read = [&](int slot, auto prod, auto buf, auto which) {
@@ -217,6 +240,7 @@ __device__ __forceinline__ void mx4_tile(const TileArgs& p, int block, int first
     wait_copies<(D - 2) * NC>();                        // (and of the last stage's those that are on their way)
     barrier_no_fence();
     read_scales(0, I0());
+    turn_scales(I0());
     unrolled<NR>([&](auto n) { read(0, I0(), I0(), n); });
 
     // One stage.  Its last product's fragments are read during the one before; behind the barrier in front of that product the stage is free and the next
@@ -235,12 +259,13 @@ __device__ __forceinline__ void mx4_tile(const TileArgs& p, int block, int first
             __builtin_amdgcn_sched_barrier(0);
             unrolled<X>([&](auto step) {
                 constexpr int x = decltype(step)::value, ct = x / RT, rt = (ct & 1) ? RT - 1 - x % RT : x % RT;
-                const uint32_t ws = sb[P][ct / 2], xs = sa[P][rt / 2];
-                constexpr int ws_at = 2 * (ct & 1) + u, xs_at = 2 * (rt & 1) + u;
+                const uint32_t ws = sb[P][ct / PER], xs = sa[P][rt / PER];
+                constexpr int ws_at = LAID ? 2 * (ct & 1) + u : u, xs_at = LAID ? 2 * (rt & 1) + u : A8 ? 0 : u;
                 if constexpr (A8) mfma_codes<ws_at, xs_at>(acc[ct][rt], fb[ONE ? 0 : B][ct], __builtin_bit_cast(v8i, __builtin_shufflevector(fa[B][rt][0], fa[B][rt][1], 0, 1, 2, 3, 4, 5, 6, 7)), ws, xs);
                 else mfma_codes<ws_at, xs_at>(acc[ct][rt], fb[ONE ? 0 : B][ct], fa[B][rt][0], ws, xs);
                 // beside it: the next product's fragments, the copies of the stage that takes this one's place
                 if constexpr (last && x == 0) read_scales(next, std::integral_constant<int, P ^ 1>());
+                if constexpr (last && x == X - 1) turn_scales(std::integral_constant<int, P ^ 1>());
                 unrolled<NR>([&](auto n) {
                     if constexpr (read_at(decltype(n)::value) == x) {
                         if constexpr (last) read(next, I0(), std::integral_constant<int, B ^ 1>(), n);
@@ -331,16 +356,16 @@ __device__ __forceinline__ void mx4_tile(const TileArgs& p, int block, int first
     }
 }
 
-template <bool A8, int RT, int CT, int D, int CD, bool SPLIT>
+template <bool A8, int RT, int CT, int D, bool LAID, int CD, bool SPLIT>
 __global__ __launch_bounds__(256, 1) void mx4_tile_kernel(TileArgs p) {
     if constexpr (RT == 4) {
         if ((int)blockIdx.x >= p.whole) {
-            mx4_tile<A8, 4, 2, D, CD, SPLIT, 2>(p, blockIdx.x - p.whole, p.whole, gridDim.x - p.whole);
+            mx4_tile<A8, 4, 2, D, LAID, CD, SPLIT, 2>(p, blockIdx.x - p.whole, p.whole, gridDim.x - p.whole);
             return;
         }
-        mx4_tile<A8, RT, CT, D, CD, SPLIT, 1>(p, blockIdx.x, 0, p.whole);
+        mx4_tile<A8, RT, CT, D, LAID, CD, SPLIT, 1>(p, blockIdx.x, 0, p.whole);
     } else {
-        mx4_tile<A8, RT, CT, D, CD, SPLIT, 1>(p, blockIdx.x, 0, gridDim.x);
+        mx4_tile<A8, RT, CT, D, LAID, CD, SPLIT, 1>(p, blockIdx.x, 0, gridDim.x);
     }
 }
 
@@ -375,7 +400,7 @@ __global__ __launch_bounds__(256) void mx4_join_kernel(const v4f* part, void* ou
         if (col + j < n) c[j] = cvt_out<CD>(s[j]);
 }
 
-struct Plan { int rt, ct, tiles_m, tiles_n, whole, slices, per_slice, steps, pack_cols; };
+struct Plan { int rt, ct, tiles_m, tiles_n, whole, slices, per_slice, steps, pack_cols; bool laid; };
 Plan plan_of(int64_t m, int64_t n, int64_t k, bool a8) {
     Plan p;
     p.steps = (int)(k / 128);
@@ -401,40 +426,44 @@ Plan plan_of(int64_t m, int64_t n, int64_t k, bool a8) {
     if (slices < 1) slices = 1;
     p.per_slice = (int)((p.steps + slices - 1) / slices) + 1 & ~1;
     p.slices = (p.steps + p.per_slice - 1) / p.per_slice;
+    // Short slices do without the launch that lays out the scales, and fetch them from where they lie, 64 lines at a time: 64 x 512 -> 32768 6.0 us in place of 8.2,
+    // 100 x 1536 -> 24576 8.9 for 11.1, 128 x 2048 -> 18432 11.5 for 13.0; with 28 steps 500 x 7168 -> 4096 28.4 for 24.6, with 32 128 x 4096 -> 18432 21.2 for 21.0, with
+    // 56 1024 x 7168 -> 4096 34 for 25.
+    p.laid = p.rt == 4 || p.per_slice > 16;
     return p;
 }
 struct Space { size_t bs, part, bytes; int64_t a_groups, b_groups; };
 Space space_of(const Plan& p) {
     Space s;
-    s.a_groups = ((int64_t)p.tiles_m * p.rt + 1) / 2; s.b_groups = ((int64_t)p.tiles_n * p.ct + 1) / 2;
+    s.a_groups = p.laid ? ((int64_t)p.tiles_m * p.rt + 1) / 2 : 0; s.b_groups = p.laid ? ((int64_t)p.tiles_n * p.ct + 1) / 2 : 0;
     s.bs = (size_t)s.a_groups * p.pack_cols * 512;
     s.part = s.bs + (size_t)s.b_groups * p.pack_cols * 512;
     s.bytes = s.part + (p.slices > 1 ? (size_t)p.slices * p.tiles_m * p.tiles_n * p.rt * p.ct * 4096 * 4 : 0);
     return s;
 }
 
-template <bool A8, int RT, int CT, int D, int CD> int launch_tiles(const TileArgs& a, const Plan& plan, hipStream_t st) {
-    using G = Geo<A8, RT, CT, D>;
+template <bool A8, int RT, int CT, int D, bool LAID, int CD> int launch_tiles(const TileArgs& a, const Plan& plan, hipStream_t st) {
+    using G = Geo<A8, RT, CT, D, LAID>;
     static_assert(G::LDS <= 160 * 1024 && 4 * 32 * CT * 64 * (RT > 1 ? 2 : 1) <= G::LDS, "the results leave through the stages");
     const unsigned tiles = (unsigned)plan.tiles_m * plan.tiles_n;
     if (plan.slices == 1) {
         static LdsGrant grant;
-        if (!grant.ensure((const void*)mx4_tile_kernel<A8, RT, CT, D, CD, false>, G::LDS)) return DSV3_ERR_LAUNCH;
-        hipLaunchKernelGGL((mx4_tile_kernel<A8, RT, CT, D, CD, false>), dim3(2 * tiles - plan.whole), dim3(256), G::LDS, st, a);
+        if (!grant.ensure((const void*)mx4_tile_kernel<A8, RT, CT, D, LAID, CD, false>, G::LDS)) return DSV3_ERR_LAUNCH;
+        hipLaunchKernelGGL((mx4_tile_kernel<A8, RT, CT, D, LAID, CD, false>), dim3(2 * tiles - plan.whole), dim3(256), G::LDS, st, a);
         return launch_status();
     }
     if constexpr (RT < 4) {
         static LdsGrant grant;
-        if (!grant.ensure((const void*)mx4_tile_kernel<A8, RT, CT, D, DSV3_F32, true>, G::LDS)) return DSV3_ERR_LAUNCH;
-        hipLaunchKernelGGL((mx4_tile_kernel<A8, RT, CT, D, DSV3_F32, true>), dim3(tiles, plan.slices), dim3(256), G::LDS, st, a);
+        if (!grant.ensure((const void*)mx4_tile_kernel<A8, RT, CT, D, LAID, DSV3_F32, true>, G::LDS)) return DSV3_ERR_LAUNCH;
+        hipLaunchKernelGGL((mx4_tile_kernel<A8, RT, CT, D, LAID, DSV3_F32, true>), dim3(tiles, plan.slices), dim3(256), G::LDS, st, a);
         hipLaunchKernelGGL((mx4_join_kernel<RT, CT, CD>), dim3(tiles, RT * CT * 4), dim3(256), 0, st, (const v4f*)a.part, a.c, a.m, a.n, plan.tiles_m, plan.tiles_n, plan.slices);
     }
     return launch_status();
 }
 template <bool A8, int CD> int launch_cd(const TileArgs& a, const Plan& plan, hipStream_t st) {
-    if (plan.rt == 4) return launch_tiles<A8, 4, 4, A8 ? 3 : 4, CD>(a, plan, st);
-    if (plan.rt == 1) return launch_tiles<A8, 1, 2, A8 ? 4 : 6, CD>(a, plan, st);
-    return launch_tiles<A8, 2, 2, A8 ? 3 : 4, CD>(a, plan, st);
+    if (plan.rt == 4) return launch_tiles<A8, 4, 4, A8 ? 3 : 4, true, CD>(a, plan, st);
+    if (plan.rt == 1) return plan.laid ? launch_tiles<A8, 1, 2, A8 ? 4 : 6, true, CD>(a, plan, st) : launch_tiles<A8, 1, 2, A8 ? 4 : 6, false, CD>(a, plan, st);
+    return plan.laid ? launch_tiles<A8, 2, 2, A8 ? 3 : 4, true, CD>(a, plan, st) : launch_tiles<A8, 2, 2, A8 ? 3 : 4, false, CD>(a, plan, st);
 }
 
 }  // namespace
@@ -447,11 +476,15 @@ int launch_mx4_tile(const Mx4Args& q, bool a8, int c_dtype, void* workspace, hip
     // (what launches hold)
     if ((int64_t)plan.tiles_m * plan.tiles_n > 0xffffff || space.a_groups + space.b_groups > 0xffffff) return DSV3_ERR_BAD_SHAPE;
     uint8_t* ws = (uint8_t*)workspace;
-    PackArgs pk = { (const uint32_t*)q.a_s, (const uint32_t*)q.b_s, (v2u*)ws, (v2u*)(ws + space.bs), space.a_groups, space.b_groups, (int)q.m, (int)q.n, (int)(q.k / 128), plan.pack_cols };
-    const dim3 grid((unsigned)(space.a_groups + space.b_groups), (unsigned)((plan.pack_cols + 15) / 16));
-    if (a8) hipLaunchKernelGGL(mx4_pack_kernel<true>, grid, dim3(256), 0, st, pk);
-    else hipLaunchKernelGGL(mx4_pack_kernel<false>, grid, dim3(256), 0, st, pk);
-    const TileArgs a = { q.a, q.b, ws, ws + space.bs, q.c, (v4f*)(ws + space.part), (int)q.m, (int)q.n, (int)q.k, plan.steps, plan.pack_cols, plan.tiles_m, plan.tiles_n, plan.per_slice, plan.whole };
+    TileArgs a = { q.a, q.b, (const uint8_t*)q.a_s, q.b_s, q.c, (v4f*)(ws + space.part), (int)q.m, (int)q.n, (int)q.k, plan.steps, plan.pack_cols, plan.tiles_m, plan.tiles_n, plan.per_slice, plan.whole };
+    if (plan.laid) {
+        PackArgs pk = { (const uint32_t*)q.a_s, (const uint32_t*)q.b_s, (v2u*)ws, (v2u*)(ws + space.bs), space.a_groups, space.b_groups, (int)q.m, (int)q.n, (int)(q.k / 128), plan.pack_cols };
+        const dim3 grid((unsigned)(space.a_groups + space.b_groups), (unsigned)((plan.pack_cols + 15) / 16));
+        if (a8) hipLaunchKernelGGL(mx4_pack_kernel<true>, grid, dim3(256), 0, st, pk);
+        else hipLaunchKernelGGL(mx4_pack_kernel<false>, grid, dim3(256), 0, st, pk);
+        a.as = ws;
+        a.bs = ws + space.bs;
+    }
     if (c_dtype == DSV3_BF16) return a8 ? launch_cd<true, DSV3_BF16>(a, plan, st) : launch_cd<false, DSV3_BF16>(a, plan, st);
     if (c_dtype == DSV3_F16) return a8 ? launch_cd<true, DSV3_F16>(a, plan, st) : launch_cd<false, DSV3_F16>(a, plan, st);
     return a8 ? launch_cd<true, DSV3_F32>(a, plan, st) : launch_cd<false, DSV3_F32>(a, plan, st);

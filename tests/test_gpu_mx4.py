@@ -161,6 +161,8 @@ PRODUCTS = [(1, 1, 128), (1, 576, 7168), (2, 17, 256), (4, 100, 384), (3, 6200, 
 # tiles of 64, 128 and 256 rows, with and without slices of k, odd numbers of steps, ragged rows and columns, columns that are no whole eights
 PRODUCTS += [(40, 8200, 8192), (64, 8203, 8320), (33, 20000, 1152), (64, 33000, 128), (300, 2304, 7168), (129, 9000, 2176), (257, 3001, 2304), (300, 7300, 384), (520, 6200, 384),
              (1030, 5000, 640), (1500, 8200, 640), (1537, 8193, 1152), (3000, 4352, 512), (1600, 8448, 128), (513, 2050, 1408)]
+# scales fetched from where they lie (16 steps of a slice at most) and laid out (more)
+PRODUCTS += [(70, 20000, 2048), (130, 20001, 2176), (60, 33000, 2048), (50, 33001, 2176)]
 # a last round of 256 x 256 in halves, the last of which may have no columns: all of them, some; in one and more bands of rows
 PRODUCTS += [(1281, 5200, 640), (1200, 5370, 384), (1800, 9300, 640), (1030, 16500, 256), (4500, 8270, 384)]
 
