@@ -1,4 +1,6 @@
 // mx4_gemm for many rows: tiles of activations and weight rows through LDS.
+#include <algorithm>
+
 #include "mla.hpp"
 #include "mx4_gemm.hpp"
 
@@ -400,7 +402,7 @@ __global__ __launch_bounds__(256) void mx4_join_kernel(const v4f* part, void* ou
         if (col + j < n) c[j] = cvt_out<CD>(s[j]);
 }
 
-struct Plan { int rt, ct, tiles_m, tiles_n, whole, slices, per_slice, steps, pack_cols; bool laid; };
+struct Plan { int rt, ct, tiles_m, tiles_n, whole, slices, per_slice, steps, pack_cols; bool laid; double time; };
 Plan plan_of(int64_t m, int64_t n, int64_t k, bool a8) {
     Plan p;
     p.steps = (int)(k / 128);
@@ -417,19 +419,25 @@ Plan plan_of(int64_t m, int64_t n, int64_t k, bool a8) {
     if (m <= 64) p.rt = 1;
     p.tiles_m = (int)((m + 64 * p.rt - 1) / (64 * p.rt));
     p.tiles_n = (int)((n + 64 * p.ct - 1) / (64 * p.ct));
-    p.whole = p.tiles_m * p.tiles_n - (p.rt == 4 && halves ? (int)left : 0);
-    // Slices of k where compute units would have no tile; with more, their sums cost more than two tiles a unit save (128 x 7168 -> 18432 without slices 32.5 us,
-    // with three 39; 500 x 7168 -> 4096 with two 24, with four 28).
+    p.whole = (int)((int64_t)p.tiles_m * p.tiles_n - (p.rt == 4 && halves ? left : 0));
+    // Slices of k where compute units would have no tile, if the shorter way pays for their sums, a launch that adds them and 8 bytes an element and slice, written and
+    // read at 5 TB/s: 300 x 7168 -> 2304 in 19.2 us with four and 21.0 without, 128 x 16384 -> 7168 29.4 and 54; 256 x 2048 -> 7168 9.9 without, 18.4 with two, 300 x 4096
+    // -> 4096 14.7 and 18.1.  A step of a tile by itself on its unit takes 0.38 us (e4m3 0.47).
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-    int64_t slices = p.rt == 4 || tiles >= 192 ? 1 : 256 / tiles;
-    slices = slices > p.steps / 8 ? p.steps / 8 : slices;
-    if (slices < 1) slices = 1;
+    const double step = a8 ? 0.47 : 0.38;
+    double least = 1e30;
+    int64_t slices = 1;
+    for (int64_t x = 1; x == 1 || (p.rt != 4 && x * tiles <= 256 && x * 2 <= p.steps); ++x) {
+        const double time = (double)((p.steps + x - 1) / x) * step + (x > 1 ? 5.0 + (double)x * m * n * 8 / 5e6 : 0.0);
+        if (time < least) { least = time; slices = x; }
+    }
     p.per_slice = (int)((p.steps + slices - 1) / slices) + 1 & ~1;
     p.slices = (p.steps + p.per_slice - 1) / p.per_slice;
     // Short slices do without the launch that lays out the scales, and fetch them from where they lie, 64 lines at a time: 64 x 512 -> 32768 6.0 us in place of 8.2,
     // 100 x 1536 -> 24576 8.9 for 11.1, 128 x 2048 -> 18432 11.5 for 13.0; with 28 steps 500 x 7168 -> 4096 28.4 for 24.6, with 32 128 x 4096 -> 18432 21.2 for 21.0, with
     // 56 1024 x 7168 -> 4096 34 for 25.
     p.laid = p.rt == 4 || p.per_slice > 16;
+    p.time = 3.0 + (p.laid ? 5.0 : 0.0) + (p.rt == 4 ? rounds * p.steps * (a8 ? 1.40 : 1.03) : tiles > 256 ? std::max(1.0, tiles / 512.0) * p.steps * (a8 ? 1.0 : 0.78) : least);
     return p;
 }
 struct Space { size_t bs, part, bytes; int64_t a_groups, b_groups; };
@@ -492,22 +500,22 @@ int launch_mx4_tile(const Mx4Args& q, bool a8, int c_dtype, void* workspace, hip
 
 // ---- which kernel takes which sizes
 
-// Up to 32 rows the weight is streamed, and beyond where that moves little: every workgroup of mx4_stream_kernel reads its weight rows and 32 activation rows (at
-// some 10 TB/s, in 3 us at least), while tiles take a launch for the scales in front and often one for the slices behind, 9 us at least.  64 x 7168 -> 2112:
-// 8.5 us streamed and 13.1 in tiles; 100 x 7168 -> 2112 10 and 14.4; 128 x 7168 -> 576 5.3 and 11.4; 300 x 2048 -> 7168 17.2 and 11.7; 64 x 512 -> 32768, many
-// workgroups, 9.6 and 8.4.
-static bool tiles(int64_t m, int64_t n, int64_t k) {
+// Up to 32 rows the weight is streamed, and beyond where that takes less time: every workgroup of mx4_stream_kernel reads its weight rows and 32 activation rows, all
+// of them at some 12 TB/s.  64 x 7168 -> 2112: 8.5 us streamed and 13.1 in tiles; 100 x 7168 -> 2112 10 and 14.4; 128 x 7168 -> 576 5.3 and 11.4; 300 x 2048 -> 7168
+// 17.2 and 10; 64 x 512 -> 32768, many workgroups, 9.6 and 6.0; 128 x 2048 -> 7168 8.9 and 9.6, e4m3 13.5 and 10.4.
+static bool tiles(int64_t m, int64_t n, int64_t k, bool a8) {
     if (m <= 32 || k == 0) return false;
     const int64_t strip = n >= 6144 ? 32 : 16, groups = (n + strip - 1) / strip * ((m + 31) / 32);
-    return groups > 1024 || groups * (strip + 32) * (k / 2) > 100000000;
+    const double time = 3.0 + groups * 0.0015 + (double)groups * (strip * (k / 2) + 32 * (a8 ? k : k / 2)) / 12e6;
+    return groups > 65535 || plan_of(m, n, k, a8).time < time;
 }
 
-size_t mx4_gemm_workspace_bytes(bool a8, int64_t m, int64_t n, int64_t k) { return tiles(m, n, k) ? mx4_tile_workspace_bytes(m, n, k, a8) : 0; }
+size_t mx4_gemm_workspace_bytes(bool a8, int64_t m, int64_t n, int64_t k) { return tiles(m, n, k, a8) ? mx4_tile_workspace_bytes(m, n, k, a8) : 0; }
 
 int launch_mx4_gemm(const void* a, const void* a_s, bool a8, const void* b, const void* b_s, void* c, int c_dtype, int64_t m, int64_t n, int64_t k,
                     void* workspace, hipStream_t st) {
     const Mx4Args p = { (const uint8_t*)a, a_s, (const uint8_t*)b, (const uint8_t*)b_s, c, m, n, k };
-    return tiles(m, n, k) ? launch_mx4_tile(p, a8, c_dtype, workspace, st) : launch_mx4_stream(p, a8, c_dtype, st);
+    return tiles(m, n, k, a8) ? launch_mx4_tile(p, a8, c_dtype, workspace, st) : launch_mx4_stream(p, a8, c_dtype, st);
 }
 
 }  // namespace dsv3
