@@ -81,7 +81,7 @@ template <int N> __device__ __forceinline__ void wait_copies() {        // all b
 // ---- the product.  Four wavefronts, 2 x 2, each 32 RT activation rows x 32 CT weight rows.  A stage of LDS holds 128 along k: rows of 64 bytes, or 128 of
 // e4m3 activations, whose chunks of 16 bytes stand at c ^ (row / 4 % 4) and c ^ (row / 2 % 8), so that 16 rows read at one place hit all banks.
 //
-// D stages, D - 1 on their way.  A compute unit has one tile of 256 x 256, or two of 128 x 128, whose barriers and copies stand beside each other's products.
+// D stages, D - 1 on their way (more make no tile faster).  A compute unit has one tile of 256 x 256, or two of 128 x 128, whose barriers and copies stand beside each other's products.
 //
 // Measured, mx4 x mx4: 4096 x 7168 -> 18432 in 272 .. 294 us by card (3.7 .. 4.0 PFLOP/s), 4096 x 18432 -> 7168 in 262 .. 271 (4.0 .. 4.1); e4m3 x mx4
 // 367 .. 389 and 360 .. 375.  1.75 rounds of tiles cost the second 12 %.  The products alone, with neither copies nor reads, would take
@@ -111,7 +111,7 @@ __device__ __forceinline__ void mx4_tile(const TileArgs& p, int block, int first
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave & 1, wn = wave >> 1, r = lane & 31, g = lane >> 5;
 
-    // workgroup -> tile: a contiguous run per XCD, in bands of 4 tile rows
+    // workgroup -> tile: a contiguous run per XCD, in bands of 4 tile rows (of 2 or 8 up to 5 % more, of 16 up to 6 %)
     int m0, n0, tile;
     {
         const int x = block % 8, q = blocks / 8, rest = blocks % 8, at = x * q + min(x, rest) + block / 8;
