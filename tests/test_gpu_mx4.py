@@ -291,3 +291,34 @@ def test_two_streams_at_once(K):
                 got[i].append(K.mx4_gemm(*sets[i]))
     torch.cuda.synchronize()
     assert all(torch.equal(c, want[i]) for i in range(2) for c in got[i])
+
+
+def test_past_32_bits_of_elements(K):
+    """2^31 elements and more: their ends are what the last rows give by themselves."""
+    x = torch.randn(300001, 7168, device="cuda", dtype=torch.bfloat16)
+    assert x.numel() > 2 ** 31
+    y, s = K.mx4_quant(x)
+    last, scale = K.mx4_quant(x[-9:].contiguous())
+    assert torch.equal(y[-9:].view(torch.uint8), last.view(torch.uint8)) and torch.equal(s[-9:].view(torch.uint8), scale.view(torch.uint8))
+    torch.set_default_dtype(torch.bfloat16)
+    assert torch.equal(K.mx4_dequant(y, s)[-9:], K.mx4_dequant(last, scale))
+
+
+@pytest.mark.parametrize("a8", [False, True], ids=["mx4", "e4m3"])
+@pytest.mark.parametrize("m,n,k", [(3, 700001, 16384), (40, 700001, 16384), (4001, 600011, 256), (70001, 40, 128)])
+def test_products_past_32_bits_of_bytes(K, m, n, k, a8):
+    """Weights of more than 2^32 bytes, results of more than 2^31 elements: exact sums, so that the last rows and columns are those of a product of their own."""
+    g = torch.Generator(device="cuda").manual_seed(m)
+    b = torch.randint(0, 256, (n, k // 2), generator=g, device="cuda", dtype=torch.uint8).view(FP4)
+    b_s = torch.full((n, k // 32), 127, device="cuda", dtype=torch.uint8).view(E8M0)
+    if a8:
+        a, a_s = torch.randint(-8, 9, (m, k), generator=g, device="cuda").float().to(FP8), torch.ones(m, k // 128, device="cuda", dtype=torch.float32)
+    else:
+        a = torch.randint(0, 256, (m, k // 2), generator=g, device="cuda", dtype=torch.uint8).view(FP4)
+        a_s = torch.full((m, k // 32), 127, device="cuda", dtype=torch.uint8).view(E8M0)
+    c = K.mx4_gemm(a, a_s, b, b_s)
+    assert c.shape == (m, n)
+    rows, cols = min(m, 3), min(n, 300)
+    ends = K.mx4_gemm(a[-rows:].contiguous(), a_s[-rows:].contiguous(), b[-cols:].contiguous(), b_s[-cols:].contiguous())
+    first = K.mx4_gemm(a[:rows].contiguous(), a_s[:rows].contiguous(), b[:cols].contiguous(), b_s[:cols].contiguous())
+    assert torch.equal(c[-rows:, -cols:], ends) and torch.equal(c[:rows, :cols], first)
