@@ -130,7 +130,8 @@ int dsv3_mx4_gemm(const void* a, const void* a_s, int a_kind, const void* b, con
     if (!mx4_gemm_sizes_ok(m, n, k)) return DSV3_ERR_BAD_SHAPE;
     if (m == 0 || n == 0) return DSV3_OK;
     if (!c || (k > 0 && (!a || !a_s || !b || !b_s))) return DSV3_ERR_NULL_POINTER;
-    if (!aligned(a, 16) || !aligned(b, 16) || !aligned(c, 16) || !aligned(a_s, 4) || !aligned(b_s, 4)) return DSV3_ERR_MISALIGNED;
+    const int scales = k % 512 == 0 ? 16 : 4;           // (rows of them are fetched in pieces)
+    if (!aligned(a, 16) || !aligned(b, 16) || !aligned(c, 16) || !aligned(a_s, scales) || !aligned(b_s, scales)) return DSV3_ERR_MISALIGNED;
     const size_t need = dsv3_mx4_gemm_workspace_bytes(a_kind, m, n, k);
     if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 256))) return DSV3_ERR_WORKSPACE;
     return launch_mx4_gemm(a, a_s, a_kind == DSV3_E4M3, b, b_s, c, c_dtype, m, n, k, workspace, (hipStream_t)stream);

@@ -87,20 +87,19 @@ template <int N> __device__ __forceinline__ void wait_copies() {        // all b
 // 367 .. 389 and 360 .. 375.  1.75 rounds of tiles cost the second 12 %.  The products alone, with neither copies nor reads, would take
 // 200 and 180 us at the 1.85 GHz that the chip's power leaves: the copies cost 50 us more, the reads 20.  More stages on their way change nothing there (three
 // or four), nor do stages of twice the length.
-// LAID: scales as mx4_pack_kernel lays them out; else a wavefront fetches four bytes of each of 64 rows a stage.
+// LAID: scales as mx4_pack_kernel lays them out; else a wavefront fetches 16 bytes of each of 64 rows every four stages, into one place of two.
 template <bool A8, int RT, int CT, int D, bool LAID> struct Geo {
     static constexpr int TM = 64 * RT, TN = 64 * CT;
     static constexpr int AB = A8 ? 128 : 64, WB = 64;   // bytes of a row
     static constexpr int SA = TM * AB, SB = TN * WB;
     static constexpr int GA = (TM + 127) / 128, GB = (TN + 127) / 128;  // 128 rows whose scales come in as one
-    static constexpr int SS = LAID ? (GA + GB + 1 & ~1) * 512 : 1024;
-    static constexpr int NA = SA / 4096, NB = SB / 4096, NS = LAID ? (GA + GB + 1) / 2 : 1, NC = NA + NB + NS;         // copies of a wavefront
-    static constexpr int B0 = D * SA, S0 = B0 + D * SB, LDS = S0 + D * SS;
+    static constexpr int SS = LAID ? (GA + GB + 1 & ~1) * 512 : 4096;
+    static constexpr int NA = SA / 4096, NB = SB / 4096, NS = LAID ? (GA + GB + 1) / 2 : 1, NC = NA + NB + (LAID ? NS : 0);      // copies of a wavefront for each stage
+    static constexpr int B0 = D * SA, S0 = B0 + D * SB, LDS = S0 + (LAID ? D : 2) * SS;
+    static_assert(LAID || D <= 4, "two places for scales");
     static_assert(NA * 4096 == SA && NB * 4096 == SB, "whole copies for every wavefront");
     static_assert((D - 1) * NC < 64, "no more copies than can be counted");
 };
-
-__device__ const uint32_t no_scale = 0u;
 
 // One of `blocks` workgroups, PARTS a tile of 64 RT x 64 CT PARTS, from tile `first` on.
 template <bool A8, int RT, int CT, int D, bool LAID, int CD, bool SPLIT, int PARTS>
@@ -122,7 +121,7 @@ __device__ __forceinline__ void mx4_tile(const TileArgs& p, int block, int first
         if (PARTS > 1 && n0 >= p.n) return;
     }
     const int k0 = blockIdx.y * p.per_slice, last = min(p.per_slice, p.steps - k0) - 1;
-    const int stages = last + 2 & ~1;                   // an odd one out is followed by itself, with scales of zero
+    const int stages = last + 2 & ~1;                   // an odd one out (LAID) is followed by itself, with scales of zero
 
     // ---- copies into LDS
     const uint32_t lds0 = lds_addr_of(lds);
@@ -144,7 +143,7 @@ __device__ __forceinline__ void mx4_tile(const TileArgs& p, int block, int first
     }
     // scales: 512 bytes for each 128 rows, wavefronts 0 and 1 (2 and 3) one group's halves; or four bytes of each of a wavefront's 64 rows, activations' first
     const uint8_t* sc0[G::NS];
-    uint64_t sc_row = 0;
+    uint32_t sc_off = 0;
     if constexpr (LAID) {
 #pragma unroll
         for (int i = 0; i < G::NS; ++i) {
@@ -152,13 +151,13 @@ __device__ __forceinline__ void mx4_tile(const TileArgs& p, int block, int first
             sc0[i] = (group < G::GA ? p.as + ((int64_t)(m0 / 128 + group) * p.pack_cols + k0) * 512 : p.bs + ((int64_t)(n0 / 128 + group - G::GA) * p.pack_cols + k0) * 512) + (wave & 1) * 256;
         }
     } else {
-        const bool of_a = wave < RT;
-        const int row = of_a ? min(m0 + wave * 64 + lane, p.m - 1) : min(n0 + min(wave - RT, CT - 1) * 64 + lane, p.n - 1);
-        sc_row = (uint64_t)(uintptr_t)(of_a ? p.as : p.bs) + (int64_t)row * (p.k / 32) + (int64_t)k0 * 4;
+        const int row0 = wave < RT ? wave * 64 : min(wave - RT, CT - 1) * 64;
+        sc0[0] = (wave < RT ? p.as + (int64_t)m0 * (p.k / 32) : p.bs + (int64_t)n0 * (p.k / 32)) + (int64_t)k0 * 4;
+        sc_off = (uint32_t)min(row0 + lane, (wave < RT ? p.m - m0 : p.n - n0) - 1) * (uint32_t)(p.k / 32);
     }
     // requests of a stage: two copies each (or what is left), then the scales
     constexpr int QA = (NA + 1) / 2, QB = (NB + 1) / 2, NQ = QA + QB + G::NS;
-    auto copy = [&](int s, int slot, auto which) {
+    auto copy = [&](int s, int slot, auto phase, auto which) {          // phase: s % 4
         constexpr int n = decltype(which)::value;
         const int at = min(s, last);
         if constexpr (n < QA) {
@@ -170,9 +169,11 @@ __device__ __forceinline__ void mx4_tile(const TileArgs& p, int block, int first
             const uint32_t to = lds0 + G::B0 + slot * G::SB + (wave * NB + t) * 1024;
             if constexpr (t + 1 < NB) copy16_two(b0 + (int64_t)at * G::WB, b_off[t], b_off[t + 1], to);
             else copy16(b0 + (int64_t)at * G::WB, b_off[t], to);
-        } else {                                        // (of the stage past an odd one out, zeros)
+        } else {                                        // (LAID: of the stage past an odd one out, zeros)
             constexpr int i = n - QA - QB;
-            if constexpr (!LAID) copy4_from(s <= last ? sc_row + (uint64_t)s * 4 : (uint64_t)(uintptr_t)&no_scale, lds0 + G::S0 + slot * G::SS + wave * 256);
+            if constexpr (!LAID) {
+                if constexpr (decltype(phase)::value % 4 == 0) copy16(sc0[0] + (int64_t)(at >> 2) * 16, sc_off, lds0 + G::S0 + (s >> 2 & 1) * G::SS + wave * 1024);
+            }
             else copy4(sc0[i] + (int64_t)min(s, p.pack_cols - 1 - k0) * 512, lane * 4, lds0 + G::S0 + slot * G::SS + i * 1024 + wave * 256);
         }
     };
@@ -190,25 +191,26 @@ __device__ __forceinline__ void mx4_tile(const TileArgs& p, int block, int first
         a_ch[u] = A8 ? r * 128 + ((2 * (u & 1) + 4 * (u >> 1) + g ^ r >> 1 & 7) << 4) : b_ch[u];
     const uint32_t a_rd = lds0 + wm * 32 * RT * G::AB, b_rd = lds0 + G::B0 + wn * 32 * CT * G::WB;
     // the wavefront's tiles in a lane's eight bytes of 128 rows (tiles of 64 rows may be the second half of them), or its rows' four bytes
-    const uint32_t as_at = lds0 + G::S0 + (LAID ? (wm * RT / 4) * 512 + ((m0 / 32 + wm * RT) & 3) * 2 + lane * 8 : (wm * RT * 32 + r) * 4);
-    const uint32_t bs_at = lds0 + G::S0 + (LAID ? (G::GA + wn * CT / 4) * 512 + ((n0 / 32 + wn * CT) & 3) * 2 + lane * 8 : (64 * RT + wn * CT * 32 + r) * 4);
+    const uint32_t as_at = lds0 + G::S0 + (LAID ? (wm * RT / 4) * 512 + ((m0 / 32 + wm * RT) & 3) * 2 + lane * 8 : (wm * RT * 32 + r) * 16);
+    const uint32_t bs_at = lds0 + G::S0 + (LAID ? (G::GA + wn * CT / 4) * 512 + ((n0 / 32 + wn * CT) & 3) * 2 + lane * 8 : (64 * RT + wn * CT * 32 + r) * 16);
     // Activations' fragments in two sets, the weight's too where there are few products; else each is read anew behind its last product, RT (CT - 1) of them before
     // it is needed.
     constexpr bool ONE = X >= 16;
     v4u fa[2][RT][A8 ? 2 : 1], fb[ONE ? 1 : 2][CT];
     constexpr int PER = LAID ? 2 : 1;                // tiles a dword of scales
     uint32_t sa[2][(RT + PER - 1) / PER], sb[2][(CT + PER - 1) / PER];  // of the stage in use and the next
-    auto read_scales = [&](int slot, auto buf) {
-        constexpr int B = decltype(buf)::value;
+    auto read_scales = [&](int s, int slot, auto phase) {               // of stage s
+        constexpr int B = decltype(phase)::value & 1;
+        const uint32_t place = LAID ? slot * G::SS : (s >> 2 & 1) * G::SS + (decltype(phase)::value & 3) * 4;
         auto some = [&](uint32_t at, auto& x, auto tiles) {
             constexpr int n = decltype(tiles)::value;
-            if constexpr (!LAID) unrolled<n>([&](auto t) { x[decltype(t)::value] = *(lds_u32)(uintptr_t)(at + decltype(t)::value * 128); });
+            if constexpr (!LAID) unrolled<n>([&](auto t) { x[decltype(t)::value] = *(lds_u32)(uintptr_t)(at + decltype(t)::value * 512); });
             else if constexpr (n == 4) { const v2u v = *(lds_read8)(uintptr_t)at; x[0] = v[0]; x[1] = v[1]; }
             else if constexpr (n == 2) x[0] = *(lds_u32)(uintptr_t)at;
             else x[0] = *(const __attribute__((address_space(3))) uint16_t*)(uintptr_t)at;
         };
-        some(as_at + slot * G::SS, sa[B], std::integral_constant<int, RT>());
-        some(bs_at + slot * G::SS, sb[B], std::integral_constant<int, CT>());
+        some(as_at + place, sa[B], std::integral_constant<int, RT>());
+        some(bs_at + place, sb[B], std::integral_constant<int, CT>());
     };
     // (what is read as it lies: the lane's two bytes of four, the exponent of a binary32)
     auto turn_scales = [&](auto buf) {
@@ -236,26 +238,28 @@ __device__ __forceinline__ void mx4_tile(const TileArgs& p, int block, int first
     unrolled<D>([&](auto d) {
         constexpr int i = decltype(d)::value;
         unrolled<NQ>([&](auto n) {
-            if constexpr (i < D - 1 || early(decltype(n)::value)) copy(i, i, n);
+            if constexpr (i < D - 1 || early(decltype(n)::value)) copy(i, i, d, n);
         });
     });
     wait_copies<(D - 2) * NC>();                        // (and of the last stage's those that are on their way)
     barrier_no_fence();
-    read_scales(0, I0());
+    read_scales(0, 0, I0());
     turn_scales(I0());
     unrolled<NR>([&](auto n) { read(0, I0(), I0(), n); });
 
     // One stage.  Its last product's fragments are read during the one before; behind the barrier in front of that product the stage is free and the next
     // one is there.
     int slot = 0, before = D - 1;                       // the stage's place and that of the one in front of it
-    auto stage = [&](int s, auto parity) {
-        constexpr int P = decltype(parity)::value;
+    auto stage = [&](int s, auto phase) {               // phase: s % 4, or s % 2
+        constexpr int F = decltype(phase)::value, P = F & 1;
+        // requests for scales among those of the D - 2 stages behind the next one
+        constexpr int MORE = LAID ? 0 : (D > 2 && (F + 2) % 4 == 0) + (D > 3 && (F + 3) % 4 == 0);
         const int next = slot + 1 == D ? 0 : slot + 1;
         unrolled<2>([&](auto prod) {
             constexpr int u = decltype(prod)::value, B = u & 1;
             constexpr bool last = u == 1;
             if constexpr (last) {
-                wait_copies<(D - 2) * NC>();            // the next stage's, of this wavefront
+                wait_copies<(D - 2) * NC + MORE>();     // the next stage's, of this wavefront
                 barrier_no_fence();                     // and of all; what was read is there
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -266,7 +270,7 @@ __device__ __forceinline__ void mx4_tile(const TileArgs& p, int block, int first
                 if constexpr (A8) mfma_codes<ws_at, xs_at>(acc[ct][rt], fb[ONE ? 0 : B][ct], __builtin_bit_cast(v8i, __builtin_shufflevector(fa[B][rt][0], fa[B][rt][1], 0, 1, 2, 3, 4, 5, 6, 7)), ws, xs);
                 else mfma_codes<ws_at, xs_at>(acc[ct][rt], fb[ONE ? 0 : B][ct], fa[B][rt][0], ws, xs);
                 // beside it: the next product's fragments, the copies of the stage that takes this one's place
-                if constexpr (last && x == 0) read_scales(next, std::integral_constant<int, P ^ 1>());
+                if constexpr (last && x == 0) read_scales(s + 1, next, std::integral_constant<int, F + 1>());
                 if constexpr (last && x == X - 1) turn_scales(std::integral_constant<int, P ^ 1>());
                 unrolled<NR>([&](auto n) {
                     if constexpr (read_at(decltype(n)::value) == x) {
@@ -276,8 +280,8 @@ __device__ __forceinline__ void mx4_tile(const TileArgs& p, int block, int first
                 });
                 unrolled<NQ>([&](auto n) {
                     constexpr int y = decltype(n)::value * 2 * X / NQ;
-                    if constexpr (last && y == x) copy(s + D, slot, n);
-                    if constexpr (!last && y == X + x) copy(s - 1 + D, before, n);
+                    if constexpr (last && y == x) copy(s + D, slot, std::integral_constant<int, F + D>(), n);
+                    if constexpr (!last && y == X + x) copy(s - 1 + D, before, std::integral_constant<int, F - 1 + D>(), n);
                 });
                 __builtin_amdgcn_sched_barrier(0);
             });
@@ -290,7 +294,11 @@ __device__ __forceinline__ void mx4_tile(const TileArgs& p, int block, int first
     do {
         stage(s, I0());
         stage(s + 1, I1());
-        s += 2;
+        if constexpr (!LAID) {
+            stage(s + 2, std::integral_constant<int, 2>());
+            stage(s + 3, std::integral_constant<int, 3>());
+        }
+        s += LAID ? 2 : 4;
     } while (s < stages);
     __builtin_amdgcn_s_waitcnt(0x0070);                 // (copies past the end are still on their way into LDS)
     barrier_no_fence();
@@ -421,8 +429,8 @@ Plan plan_of(int64_t m, int64_t n, int64_t k, bool a8) {
     p.tiles_n = (int)((n + 64 * p.ct - 1) / (64 * p.ct));
     p.whole = (int)((int64_t)p.tiles_m * p.tiles_n - (p.rt == 4 && halves ? left : 0));
     // Slices of k where compute units would have no tile, if the shorter way pays for their sums, a launch that adds them and 8 bytes an element and slice, written and
-    // read at 5 TB/s: 300 x 7168 -> 2304 in 19.2 us with four and 21.0 without, 128 x 16384 -> 7168 29.4 and 54; 256 x 2048 -> 7168 9.9 without, 18.4 with two, 300 x 4096
-    // -> 4096 14.7 and 18.1.  A step of a tile by itself on its unit takes 0.38 us (e4m3 0.47).
+    // read at 5 TB/s: with scales laid out in front, 300 x 7168 -> 2304 in 19.2 us with four and 21.0 without, 128 x 16384 -> 7168 29.4 and 54; 256 x 2048 ->
+    // 7168 9.9 without, 18.4 with two, 300 x 4096 -> 4096 14.7 and 18.1.  A step of a tile by itself on its unit takes 0.38 us (e4m3 0.47).
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
     const double step = a8 ? 0.47 : 0.38;
     double least = 1e30;
@@ -431,12 +439,13 @@ Plan plan_of(int64_t m, int64_t n, int64_t k, bool a8) {
         const double time = (double)((p.steps + x - 1) / x) * step + (x > 1 ? 5.0 + (double)x * m * n * 8 / 5e6 : 0.0);
         if (time < least) { least = time; slices = x; }
     }
-    p.per_slice = (int)((p.steps + slices - 1) / slices) + 1 & ~1;
+    const int whole = k % 512 != 0 ? 2 : 4;             // stages that the kernel does at once
+    p.per_slice = ((int)((p.steps + slices - 1) / slices) + whole - 1) / whole * whole;
     p.slices = (p.steps + p.per_slice - 1) / p.per_slice;
-    // Short slices do without the launch that lays out the scales, and fetch them from where they lie, 64 lines at a time: 64 x 512 -> 32768 6.0 us in place of 8.2,
-    // 100 x 1536 -> 24576 8.9 for 11.1, 128 x 2048 -> 18432 11.5 for 13.0; with 28 steps 500 x 7168 -> 4096 28.4 for 24.6, with 32 128 x 4096 -> 18432 21.2 for 21.0, with
-    // 56 1024 x 7168 -> 4096 34 for 25.
-    p.laid = p.rt == 4 || p.per_slice > 16;
+    // Small tiles fetch their scales from where they lie, 16 bytes a row, where rows begin at multiples of that: without the launch that lays them out 64 x 512 ->
+    // 32768 takes 5.1 us in place of 8.2, 500 x 7168 -> 4096 19.2 for 21.8, 64 x 16384 -> 7168 21 for 27, 1024 x 7168 -> 4096 24.8 for 25.0 (four bytes a row every
+    // stage would take 34 there).
+    p.laid = p.rt == 4 || k % 512 != 0;
     p.time = 3.0 + (p.laid ? 5.0 : 0.0) + (p.rt == 4 ? rounds * p.steps * (a8 ? 1.40 : 1.03) : tiles > 256 ? std::max(1.0, tiles / 512.0) * p.steps * (a8 ? 1.0 : 0.78) : least);
     return p;
 }
@@ -470,7 +479,7 @@ template <bool A8, int RT, int CT, int D, bool LAID, int CD> int launch_tiles(co
 }
 template <bool A8, int CD> int launch_cd(const TileArgs& a, const Plan& plan, hipStream_t st) {
     if (plan.rt == 4) return launch_tiles<A8, 4, 4, A8 ? 3 : 4, true, CD>(a, plan, st);
-    if (plan.rt == 1) return plan.laid ? launch_tiles<A8, 1, 2, A8 ? 4 : 6, true, CD>(a, plan, st) : launch_tiles<A8, 1, 2, A8 ? 4 : 6, false, CD>(a, plan, st);
+    if (plan.rt == 1) return plan.laid ? launch_tiles<A8, 1, 2, A8 ? 4 : 6, true, CD>(a, plan, st) : launch_tiles<A8, 1, 2, 4, false, CD>(a, plan, st);
     return plan.laid ? launch_tiles<A8, 2, 2, A8 ? 3 : 4, true, CD>(a, plan, st) : launch_tiles<A8, 2, 2, A8 ? 3 : 4, false, CD>(a, plan, st);
 }
 
@@ -502,7 +511,7 @@ int launch_mx4_tile(const Mx4Args& q, bool a8, int c_dtype, void* workspace, hip
 
 // Up to 32 rows the weight is streamed, and beyond where that takes less time: every workgroup of mx4_stream_kernel reads its weight rows and 32 activation rows, all
 // of them at some 12 TB/s.  64 x 7168 -> 2112: 8.5 us streamed and 13.1 in tiles; 100 x 7168 -> 2112 10 and 14.4; 128 x 7168 -> 576 5.3 and 11.4; 300 x 2048 -> 7168
-// 17.2 and 10; 64 x 512 -> 32768, many workgroups, 9.6 and 6.0; 128 x 2048 -> 7168 8.9 and 9.6, e4m3 13.5 and 10.4.
+// 17.2 and 9; 64 x 512 -> 32768, many workgroups, 9.6 and 5.1; 128 x 2048 -> 7168 8.9 and 8.5, e4m3 13.5 and 9.6.
 static bool tiles(int64_t m, int64_t n, int64_t k, bool a8) {
     if (m <= 32 || k == 0) return false;
     const int64_t strip = n >= 6144 ? 32 : 16, groups = (n + strip - 1) / strip * ((m + 31) / 32);

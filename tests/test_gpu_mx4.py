@@ -161,7 +161,7 @@ PRODUCTS = [(1, 1, 128), (1, 576, 7168), (2, 17, 256), (4, 100, 384), (3, 6200, 
 # tiles of 64, 128 and 256 rows, with and without slices of k, odd numbers of steps, ragged rows and columns, columns that are no whole eights
 PRODUCTS += [(40, 8200, 8192), (64, 8203, 8320), (33, 20000, 1152), (64, 33000, 128), (300, 2304, 7168), (129, 9000, 2176), (257, 3001, 2304), (300, 7300, 384), (520, 6200, 384),
              (1030, 5000, 640), (1500, 8200, 640), (1537, 8193, 1152), (3000, 4352, 512), (1600, 8448, 128), (513, 2050, 1408)]
-# scales fetched from where they lie (16 steps of a slice at most) and laid out (more)
+# scales fetched from where they lie (k a multiple of 512) and laid out
 PRODUCTS += [(70, 20000, 2048), (130, 20001, 2176), (60, 33000, 2048), (50, 33001, 2176)]
 # a last round of 256 x 256 in halves, the last of which may have no columns: all of them, some; in one and more bands of rows
 PRODUCTS += [(1281, 5200, 640), (1200, 5370, 384), (1800, 9300, 640), (1030, 16500, 256), (4500, 8270, 384)]
@@ -207,11 +207,11 @@ def test_products_of_whole_numbers(K, m, n, k, a8):
     assert torch.equal(K.mx4_gemm(a, a_s, b, b_s).cpu().double(), va @ held(b, b_s).t())
 
 
+@pytest.mark.parametrize("k", [640, 1024])
 @pytest.mark.parametrize("a8", [False, True], ids=["mx4", "e4m3"])
 @pytest.mark.parametrize("m,n", [(3, 50), (80, 300), (300, 7000), (50, 20000), (1500, 9000), (1900, 8330)])
-def test_a_scale_of_nan_reaches_its_row(K, m, n, a8):
+def test_a_scale_of_nan_reaches_its_row(K, m, n, a8, k):
     g = torch.Generator().manual_seed(m)
-    k = 640
     a, a_s, b, b_s, _, _ = operands(g, m, n, k, a8)
     plain = K.mx4_gemm(a, a_s, b, b_s)
     b_s.view(torch.uint8)[n - 2, 7] = 255
@@ -236,6 +236,16 @@ def test_shapes(K, m, n, k, lead):
     assert torch.allclose(c.cpu().double().reshape(m, n), ref, rtol=2.0 ** -8, atol=1e-5)
     y, s = K.mx4_quant(torch.randn(*lead, k, device="cuda"))
     assert K.mx4_dequant(y, s).shape == (*lead, k)
+
+
+@pytest.mark.parametrize("a8", [False, True], ids=["mx4", "e4m3"])
+@pytest.mark.parametrize("m,n,k", [(5, 40, 384), (300, 700, 384), (300, 7000, 384), (300, 2304, 512)])
+def test_rows_of_larger_tensors(K, m, n, k, a8):
+    """From the second row on, where scales begin at no more than multiples of four bytes, or of 16."""
+    g = torch.Generator().manual_seed(m)
+    a, a_s, b, b_s, _, _ = operands(g, m + 1, n + 1, k, a8)
+    want = K.mx4_gemm(a[1:].clone(), a_s[1:].clone(), b[1:].clone(), b_s[1:].clone())
+    assert torch.equal(K.mx4_gemm(a[1:], a_s[1:], b[1:], b_s[1:]), want)
 
 
 def test_the_same_sums_in_every_call(K):

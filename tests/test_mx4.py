@@ -34,6 +34,7 @@ def test_product_validation(L):
     for name in ("a", "a_s", "b", "b_s", "c"):
         assert call(**{name: None}) == 1
         assert call(**{name: A16 + (2 if name.endswith("_s") else 8)}) == 4
+    assert call(k=512, a_s=A16 + 8) == 4 and call(k=1024, b_s=A16 + 4) == 4      # (pieces of 16 bytes are fetched)
     assert call(kind=2) == 5 and call(kind=-1) == 5 and call(dtype=3) == 5
     for bad in (dict(m=-1), dict(n=-1), dict(k=-128), dict(k=64), dict(k=192), dict(k=(1 << 22) + 128), dict(m=1 << 31), dict(n=1 << 31)):
         assert call(**bad) == 2, bad
