@@ -596,9 +596,10 @@ class MLA(nn.Module):
         adds = (entries.remainder(pages) == entries).log().repeat_interleave(page, 1)[:, :positions]       # (of one and zero)
         adds[:, 0].clamp_(min=torch.finfo(adds.dtype).min)
         # A row that is not finite: zeros, so that it reaches nobody through a score that is hidden or a weight of zero, and NaN for those who see it
-        # (a latent that is not finite is NaN in all elements)
-        adds = adds.add(torch.linalg.vector_norm(pe, float("inf"), -1), alpha=0).add_(kv[..., 0], alpha=0)
-        kv.nan_to_num_(0.0, float("inf"), float("-inf"))
+        # (an e4m3 row has one scale, so that a latent that is not finite is NaN in all elements; one of four bits has 16, and numbers up to 6 * 2^126)
+        four, inf = cache.kv.dtype == FP4, float("inf")
+        adds = adds.add(torch.linalg.vector_norm(pe, inf, -1), alpha=0).add_(torch.linalg.vector_norm(kv, inf, -1) if four else kv[..., 0], alpha=0)
+        kv.nan_to_num_(0.0, 0.0 if four else inf, 0.0 if four else -inf)
         pe.nan_to_num_(0.0, 0.0, 0.0)
         last, hidden, parts = starts.unsqueeze(-1) + new, adds.new_full((), float("-inf")), []         # last: what token t sees, itself
         for i in range(b):

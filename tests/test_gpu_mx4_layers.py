@@ -206,3 +206,62 @@ def test_a_captured_step_serves_every_length(M):  # noqa: F811
             assert torch.equal(y.view(torch.int16), want.view(torch.int16))
     for a, c in zip(raw(cache), raw(other)):
         assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("s,what", [(3, "block"), (3, "first block"), (3, "last block"), (70, "block"), (70, "first block"), (70, "last block"), (70, "infinity")])
+def test_rows_of_which_a_part_is_not_finite_reach_the_tokens_that_see_them(M, s, what):  # noqa: F811
+    """A cached row from elsewhere with one scale of NaN, or (in a prompt, which reads rows as bf16) with a number of 2^128: NaN for the tokens of its sequence, which all see
+    it, and the bits that they get without it for the others'."""
+    from dsv3fp8.model import LatentPages
+    layer = _layer(M, small_mla_params(DIM, HEADS, RANK, C, NOPE, ROPE, V, 55), DIM, HEADS, RANK, 8)
+    g = torch.Generator().manual_seed(56)
+    table = torch.tensor([[3, 1, 5, 0, 9], [2, 4, 6, 7, 8]], dtype=torch.int32).cuda()
+    first, freqs0 = _tokens(g, 2, 40, [list(range(40))] * 2)
+    x, freqs = _tokens(g, 2, s, [list(range(40, 40 + s))] * 2)
+    out = []
+    for bad in (False, True):
+        cache = LatentPages(10, 24, device="cuda", bits=4)
+        with torch.inference_mode():
+            layer.forward_paged(first, cache, table, _ints(0, 0), _ints(40, 40), freqs0, 40)
+            if bad:
+                row = cache.scale.view(torch.uint8)[1, 9], cache.kv.view(torch.uint8)[1, 9]           # position 33 of sequence 0
+                if what == "infinity":
+                    row[0].fill_(245)
+                    row[0][11], row[1][11 * 16 + 5] = 253, 0x60                                          # 4 * 2^126
+                else:
+                    row[0][{"block": 9, "first block": 0, "last block": 15}[what]] = 255
+            out.append(layer.forward_paged(x, cache, table, _ints(40, 40), _ints(s, s), freqs, 40 + s))
+    clean, got = out
+    assert clean.isfinite().all() and got[0].isnan().all() and torch.equal(got[1].view(torch.int16), clean[1].view(torch.int16))
+
+
+def test_a_prompt_captured_and_replayed(M):  # noqa: F811
+    """One graph of a prompt's step on 4-bit rows; rows of which a block is NaN come and go between the replays."""
+    from dsv3fp8.model import LatentPages
+    layer = _layer(M, small_mla_params(DIM, HEADS, RANK, C, NOPE, ROPE, V, 57), DIM, HEADS, RANK, 8)
+    g = torch.Generator().manual_seed(58)
+    table = torch.tensor([[3, 1, 5, 0, 9], [2, 4, 6, 7, 8]], dtype=torch.int32).cuda()
+    cache, start, other = (LatentPages(10, 24, device="cuda", bits=4) for _ in range(3))
+    raw = lambda c: (c.kv.view(torch.uint8), c.scale.view(torch.uint8), c.pe)  # noqa: E731
+    first, freqs0 = _tokens(g, 2, 40, [list(range(40))] * 2)
+    x, freqs = _tokens(g, 2, 70, [list(range(40, 110))] * 2)
+    starts, counts = _ints(40, 40), _ints(70, 70)
+    with torch.inference_mode():
+        layer.forward_paged(first, start, table, _ints(0, 0), _ints(40, 40), freqs0, 40)
+        layer.forward_paged(x, other, table, starts, counts, freqs, 120)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = layer.forward_paged(x, cache, table, starts, counts, freqs, 120)
+        for step in range(6):
+            x.copy_(_tokens(g, 2, 70, [list(range(70))] * 2)[0])
+            for c in (cache, other):
+                for mine, theirs in zip(raw(c), raw(start)):
+                    mine.copy_(theirs)
+                if step % 2:
+                    raw(c)[1][4, 3, step] = 255                     # position 27 of sequence 1
+            graph.replay()
+            want = layer.forward_paged(x, other, table, starts, counts, freqs, 120)
+            torch.cuda.synchronize()
+            assert torch.equal(y.view(torch.int16), want.view(torch.int16))
+            assert y[0].isfinite().all() and (y[1].isnan().all() if step % 2 else y[1].isfinite().all())

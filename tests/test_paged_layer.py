@@ -199,3 +199,32 @@ def test_prompts_with_starts_and_counts_out_of_range(layer, calls, start, count)
     sees = at <= start + token
     assert lengths.dtype == torch.int32 and torch.equal(mask == 0, sees) and y.shape == (1, 70, 256)
     assert (not mine.any() or start < 0 or int(lengths[0]) > int(sees[mine].nonzero()[:, 1].max()))
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_prompts_see_rows_of_which_a_part_is_not_finite(layer, calls, monkeypatch, bits):  # noqa: F811
+    """A 4-bit row has 16 scales, of which one may be NaN, and numbers that bf16 does not hold: such a row is marked wherever that part lies.  (An e4m3 row has one scale.)"""
+    from dsv3fp8.model import LatentPages
+    args, s, positions = _arguments(1, 70), 70, 128
+    args[1], args[3] = LatentPages(4, 64, bits=bits), torch.tensor([50], dtype=torch.int32)
+    kv, pe = torch.randn(1, positions, 512).bfloat16(), torch.randn(1, positions, 64).bfloat16()
+    kv[0, 3] = float("nan")
+    kv[0, 4, 1:3] = torch.finfo(torch.bfloat16).max                 # (finite)
+    bad = [3]
+    if bits == 4:
+        for row, block in ((7, 0), (20, 1), (33, 9), (77, 15)):
+            kv[0, row, 32 * block:32 * block + 32] = float("nan")
+        kv[0, 41, 500], kv[0, 100, 0], kv[0, 101, 40:42] = float("inf"), float("-inf"), torch.tensor([float("inf"), float("-inf")])
+        bad += [7, 20, 33, 41, 77, 100, 101]
+    read = kv.clone(), pe.clone()
+    monkeypatch.setattr(torch.ops.dsv3fp8, "mla_cache_read", lambda *a: read)
+    with torch.no_grad():
+        layer.forward_paged(*args)
+    mask, given = _masks(calls)[0], next(c[1] for c in calls if c[0] == "prefill")
+    want = torch.zeros(s, positions)
+    want[:, bad] = float("nan")
+    want[torch.arange(positions) > 50 + torch.arange(s)[:, None]] = float("-inf")
+    assert torch.equal(mask.isnan(), want.isnan()) and torch.equal(mask[~want.isnan()].float(), want[~want.isnan()].float())
+    good = torch.ones(positions, dtype=torch.bool)
+    good[bad] = False
+    assert given[2].isfinite().all() and torch.equal(given[2][:, good], kv[:, good])
