@@ -37,7 +37,7 @@ void* static_scratch() {
 
 extern "C" {
 
-int dsv3_version(void) { return 200; }
+int dsv3_version(void) { return 201; }
 
 const char* dsv3_status_string(int status) {
     switch (status) {
@@ -514,22 +514,25 @@ int dsv3_mla_latent_gemm(const void* x, const float* x_s, const void* w, const f
 }
 
 // What the functions of the paged cache share (no GPU call).
-static int mla_pages_validate(const dsv3_mla_pages* cache, int64_t batch) {
-    if (!cache) return DSV3_ERR_NULL_POINTER;
+static int mla_pages_of(const dsv3_mla_pages* host, int64_t batch, MlaPages* cache) {
+    if (!host) return DSV3_ERR_NULL_POINTER;
+    const int bits = host->page_size >> 24;
+    *cache = MlaPages{ host->kv, host->kv_scale, host->pe, host->pages, host->page_size & 0xffffff, host->table, host->table_width, bits == 4 };
     if (cache->pages < 1 || cache->pages > 0x7fffffff || cache->page_size < 8 || cache->page_size > 16384 || cache->page_size % 8 != 0 ||
         cache->table_width < 1 || cache->table_width > 0x7fffffff || batch < 0 || batch > 65535)
         return DSV3_ERR_BAD_SHAPE;
-    if (cache->kv_bits != 0 && cache->kv_bits != 8 && cache->kv_bits != 4) return DSV3_ERR_BAD_DTYPE;
+    if (bits != 0 && bits != 8 && bits != 4) return DSV3_ERR_BAD_DTYPE;
     if (batch == 0) return DSV3_OK;
     if (!cache->kv || !cache->kv_scale || !cache->pe || !cache->table) return DSV3_ERR_NULL_POINTER;
-    if (!aligned(cache->kv, 16) || !aligned(cache->kv_scale, cache->kv_bits == 4 ? 16 : 4) || !aligned(cache->pe, 16) || !aligned(cache->table, 4)) return DSV3_ERR_MISALIGNED;
+    if (!aligned(cache->kv, 16) || !aligned(cache->kv_scale, cache->four ? 16 : 4) || !aligned(cache->pe, 16) || !aligned(cache->table, 4)) return DSV3_ERR_MISALIGNED;
     return DSV3_OK;
 }
 
 int dsv3_mla_latent_paged(const void* a, int64_t a_stride, const void* q_norm, const void* kv_norm, const float* freqs,
                           const dsv3_mla_pages* cache, const int32_t* starts, const int32_t* counts, void* y, float* s, int64_t batch,
                           int64_t rows, int64_t q_rank, int64_t kv_rank, int rope_dim, float q_eps, float kv_eps, void* stream) {
-    const int rc = mla_pages_validate(cache, batch);
+    MlaPages pages;
+    const int rc = mla_pages_of(cache, batch, &pages);
     if (rc != DSV3_OK) return rc;
     if (kv_rank != 512 || rope_dim != 64 || q_rank < 0 || q_rank > 2048 || q_rank % 128 != 0 || rows < 0 || rows > 0x7fffff ||
         batch * rows > 0x7fffffff || a_stride % 8 != 0 || a_stride < q_rank + kv_rank + rope_dim)
@@ -539,30 +542,32 @@ int dsv3_mla_latent_paged(const void* a, int64_t a_stride, const void* q_norm, c
     if (!aligned(a, 16) || !aligned(kv_norm, 16) || !aligned(freqs, 8) || !aligned(starts, 4) || !aligned(counts, 4) ||
         (q_rank && (!aligned(q_norm, 16) || !aligned(y, 8) || !aligned(s, 4))))
         return DSV3_ERR_MISALIGNED;
-    return launch_mla_latent_paged(a, a_stride, q_norm, kv_norm, freqs, *cache, starts, counts, y, s, batch, rows, (int)q_rank, q_eps, kv_eps,
+    return launch_mla_latent_paged(a, a_stride, q_norm, kv_norm, freqs, pages, starts, counts, y, s, batch, rows, (int)q_rank, q_eps, kv_eps,
                                    (hipStream_t)stream);
 }
 
 int dsv3_mla_cache_read(const dsv3_mla_pages* cache, const int32_t* lengths, void* kv, void* pe, int64_t batch, int64_t positions,
                         void* stream) {
-    const int rc = mla_pages_validate(cache, batch);
+    MlaPages pages;
+    const int rc = mla_pages_of(cache, batch, &pages);
     if (rc != DSV3_OK) return rc;
     if (positions < 0 || positions > 0x7fffff || batch * ((positions + 7) / 8) > 0x7fffffff) return DSV3_ERR_BAD_SHAPE;
     if (batch == 0 || positions == 0) return DSV3_OK;
     if (!lengths || !kv || !pe) return DSV3_ERR_NULL_POINTER;
     if (!aligned(lengths, 4) || !aligned(kv, 16) || !aligned(pe, 16)) return DSV3_ERR_MISALIGNED;
-    return launch_mla_cache_read(*cache, lengths, kv, pe, batch, positions, (hipStream_t)stream);
+    return launch_mla_cache_read(pages, lengths, kv, pe, batch, positions, (hipStream_t)stream);
 }
 
 int dsv3_mla_cache_keep(const dsv3_mla_pages* cache, const int32_t* starts, const int32_t* path, const int32_t* kept, int64_t batch,
                         int most, void* stream) {
-    const int rc = mla_pages_validate(cache, batch);
+    MlaPages pages;
+    const int rc = mla_pages_of(cache, batch, &pages);
     if (rc != DSV3_OK) return rc;
     if (most < 0 || most > 64) return DSV3_ERR_BAD_SHAPE;
     if (batch == 0 || most == 0) return DSV3_OK;
     if (!starts || !path || !kept) return DSV3_ERR_NULL_POINTER;
     if (!aligned(starts, 4) || !aligned(path, 4) || !aligned(kept, 4)) return DSV3_ERR_MISALIGNED;
-    return launch_mla_cache_keep(*cache, starts, path, kept, batch, most, (hipStream_t)stream);
+    return launch_mla_cache_keep(pages, starts, path, kept, batch, most, (hipStream_t)stream);
 }
 
 size_t dsv3_mla_decode_paged_workspace_bytes(int64_t batch, int64_t rows, int heads) {
@@ -574,10 +579,11 @@ static int mla_decode_paged_checked(const void* q, const float* freqs, const dsv
                                     const int64_t* tree, const void* wkv_b, const float* wkv_b_scale, void* y, float* s, bool quant, int64_t batch,
                                     int64_t rows, int64_t positions, int heads, int nope_dim, int rope_dim, int v_dim, int64_t kv_rank,
                                     float softmax_scale, void* workspace, size_t workspace_bytes, void* stream) {
-    const int rc = mla_pages_validate(cache, batch);
+    MlaPages pages;
+    const int rc = mla_pages_of(cache, batch, &pages);
     if (rc != DSV3_OK) return rc;
     if (nope_dim != 128 || rope_dim != 64 || v_dim != 128 || kv_rank != 512 || rows < 0 || rows > 64 || heads < 0 || heads > 65535 ||
-        positions < 1 || positions > 0x7fffff || positions > cache->table_width * cache->page_size ||
+        positions < 1 || positions > 0x7fffff || positions > pages.table_width * pages.page_size ||
         batch * ((positions + 31) / 32) > 0x7fffffff || !(softmax_scale > 1e-30f && softmax_scale < 1e30f))
         return DSV3_ERR_BAD_SHAPE;
     if (batch == 0 || rows == 0 || heads == 0) return DSV3_OK;
@@ -586,7 +592,7 @@ static int mla_decode_paged_checked(const void* q, const float* freqs, const dsv
         !aligned(wkv_b_scale, 4) || !aligned(y, 16) || !aligned(s, 4))
         return DSV3_ERR_MISALIGNED;
     if (!workspace || !aligned(workspace, 256) || workspace_bytes < mla_decode_paged_workspace_bytes(batch, rows, heads)) return DSV3_ERR_WORKSPACE;
-    return launch_mla_decode_paged(q, freqs, *cache, starts, counts, tree, wkv_b, wkv_b_scale, y, s, batch, rows, positions, heads, softmax_scale,
+    return launch_mla_decode_paged(q, freqs, pages, starts, counts, tree, wkv_b, wkv_b_scale, y, s, batch, rows, positions, heads, softmax_scale,
                                    workspace, (hipStream_t)stream);
 }
 

@@ -238,7 +238,7 @@ template <bool FOUR> __global__ __launch_bounds__(512) void mla_keep_kernel(Keep
 
 }  // namespace
 
-int launch_mla_latent_paged(const void* a, int64_t a_stride, const void* q_w, const void* kv_w, const void* freqs, const dsv3_mla_pages& cache,
+int launch_mla_latent_paged(const void* a, int64_t a_stride, const void* q_w, const void* kv_w, const void* freqs, const MlaPages& cache,
                             const int32_t* starts, const int32_t* counts, void* y, float* ys, int64_t batch, int64_t rows, int q_rank,
                             float q_eps, float kv_eps, hipStream_t st) {
     WriteArgs p;
@@ -251,28 +251,28 @@ int launch_mla_latent_paged(const void* a, int64_t a_stride, const void* q_w, co
     if (grid * threads > kMostItems) return DSV3_ERR_BAD_SHAPE;
     static void (*const kernels[2][2])(WriteArgs) = { { mla_write_kernel<false, false>, mla_write_kernel<false, true> },
                                                       { mla_write_kernel<true, false>, mla_write_kernel<true, true> } };
-    hipLaunchKernelGGL(kernels[q_rank != 0][cache.kv_bits == 4], dim3((unsigned)grid), dim3((unsigned)threads), 0, st, p);
+    hipLaunchKernelGGL(kernels[q_rank != 0][cache.four], dim3((unsigned)grid), dim3((unsigned)threads), 0, st, p);
     return launch_status();
 }
 
-int launch_mla_cache_read(const dsv3_mla_pages& cache, const int32_t* lengths, void* kv, void* pe, int64_t batch, int64_t positions, hipStream_t st) {
+int launch_mla_cache_read(const MlaPages& cache, const int32_t* lengths, void* kv, void* pe, int64_t batch, int64_t positions, hipStream_t st) {
     ReadArgs p;
     p.kv = (const uint8_t*)cache.kv; p.scale = cache.kv_scale; p.pe = (const uint16_t*)cache.pe;
     p.table = cache.table; p.width = cache.table_width; p.pages = cache.pages; p.page = cache.page_size;
     p.lengths = lengths; p.out = (uint16_t*)kv; p.out_pe = (uint16_t*)pe;
     p.positions = (int)positions; p.per_seq = (int)((positions + 7) / 8); p.groups = batch * p.per_seq;
     if ((p.groups + 3) / 4 * 256 > kMostItems) return DSV3_ERR_BAD_SHAPE;
-    hipLaunchKernelGGL(cache.kv_bits == 4 ? mla_read_kernel<true> : mla_read_kernel<false>, dim3((unsigned)((p.groups + 3) / 4)), dim3(256), 0, st, p);
+    hipLaunchKernelGGL(cache.four ? mla_read_kernel<true> : mla_read_kernel<false>, dim3((unsigned)((p.groups + 3) / 4)), dim3(256), 0, st, p);
     return launch_status();
 }
 
-int launch_mla_cache_keep(const dsv3_mla_pages& cache, const int32_t* starts, const int32_t* path, const int32_t* kept, int64_t batch, int most,
+int launch_mla_cache_keep(const MlaPages& cache, const int32_t* starts, const int32_t* path, const int32_t* kept, int64_t batch, int most,
                           hipStream_t st) {
     KeepArgs p;
     p.kv = (uint8_t*)cache.kv; p.scale = (uint8_t*)cache.kv_scale; p.pe = (uint8_t*)cache.pe;
     p.table = cache.table; p.width = cache.table_width; p.pages = cache.pages; p.page = cache.page_size;
     p.starts = starts; p.path = path; p.kept = kept; p.most = most;
-    hipLaunchKernelGGL(cache.kv_bits == 4 ? mla_keep_kernel<true> : mla_keep_kernel<false>, dim3((unsigned)batch), dim3(512), 0, st, p);
+    hipLaunchKernelGGL(cache.four ? mla_keep_kernel<true> : mla_keep_kernel<false>, dim3((unsigned)batch), dim3(512), 0, st, p);
     return launch_status();
 }
 

@@ -895,7 +895,7 @@ PagedSpace paged_space(const PagedPlan& a, int64_t batch) {
 
 size_t mla_decode_paged_workspace_bytes(int64_t batch, int64_t tokens, int heads) { return paged_space(paged_plan(batch, tokens * heads), batch).bytes; }
 
-int launch_mla_decode_paged(const void* q, const void* freqs, const dsv3_mla_pages& cache, const int32_t* starts, const int32_t* counts,
+int launch_mla_decode_paged(const void* q, const void* freqs, const MlaPages& cache, const int32_t* starts, const int32_t* counts,
                             const int64_t* tree, const void* w, const float* ws, void* y, float* ys, int64_t batch, int64_t tokens,
                             int64_t positions, int heads, float scale, void* workspace, hipStream_t st) {
     const int64_t rows = tokens * heads;
@@ -905,7 +905,7 @@ int launch_mla_decode_paged(const void* q, const void* freqs, const dsv3_mla_pag
     PagedArgs a;
     uint8_t* wsp = (uint8_t*)workspace;
     a.ql = wsp; a.qe = wsp + space.exponents; a.q = (const uint16_t*)q; a.freqs = (const v2f*)freqs;
-    const bool four = cache.kv_bits == 4;
+    const bool four = cache.four;
     a.kv = (const uint8_t*)cache.kv; a.scales = cache.kv_scale; a.pe = (const uint8_t*)cache.pe;
     a.table = cache.table; a.width = cache.table_width; a.pages = cache.pages;
     a.starts = starts; a.counts = counts; a.tree = tree;

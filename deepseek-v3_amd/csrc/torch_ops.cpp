@@ -404,7 +404,7 @@ dsv3_mla_pages checked_pages(const char* what, const Tensor& kv, const Tensor& s
     TORCH_CHECK(kv.size(2) == (four ? kRank / 2 : kRank) && pe.size(2) == 64, what, ": latents of 512 and rotary keys of 64 are implemented, got ", kv.size(2) * (four ? 2 : 1), " and ", pe.size(2));
     TORCH_CHECK(table.dim() == 2 && table.scalar_type() == at::kInt && table.is_contiguous() && table.size(0) == batch && table.size(1) > 0,
                 what, ": page_table must be a contiguous int32 [batch, width]");
-    return { kv.data_ptr(), scale.data_ptr(), pe.data_ptr(), kv.size(0), (int)kv.size(1), (const int32_t*)table.data_ptr(), table.size(1), four ? 4 : 8 };
+    return { kv.data_ptr(), scale.data_ptr(), pe.data_ptr(), kv.size(0), (int)kv.size(1) | (four ? DSV3_PAGES_OF_4_BITS : 0), (const int32_t*)table.data_ptr(), table.size(1) };
 }
 const int32_t* checked_ints(const char* what, const char* name, const Tensor& t, int64_t batch) {
     TORCH_CHECK(t.dim() == 1 && t.scalar_type() == at::kInt && t.is_contiguous() && t.size(0) == batch, what, ": ", name, " must be a contiguous int32 [batch]");

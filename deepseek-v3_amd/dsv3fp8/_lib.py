@@ -22,9 +22,12 @@ OK = 0
 
 
 class MlaPages(ctypes.Structure):
-    """dsv3_mla_pages (include/dsv3_fp8.h)."""
+    """dsv3_mla_pages (include/dsv3_fp8.h); ``kv_bits``, 0 and 8 for e4m3 rows and 4, stands in the upper eight bits of its ``page_size``."""
     _fields_ = [("kv", c_void_p), ("kv_scale", c_void_p), ("pe", c_void_p), ("pages", c_int64), ("page_size", c_int),
-                ("table", c_void_p), ("table_width", c_int64), ("kv_bits", c_int)]
+                ("table", c_void_p), ("table_width", c_int64)]
+
+    def __init__(self, kv=None, kv_scale=None, pe=None, pages=0, page_size=0, table=None, table_width=0, kv_bits=0):
+        super().__init__(kv, kv_scale, pe, pages, page_size | kv_bits << 24, table, table_width)
 
 
 _pages_p = ctypes.POINTER(MlaPages)

@@ -453,7 +453,7 @@ int dsv3_mla_latent_gemm(const void* x, const float* x_s, const void* w, const f
  *     kv       e4m3 [pages, page_size, 512]     the latent's codes (16-byte aligned)
  *     kv_scale binary32 [pages, page_size]      a power of two: latent = code * scale, a bf16 number (4-byte aligned)
  *     pe       bf16 [pages, page_size, 64]      the rotated key (16-byte aligned)
- * or, with kv_bits 4, microscaled 4-bit numbers (dsv3_mx4_quant),
+ * or, with DSV3_PAGES_OF_4_BITS in the struct's page_size, microscaled 4-bit numbers (dsv3_mx4_quant),
  *     kv       e2m1 [pages, page_size, 256]     two codes a byte (16-byte aligned)
  *     kv_scale e8m0 [pages, page_size, 16]      a power of two per 32 latents (16-byte aligned), byte 253 the largest
  * 400 bytes a position where eight bits take 644 and the dense cache 1152.  The attention takes latents as they are down to 2^-15 of their row's
@@ -469,11 +469,14 @@ typedef struct dsv3_mla_pages {
     void* kv_scale;
     void* pe;
     int64_t pages;
-    int page_size;
+    int page_size;              /* | DSV3_PAGES_OF_4_BITS for rows of four bits */
     const int32_t* table;       /* int32 [batch, table_width] */
     int64_t table_width;
-    int kv_bits;                /* 8 (or 0): e4m3 codes, one scale a row; 4: see above */
 } dsv3_mla_pages;
+
+/* A row's bits stand in page_size's upper eight: 0 (or 8) e4m3 codes and one scale, 4 as above, anything else DSV3_ERR_BAD_DTYPE.  So the struct is as long as
+ * in version 100, whose hosts need no change. */
+#define DSV3_PAGES_OF_4_BITS (4 << 24)
 
 /*
  * dsv3_mla_latent whose cache rows go into pages (inference/model.py:457-466, :480-483), for rows a[i] = [ query latent (q_rank) | latent (512) | rotary key (64) ]:

@@ -268,3 +268,26 @@ def test_widened_codes_are_e4m3():
         v = magnitudes * 2.0 ** (6 - step)
         assert torch.equal(v.float().to(FP8).double(), v)
     assert not torch.equal((magnitudes * 2.0 ** -9).float().to(FP8).double(), magnitudes * 2.0 ** -9)
+
+
+@pytest.mark.parametrize("behind", [0, 4, 7, 8, -1])
+def test_what_lies_behind_the_struct_of_pages_is_not_read(L, behind):
+    """A host's struct has seven fields, of which page_size alone says that rows are e4m3; what follows it in the host's memory is not the library's."""
+    import ctypes
+
+    class Seven(ctypes.Structure):
+        _fields_ = [("kv", ctypes.c_void_p), ("kv_scale", ctypes.c_void_p), ("pe", ctypes.c_void_p), ("pages", ctypes.c_int64), ("page_size", ctypes.c_int),
+                    ("table", ctypes.c_void_p), ("table_width", ctypes.c_int64)]
+
+    class Held(ctypes.Structure):
+        _fields_ = [("pages", Seven), ("behind", ctypes.c_int * 4)]
+    # kv_scale: 4-byte aligned, which is what e4m3 rows ask for
+    held = Held(Seven(A16, A16 + 4, A16, 4, 64, A16, 2), (ctypes.c_int * 4)(*[behind] * 4))
+    cache = ctypes.cast(ctypes.byref(held), ctypes.POINTER(L.MlaPages))
+    # (a null pointer is looked for behind the struct's checks, so that nothing is launched)
+    assert L.lib.dsv3_mla_cache_read(cache, None, A16, A16, 2, 100, None) == 1
+    assert L.lib.dsv3_mla_cache_keep(cache, None, A16, A16, 2, 5, None) == 1
+    assert L.lib.dsv3_mla_latent_paged(None, 2112, A16, A16, A16, cache, A16, A16, A16, A16, 2, 3, 1536, 512, 64, 1e-6, 1e-6, None) == 1
+    assert L.lib.dsv3_mla_decode_paged(None, A16, cache, A16, A16, A16, A16, A16, A16, 2, 3, 100, 4, 128, 64, 128, 512, 0.1, A16, 1 << 30, None) == 1
+    assert L.lib.dsv3_mla_decode_paged_quant(None, A16, cache, A16, A16, A16, A16, A16, A16, A16, 2, 3, 100, 4, 128, 64, 128, 512, 0.1, A16, 1 << 30, None) == 1
+    assert ctypes.sizeof(L.MlaPages) == ctypes.sizeof(Seven)
