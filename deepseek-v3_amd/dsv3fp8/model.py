@@ -749,7 +749,7 @@ class MoE(nn.Module):
     With FP8 experts and ``gemm_impl == "fp8"`` the token lists stay on the device: the routed experts run as
     two grouped GEMMs over expert-sorted rows (w1|w3 stacked, then w2) with SwiGLU and the re-quantisation fused
     between them, and one kernel adds the weighted outputs per token in the order the reference's loop does.
-    ``MoE.grouped = False`` selects the reference's expert-by-expert loop (same kernels, one expert at a time), which experts of 4-bit weights take too.
+    ``MoE.grouped = False`` selects the reference's expert-by-expert loop (same kernels, one expert at a time), which experts take too of whose layers any is of 4-bit weights.
     """
 
     grouped: bool = True
@@ -788,7 +788,7 @@ class MoE(nn.Module):
         assert inter % block_size == 0 and dim % block_size == 0
         dev, fp8 = exs[0].w1.weight.device, exs[0].w1.weight.dtype
         sh = self.shared_experts
-        self._shared_stacked = (sh.w1.out_features == inter and sh.w1.weight.dtype == fp8 and sh.w2.weight.dtype != FP4
+        self._shared_stacked = (sh.w1.out_features == inter and all(lin.weight.dtype == fp8 for lin in (sh.w1, sh.w2, sh.w3))
                                 and sh.w1.weight.device == dev)
         if self._shared_stacked:
             exs.append(sh)
@@ -808,6 +808,10 @@ class MoE(nn.Module):
                     lin.scale.data = sv
         self._stacked = (w13, s13, w2, s2)
 
+    def _stackable(self) -> bool:
+        """Whether every routed expert's weights are of e4m3 codes (looked at until they are stacked)."""
+        return self._stacked is not None or all(_eight_bits(lin.weight) for ex in self.experts if ex is not None for lin in (ex.w1, ex.w2, ex.w3))
+
     def _grouped_ok(self, x: torch.Tensor) -> bool:
         ex = self.experts[self.experts_start_idx]
         inter = ex.w1.out_features
@@ -818,7 +822,7 @@ class MoE(nn.Module):
         return (self.grouped and fits and gemm_impl == "fp8" and world_size == 1 and x.is_cuda
                 and _eight_bits(ex.w1.weight) and ex.w2.weight.dtype != FP4 and x.dtype == torch.bfloat16
                 and torch.get_default_dtype() == torch.bfloat16
-                and ex.w1.out_features % block_size == 0 and self.dim % block_size == 0)
+                and ex.w1.out_features % block_size == 0 and self.dim % block_size == 0 and self._stackable())
 
     def _forward_grouped(self, x: torch.Tensor, weights: torch.Tensor, indices: torch.Tensor) -> torch.Tensor:
         self.stack_experts()

@@ -291,3 +291,51 @@ def test_what_lies_behind_the_struct_of_pages_is_not_read(L, behind):
     assert L.lib.dsv3_mla_decode_paged(None, A16, cache, A16, A16, A16, A16, A16, A16, 2, 3, 100, 4, 128, 64, 128, 512, 0.1, A16, 1 << 30, None) == 1
     assert L.lib.dsv3_mla_decode_paged_quant(None, A16, cache, A16, A16, A16, A16, A16, A16, A16, 2, 3, 100, 4, 128, 64, 128, 512, 0.1, A16, 1 << 30, None) == 1
     assert ctypes.sizeof(L.MlaPages) == ctypes.sizeof(Seven)
+
+
+def _moe(monkeypatch):
+    from dsv3fp8 import model
+    monkeypatch.setattr(model.Linear, "dtype", FP8)
+    monkeypatch.setattr(model, "gemm_impl", "fp8")
+    old = torch.get_default_dtype()
+    torch.set_default_dtype(torch.bfloat16)
+    monkeypatch.setattr(torch, "get_default_dtype", lambda: torch.bfloat16)
+    try:
+        moe = model.MoE(model.ModelArgs(dim=256, n_routed_experts=4, n_activated_experts=2, n_expert_groups=1, n_limited_groups=1, moe_inter_dim=128, n_shared_experts=1))
+    finally:
+        torch.set_default_dtype(old)
+    for module in moe.modules():
+        if isinstance(module, model.Linear):
+            module.weight.data.view(torch.uint8).fill_(0x38)
+            module.scale.data.fill_(1.0)
+    return model, moe
+
+
+@pytest.mark.parametrize("expert,name", [(None, None), (0, "w1"), (0, "w2"), (0, "w3"), (2, "w1"), (3, "w2"), (1, "w3")])
+def test_experts_of_which_some_are_of_4_bits(monkeypatch, expert, name):
+    """One layer of four bits among the routed experts: they are not grouped, and no weight is moved."""
+    from test_mla_dispatch import _OnGpu
+    model, moe = _moe(monkeypatch)
+    x = torch.zeros(2, 256, dtype=torch.bfloat16).as_subclass(_OnGpu)
+    if expert is None:
+        assert moe._grouped_ok(x)
+        moe.stack_experts()
+        assert moe._grouped_ok(x) and moe._shared_stacked and moe._stacked[0].shape == (5, 256, 256)
+        return
+    lin = getattr(moe.experts[expert], name)
+    setattr(moe.experts[expert], name, model.Linear(lin.in_features, lin.out_features, dtype=FP4))
+    assert not moe._grouped_ok(x) and moe._stacked is None
+
+
+@pytest.mark.parametrize("name", ["w1", "w2", "w3"])
+def test_a_shared_expert_with_a_layer_of_4_bits(monkeypatch, name):
+    """It stays by itself; the routed experts are grouped without it."""
+    from test_mla_dispatch import _OnGpu
+    model, moe = _moe(monkeypatch)
+    sh = moe.shared_experts
+    lin = getattr(sh, name)
+    setattr(sh, name, type(lin)(lin.in_features, lin.out_features, dtype=FP4))
+    before = {n: getattr(sh, n).weight.data_ptr() for n in ("w1", "w2", "w3")}
+    assert moe._grouped_ok(torch.zeros(2, 256, dtype=torch.bfloat16).as_subclass(_OnGpu))
+    moe.stack_experts()
+    assert not moe._shared_stacked and moe._stacked[0].shape == (4, 256, 256) and before == {n: getattr(sh, n).weight.data_ptr() for n in before}
