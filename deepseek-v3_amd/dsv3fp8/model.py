@@ -563,10 +563,11 @@ class MLA(nn.Module):
         246 in two pieces of 64, 1610 and 8510 for 1 x 4096; few new tokens on their own (1 x 70: 220 and 182, bound by the host) or far into a long
         context (1 x 128 at 8192: 624 and 398) lose.
 
-        There is no slower path behind the kernels: a layer or call that they do not take raises."""
+        There is no slower path behind the kernels: a layer or call that they do not take raises, one with a projection of 4-bit weights too, whatever the bits of the
+        cache's rows."""
         latent = self._latent_kernel_ok(x) if self._paged_ok(x, freqs_cis) else None
         if latent is None:
-            raise RuntimeError("MLA.forward_paged needs an FP8 layer of the 671B head dimensions with a low-rank query and plain submodules, bf16 input [b, s, dim] "
+            raise RuntimeError("MLA.forward_paged needs a layer of e4m3 weights (none of 4 bits), of the 671B head dimensions, with a low-rank query and plain submodules, bf16 input [b, s, dim] "
                                "on the GPU, gemm_impl 'fp8', no gradients, and freqs_cis complex64 [b, s, 32]")
         b, s = x.size(0), x.size(1)
         if s > 64 and tree is not None:

@@ -228,3 +228,20 @@ def test_prompts_see_rows_of_which_a_part_is_not_finite(layer, calls, monkeypatc
     good = torch.ones(positions, dtype=torch.bool)
     good[bad] = False
     assert given[2].isfinite().all() and torch.equal(given[2][:, good], kv[:, good])
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("name", ["wq_a", "wkv_a", "wq_b", "wkv_b", "wo"])
+def test_layers_with_a_projection_of_4_bits_are_refused(layer, calls, name, bits):  # noqa: F811
+    """Before a row is written, and by their reason."""
+    from dsv3fp8.model import LatentPages
+    lin, args = getattr(layer, name), _arguments(2, 3)
+    args[1] = LatentPages(4, 64, bits=bits)
+    with torch.no_grad():
+        layer.forward_paged(*args)
+        assert calls
+        calls.clear()
+        setattr(layer, name, type(lin)(lin.in_features, lin.out_features, dtype=torch.float4_e2m1fn_x2))
+        with pytest.raises(RuntimeError, match="e4m3 weights .none of 4 bits"):
+            layer.forward_paged(*args)
+    assert not calls
