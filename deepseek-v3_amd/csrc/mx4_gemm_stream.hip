@@ -201,7 +201,17 @@ template <bool A8> int launch_a(const Mx4Args& p, int c_dtype, hipStream_t st) {
 }  // namespace
 
 int launch_mx4_stream(const Mx4Args& p, bool a8, int c_dtype, hipStream_t st) {
-    return a8 ? launch_a<true>(p, c_dtype, st) : launch_a<false>(p, c_dtype, st);
+    constexpr int64_t most = 65535 * 32;                // rows of a launch, which k == 0 alone brings more of
+    for (int64_t m0 = 0; m0 < p.m; m0 += most) {
+        Mx4Args q = p;
+        q.m = p.m - m0 < most ? p.m - m0 : most;
+        q.a += m0 * (a8 ? p.k : p.k / 2);
+        q.a_s = (const uint8_t*)p.a_s + m0 * (p.k / 32);
+        q.c = (uint8_t*)p.c + m0 * p.n * (c_dtype == DSV3_F32 ? 4 : 2);
+        const int rc = a8 ? launch_a<true>(q, c_dtype, st) : launch_a<false>(q, c_dtype, st);
+        if (rc != DSV3_OK) return rc;
+    }
+    return DSV3_OK;
 }
 
 }  // namespace dsv3

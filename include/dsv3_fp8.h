@@ -217,7 +217,8 @@ int dsv3_mx4_dequant(const void* x, const void* s, void* y, int y_dtype, int64_t
  *     c[i, j] = c_dtype( sum_k a[i, k] * b[j, k] )
  * b: codes [n, k / 2] and bytes [n, k / 32]; a: the same, [m, k / 2] and [m, k / 32], for a_kind DSV3_MX4, or e4m3 codes [m, k] and binary32
  * scales [m, k / 128] for DSV3_E4M3, powers of two as dsv3_act_quant's DSV3_SCALE_FMT_UE8M0 makes them (the caller's guarantee; of any other scale its
- * exponent alone counts).  k a multiple of 128 up to 2^22; any m, n >= 0 whose tiles a launch holds (2^24 of 128 x 128); k == 0 gives zeros.
+ * exponent alone counts).  k a multiple of 128 up to 2^22; any m, n >= 0 whose tiles a launch holds (2^24 of 128 x 128; of up to 4 rows,
+ * n * ceil(k / 512) below 2^30 - 32); k == 0 gives zeros.
  * Products of 4-bit activations are exact; of e4m3 ones the matrix cores cut off what lies more than 2^13 below the largest of eight.  Sums are binary32, in an
  * order of the kernels' own, the same for the same sizes.  A NaN scale makes NaN of the results that its row takes part in, and of no others.
  * a, b and c 16-byte aligned, a_s and b_s 4-byte, where k is a multiple of 512 16-byte.  workspace: dsv3_mx4_gemm_workspace_bytes() bytes where that is not 0, 256-byte

@@ -332,3 +332,18 @@ def test_products_past_32_bits_of_bytes(K, m, n, k, a8):
     ends = K.mx4_gemm(a[-rows:].contiguous(), a_s[-rows:].contiguous(), b[-cols:].contiguous(), b_s[-cols:].contiguous())
     first = K.mx4_gemm(a[:rows].contiguous(), a_s[:rows].contiguous(), b[:cols].contiguous(), b_s[:cols].contiguous())
     assert torch.equal(c[-rows:, -cols:], ends) and torch.equal(c[:rows, :cols], first)
+
+
+@pytest.mark.parametrize("a8", [False, True], ids=["mx4", "e4m3"])
+@pytest.mark.parametrize("m,n", [(2097120, 5), (2097121, 9), (4194250, 16)])
+def test_no_terms_and_more_rows_than_a_launch_holds(K, m, n, a8):
+    """k == 0: zeros, for any number of rows."""
+    b, b_s = torch.empty(n, 0, dtype=torch.uint8, device="cuda").view(FP4), torch.empty(n, 0, dtype=torch.uint8, device="cuda").view(E8M0)
+    a = torch.empty(m, 0, dtype=torch.uint8, device="cuda").view(FP8 if a8 else FP4)
+    a_s = torch.empty(m, 0, dtype=torch.float32, device="cuda") if a8 else torch.empty(m, 0, dtype=torch.uint8, device="cuda").view(E8M0)
+    for dtype in (torch.bfloat16, torch.float32):
+        torch.set_default_dtype(dtype)
+        spoilt = torch.full((m * n,), 7.0, dtype=dtype, device="cuda")
+        del spoilt                                                  # (what the result's memory holds beforehand)
+        c = K.mx4_gemm(a, a_s, b, b_s)
+        assert c.shape == (m, n) and c.dtype == dtype and (c == 0).all()
