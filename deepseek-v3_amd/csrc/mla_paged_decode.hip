@@ -480,6 +480,7 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     float off = kNoScore, l = 0.f;                      // exponentials are of 2^(score - off), off a whole number; this lane's share of their sum
     int ks[2];                                          // scale byte of position i, by halves
     uint32_t none[2];                                   // positions that nobody sees for want of a page, by halves
+    uint32_t great[2];                                  // and those whose scale is above 2^30
     float sc;                                           // the scale that the next scores need
     auto scale_at = [&](uint32_t stage, int half) -> float {
         const int i = lane_now() & 31;
@@ -488,6 +489,7 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
     auto look_at_scale = [&](int half) {
         ks[half] = (int)(f32_as_u32(sc) >> 23 & 0xff);  // (NaN: 255, which makes the products NaN)
         none[half] = (uint32_t)__ballot(sc == kNothing);
+        great[half] = (uint32_t)__ballot(sc > 0x1p30f);  // (not NaN)
     };
 
     // The exponentials of half h, in 17 steps that stand beside the MFMAs of 20.
@@ -528,8 +530,9 @@ __global__ __launch_bounds__(256, 1) void mla_paged_kernel(PagedArgs p) {
             const float top = fmaxf(both.x, both.y) * p.scale;
             // `off` is only raised when a score passes it by more than 2^64: exponentials and sums have room for that in binary32, and so the 256
             // multiplications are needed in the rarest of cases.  By whole powers of two: the first half's codes change their exponent only.
-            // (Rows that nobody reads do not ask for it.)
-            const uint64_t raise = __ballot(top - off > 64.f) & alive;
+            // (Rows that nobody reads do not ask for it.)  That much room there is beside scales up to 2^30: 2^64 2^30 448 for each of 2^23 positions is less than
+            // 2^127.  Beside larger ones exponentials are up to 1, and the sums finite as long as as many latents of the largest one's size are.
+            const uint64_t raise = __ballot(top - off > (great[h] ? 0.f : 64.f)) & alive;
             if (raise) {
                 const bool mine = raise >> lane_now() & 1;
                 const float on = mine ? __builtin_ceilf(top) : off, a = __builtin_amdgcn_exp2f(off - on);

@@ -395,3 +395,69 @@ def test_two_streams_at_once():
     for k in (0, 1):
         for y in got[k]:
             assert torch.equal(_bits(y), _bits(want[k]))
+
+
+@pytest.mark.parametrize("h", [64, 8])
+@pytest.mark.parametrize("lo,hi,weights", [(0, 1, 100), (0, 3, 100), (5, 9, 100), (6, 20, 100), (100, 107, 0), (200, 206, -60), (225, 231, -80), (243, 247, -100), (240, 254, -100), (250, 254, -100), (253, 254, -100)])
+def test_rows_of_scales_at_both_ends(lo, hi, weights, h):
+    """Scales from 2^-127 to 2^126, the byte in front of the one that stands for no row, beside weights of 2^`weights` that bring the results to where bf16 has
+    them: bit for bit the e4m3 rows of the same values, whose scale is 2^-6 times the row's largest (2^-125 the least), and as near to 64 bits as the scores' size lets them
+    be.  Scores of the largest rows are so large that their rounding alone says which position is the largest; four and six times 2^126 are more than binary32 holds, in
+    which the sums are: infinite there, or NaN."""
+    four, _, seen = _case(2, 2, h, 200, 24, None, 3)
+    g = torch.Generator().manual_seed(lo * 256 + hi)
+    byte = torch.randint(lo, hi, four[3].shape, generator=g)
+    byte[0, :, 0] = hi - 1
+    four[0] = torch.randn(four[0].shape, generator=g).bfloat16().cuda()
+    four[3] = byte.to(torch.uint8).cuda().view(E8M0)
+    four[4].nan_to_num_(0.0)
+    kv = four[2].view(torch.uint8)
+    kv[:] = torch.randint(0, 256, kv.shape, generator=g).to(torch.uint8).cuda()
+    four[10] = four[10] * 2.0 ** weights
+    if lo >= 200:
+        four[0][..., :NOPE] *= 2.0 ** (-(lo - 127) - weights if lo < 240 else -20)
+    one = kv.cpu().long()
+    values = VALUES[torch.stack((one & 15, one >> 4), -1).flatten(-2)].unflatten(-1, (-1, 32))
+    base = byte.amax(-1, keepdim=True).clamp_min(8)
+    wide = (values * torch.exp2((6 + byte - base).double())[..., None]).flatten(-2)
+    codes, row_scale = wide.float().to(FP8), torch.exp2((base - 133).double()).squeeze(-1).float()
+    assert torch.equal(codes.double(), wide)
+    eight = [*four[:2], codes.cuda(), row_scale.cuda(), *four[4:]]
+    got = torch.ops.dsv3fp8.mla_decode_paged(*four)
+    assert torch.equal(_bits(got), _bits(torch.ops.dsv3fp8.mla_decode_paged(*eight)))
+    ref = _attention_reference(eight, seen)
+    live = ref.abs().amax(-1) > 0
+    got = got.view(ref.shape).double()
+    assert live.any() and (got[~live] == 0).all()
+    if hi <= 250:
+        assert got.isfinite().all() and (got[live].abs().amax(-1) > 2.0 ** -60).all()
+    if hi < 240:
+        assert ((got - ref).norm(dim=-1) <= 2.0 ** -7 * ref.norm(dim=-1) + _at_both_ends(eight, seen)).all()
+
+
+def _at_both_ends(args, seen):
+    """What numbers near binary32's smallest and scores of any size add to an attention's error, as a norm [b, s, h].  Exponentials times their row's scale 2^r are pairs of e4m3 codes whose second
+    one has a scale of 2^-126 at least: off by half of 2^-9 of that, 2^-136, which is 2^(-136 - r) of an exponential.  The largest of these is above 1/2 (offsets
+    are scores rounded up to whole numbers), so that a weight is off by 2^(-136 - r) * 2 * the largest weight.  And the sums of latents go into the last product as two bf16
+    numbers, multiples of 2^-133: off by 2^-134 for each of 512.  A folded query is a pair of codes, off by 2^-9 of itself or 2^-21 of the largest beside it, and of the
+    products of eight features 7 * 2^-13 of their sizes are cut: a score is off by d = softmax_scale * (sum |q| |c| (2^-9 + 7 * 2^-13) + 2^-21 max |q| sum |c|), and a weight
+    by a factor of e^(d + the largest d) at most."""
+    q, freqs, kv, scale, pe, table, starts, counts, _, w8, ws, positions, softmax_scale = args
+    b, s, h, _ = q.shape
+    pages, page = scale.shape
+    w = (w8.float() * ws.repeat_interleave(128, 0).repeat_interleave(128, 1)).bfloat16().double().view(h, NOPE + V, C)
+    out = torch.zeros(b, s, h, dtype=torch.float64, device=q.device)
+    for i in range(b):
+        first = int(starts[i])
+        for t in range(int(counts[i])):
+            rows = _rows(table.cpu(), page, pages, i, list(range(first)) + [first + j for j in sorted(seen[i][t])]).cuda()
+            r = scale.view(-1)[rows].double()
+            c, k = kv.view(-1, C)[rows].double() * r[:, None], pe.view(-1, ROPE)[rows].double()
+            turned = _rotated(q[i, t, :, NOPE:], freqs[i, t, None]).bfloat16().double()
+            for a in range(h):
+                folded = q[i, t, a, :NOPE].double() @ w[a, :NOPE]
+                p = ((folded @ c.T + turned[a] @ k.T) * softmax_scale).softmax(-1)
+                d = softmax_scale * ((2.0 ** -9 + 7 * 2.0 ** -13) * (folded.abs() @ c.abs().T) + 2.0 ** -21 * folded.abs().max() * c.abs().sum(-1))
+                off = p * torch.expm1(d + d.max()) + (2.0 ** -135 / r) * p.max()
+                out[i, t, a] = (off * (c @ w[a, NOPE:].T).norm(dim=-1)).sum() + 2.0 ** -134 * w[a, NOPE:].abs().sum(-1).norm()
+    return out
