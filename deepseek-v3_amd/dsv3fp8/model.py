@@ -141,7 +141,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
 class Linear(nn.Module):
     """Linear layer whose weight may be fp8 with a block-scale tensor attached as ``weight.scale``
     (shape ``[ceil(out/128), ceil(in/128)]``, fp32), as in model.py:166-205.  With ``dtype`` ``torch.float4_e2m1fn_x2`` the weight is of microscaled
-    4-bit numbers, ``[out, in / 2]`` with ``scale`` e8m0 ``[out, in / 32]``; ``in`` is a multiple of 128 then."""
+    4-bit numbers, ``[out, in / 2]`` with ``scale`` e8m0 ``[out, in / 32]``; ``in`` is a multiple of 128 then, and ``to(dtype)``, ``half()`` and their like leave both as they are."""
     dtype = torch.bfloat16
     scale_fmt: Optional[str] = None
 
@@ -165,6 +165,18 @@ class Linear(nn.Module):
             self.bias = nn.Parameter(torch.empty(out_features))
         else:
             self.register_parameter("bias", None)
+
+    def _apply(self, fn, recurse: bool = True):
+        # (to(), cuda(), half() and their like.)  Codes of 4 bits and their scales go through as bytes, which move and are not converted: torch has no conversion
+        # of float4_e2m1fn_x2, and on the GPU its attempt is a fault.
+        def of_bytes(t: torch.Tensor) -> torch.Tensor:
+            if t.dtype not in (FP4, ops.E8M0):
+                return fn(t)
+            raw = fn(t.detach().view(torch.uint8))
+            if raw.dtype != torch.uint8:
+                raise TypeError(f"Linear: weights of 4 bits cannot become {raw.dtype}")
+            return raw.view(t.dtype)
+        return super()._apply(of_bytes if self.weight.dtype == FP4 else fn, recurse)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return linear(x, self.weight, self.bias, self.scale_fmt)

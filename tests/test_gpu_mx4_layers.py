@@ -265,3 +265,21 @@ def test_a_prompt_captured_and_replayed(M):  # noqa: F811
             torch.cuda.synchronize()
             assert torch.equal(y.view(torch.int16), want.view(torch.int16))
             assert y[0].isfinite().all() and (y[1].isnan().all() if step % 2 else y[1].isfinite().all())
+
+
+def test_conversions_of_a_layer_leave_its_codes(four):
+    """Moved and converted as a whole, with another layer and a bias: the same products."""
+    g = torch.Generator().manual_seed(8)
+    lin = four.Linear(256, 48, bias=True)
+    block = torch.nn.Sequential(lin, torch.nn.LayerNorm(48)).cuda()
+    _fill(lin, g)
+    codes, scale = lin.weight.data.view(torch.uint8).clone(), lin.scale.data.view(torch.uint8).clone()
+    x = torch.randn(5, 256, generator=g).bfloat16().cuda()
+    with torch.no_grad():
+        want = lin(x)
+        block.float()
+        assert lin.bias.dtype == torch.float32
+        block.to("cpu", torch.float16).to("cuda", torch.bfloat16)
+        assert lin.weight.is_cuda and lin.scale.is_cuda and lin.weight.scale is lin.scale and lin.bias.dtype == torch.bfloat16
+        assert torch.equal(lin.weight.data.view(torch.uint8), codes) and torch.equal(lin.scale.data.view(torch.uint8), scale)
+        assert torch.equal(lin(x), want)

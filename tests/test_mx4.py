@@ -339,3 +339,42 @@ def test_a_shared_expert_with_a_layer_of_4_bits(monkeypatch, name):
     assert moe._grouped_ok(torch.zeros(2, 256, dtype=torch.bfloat16).as_subclass(_OnGpu))
     moe.stack_experts()
     assert not moe._shared_stacked and moe._stacked[0].shape == (4, 256, 256) and before == {n: getattr(sh, n).weight.data_ptr() for n in before}
+
+
+def _four_bit_linear():
+    from dsv3fp8 import model
+    lin = model.Linear(256, 48, bias=True, dtype=FP4)
+    _u8(lin.weight.data).copy_(torch.randint(0, 256, (48, 128)).to(torch.uint8))
+    _u8(lin.scale.data).copy_(torch.randint(0, 255, (48, 8)).to(torch.uint8))
+    return lin
+
+
+@pytest.mark.parametrize("convert", ["to", "half", "float", "double", "bfloat16", "in a model", "to a device and type"])
+def test_conversions_of_a_layer_leave_its_codes(convert):
+    """torch has no conversion of float4_e2m1fn_x2 (an error on the host, a fault on the GPU): codes and scales stay what they are, the bias is converted."""
+    lin = _four_bit_linear()
+    codes, scale, weight = _u8(lin.weight.data).clone(), _u8(lin.scale.data).clone(), lin.weight
+    module = torch.nn.Sequential(torch.nn.LayerNorm(4), lin) if convert == "in a model" else lin
+    dtype = {"half": torch.float16, "float": torch.float32, "double": torch.float64}.get(convert, torch.bfloat16)
+    if convert in ("to", "in a model"):
+        module.to(dtype)
+    elif convert == "to a device and type":
+        module.to("cpu", dtype)
+    else:
+        getattr(module, convert)()
+    assert lin.weight is weight and lin.weight.scale is lin.scale and lin.weight.dtype == FP4 and lin.scale.dtype == E8M0 and lin.bias.dtype == dtype
+    assert torch.equal(_u8(lin.weight.data), codes) and torch.equal(_u8(lin.scale.data), scale)
+
+
+def test_layers_of_4_bit_weights_on_other_devices():
+    lin = _four_bit_linear()
+    with pytest.raises(TypeError, match="4 bits"):
+        lin.type(torch.float32)
+    assert lin.weight.shape == (48, 128) and lin.weight.dtype == FP4
+    lin.to("meta")
+    assert lin.weight.device.type == "meta" and lin.weight.dtype == FP4 and lin.scale.dtype == E8M0 and lin.weight.shape == (48, 128)
+    lin.to_empty(device="cpu")
+    assert lin.weight.device.type == "cpu" and lin.weight.dtype == FP4 and lin.scale.shape == (48, 8)
+    # e4m3 weights are converted as before
+    from dsv3fp8 import model
+    assert model.Linear(128, 8, dtype=FP8).to(torch.bfloat16).weight.dtype == torch.bfloat16
