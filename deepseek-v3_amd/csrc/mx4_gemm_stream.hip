@@ -20,9 +20,10 @@ constexpr int kMostWaves = 8;
 //
 // AR: activation rows that are copied (rows past them repeat the last one).
 //
-// 7168 -> 18432 (70 MB of weight, 10.8 us at the 6.5 TB/s that a read stream reaches): 14.4 us for one row, 18.3 for 16, 22.4 for 32; straight from memory
-// into the fragments, 1 KiB of both a product, 23, 37 and 53.  Bound by the weight's way from memory, behind it by the launch and its first line, and with 32 rows by
-// the activations, which every workgroup reads (58 MB).
+// 7168 -> 18432 (70 MB of weight, 10.8 us at the 6.5 TB/s that a read stream reaches), a weight from memory in every call: 14.4 us for one row, 18.2 for 16, 22.3 for 32
+// (e4m3 15.5, 21.3 and 25.4; the first form, straight from memory into the fragments, 1 KiB of both a product, 23, 37 and 53).  One weight call after call, most of which
+// the last cache keeps: 12.0, 13.9 and 17.1 (12.7, 16.4 and 19.1).  Bound by the weight's way from memory, behind it by the launch and its first line, and with 32 rows
+// by the activations, which every workgroup reads (58 MB).
 template <bool A8, int AR, int NT, int DEPTH> struct Geo {
     static constexpr int MT = (AR + 15) / 16, AB = A8 ? 512 : 256;      // activation tiles, bytes of an activation row in a chunk
     static constexpr int NB = 4 * NT, NA = AR * AB / 1024;              // copies of a chunk's codes
@@ -175,8 +176,8 @@ template <bool A8, int AR, int NT> int launch_ar(const Mx4Args& p, int c_dtype, 
     using G = Geo<A8, AR, NT, DEPTH>;
     static_assert(DEPTH * G::STAGE <= 80 * 1024, "a wavefront's chunks");
     // Wavefronts of a workgroup: what fits a compute unit's LDS beside the workgroups that share it.  One a unit where there are no more (32 rows of e4m3,
-    // 7168 -> 2112: 11.6 us with one wavefront in half of it); three where activations take little room (one row, 7168 -> 18432: 14.4 us, two of them 15.3,
-    // one 20), else two.
+    // 7168 -> 2112: 7.0 us, with one wavefront in half of it 11.6); three where activations take little room (one row of e4m3, 7168 -> 18432: 15.5 us, two of them
+    // 16.3, one 20.5), else two (16 rows 21.3, one of them 22.6).
     const int64_t strips = (p.n + 16 * NT - 1) / (16 * NT) * ((p.m + AR - 1) / AR), chunks = (p.k + 511) / 512;
     const int room = strips <= 256 ? 160 * 1024 : AR <= 4 ? 54 * 1024 : 80 * 1024;
     int64_t w = room / (DEPTH * G::STAGE);
@@ -187,8 +188,8 @@ template <bool A8, int AR, int NT> int launch_ar(const Mx4Args& p, int c_dtype, 
     if (c_dtype == DSV3_F16) return launch_cd<A8, AR, NT, DEPTH, DSV3_F16>(p, (int)w, st);
     return launch_cd<A8, AR, NT, DEPTH, DSV3_F32>(p, (int)w, st);
 }
-// Two strips a workgroup read the activations half as often, and leave half as many workgroups: 16 x 16384 -> 7168 13.9 us with two and 15.5 with one,
-// 16 x 7168 -> 4096 5.65 and 5.15.
+// Two strips a workgroup read the activations half as often, and leave half as many workgroups: 16 x 16384 -> 7168 15.5 us with two and 17.7 with one,
+// 16 x 7168 -> 4096 5.9 and 5.3.
 template <bool A8, int AR> int launch_nt(const Mx4Args& p, int c_dtype, hipStream_t st) {
     return p.n >= 6144 ? launch_ar<A8, AR, 2>(p, c_dtype, st) : launch_ar<A8, AR, 1>(p, c_dtype, st);
 }

@@ -418,8 +418,9 @@ Plan plan_of(int64_t m, int64_t n, int64_t k, bool a8) {
     // Tiles of 256 where their rounds take less time: a round of one each takes 1.03 us a step (e4m3 1.40), one of two small ones 0.78 (1.0), of one half of that,
     // and where there are no whole rounds of those the next ones fill them.  Of a last round that is half empty each tile goes to two workgroups, 0.58 of the
     // time: 4096 x 7168 -> 18432 (4.5 rounds) 272 us in place of 284, e4m3 367 for 379, 2304 x 7168 -> 9216 (1.27) 91 for 116.  2000 x 7168 -> 7168: 61 us with 224
-    // tiles of 256 and 82 with 896 small ones; 1024 x 7168 -> 18432 98 with 256 tiles and 32 in halves, 106 with small ones (e4m3: 122 and 130); 2048 x 7168 -> 4096
-    // 43 with 128 in halves and 49; 1024 x 7168 -> 4096 32 with 64 in halves and 25 with 256 small ones.
+    // tiles of 256 and 82 with 896 small ones; 1024 x 7168 -> 18432 98 with 256 tiles and 32 in halves, 116 with small ones (e4m3: 123 and 135); 2048 x 7168 -> 4096
+    // 43 with 128 in halves and 49; 1024 x 7168 -> 4096 32 with 64 in halves and 26 with 256 small ones.  The costs are of k = 7168 and count steps alone: 4096 x 2048 -> 7168 takes 47
+    // and 52, 4096 x 512 -> 32768 111 and 129, but 1024 x 512 -> 32768 29 and 26, and 512 x 7168 -> 18432 gets small tiles, 73, where large ones take 57.
     const int64_t large = ((m + 255) / 256) * ((n + 255) / 256), small = ((m + 127) / 128) * ((n + 127) / 128), left = large % 256;
     const bool halves = left > 0 && left <= 128;
     const double rounds = (double)((large + 255) / 256) - (halves ? 0.42 : 0.0), some = small > 512 ? small / 512.0 : small > 256 ? 1.0 : 0.5;
@@ -510,8 +511,9 @@ int launch_mx4_tile(const Mx4Args& q, bool a8, int c_dtype, void* workspace, hip
 // ---- which kernel takes which sizes
 
 // Up to 32 rows the weight is streamed, and beyond where that takes less time: every workgroup of mx4_stream_kernel reads its weight rows and 32 activation rows, all
-// of them at some 12 TB/s.  64 x 7168 -> 2112: 8.5 us streamed and 13.1 in tiles; 100 x 7168 -> 2112 10 and 14.4; 128 x 7168 -> 576 5.3 and 11.4; 300 x 2048 -> 7168
-// 17.2 and 9; 64 x 512 -> 32768, many workgroups, 9.6 and 5.1; 128 x 2048 -> 7168 8.9 and 8.5, e4m3 13.5 and 9.6.
+// of them at some 12 TB/s.  64 x 7168 -> 2112: 8.5 us streamed and 9.5 in tiles; 100 x 7168 -> 2112 10.0 and 11.6; 128 x 7168 -> 576 5.3 and 9.9; 300 x 2048 -> 7168
+// 16.9 and 8.2; 64 x 512 -> 32768, many workgroups, 9.7 and 5.0; 128 x 2048 -> 7168 9.1 and 8.2, e4m3 13.7 and 9.3.  Of 40 sizes with both kinds of activations 77 of 80 get a way
+// within 5 % of the better one; 90 x 4096 -> 4096 of e4m3 does not, 12.4 in tiles and 9.5 streamed, and 200 x 7168 -> 2112, 16.0 and 12.9.
 static bool tiles(int64_t m, int64_t n, int64_t k, bool a8) {
     if (m <= 32 || k == 0) return false;
     const int64_t strip = n >= 6144 ? 32 : 16, groups = (n + strip - 1) / strip * ((m + 31) / 32);
