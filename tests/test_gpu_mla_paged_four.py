@@ -461,3 +461,26 @@ def _at_both_ends(args, seen):
                 off = p * torch.expm1(d + d.max()) + (2.0 ** -135 / r) * p.max()
                 out[i, t, a] = (off * (c @ w[a, NOPE:].T).norm(dim=-1)).sum() + 2.0 ** -134 * w[a, NOPE:].abs().sum(-1).norm()
     return out
+
+
+@pytest.mark.parametrize("size", [-133, -126, -120, -60, 60, 120, 126])
+def test_rows_of_any_size_are_written_and_read(size):
+    """Norm weights of 2^size: latents from binary32's subnormal numbers up to its largest, bit for bit."""
+    g = torch.Generator().manual_seed(size + 200)
+    b, s, page, pages = 2, 9, 8, 6
+    table = torch.randperm(pages, generator=g)[:4].view(2, 2).int()
+    starts, counts = torch.tensor([3, 0], dtype=torch.int32), torch.tensor([9, 9], dtype=torch.int32)
+    a = torch.randn(b, s, C + ROPE, generator=g).bfloat16()
+    a[0, 2, :C - 40] *= 2.0 ** -7
+    kn = (torch.randn(C, generator=g) * 2.0 ** size).bfloat16().clamp(torch.finfo(torch.bfloat16).min, torch.finfo(torch.bfloat16).max)
+    pool, freqs = _pool(g, pages, page), _phases(g, b, s)
+    want = _write_reference(a, None, kn, freqs, *pool, table, starts, counts)
+    dev = [t.cuda() for t in pool]
+    torch.ops.dsv3fp8.mla_latent_paged(a.cuda(), None, kn.cuda(), freqs.cuda(), *dev, table.cuda(), starts.cuda(), counts.cuda(), EPS, EPS)
+    for got, ref in zip(dev, want):
+        assert torch.equal(_bits(got), _bits(ref))
+    kv, _ = torch.ops.dsv3fp8.mla_cache_read(*dev, table.cuda(), torch.tensor([12, 9], dtype=torch.int32).cuda(), 12)
+    values = held(*want[:2]).view(-1, C)
+    for i, n in ((0, 12), (1, 9)):
+        back = values[_rows(table, page, pages, i, range(n))].float().bfloat16()
+        assert torch.equal(kv[i, :n].cpu().isnan(), back.isnan()) and torch.equal(kv[i, :n].cpu().nan_to_num(7.0), back.nan_to_num(7.0))

@@ -347,3 +347,43 @@ def test_no_terms_and_more_rows_than_a_launch_holds(K, m, n, a8):
         del spoilt                                                  # (what the result's memory holds beforehand)
         c = K.mx4_gemm(a, a_s, b, b_s)
         assert c.shape == (m, n) and c.dtype == dtype and (c == 0).all()
+
+
+@pytest.mark.parametrize("a8", [False, True], ids=["mx4", "e4m3"])
+@pytest.mark.parametrize("m,n,k", [(1, 40, 640), (20, 70, 512), (40, 300, 1152), (70, 8200, 512), (300, 700, 640), (1030, 5000, 640)])
+def test_products_of_scales_at_both_ends(K, m, n, k, a8):
+    """Scales of 2^-127 beside scales of 2^127, block by block, so that every product is an ordinary number; the bound is `test_product`'s.  (Activations' e4m3 scales
+    are powers of two that binary32 has as normal numbers.)"""
+    g = torch.Generator().manual_seed(m + k)
+    ends = torch.tensor([0, 1, 2, 3, 60, 127, 190, 251, 252, 253, 254])
+    pick = ends[torch.randint(0, 11, (k // 128,), generator=g)] if a8 else ends[torch.randint(0, 11, (k // 32,), generator=g)]
+    if a8:
+        pick = pick.clamp(1, 253)
+        a = (torch.randn(m, k, generator=g, dtype=torch.float32) * 40).to(FP8)
+        a_s = torch.exp2(pick.double() - 127).float().expand(m, -1).contiguous()
+        va = a.double() * a_s.double().repeat_interleave(128, -1)
+        a, a_s, other = a.cuda(), a_s.cuda(), (254 - pick).repeat_interleave(4)
+    else:
+        a, a_s = numbers(torch.randint(0, 16, (m, k), generator=g), pick.expand(m, -1))
+        va, other = held(a, a_s), 254 - pick
+    b, b_s = numbers(torch.randint(0, 16, (n, k), generator=g), other.expand(n, -1))
+    vb = held(b, b_s)
+    ref, size = va @ vb.t(), va.abs() @ vb.abs().t()
+    bound = size * (k / 32 + 7) * 2.0 ** -23 + (size * 7 * 2.0 ** -13 if a8 else 0)
+    torch.set_default_dtype(torch.float32)
+    c = K.mx4_gemm(a, a_s, b, b_s).cpu().double()
+    assert ref.abs().max() > 1 and ((c - ref).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 40, 640), (40, 300, 1152), (300, 700, 640), (1030, 5000, 640)])
+def test_products_smaller_and_larger_than_binary32(K, m, n, k):
+    """Scales of 2^-127 on both sides: zeros.  Of 2^127 on both: infinities of the sums' sign where all terms have one sign."""
+    torch.set_default_dtype(torch.float32)
+    a, _ = numbers(torch.full((m, k), 7), torch.zeros(m, k // 32))
+    codes = torch.full((n, k), 7)
+    codes[1::2] = 15
+    b, _ = numbers(codes, torch.zeros(n, k // 32))
+    scales = lambda rows, byte: torch.full((rows, k // 32), byte, dtype=torch.uint8).cuda().view(E8M0)  # noqa: E731
+    assert (K.mx4_gemm(a, scales(m, 0), b, scales(n, 0)) == 0).all()
+    c = K.mx4_gemm(a, scales(m, 254), b, scales(n, 254))
+    assert (c[:, 0::2] == float("inf")).all() and (c[:, 1::2] == float("-inf")).all()
