@@ -176,7 +176,7 @@ class Linear(nn.Module):
             if raw.dtype != torch.uint8:
                 raise TypeError(f"Linear: weights of 4 bits cannot become {raw.dtype}")
             return raw.view(t.dtype)
-        return super()._apply(of_bytes if self.weight.dtype == FP4 else fn, recurse)
+        return super()._apply(of_bytes, recurse)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return linear(x, self.weight, self.bias, self.scale_fmt)

@@ -378,3 +378,10 @@ def test_layers_of_4_bit_weights_on_other_devices():
     # e4m3 weights are converted as before
     from dsv3fp8 import model
     assert model.Linear(128, 8, dtype=FP8).to(torch.bfloat16).weight.dtype == torch.bfloat16
+
+
+def test_layers_without_a_weight_are_moved_as_before():
+    from dsv3fp8 import model
+    lin = model.Linear(128, 8, bias=True)
+    del lin.weight
+    assert lin.to(torch.float16).bias.dtype == torch.float16
