@@ -508,8 +508,8 @@ int dsv3_mla_cache_read(const dsv3_mla_pages* cache, const int32_t* lengths, voi
  * sequence b sees every position below starts[b], and position starts[b] + j where bit j of tree[b, i] is set and j < counts[b]
  * (tree: int64 [batch, rows], 8-byte aligned, or NULL: bits 0 .. i).  Ancestors and the token itself for a tree; any other bits do.
  * A token that sees nothing, and tokens from counts[b] on, give zeros.  A latent of NaN reaches the tokens that see it and no others.
- * Sums are binary32, of weights up to 1 wherever latents are large: finite as long as `positions` latents of the largest one's size are below 2^127 in sum.  A weight
- * times its row's scale is kept down to 2^-135: below 2^-108, scales leave their weights fewer bits than elsewhere.
+ * Sums are binary32, of weights up to 1 wherever latents are large: finite as long as `positions` latents of the largest one's size are below 2^127 in sum.  Weights
+ * times their rows' scales are codes whose exponent ends at 2^-122: where all rows that a token sees have scales below 2^-108, results may be off by latents of that size.
  * `positions`: no sequence has more (what lies behind is not seen); at most table_width * page_size.  It and the other sizes are all that
  * the host knows: lengths are read on the device, the work is divided there.
  * q: bf16 [batch, rows, heads, 192], its last 64 elements not yet rotated; freqs: binary32 (cos, sin) pairs [batch, rows, 32], each
